@@ -679,6 +679,120 @@ typedef struct mote_dechunk_step_args {
 
 int mote_dechunk_step(const mote_dechunk_step_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The {P2, I~} cache held in 4 bits. No counterpart in the reference, whose arena holds its rows in
+ * the model's dtype (mote/model/arena.py:30-51).
+ * Format. A row's D values (D % 8 == 0, D <= 128) form G = ceil(D / 32) groups of 32. A group holds the
+ * bf16 scale s = bf16(max|x| / 6) and one e2m1 code per value: the magnitude among 0, 0.5, 1, 1.5, 2, 3,
+ * 4, 6 nearest to min(|x (1 / s)|, 6) (fp32 quotient and product, ties to the even code) and the sign of x;
+ * the value is code * s. A group whose s is below 2^-126 stores zeros; one with a NaN or an infinity
+ * stores the scale NaN, so every value read from it is NaN. Dim 2 i of a row is the low half of its
+ * byte i, dim 2 i + 1 the high half; a row's codes are padded to whole groups (16 G bytes).
+ * mote_cache4: codes [B, H, capacity, 16 G] bytes and scales [B, H, capacity, G] bf16 of P2 and I~,
+ * rows of one head back to back; batch and head strides in bytes for the codes (codes on 16-byte
+ * boundaries), in elements for the scales.
+ * ------------------------------------------------------------------------------------------------ */
+typedef struct mote_cache4 {
+  void* p2;
+  void* p2_scale;
+  void* info;
+  void* info_scale;
+  int64_t codes_sb;
+  int64_t codes_sh;
+  int64_t scale_sb;
+  int64_t scale_sh;
+} mote_cache4;
+
+/* mote_cache4_write: rows start + t, t < T, of every sequence and head from p2 / info [B, H, T, D]
+ * (dtype; rows on 16-byte boundaries). start is `start`, or start_dev[b] (device) when start_dev is not
+ * NULL; with lens (device, [B], or NULL) sequence b writes its first lens[b] rows only. Rows outside
+ * [0, capacity) are skipped. Replaces: ArenaLayer.write (mote/model/arena.py:133-139).
+ * mote_cache4_read: rows start + t, t < T, into the views p2 / info (dtype), each value rounded once;
+ * rows outside [0, capacity) read as NaN; lens is not used. */
+typedef struct mote_cache4_rows_args {
+  int dtype;
+  int B, H, T, D, capacity;
+  mote_view p2, info;
+  mote_cache4 cache;
+  int64_t start;
+  const int64_t* start_dev;
+  const int64_t* lens;
+} mote_cache4_rows_args;
+
+int mote_cache4_write(const mote_cache4_rows_args* args, void* stream);
+int mote_cache4_read(const mote_cache4_rows_args* args, void* stream);
+
+/* One decode step over that cache: mote_relation_decode (see there for every argument they share) with
+ * the past rows j < S at their 4-bit values. The Self term and the new chunk's share of y take the new
+ * rows as they are; they are then stored in 4 bits at row S. S[b] outside [0, capacity) writes NaN into
+ * y[b] and g[b] and stores nothing. The workspace (mote_relation_decode4_workspace() bytes, zeroed once
+ * before its first call) is left with its counters at zero; it serves calls of one B and H (the counters'
+ * places follow from them), one after the other. */
+typedef struct mote_relation_decode4_args {
+  int dtype;
+  int B, H, D, capacity, layer_parity, flags;
+  float tau_s;
+  const float* lam;
+  const float* inv_freq;
+  const float* theta;
+  int64_t* S;
+  const void* p1;
+  const void* p2;
+  const void* info;
+  int64_t in_sb;
+  mote_cache4 cache;
+  void* y;
+  int64_t y_sb;
+  float* g;
+  void* workspace;
+  size_t workspace_bytes;
+  float* xm;
+  const unsigned char* run;
+} mote_relation_decode4_args;
+
+size_t mote_relation_decode4_workspace(const mote_relation_decode4_args* args);
+int mote_relation_decode4(const mote_relation_decode4_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Products in 8-bit integers with one fp32 scale per row of either operand (a token of x, an output
+ * channel of W). No counterpart in the reference (its projections are nn.Linear in the model's dtype).
+ * mote_quantize_rows: row m of x [M, K] (dtype) as q [M, Kp] int8 and scale[m] fp32, Kp = K rounded up
+ * to 128: scale = max|x| / 127, q = rint(x (127 / max|x|)) (fp32 quotient and product, ties to even),
+ * zeros past K. A row whose maximum is below 2^-120 stores zeros with scale 0; one with a NaN or an
+ * infinity stores zeros with scale NaN.
+ * mote_int8_linear: y [M, N] (dtype) = ((float(acc) sx[m]) sw[n]) rounded once, acc = sum_k xq wq exact in
+ * 32-bit integers (K <= 131072); x is quantised in the call, wq [N, Kp] and sw [N] come from
+ * mote_quantize_rows. Up to 16 rows with K <= 4096 are one launch, which takes the decode step's predicate
+ * and exchange mass as mote_skinny_gemm does; others quantise x into the workspace first
+ * (mote_int8_linear_workspace() bytes; its contents on entry do not matter) and take neither.
+ * Row strides in elements; wq on a 16-byte boundary with its rows Kp apart.
+ * ------------------------------------------------------------------------------------------------ */
+typedef struct mote_quantize_rows_args {
+  int dtype;
+  int M, K;
+  const void* x; int64_t x_sr;
+  int8_t* q;
+  float* scale;
+} mote_quantize_rows_args;
+
+int mote_quantize_rows(const mote_quantize_rows_args* args, void* stream);
+
+typedef struct mote_int8_linear_args {
+  int dtype;
+  int M, N, K;
+  const void* x; int64_t x_sr;
+  const int8_t* wq;
+  const float* w_scale;
+  void* y; int64_t y_sr;
+  void* workspace;
+  size_t workspace_bytes;
+  const unsigned char* run;
+  const float* g; float* xm; int heads;
+} mote_int8_linear_args;
+
+size_t mote_int8_linear_workspace(const mote_int8_linear_args* args);
+int mote_int8_linear(const mote_int8_linear_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,7 @@ HIP stream of the tensors' device.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import importlib.util
 import os
@@ -247,6 +248,48 @@ class DechunkStepArgs(C.Structure):
     ]
 
 
+class Cache4View(C.Structure):
+    _fields_ = [
+        ("p2", C.c_void_p), ("p2_scale", C.c_void_p), ("info", C.c_void_p), ("info_scale", C.c_void_p),
+        ("codes_sb", C.c_int64), ("codes_sh", C.c_int64), ("scale_sb", C.c_int64), ("scale_sh", C.c_int64),
+    ]
+
+
+class Cache4RowsArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("B", C.c_int), ("H", C.c_int), ("T", C.c_int), ("D", C.c_int), ("capacity", C.c_int),
+        ("p2", View), ("info", View), ("cache", Cache4View),
+        ("start", C.c_int64), ("start_dev", C.c_void_p), ("lens", C.c_void_p),
+    ]
+
+
+class Decode4Args(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("B", C.c_int), ("H", C.c_int), ("D", C.c_int), ("capacity", C.c_int),
+        ("layer_parity", C.c_int), ("flags", C.c_int), ("tau_s", C.c_float),
+        ("lam", C.c_void_p), ("inv_freq", C.c_void_p), ("theta", C.c_void_p), ("S", C.c_void_p),
+        ("p1", C.c_void_p), ("p2", C.c_void_p), ("info", C.c_void_p), ("in_sb", C.c_int64),
+        ("cache", Cache4View), ("y", C.c_void_p), ("y_sb", C.c_int64), ("g", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("xm", C.c_void_p), ("run", C.c_void_p),
+    ]
+
+
+class QuantizeRowsArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("M", C.c_int), ("K", C.c_int), ("x", C.c_void_p), ("x_sr", C.c_int64),
+        ("q", C.c_void_p), ("scale", C.c_void_p),
+    ]
+
+
+class Int8LinearArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("M", C.c_int), ("N", C.c_int), ("K", C.c_int), ("x", C.c_void_p), ("x_sr", C.c_int64),
+        ("wq", C.c_void_p), ("w_scale", C.c_void_p), ("y", C.c_void_p), ("y_sr", C.c_int64),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("run", C.c_void_p),
+        ("g", C.c_void_p), ("xm", C.c_void_p), ("heads", C.c_int),
+    ]
+
+
 # every symbol the header declares, with its argument types
 EXPORTS = {
     "mote_last_error": ([], C.c_char_p),
@@ -287,6 +330,13 @@ EXPORTS = {
     "mote_dechunk_bwd_workspace": ([C.POINTER(DechunkBwdArgs)], C.c_size_t),
     "mote_dechunk_bwd": ([C.POINTER(DechunkBwdArgs), C.c_void_p], C.c_int),
     "mote_dechunk_step": ([C.POINTER(DechunkStepArgs), C.c_void_p], C.c_int),
+    "mote_cache4_write": ([C.POINTER(Cache4RowsArgs), C.c_void_p], C.c_int),
+    "mote_cache4_read": ([C.POINTER(Cache4RowsArgs), C.c_void_p], C.c_int),
+    "mote_relation_decode4_workspace": ([C.POINTER(Decode4Args)], C.c_size_t),
+    "mote_relation_decode4": ([C.POINTER(Decode4Args), C.c_void_p], C.c_int),
+    "mote_quantize_rows": ([C.POINTER(QuantizeRowsArgs), C.c_void_p], C.c_int),
+    "mote_int8_linear_workspace": ([C.POINTER(Int8LinearArgs)], C.c_size_t),
+    "mote_int8_linear": ([C.POINTER(Int8LinearArgs), C.c_void_p], C.c_int),
     "mote_abi_layout": ([], C.c_char_p),
     "mote_clock_probe": ([C.c_void_p, C.c_int, C.c_int, C.c_void_p], C.c_int),
 }
@@ -303,7 +353,9 @@ STRUCTS = {
     "mote_page_copy_args": PageCopyArgs, "mote_chunk_route_args": ChunkRouteArgs,
     "mote_chunk_gather_args": ChunkGatherArgs, "mote_chunk_gather_bwd_args": ChunkGatherBwdArgs,
     "mote_dechunk_args": DechunkArgs, "mote_dechunk_bwd_args": DechunkBwdArgs,
-    "mote_dechunk_step_args": DechunkStepArgs,
+    "mote_dechunk_step_args": DechunkStepArgs, "mote_cache4": Cache4View, "mote_cache4_rows_args": Cache4RowsArgs,
+    "mote_relation_decode4_args": Decode4Args, "mote_quantize_rows_args": QuantizeRowsArgs,
+    "mote_int8_linear_args": Int8LinearArgs,
 }
 
 
@@ -384,6 +436,23 @@ def view(t: torch.Tensor) -> View:
 def stream_of(t: torch.Tensor) -> int:
     """The current stream of t's device as a raw handle (without the Stream object around it)."""
     return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+def stream_or_null(t: torch.Tensor) -> int:
+    """stream_of for calls whose checks come with the launch: null for a tensor on the CPU, which they refuse."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index) if t.is_cuda else 0
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def device_of(t):
+    """A context in which a tensor's (or a given) GPU is the current device, which is where a launch goes.
+    Nothing is entered where it is current already, and for the CPU, whose calls the checks refuse."""
+    dev = t.device if torch.is_tensor(t) else torch.device(t)
+    if dev.type != "cuda" or dev.index is None or dev.index == torch._C._cuda_getDevice():
+        return _HERE_ALREADY
+    return torch.cuda.device(dev)
 
 
 def ptr(t) -> int:

@@ -33,6 +33,13 @@ int launch_wgrad(const mote_wgrad_args* a, hipStream_t stream);
 size_t linear_wgrad_workspace_bytes(const mote_linear_wgrad_args* a);
 int launch_qkv_rope_parts_fwd(const mote_qkv_rope_args* a, const void* w2, const void* wi, hipStream_t stream);
 int launch_linear_wgrad(const mote_linear_wgrad_args* a, hipStream_t stream);
+int launch_cache4_write(const mote_cache4_rows_args* a, hipStream_t stream);
+int launch_cache4_read(const mote_cache4_rows_args* a, hipStream_t stream);
+size_t decode4_workspace_bytes(const mote_relation_decode4_args* a);
+int launch_decode4(const mote_relation_decode4_args* a, hipStream_t stream);
+int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream);
+size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a);
+int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream);
 
 }  // namespace mote
 
@@ -187,6 +194,39 @@ int mote_dechunk_bwd(const mote_dechunk_bwd_args* args, void* stream) {
 int mote_dechunk_step(const mote_dechunk_step_args* args, void* stream) {
   mote::g_err[0] = 0;
   return mote::launch_dechunk_step(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+int mote_cache4_write(const mote_cache4_rows_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_cache4_write(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+int mote_cache4_read(const mote_cache4_rows_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_cache4_read(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t mote_relation_decode4_workspace(const mote_relation_decode4_args* args) {
+  return args ? mote::decode4_workspace_bytes(args) : 0;
+}
+
+int mote_relation_decode4(const mote_relation_decode4_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_decode4(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+int mote_quantize_rows(const mote_quantize_rows_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_quantize_rows(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t mote_int8_linear_workspace(const mote_int8_linear_args* args) {
+  return args ? mote::int8_linear_workspace_bytes(args) : 0;
+}
+
+int mote_int8_linear(const mote_int8_linear_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_int8_linear(args, reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -1,0 +1,105 @@
+// Values in 4 bits: groups of 32 share a bf16 scale, codes are e2m1 (mote_relation.h has the format).
+//
+// Four lanes of a quad hold one group of a row while it is encoded, eight values (an octet) each. The
+// group's maximum goes over the bits of |x|: as unsigned integers they order as the magnitudes do, with
+// infinities and NaNs on top, so one comparison finds the groups that have no scale.
+#pragma once
+
+#include "common.hpp"
+
+namespace mote {
+
+constexpr int kGroup4 = 32;            // values per scale
+constexpr float kTiny4 = 0x1p-126f;    // a smaller scale stores zeros (its inverse would overflow)
+constexpr bf16_t kNanScale4 = 0x7fc0;
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
+typedef __attribute__((ext_vector_type(2))) float f32x2;
+
+// byte i (0..3) of a code word: values 2 i and 2 i + 1
+template <int I>
+__device__ __forceinline__ bf16x2 codes_bf16(uint32_t w) {
+  return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, 1.0f, I);
+}
+template <int I>
+__device__ __forceinline__ f32x2 codes_f32(uint32_t w) {
+  return __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, I);
+}
+
+__device__ __forceinline__ uint32_t quad_umax(uint32_t m) {
+  m = max(m, uint32_t(__builtin_amdgcn_mov_dpp(int(m), kDppXor1, 0xF, 0xF, false)));
+  return max(m, uint32_t(__builtin_amdgcn_mov_dpp(int(m), kDppXor2, 0xF, 0xF, false)));
+}
+
+// The quad's group in 4 bits: this lane's eight codes, and the group's scale. All four lanes must be here
+// (lanes past the head dim with zeros). Rounding points: the scale once to bf16 (a wider one would cost
+// more than it gains: codes are 2^-2 apart), the inverse and the products in fp32.
+__device__ __forceinline__ uint32_t encode4(const float (&x)[8], bf16_t& scale) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
+  top = quad_umax(top);
+  const bool finite = top < 0x7f800000u;
+  bf16_t sb = f2bf(__uint_as_float(finite ? top : 0u) / 6.0f);
+  if (bf2f(sb) < kTiny4) sb = 0;
+  const float inv = sb ? 1.0f / bf2f(sb) : 0.f;
+  scale = finite ? sb : kNanScale4;
+  float t[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) t[j] = finite ? __builtin_amdgcn_fmed3f(x[j] * inv, -6.0f, 6.0f) : 0.f;
+  uint32_t w = 0;  // v_cvt_scalef32_pk_fp4_f32 rounds to nearest, ties to the even code
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[0], t[1], 1.0f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[2], t[3], 1.0f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[4], t[5], 1.0f, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[6], t[7], 1.0f, 3);
+  return w;
+}
+
+__device__ __forceinline__ void decode4(uint32_t w, float s, float (&x)[8]) {
+  const f32x2 a = codes_f32<0>(w), b = codes_f32<1>(w), c = codes_f32<2>(w), d = codes_f32<3>(w);
+  x[0] = a.x * s; x[1] = a.y * s; x[2] = b.x * s; x[3] = b.y * s;
+  x[4] = c.x * s; x[5] = c.y * s; x[6] = d.x * s; x[7] = d.y * s;
+}
+
+// eight elements of a 16-byte aligned row
+template <typename T>
+__device__ __forceinline__ void load_octet(const T* p, float (&x)[8]);
+template <>
+__device__ __forceinline__ void load_octet<bf16_t>(const bf16_t* p, float (&x)[8]) {
+  const Chunk c = load_chunk(p);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = __uint_as_float(c.w[j] << 16);
+    x[2 * j + 1] = __uint_as_float(c.w[j] & 0xffff0000u);
+  }
+}
+template <>
+__device__ __forceinline__ void load_octet<float>(const float* p, float (&x)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+template <typename T>
+__device__ __forceinline__ void store_octet(T* p, const float (&x)[8]);
+template <>
+__device__ __forceinline__ void store_octet<bf16_t>(bf16_t* p, const float (&x)[8]) {
+  Chunk c;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) c.w[j] = uint32_t(f2bf(x[2 * j])) | uint32_t(f2bf(x[2 * j + 1])) << 16;
+  store_chunk(p, c);
+}
+template <>
+__device__ __forceinline__ void store_octet<float>(float* p, const float (&x)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+
+// what a launcher checks of a cache in 4 bits: null pointers, alignment, strides that hold a row each
+inline const char* bad_cache4(const mote_cache4& c) {
+  if (!c.p2 || !c.p2_scale || !c.info || !c.info_scale) return "null pointer";
+  const uintptr_t codes = reinterpret_cast<uintptr_t>(c.p2) | reinterpret_cast<uintptr_t>(c.info);
+  const uintptr_t scales = reinterpret_cast<uintptr_t>(c.p2_scale) | reinterpret_cast<uintptr_t>(c.info_scale);
+  if (codes % 16 || c.codes_sb % 16 || c.codes_sh % 16 || scales % 2) return "codes must start on 16-byte boundaries";
+  return nullptr;
+}
+
+}  // namespace mote

@@ -7,8 +7,11 @@
 // when a call fails. Host code only; streams come as raw handles.
 #include <torch/extension.h>
 
+#include <climits>
+#include <initializer_list>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include "../../include/mote_relation.h"
 
@@ -389,6 +392,266 @@ std::tuple<Tensor, Tensor> dechunk_bwd(const Tensor& g, const Tensor& h, const T
   return {dh, dp};
 }
 
+// ---- the cache in 4 bits and the 8-bit products: checks, allocation and launch in one call ----------
+template <typename... A>
+[[noreturn]] void bad_value(A&&... a) { throw py::value_error(c10::str(std::forward<A>(a)...)); }
+void on_gpu(const Tensor& t, const char* what) {
+  if (!t.is_cuda()) throw std::runtime_error(c10::str(what, " needs the HIP library and an MI355X"));
+}
+void no_grad(const char* what, std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor* t : ts)
+    if (t->requires_grad()) throw std::runtime_error(c10::str(what, " has no backward: call it under torch.no_grad()"));
+}
+// an int64 position per sequence (read, and with `advance` written, by the kernel as it is)
+void positions(const Tensor& t, int64_t B, c10::Device dev, const char* what, const char* name) {
+  if (t.scalar_type() != at::kLong || t.device() != dev || t.numel() != B || !t.is_contiguous())
+    bad_value(what, ": ", name, " must be a contiguous int64 tensor of B = ", B, " on the rows' device");
+}
+
+struct Cache4 {
+  mote_cache4 c;
+  int64_t capacity;
+};
+Cache4 cache4(const Tensor& p2, const Tensor& s2, const Tensor& info, const Tensor& si, int64_t B, int64_t H, int64_t D,
+              c10::Device dev, bool writes, const char* what) {
+  if (D <= 0 || D > 128 || D % 8) bad_value(what, ": head dim ", D, " unsupported (need 8 <= D <= 128, D % 8 == 0)");
+  const int64_t G = (D + 31) / 32;
+  const int64_t cap = p2.dim() == 4 ? p2.size(2) : 0;
+  auto check = [&](const Tensor& t, const Tensor& like, int64_t width, at::ScalarType dt, const char* name) {
+    if (t.dim() != 4 || t.size(0) != B || t.size(1) != H || t.size(2) != cap || t.size(3) != width || cap < 1)
+      bad_value(what, ": ", name, " must be [B, H, capacity, ", width, "] = [", B, ", ", H, ", ", cap, ", ", width, "], got ", t.sizes());
+    if (t.scalar_type() != dt || t.device() != dev)
+      throw py::type_error(c10::str(what, ": ", name, " must be ", c10::toString(dt), " on the rows' device"));
+    if ((width > 1 && t.stride(3) != 1) || (cap > 1 && t.stride(2) != width))
+      bad_value(what, ": the rows of a head must lie back to back (", name, ")");
+    for (int d = 0; d < 2; ++d) {
+      if (t.size(d) > 1 && t.stride(d) != like.stride(d)) bad_value(what, ": P2 and I~ must have the same strides");
+      // heads (or sequences) that share rows would be written over one another
+      if (writes && t.size(d) > 1 && t.stride(d) == 0) bad_value(what, ": ", name, " holds its rows for several heads at once");
+    }
+  };
+  check(p2, p2, 16 * G, at::kByte, "the codes of P2");
+  check(info, p2, 16 * G, at::kByte, "the codes of I~");
+  check(s2, s2, G, at::kBFloat16, "the scales of P2");
+  check(si, s2, G, at::kBFloat16, "the scales of I~");
+  Cache4 r;
+  r.c = mote_cache4{p2.data_ptr(), s2.data_ptr(), info.data_ptr(), si.data_ptr(),
+                    p2.size(0) > 1 ? p2.stride(0) : 0, p2.size(1) > 1 ? p2.stride(1) : 0,
+                    s2.size(0) > 1 ? s2.stride(0) : 0, s2.size(1) > 1 ? s2.stride(1) : 0};
+  r.capacity = cap;
+  if (cap > (int64_t(1) << 30)) bad_value(what, ": a capacity of ", cap, " rows (at most 2^30)");
+  return r;
+}
+
+void rows_of_start(mote_cache4_rows_args& a, const Cache4& c, int64_t start, const OptTensor& start_dev, const OptTensor& lens,
+                   int64_t B, int64_t T, c10::Device dev, const char* what) {
+  if (start_dev) {
+    positions(*start_dev, B, dev, what, "start");
+    a.start_dev = static_cast<const int64_t*>(start_dev->data_ptr());
+  } else if (start < 0 || T < 0 || start > c.capacity - T) {
+    throw std::runtime_error(c10::str(what, ": rows ", start, " to ", start + T, " in a capacity of ", c.capacity));
+  }
+  a.start = start;
+  if (lens) {
+    positions(*lens, B, dev, what, "lens");
+    a.lens = static_cast<const int64_t*>(lens->data_ptr());
+  }
+  a.cache = c.c;
+  a.capacity = int(c.capacity);
+}
+
+void cache4_write(const Tensor& k, const Tensor& ks, const Tensor& v, const Tensor& vs, Tensor p2, Tensor info, int64_t start,
+                  const OptTensor& start_dev, const OptTensor& lens, int64_t stream) {
+  const char* what = "cache4_write";
+  if (p2.dim() != 4 || info.sizes() != p2.sizes()) bad_value(what, ": p2 and info must both be [B, H, T, D]");
+  if (info.scalar_type() != p2.scalar_type() || info.device() != p2.device())
+    throw py::type_error("cache4_write: p2 and info must share a dtype and a device");
+  const int64_t B = p2.size(0), H = p2.size(1), T = p2.size(2), D = p2.size(3);
+  const Cache4 c = cache4(k, ks, v, vs, B, H, D, p2.device(), true, what);
+  mote_cache4_rows_args a{};
+  a.dtype = code(p2);
+  rows_of_start(a, c, start, start_dev, lens, B, T, p2.device(), what);
+  no_grad(what, {&p2, &info});
+  on_gpu(p2, what);
+  p2 = aligned(p2); info = aligned(info);
+  a.B = int(B); a.H = int(H); a.T = int(T); a.D = int(D);
+  a.p2 = view(p2); a.info = view(info);
+  check(mote_cache4_write(&a, reinterpret_cast<void*>(stream)), "mote_cache4_write");
+}
+
+std::tuple<Tensor, Tensor> cache4_read(const Tensor& k, const Tensor& ks, const Tensor& v, const Tensor& vs, int64_t D,
+                                       int64_t start, const OptTensor& start_dev, int64_t rows, at::ScalarType dtype,
+                                       const OptTensor& out2, const OptTensor& outi, int64_t stream) {
+  const char* what = "cache4_read";
+  if (k.dim() != 4) bad_value(what, ": the codes of P2 must be [B, H, capacity, 16 G]");
+  const int64_t B = k.size(0), H = k.size(1);
+  const Cache4 c = cache4(k, ks, v, vs, B, H, D, k.device(), false, what);
+  mote_cache4_rows_args a{};
+  if (rows < 0) bad_value(what, ": ", rows, " rows");
+  rows_of_start(a, c, start, start_dev, std::nullopt, B, rows, k.device(), what);
+  Tensor p2, info;
+  if (out2) {
+    p2 = *out2; info = *outi;
+    for (const Tensor* t : {&p2, &info}) {
+      if (t->dim() != 4 || t->size(0) != B || t->size(1) != H || t->size(2) != rows || t->size(3) != D || t->device() != k.device())
+        bad_value(what, ": out must be two [B, H, rows, D] tensors on the cache's device");
+      for (int d = 0; d < 3; ++d)
+        if (t->size(d) > 1 && t->stride(d) == 0) bad_value(what, ": out holds its rows for several places at once");
+    }
+    if (info.scalar_type() != p2.scalar_type()) throw py::type_error("cache4_read: out must be two tensors of one dtype");
+    if (p2.requires_grad() || info.requires_grad()) throw std::runtime_error("cache4_read: out must not require a gradient");
+  }
+  a.dtype = code(out2 ? p2.scalar_type() : dtype);
+  on_gpu(k, what);
+  if (!out2) {
+    p2 = empty({B, H, rows, D}, k, dtype);
+    info = empty({B, H, rows, D}, k, dtype);
+  }
+  a.B = int(B); a.H = int(H); a.T = int(rows); a.D = int(D);
+  a.p2 = view(p2); a.info = view(info);
+  check(mote_cache4_read(&a, reinterpret_cast<void*>(stream)), "mote_cache4_read");
+  return {p2, info};
+}
+
+// a small fp32 parameter of n values on `like`'s device (itself when it is that already)
+Tensor small_f32(const Tensor& t, int64_t n, const Tensor& like, const char* what, const char* name) {
+  if (t.numel() != n || t.device() != like.device())
+    bad_value(what, ": ", name, " must be a tensor of ", n, " element(s) on the inputs' device");
+  return t.scalar_type() == at::kFloat && t.is_contiguous() ? t : t.detach().to(at::kFloat).contiguous();
+}
+void check_run(const OptTensor& run, const Tensor& like, const char* what) {
+  if (run && ((run->scalar_type() != at::kBool && run->scalar_type() != at::kByte) || run->numel() != 1 || run->device() != like.device()))
+    bad_value(what, ": run must be a one-element bool or uint8 tensor on the inputs' device");
+}
+
+std::tuple<Tensor, Tensor> relation_decode4(const Tensor& p1, const Tensor& p2, const Tensor& info, const Tensor& S, const Tensor& k,
+                                            const Tensor& ks, const Tensor& v, const Tensor& vs, const Tensor& lam, double tau,
+                                            const OptTensor& inv_freq, const OptTensor& theta, int64_t layer_idx, bool advance,
+                                            const OptTensor& workspace, const OptTensor& y_, const OptTensor& g_, const OptTensor& xm,
+                                            const OptTensor& run, bool rope_f32, int64_t stream) {
+  const char* what = "relation_decode4";
+  if (p1.dim() != 3) bad_value(what, ": p1/p2/info must be [B, H, dh]");
+  const int64_t B = p1.size(0), H = p1.size(1), D = p1.size(2);
+  const c10::Device dev = p1.device();
+  for (const Tensor* t : {&p1, &p2, &info}) {
+    if (t->sizes() != p1.sizes() || t->stride(2) != 1 || t->stride(1) != D || (B > 1 && t->stride(0) != p1.stride(0)))
+      bad_value(what, ": p1/p2/info must be [B, H, dh] with head stride dh and one batch stride");
+    if (t->scalar_type() != p1.scalar_type() || t->device() != dev)
+      throw py::type_error("relation_decode4: p1, p2 and info must share a dtype and a device");
+  }
+  if (B < 1 || H < 1 || H % 2) bad_value(what, ": B = ", B, " sequences of H = ", H, " heads (an even number)");
+  mote_relation_decode4_args a{};
+  a.dtype = code(p1);
+  const Cache4 c = cache4(k, ks, v, vs, B, H, D, dev, true, what);
+  positions(S, B, dev, what, "S");
+  const Tensor lam32 = small_f32(lam, 1, p1, what, "lam");
+  Tensor inv, th;
+  if (inv_freq) inv = small_f32(*inv_freq, D / 2, p1, what, "inv_freq");
+  if (theta) th = small_f32(*theta, H / 2, p1, what, "theta");
+  if (xm && (xm->scalar_type() != at::kFloat || xm->numel() != B || !xm->is_contiguous() || xm->device() != dev))
+    bad_value(what, ": xm must be a contiguous fp32 tensor of B elements");
+  check_run(run, p1, what);
+  if (workspace && (workspace->device() != dev || !workspace->is_contiguous()))
+    bad_value(what, ": workspace must be a contiguous tensor on the inputs' device");
+  if (y_ && (y_->sizes() != p1.sizes() || y_->scalar_type() != p1.scalar_type() || y_->device() != dev || y_->stride(2) != 1 ||
+             y_->stride(1) != D || (B > 1 && y_->stride(0) < H * D)))
+    bad_value(what, ": y must be [B, H, dh] in the inputs' dtype with head stride dh");
+  if (g_ && (g_->dim() != 2 || g_->size(0) != B || g_->size(1) != H || g_->scalar_type() != at::kFloat || g_->device() != dev ||
+             !g_->is_contiguous()))
+    bad_value(what, ": g must be a contiguous fp32 [B, H] tensor");
+  no_grad(what, {&p1, &p2, &info});
+  on_gpu(p1, what);
+  Tensor y = y_ ? *y_ : empty({B, H, D}, p1, p1.scalar_type());
+  Tensor g = g_ ? *g_ : empty({B, H}, p1, at::kFloat);
+  a.B = int(B); a.H = int(H); a.D = int(D); a.capacity = int(c.capacity);
+  a.layer_parity = int(((layer_idx % 2) + 2) % 2);
+  a.flags = (advance ? MOTE_DECODE_ADVANCE : 0) | (rope_f32 ? MOTE_DECODE_ROPE_F32 : 0);
+  a.tau_s = float(tau);
+  a.lam = fptr(lam32);
+  a.inv_freq = inv_freq ? fptr(inv) : nullptr;
+  a.theta = theta ? fptr(th) : nullptr;
+  a.S = static_cast<int64_t*>(S.data_ptr());
+  a.p1 = p1.data_ptr(); a.p2 = p2.data_ptr(); a.info = info.data_ptr(); a.in_sb = p1.stride(0);
+  a.cache = c.c;
+  a.y = y.data_ptr(); a.y_sb = y.stride(0); a.g = fptr(g);
+  const int64_t need = int64_t(mote_relation_decode4_workspace(&a));
+  // another shape's counters lie elsewhere: its workspace would not be zero where this call counts
+  if (workspace && workspace->numel() * workspace->element_size() != need)
+    bad_value(what, ": a workspace of ", workspace->numel() * workspace->element_size(), " bytes, ", need,
+              " needed (decode4_workspace makes one for these sizes)");
+  const Tensor ws = workspace ? *workspace : at::zeros({need}, p1.options().dtype(at::kByte));
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = size_t(ws.numel()) * ws.element_size();
+  a.xm = xm ? fptr(*xm) : nullptr;
+  a.run = run ? static_cast<const unsigned char*>(run->data_ptr()) : nullptr;
+  check(mote_relation_decode4(&a, reinterpret_cast<void*>(stream)), "mote_relation_decode4");
+  return {y, g};
+}
+
+std::tuple<Tensor, Tensor> quantize_rows(Tensor x, int64_t stream) {
+  if (x.dim() != 2 || x.size(1) < 1) bad_value("quantize_rows: x must be [M, K]");
+  mote_quantize_rows_args a{};
+  a.dtype = code(x);
+  no_grad("quantize_rows", {&x});
+  on_gpu(x, "quantize_rows");
+  x = unit(x);
+  const int64_t M = x.size(0), K = x.size(1);
+  Tensor q = empty({M, (K + 127) / 128 * 128}, x, at::kChar), scale = empty({M}, x, at::kFloat);
+  TORCH_CHECK(M <= INT_MAX && K <= INT_MAX, "quantize_rows: sizes beyond 32 bits");
+  a.M = int(M); a.K = int(K);
+  a.x = x.data_ptr(); a.x_sr = x.stride(0);
+  a.q = static_cast<int8_t*>(q.data_ptr()); a.scale = fptr(scale);
+  check(mote_quantize_rows(&a, reinterpret_cast<void*>(stream)), "mote_quantize_rows");
+  return {q, scale};
+}
+
+Tensor int8_linear(const Tensor& x_, const Tensor& wq, const Tensor& ws, int64_t K, const OptTensor& out, const OptTensor& run,
+                   const OptTensor& g, const OptTensor& xm, int64_t stream) {
+  const char* what = "int8_linear";
+  if (x_.dim() < 1 || x_.size(-1) != K || K < 1) bad_value(what, ": x must be [..., ", K, "], got ", x_.sizes());
+  const int64_t Kp = (K + 127) / 128 * 128;
+  if (wq.dim() != 2 || wq.size(0) < 1 || wq.size(1) != Kp || !wq.is_contiguous() || ws.numel() != wq.size(0) || !ws.is_contiguous())
+    bad_value(what, ": the weight must be contiguous codes [N, ", Kp, "] with N scales");
+  if (wq.scalar_type() != at::kChar || ws.scalar_type() != at::kFloat || wq.device() != x_.device() || ws.device() != x_.device())
+    throw py::type_error("int8_linear: the weight must be int8 codes and fp32 scales on x's device");
+  const int64_t N = wq.size(0), M = x_.numel() / K;
+  mote_int8_linear_args a{};
+  a.dtype = code(x_);
+  check_run(run, x_, what);
+  std::vector<int64_t> sizes = x_.sizes().vec();
+  sizes.back() = N;
+  if (out && (out->sizes() != at::IntArrayRef(sizes) || out->scalar_type() != x_.scalar_type() || out->device() != x_.device() ||
+              out->stride(-1) != 1))
+    bad_value(what, ": out must be ", at::IntArrayRef(sizes), " in x's dtype with unit element stride");
+  if (xm && (!g || g->scalar_type() != at::kFloat || xm->scalar_type() != at::kFloat || !g->is_contiguous() || !xm->is_contiguous() ||
+             g->dim() != 2 || g->size(0) != M || xm->numel() != M || g->device() != x_.device() || xm->device() != x_.device()))
+    bad_value(what, ": xm needs fp32 contiguous g [M, H] and xm [M] on x's device");
+  no_grad(what, {&x_});
+  on_gpu(x_, what);
+  TORCH_CHECK(M <= INT_MAX && N <= INT_MAX && K <= INT_MAX, "int8_linear: sizes beyond 32 bits");
+  const Tensor x = unit(x_.dim() == 2 ? x_ : x_.reshape({M, K}));
+  Tensor y = out ? *out : empty(sizes, x_, x_.scalar_type());
+  const Tensor y2 = y.dim() == 2 ? y : y.view({M, N});  // an output that is no [M, N] in memory is refused
+  if (M > 1 && y2.stride(0) < N) bad_value(what, ": the rows of out overlap");
+  a.M = int(M); a.N = int(N); a.K = int(K);
+  a.x = x.data_ptr(); a.x_sr = x.stride(0);
+  a.wq = static_cast<const int8_t*>(wq.data_ptr()); a.w_scale = fptr(ws);
+  a.y = y2.data_ptr(); a.y_sr = y2.stride(0);
+  a.run = run ? static_cast<const unsigned char*>(run->data_ptr()) : nullptr;
+  if (xm) {
+    a.g = fptr(*g); a.xm = fptr(*xm); a.heads = int(g->size(1));
+  }
+  Tensor wk;
+  if (const size_t n = mote_int8_linear_workspace(&a)) {
+    wk = bytes(n, x);
+    a.workspace = wk.data_ptr();
+    a.workspace_bytes = n;
+  }
+  check(mote_int8_linear(&a, reinterpret_cast<void*>(stream)), "mote_int8_linear");
+  return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_launch, m) {
@@ -405,4 +668,9 @@ PYBIND11_MODULE(_torch_launch, m) {
   m.def("chunk_route", &chunk_route, nogil());
   m.def("dechunk", &dechunk, nogil());
   m.def("dechunk_bwd", &dechunk_bwd, nogil());
+  m.def("cache4_write", &cache4_write, nogil());
+  m.def("cache4_read", &cache4_read, nogil());
+  m.def("relation_decode4", &relation_decode4, nogil());
+  m.def("quantize_rows", &quantize_rows, nogil());
+  m.def("int8_linear", &int8_linear, nogil());
 }
