@@ -227,12 +227,16 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
 }
 
 // ------------------------------------------------------------------------------------------------
-// Many tokens: a tile of 128 tokens x 128 channels per workgroup (4 waves, 64 x 64 each), stages of 128 k
-// brought to LDS with global_load_lds, 16-byte chunks swizzled by the row's low bits.
+// Many tokens: a tile of 16 FA WN channels x 16 FB WM tokens per workgroup of WN x WM waves.
+//
+// k goes in steps of 64 through a ring of four LDS stages filled by global_load_lds (rows of 64 bytes, the
+// four 16-byte chunks of row r swizzled by (r / 2) % 4, so the eight rows that a quarter of a wave reads at
+// once cover every bank). While a wave multiplies step kb from registers it reads the fragments of step
+// kb + 1 into a second set and the steps kb + 2 to kb + 4 are in flight, so neither LDS nor memory latency
+// stands in front of a product: one barrier a step.
+// What bounds it is the LDS: per step a wave reads FA + FB KB for FA FB products of 16 cycles, and the ring
+// takes (FA WN + FB WM) KB; a 256 x 256 tile (FA, FB = 8, 4 on 2 x 4 waves) asks for 128 bytes a cycle.
 // ------------------------------------------------------------------------------------------------
-constexpr int kTile8 = 128;
-constexpr int kStage8 = 2 * kTile8 * 128;  // bytes
-
 struct Many8Params {
   const int8_t* x;   // [M, Kp]
   const float* sx;
@@ -240,73 +244,151 @@ struct Many8Params {
   const float* sw;
   void* y; int64_t y_sr;
   int M, N, Kp, ntok, nch;
+  int wide;          // y's rows start on 16-byte boundaries
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) int8_many_kernel(const Many8Params p) {
+template <int FA, int FB, int WN, int WM>
+struct Tile8 {
+  static constexpr int CH = 16 * FA * WN, TOK = 16 * FB * WM, NW = WN * WM;
+  static constexpr int ROWS = CH + TOK;             // rows of a stage: channels, then tokens
+  static constexpr int STAGE = 64 * ROWS;           // bytes
+  static constexpr int PER = ROWS / 16 / NW;        // transfers of a wave per stage (16 rows each)
+  static constexpr int RING = 4;
+  static constexpr int OUTW = 16 * FA + 8;          // a row of a wave's output tile in LDS (padded, in elements)
+  static_assert(ROWS % (16 * NW) == 0, "every wave issues as many transfers");
+};
+
+template <typename T, int FA, int FB, int WN, int WM>
+__global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2)))
+int8_many_kernel(const Many8Params p) {
   using E = Elem<T>;
-  __shared__ __align__(16) int8_t smem[2 * kStage8];
+  using S = Tile8<FA, FB, WN, WM>;
+  constexpr int kOut = S::NW * 16 * S::OUTW * int(sizeof(T));  // 16 tokens of every wave's tile at a time
+  __shared__ __align__(16) int8_t smem[S::RING * S::STAGE > kOut ? S::RING * S::STAGE : kOut];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // workgroups go round-robin over the 8 XCDs: XCD j takes the j-th run of (token tile, channel tile)
   const int nwg = p.ntok * p.nch, per = (nwg + 7) / 8;
   const int seq = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (seq >= nwg) return;
-  const int m0 = seq / p.nch * kTile8, n0 = seq % p.nch * kTile8;
-  // a stage is 256 rows (128 of W, 128 of x) of 8 chunks: 32 wave transfers of 8 rows, 8 per wave
-  const int lrow = lane >> 3, lch = (lane & 7) ^ lrow;  // rows 8 g + lrow: the swizzle is row & 7 = lrow
-  const int8_t* src[8];
+  const int m0 = seq / p.nch * S::TOK, n0 = seq % p.nch * S::CH;
+
+  const int8_t* wb = p.w + int64_t(n0) * p.Kp;
+  const int8_t* xb = p.x + int64_t(m0) * p.Kp;
+  uint32_t voff[S::PER];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int row = (wave * 8 + i) * 8 + lrow;
-    src[i] = (row < kTile8 ? p.w + int64_t(min(n0 + row, p.N - 1)) * p.Kp
-                           : p.x + int64_t(min(m0 + row - kTile8, p.M - 1)) * p.Kp) + 16 * lch;
+  for (int i = 0; i < S::PER; ++i) {
+    const int row = (wave * S::PER + i) * 16 + (lane >> 2);
+    const int r = row < S::CH ? min(row, p.N - 1 - n0) : min(row - S::CH, p.M - 1 - m0);
+    voff[i] = uint32_t(r) * uint32_t(p.Kp) + 16u * ((lane & 3) ^ ((row >> 1) & 3));
   }
-  auto issue = [&](int kb, int slot) {
+  const uint32_t ring = lds_addr(smem);
+  auto issue = [&](int kb) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) lds_dma16(src[i] + 128 * kb, smem + slot * kStage8 + (wave * 8 + i) * 1024);
+    for (int i = 0; i < S::PER; ++i) {
+      const int g = wave * S::PER + i;
+      lds_dma16_sa((g < S::CH / 16 ? wb : xb) + 64 * kb, voff[i],
+                   ring + uint32_t((kb & (S::RING - 1)) * S::STAGE + g * 1024));
+    }
   };
-  const int wn = wave & 1, wm = wave >> 1;
-  i32x4 acc[4][4];
+
+  const int wn = wave % WN, wm = wave / WN;
+  const int r = lane & 15, q = lane >> 4;
+  const int foff = r * 64 + 16 * (q ^ ((r >> 1) & 3));
+  const int8_t* fa = smem + wn * FA * 1024 + foff;
+  const int8_t* fb = smem + (S::CH / 16 + wm * FB) * 1024 + foff;
+  struct Frags {
+    Chunk a[FA], b[FB];
+  };
+  auto read = [&](Frags& f, int kb) __attribute__((always_inline)) {
+    const int st = (kb & (S::RING - 1)) * S::STAGE;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < FB; ++i) f.b[i] = load_chunk(fb + st + i * 1024);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-  const int nk = p.Kp / 128;
-  issue(0, 0);
-  for (int kb = 0; kb < nk; ++kb) {
-    __builtin_amdgcn_s_waitcnt(0);
-    lds_barrier();  // stage kb is in LDS, and every wave is done with the slot the next one goes to
-    if (kb + 1 < nk) issue(kb + 1, (kb + 1) & 1);
-    const int8_t* st = smem + (kb & 1) * kStage8;
+    for (int i = 0; i < FA; ++i) f.a[i] = load_chunk(fa + st + i * 1024);
+  };
+  i32x4 acc[FA][FB];
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const int ch = 4 * kk + (lane >> 4), r = lane & 15;
-      Chunk a[4], b[4];
+  for (int i = 0; i < FA; ++i)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        a[i] = load_chunk(st + (wn * 64 + 16 * i + r) * 128 + ((ch ^ (r & 7)) * 16));
-        b[i] = load_chunk(st + (kTile8 + wm * 64 + 16 * i + r) * 128 + ((ch ^ (r & 7)) * 16));
-      }
+    for (int j = 0; j < FB; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+  auto multiply = [&](const Frags& f) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < FA; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = mma8(a[i], b[j], acc[i][j]);
-    }
+      for (int j = 0; j < FB; ++j) acc[i][j] = mma8(f.a[i], f.b[j], acc[i][j]);
+  };
+
+  const int nk = p.Kp / 64;  // even, at least 2
+  Frags f0, f1;
+#pragma unroll
+  for (int s = 0; s < S::RING; ++s)
+    if (s < nk) issue(s);
+  if (nk >= S::RING) __builtin_amdgcn_s_waitcnt(kVmWaitStage<(S::RING - 1) * S::PER>());
+  else __builtin_amdgcn_s_waitcnt(kVmWaitStage<0>());
+  lds_barrier();
+  read(f0, 0);
+  // Step kb: this wave's part of stage kb + 1 has arrived once at most two younger stages are outstanding
+  // (near the end, where nothing younger is issued, once none is). Behind the barrier every wave's part has,
+  // and every wave holds step kb in registers, so stage kb's slot takes stage kb + 4.
+  auto step = [&](const Frags& cur, Frags& next, int kb) __attribute__((always_inline)) {
+    if (kb + S::RING <= nk) __builtin_amdgcn_s_waitcnt(kVmWaitStage<2 * S::PER>());
+    else __builtin_amdgcn_s_waitcnt(kVmWaitStage<0>());
+    lds_barrier();
+    if (kb + S::RING < nk) issue(kb + S::RING);
+    if (kb + 1 < nk) read(next, kb + 1);
+    multiply(cur);
+  };
+  for (int kb = 0; kb < nk; kb += 2) {
+    step(f0, f1, kb);
+    step(f1, f0, kb + 1);
   }
-  // acc[i][j]: channels n0 + 64 wn + 16 i + 4 (lane / 16) + e of token m0 + 64 wm + 16 j + lane % 16
+
+  // acc[i][j]: channels n0 + 16 (wn FA + i) + 4 q + e of token m0 + 16 (wm FB + j) + r. Sixteen tokens at a
+  // time go through LDS (each wave its own part), so that a store instruction writes whole rows.
+  lds_barrier();  // the ring is no longer read
+  T* tile = reinterpret_cast<T*>(smem) + wave * 16 * S::OUTW;
+  const int nw0 = n0 + wn * 16 * FA;
+  float sw[FA][4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int m = m0 + 64 * wm + 16 * j + (lane & 15);
-    if (m >= p.M) continue;
-    const float sx = p.sx[m];
-    T* yr = reinterpret_cast<T*>(p.y) + int64_t(m) * p.y_sr;
+  for (int i = 0; i < FA; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = n0 + 64 * wn + 16 * i + 4 * (lane >> 4);
+    for (int e = 0; e < 4; ++e) sw[i][e] = p.sw[min(nw0 + 16 * i + 4 * q + e, p.N - 1)];
+  constexpr int EPC = 16 / int(sizeof(T));      // elements of a 16-byte store
+  constexpr int CPR = 16 * FA / EPC;            // stores of a row
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.N) yr[n + e] = E::from_f(float(acc[i][j][e]) * sx * p.sw[n + e]);
+  for (int j = 0; j < FB; ++j) {
+    const int mt = m0 + 16 * (wm * FB + j);
+    const float sx = p.sx[min(mt + r, p.M - 1)];
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+      float v[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = float(acc[i][j][e]) * sx * sw[i][e];
+      T* d = tile + r * S::OUTW + 16 * i + 4 * q;
+      if constexpr (sizeof(T) == 2) {
+        *reinterpret_cast<uint2*>(d) = make_uint2(uint32_t(f2bf(v[0])) | uint32_t(f2bf(v[1])) << 16,
+                                                  uint32_t(f2bf(v[2])) | uint32_t(f2bf(v[3])) << 16);
+      } else {
+        *reinterpret_cast<float4*>(d) = make_float4(v[0], v[1], v[2], v[3]);
+      }
     }
+    // the wave's own writes, read back by the wave: LDS operations of a wave complete in order
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int c = lane; c < 16 * CPR; c += 64) {
+      const int row = c / CPR, col = c % CPR * EPC;
+      const int m = mt + row, n = nw0 + col;
+      if (m >= p.M || n >= p.N) continue;
+      T* yr = reinterpret_cast<T*>(p.y) + int64_t(m) * p.y_sr + n;
+      const T* src = tile + row * S::OUTW + col;
+      if (p.wide && n + EPC <= p.N) {
+        store_chunk(yr, load_chunk(src));
+      } else {
+        for (int e = 0; e < EPC && n + e < p.N; ++e) yr[e] = src[e];
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
@@ -333,6 +415,7 @@ int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream) {
   return check_launch(what);
 }
 
+constexpr int64_t kBigTiles8 = 128;
 static bool few8(const mote_int8_linear_args* a) { return a->M <= 16 && a->K <= kFewMaxK; }
 
 size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a) {
@@ -363,9 +446,15 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
   Many8Params p;
   p.x = xq; p.sx = sx; p.w = a->wq; p.sw = a->w_scale; p.y = a->y; p.y_sr = a->y_sr;
   p.M = a->M; p.N = a->N; p.Kp = Kp;
-  p.ntok = (a->M + kTile8 - 1) / kTile8; p.nch = (a->N + kTile8 - 1) / kTile8;
-  const unsigned per = unsigned((int64_t(p.ntok) * p.nch + 7) / 8);
-  hipLaunchKernelGGL(int8_many_kernel<T>, dim3(8 * per), dim3(256), 0, stream, p);
+  p.wide = reinterpret_cast<uintptr_t>(a->y) % 16 == 0 && (a->y_sr * int64_t(sizeof(T))) % 16 == 0;
+  const int64_t big = (int64_t(a->M) + 255) / 256 * ((a->N + 255) / 256);
+  auto go = [&](auto kernel, int ch, int tok, int waves) {
+    p.ntok = (a->M + tok - 1) / tok; p.nch = (a->N + ch - 1) / ch;
+    const unsigned per = unsigned((int64_t(p.ntok) * p.nch + 7) / 8);
+    hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * waves), 0, stream, p);
+  };
+  if (big >= kBigTiles8) go(int8_many_kernel<T, 8, 4, 2, 4>, 256, 256, 8);
+  else go(int8_many_kernel<T, 4, 4, 2, 2>, 128, 128, 4);
 }
 
 int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream) {
@@ -374,7 +463,7 @@ int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream) {
   if (a->dtype != MOTE_F32 && a->dtype != MOTE_BF16) return set_error(MOTE_ERR_ARGUMENT, "%s: bad dtype %d", what, a->dtype);
   if (a->M < 0 || a->N <= 0 || a->K <= 0 || a->K > kMaxK8)
     return set_error(MOTE_ERR_SHAPE, "%s: M = %d, N = %d, K = %d (K at most %d)", what, a->M, a->N, a->K, kMaxK8);
-  if (int64_t((a->M + kTile8 - 1) / kTile8) * ((a->N + kTile8 - 1) / kTile8) >= (int64_t(1) << 30))
+  if (((int64_t(a->M) + 127) / 128) * ((int64_t(a->N) + 127) / 128) >= (int64_t(1) << 30))
     return set_error(MOTE_ERR_SHAPE, "%s: too many tiles for one launch", what);
   if (a->M == 0) return MOTE_OK;
   if (!a->x || !a->wq || !a->w_scale || !a->y) return set_error(MOTE_ERR_ARGUMENT, "%s: null pointer", what);
