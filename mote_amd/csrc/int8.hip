@@ -4,6 +4,7 @@
 // acc = sum_k xq wq runs on v_mfma_i32_16x16x64_i8, exact in 32 bits; y = (acc sx) sw in fp32, rounded once.
 // One fragment convention for both operands: lane l holds 16 consecutive k of row l % 16, k group l / 16.
 // Rows of xq and wq are Kp = K rounded up to 128 bytes, xq's zero past K, so no product looks at K.
+#include <stdlib.h>
 #include "tiles.hpp"
 #include "params.hpp"
 
@@ -247,22 +248,32 @@ struct Many8Params {
   int wide;          // y's rows start on 16-byte boundaries
 };
 
-template <int FA, int FB, int WN, int WM>
+template <int FA, int FB, int WN, int WM, int RING_>
 struct Tile8 {
   static constexpr int CH = 16 * FA * WN, TOK = 16 * FB * WM, NW = WN * WM;
   static constexpr int ROWS = CH + TOK;             // rows of a stage: channels, then tokens
   static constexpr int STAGE = 64 * ROWS;           // bytes
   static constexpr int PER = ROWS / 16 / NW;        // transfers of a wave per stage (16 rows each)
-  static constexpr int RING = 4;
+  static constexpr int RING = RING_;                // stages, a power of two of at least 4
   static constexpr int OUTW = 16 * FA + 8;          // a row of a wave's output tile in LDS (padded, in elements)
   static_assert(ROWS % (16 * NW) == 0, "every wave issues as many transfers");
 };
 
-template <typename T, int FA, int FB, int WN, int WM>
+// the wave's LDS reads are done, at most N of its transfers are outstanding, and every wave is here (the
+// waits as builtins: the compiler then knows that the fragments have arrived)
+template <int N>
+__device__ __forceinline__ void arrive() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(kVmWaitStage<N>() & ~(0xF << 8));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+template <typename T, int FA, int FB, int WN, int WM, int RING>
 __global__ void __launch_bounds__(64 * WN * WM) __attribute__((amdgpu_waves_per_eu(2)))
 int8_many_kernel(const Many8Params p) {
   using E = Elem<T>;
-  using S = Tile8<FA, FB, WN, WM>;
+  using S = Tile8<FA, FB, WN, WM, RING>;
   constexpr int kOut = S::NW * 16 * S::OUTW * int(sizeof(T));  // 16 tokens of every wave's tile at a time
   __shared__ __align__(16) int8_t smem[S::RING * S::STAGE > kOut ? S::RING * S::STAGE : kOut];
   const int lane = threadIdx.x & 63;
@@ -283,12 +294,12 @@ int8_many_kernel(const Many8Params p) {
     voff[i] = uint32_t(r) * uint32_t(p.Kp) + 16u * ((lane & 3) ^ ((row >> 1) & 3));
   }
   const uint32_t ring = lds_addr(smem);
-  auto issue = [&](int kb) __attribute__((always_inline)) {
+  auto issue = [&](int kb, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < S::PER; ++i) {
       const int g = wave * S::PER + i;
       lds_dma16_sa((g < S::CH / 16 ? wb : xb) + 64 * kb, voff[i],
-                   ring + uint32_t((kb & (S::RING - 1)) * S::STAGE + g * 1024));
+                   ring + uint32_t(slot * S::STAGE + g * 1024));
     }
   };
 
@@ -300,8 +311,8 @@ int8_many_kernel(const Many8Params p) {
   struct Frags {
     Chunk a[FA], b[FB];
   };
-  auto read = [&](Frags& f, int kb) __attribute__((always_inline)) {
-    const int st = (kb & (S::RING - 1)) * S::STAGE;
+  auto read = [&](Frags& f, int slot) __attribute__((always_inline)) {
+    const int st = slot * S::STAGE;
 #pragma unroll
     for (int i = 0; i < FB; ++i) f.b[i] = load_chunk(fb + st + i * 1024);
 #pragma unroll
@@ -323,26 +334,37 @@ int8_many_kernel(const Many8Params p) {
   Frags f0, f1;
 #pragma unroll
   for (int s = 0; s < S::RING; ++s)
-    if (s < nk) issue(s);
-  if (nk >= S::RING) __builtin_amdgcn_s_waitcnt(kVmWaitStage<(S::RING - 1) * S::PER>());
-  else __builtin_amdgcn_s_waitcnt(kVmWaitStage<0>());
-  lds_barrier();
+    if (s < nk) issue(s, s);
+  if (nk >= S::RING) arrive<(S::RING - 1) * S::PER>();
+  else arrive<0>();
   read(f0, 0);
-  // Step kb: this wave's part of stage kb + 1 has arrived once at most two younger stages are outstanding
-  // (near the end, where nothing younger is issued, once none is). Behind the barrier every wave's part has,
-  // and every wave holds step kb in registers, so stage kb's slot takes stage kb + 4.
-  auto step = [&](const Frags& cur, Frags& next, int kb) __attribute__((always_inline)) {
-    if (kb + S::RING <= nk) __builtin_amdgcn_s_waitcnt(kVmWaitStage<2 * S::PER>());
-    else __builtin_amdgcn_s_waitcnt(kVmWaitStage<0>());
-    lds_barrier();
-    if (kb + S::RING < nk) issue(kb + S::RING);
-    if (kb + 1 < nk) read(next, kb + 1);
+  // Step kb: this wave's part of stage kb + 1 has arrived once at most YOUNGER transfers are outstanding.
+  // Behind the barrier every wave's part has, and every wave holds step kb in registers, so stage kb's slot
+  // takes stage kb + RING. No step is conditional: at a join the compiler would wait for the reads of the
+  // next fragments before the products of the current ones (the last step reads a slot for nothing).
+  int slot = 0;  // of stage kb
+  auto step = [&](const Frags& cur, Frags& next, int kb, auto younger, auto more) __attribute__((always_inline)) {
+    arrive<decltype(younger)::value>();
+    if constexpr (decltype(more)::value) issue(kb + S::RING, slot);
+    slot = (slot + 1) & (S::RING - 1);
+    read(next, slot);
+    __builtin_amdgcn_sched_barrier(0);  // the reads ahead of the products, the products ahead of the barrier
     multiply(cur);
+    __builtin_amdgcn_sched_barrier(0);
   };
-  for (int kb = 0; kb < nk; kb += 2) {
-    step(f0, f1, kb);
-    step(f1, f0, kb + 1);
+  using More = std::true_type;
+  using Last = std::false_type;
+  int kb = 0;
+  for (; kb + S::RING < nk; kb += 2) {
+    step(f0, f1, kb, std::integral_constant<int, 2 * S::PER>{}, More{});
+    step(f1, f0, kb + 1, std::integral_constant<int, 2 * S::PER>{}, More{});
   }
+  if (nk >= S::RING) {
+    step(f0, f1, kb, std::integral_constant<int, 2 * S::PER>{}, Last{});
+    step(f1, f0, kb + 1, std::integral_constant<int, S::PER>{}, Last{});
+  }
+  step(f0, f1, nk - 2, std::integral_constant<int, 0>{}, Last{});
+  step(f1, f0, nk - 1, std::integral_constant<int, 0>{}, Last{});
 
   // acc[i][j]: channels n0 + 16 (wn FA + i) + 4 q + e of token m0 + 16 (wm FB + j) + r. Sixteen tokens at a
   // time go through LDS (each wave its own part), so that a store instruction writes whole rows.
@@ -453,8 +475,13 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
     const unsigned per = unsigned((int64_t(p.ntok) * p.nch + 7) / 8);
     hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * waves), 0, stream, p);
   };
-  if (big >= kBigTiles8) go(int8_many_kernel<T, 8, 4, 2, 4>, 256, 256, 8);
-  else go(int8_many_kernel<T, 4, 4, 2, 2>, 128, 128, 4);
+  static const int var = getenv("V8") ? atoi(getenv("V8")) : 0;
+  if (var == 5) go(int8_many_kernel<T, 4, 4, 2, 2, 4>, 128, 128, 4);
+  else if (var == 7) go(int8_many_kernel<T, 2, 2, 2, 2, 4>, 64, 64, 4);
+  else if (var == 8) go(int8_many_kernel<T, 4, 8, 4, 2, 4>, 256, 256, 8);
+  else if (var == 9) go(int8_many_kernel<T, 8, 4, 1, 4, 4>, 128, 256, 4);
+  else if (big >= kBigTiles8) go(int8_many_kernel<T, 8, 4, 2, 4, 4>, 256, 256, 8);
+  else go(int8_many_kernel<T, 4, 4, 2, 2, 4>, 128, 128, 4);
 }
 
 int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream) {

@@ -117,11 +117,27 @@ __device__ __forceinline__ void add4(float (&z)[32], const Chunk& c, float w) {
   }
 }
 
+// the sum of a row's LPR neighbouring lanes, in each of them (c: the lane's place among them); three lanes
+// lie across the rows of 16 that DPP works in, so they take its whole-wave shifts
+template <int LPR>
+__device__ __forceinline__ float row_sum(float x, int c) {
+  if constexpr (LPR == 2 || LPR == 4) x += dpp<kDppXor1>(x);
+  if constexpr (LPR == 4) x += dpp<kDppXor2>(x);
+  if constexpr (LPR == 3) {
+    constexpr int kNext = 0x130, kPrev = 0x138;  // wave_shl:1 reads lane + 1, wave_shr:1 lane - 1
+    const float x1 = dpp<kNext>(x), x2 = dpp<kNext>(x1);
+    const float s = (x + x1) + x2;  // the row's, in its first lane
+    const float s1 = dpp<kPrev>(s), s2 = dpp<kPrev>(s1);
+    x = c == 0 ? s : c == 1 ? s1 : s2;
+  }
+  return x;
+}
+
 template <typename T, int G>
 __global__ void __launch_bounds__(kD4Threads) relation_decode4_kernel(const Dec4Params p) {
   using E = Elem<T>;
-  constexpr int LPR = G <= 2 ? G : 4;             // lanes of a row
-  constexpr int RPW = 64 / LPR;                   // rows of a wave's step
+  constexpr int LPR = G;                          // lanes of a row, one per group
+  constexpr int RPW = 64 / LPR;                   // rows of a wave's step (three groups: lane 63 has none)
   constexpr int ROWS = RPW * kD4Waves;            // rows of a step
   constexpr int DP = 32 * G, ZS = DP + 4;         // a row group's z in LDS (16-byte aligned)
   constexpr int CL = 32 * LPR, PARTS = kD4Threads / CL;  // column sums: PARTS threads a column
@@ -141,13 +157,14 @@ __global__ void __launch_bounds__(kD4Threads) relation_decode4_kernel(const Dec4
   const int b = bh / p.H, h = bh % p.H;
   const int D = p.D, half = D / 2;
   const int nsp = p.nsplit;
-  const int rr = lane / LPR, c = lane % LPR;
-  const int cg = min(c, G - 1);          // this lane's group (three groups: the fourth lane repeats the last)
-  const int roff = wave * RPW + rr;      // this lane's row within a step
-  const uint8_t* kbase = p.kc + b * p.c_sb + h * p.c_sh + 16 * cg;
-  const uint8_t* vbase = p.vc + b * p.c_sb + h * p.c_sh + 16 * cg;
-  const bf16_t* ksb = p.ks + b * p.s_sb + h * p.s_sh + cg;
-  const bf16_t* vsb = p.vs + b * p.s_sb + h * p.s_sh + cg;
+  const int c = lane % LPR;                   // this lane's group
+  const bool act = lane < RPW * LPR;
+  const int rr = min(lane / LPR, RPW - 1);
+  const int roff = wave * RPW + rr;           // its row within a step
+  const uint8_t* kbase = p.kc + b * p.c_sb + h * p.c_sh + 16 * c;
+  const uint8_t* vbase = p.vc + b * p.c_sb + h * p.c_sh + 16 * c;
+  const bf16_t* ksb = p.ks + b * p.s_sb + h * p.s_sh + c;
+  const bf16_t* vsb = p.vs + b * p.s_sb + h * p.s_sh + c;
 
   // the small loads first: they complete in order, ahead of the cache rows issued after them
   int vzero;
@@ -236,7 +253,7 @@ __global__ void __launch_bounds__(kD4Threads) relation_decode4_kernel(const Dec4
   {
     float qf[32];
 #pragma unroll
-    for (int j = 0; j < 32; ++j) qf[j] = c < G ? sq[32 * cg + j] : 0.f;
+    for (int j = 0; j < 32; ++j) qf[j] = sq[32 * c + j];
     q.set(qf);
   }
   float m = kNegInf, l = 0.f;
@@ -248,12 +265,9 @@ __global__ void __launch_bounds__(kD4Threads) relation_decode4_kernel(const Dec4
   auto consume = [&](int jstep, auto u) {
     constexpr int U = decltype(u)::value;
     if (jstep >= ns) return;
-    const float sk = c < G ? bf2f(ksr[U]) : 0.f;
-    float dot = q.dot(kr[U]) * sk;
-    if constexpr (LPR >= 2) dot += dpp<kDppXor1>(dot);
-    if constexpr (LPR == 4) dot += dpp<kDppXor2>(dot);
+    const float dot = row_sum<LPR>(q.dot(kr[U]) * bf2f(ksr[U]), c);
     const int row = (split + jstep * nsp) * ROWS + roff;
-    if (row < S) {
+    if (act && row < S) {
       const float u2 = dot * c2;
       const float ev = u2 * frcp(1.0f + fexp2(-u2));
       if (ev > m + kRescale) {
@@ -280,25 +294,17 @@ __global__ void __launch_bounds__(kD4Threads) relation_decode4_kernel(const Dec4
   }
 
   // ---- merge of the workgroup's row groups (the lanes of a row hold the same m and l) ----
-  float mw = m;
-  if constexpr (LPR == 1) mw = fmaxf(mw, dpp<kDppXor1>(mw));
-  if constexpr (LPR <= 2) mw = fmaxf(mw, dpp<kDppXor2>(mw));
-  mw = fmaxf(mw, dpp<kDppNext4>(mw));
-  mw = lanegroup_max(fmaxf(mw, dpp<kDppRor8>(mw)));  // in lane 0
+  const float mw = wave_max(m);
   if (lane == 0) sm[wave] = mw;
   __syncthreads();
   float M = sm[0];
 #pragma unroll
   for (int w = 1; w < kD4Waves; ++w) M = fmaxf(M, sm[w]);
   const float a = fexp2(m - (M == kNegInf ? 0.f : M));  // 0 for a row group without rows
-  float lw = l * a;
-  if constexpr (LPR == 1) lw += dpp<kDppXor1>(lw);
-  if constexpr (LPR <= 2) lw += dpp<kDppXor2>(lw);
-  lw += dpp<kDppNext4>(lw);
-  lw = lanegroup_sum(lw + dpp<kDppRor8>(lw));
+  const float lw = wave_sum_lane0(act && c == 0 ? l * a : 0.f);
   if (lane == 0) sl[wave] = lw;
-  float* zg = zred + roff * ZS + 32 * cg;
-  if (c < G) {
+  float* zg = zred + roff * ZS + 32 * c;
+  if (act) {
 #pragma unroll
     for (int j = 0; j < 32; j += 4)
       *reinterpret_cast<float4*>(zg + j) = make_float4(z[j] * a, z[j + 1] * a, z[j + 2] * a, z[j + 3] * a);
@@ -306,7 +312,7 @@ __global__ void __launch_bounds__(kD4Threads) relation_decode4_kernel(const Dec4
   __syncthreads();
   {
     const int d = tid % CL, part = tid / CL;
-    if (d < DP) {
+    if (part < PARTS) {
       constexpr int N = ROWS / PARTS;
       const float* col = zred + part * N * ZS + d;
       float s0 = 0.f, s1 = 0.f;
@@ -319,44 +325,51 @@ __global__ void __launch_bounds__(kD4Threads) relation_decode4_kernel(const Dec4
     }
   }
   __syncthreads();
-  {
-    float* part = p.part + (int64_t(bh) * nsp + split) * (D + 2);
-    if (tid < D) {
-      float s = csum[0][tid];
+  float zs = 0.f, L4 = 0.f;
+  if (tid < D) {
 #pragma unroll
-      for (int k = 1; k < PARTS; ++k) s += csum[k][tid];
-      put_coherent(part + 2 + tid, s);
-    }
+    for (int k = 0; k < PARTS; ++k) zs += csum[k][tid];
+  }
+#pragma unroll
+  for (int w = 0; w < kD4Waves; ++w) L4 += sl[w];
+  if (nsp == 1) {
+    // one split: its sums are the head's, and no other workgroup counts (start of a conversation at
+    // batch 1, head dim 48: 6.7 us a step with the publication, see the figures above)
+    if (tid < D) zred[2 + tid] = zs;
     if (tid == 0) {
-      float L = 0.f;
-#pragma unroll
-      for (int w = 0; w < kD4Waves; ++w) L += sl[w];
-      put_coherent(part, M);
-      put_coherent(part + 1, L);
+      zred[0] = M;
+      zred[1] = L4;
     }
-  }
-  // publish, then count: agent-scope stores are acknowledged at the device-coherent level before the
-  // barrier, the count's add is issued after it, and the workgroup that sees the last count reads the
-  // partials with agent-scope loads
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (tid == 0) {
-    const int before = __hip_atomic_fetch_add(p.cnt + bh * kD4CntStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s_last = before == nsp - 1;
-  }
-  __syncthreads();
-  if (!s_last) return;
+  } else {
+    float* part = p.part + (int64_t(bh) * nsp + split) * (D + 2);
+    if (tid < D) put_coherent(part + 2 + tid, zs);
+    if (tid == 0) {
+      put_coherent(part, M);
+      put_coherent(part + 1, L4);
+    }
+    // publish, then count: agent-scope stores are acknowledged at the device-coherent level before the
+    // barrier, the count's add is issued after it, and the workgroup that sees the last count reads the
+    // partials with agent-scope loads
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+      const int before = __hip_atomic_fetch_add(p.cnt + bh * kD4CntStride, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_last = before == nsp - 1;
+    }
+    __syncthreads();
+    if (!s_last) return;
 
-  // ---- the last workgroup of the head ----
-  const int np = nsp * (D + 2);
-  const float* pb = p.part + int64_t(bh) * np;
-  constexpr int KP = (kD4MaxSplits * (DP + 2) + kD4Threads - 1) / kD4Threads;
-  float pv[KP];
+    // ---- the last workgroup of the head ----
+    const int np = nsp * (D + 2);
+    const float* pb = p.part + int64_t(bh) * np;
+    constexpr int KP = (kD4MaxSplits * (DP + 2) + kD4Threads - 1) / kD4Threads;
+    float pv[KP];
 #pragma unroll
-  for (int k = 0; k < KP; ++k) pv[k] = get_coherent(pb + min(tid + k * kD4Threads, np - 1));
+    for (int k = 0; k < KP; ++k) pv[k] = get_coherent(pb + min(tid + k * kD4Threads, np - 1));
 #pragma unroll
-  for (int k = 0; k < KP; ++k)
-    if (tid + k * kD4Threads < np) zred[tid + k * kD4Threads] = pv[k];
+    for (int k = 0; k < KP; ++k)
+      if (tid + k * kD4Threads < np) zred[tid + k * kD4Threads] = pv[k];
+  }
   __syncthreads();
   const int stride = D + 2;
   if (wave == 0) {
@@ -407,7 +420,7 @@ __global__ void __launch_bounds__(kD4Threads) relation_decode4_kernel(const Dec4
     y[d] = E::from_f(bad ? __builtin_nanf("") : yv);
   }
   if (tid == 0) {
-    __hip_atomic_store(p.cnt + bh * kD4CntStride, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (nsp > 1) __hip_atomic_store(p.cnt + bh * kD4CntStride, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     p.g[bh] = bad ? __builtin_nanf("") : gate;
     if ((p.flags & MOTE_DECODE_ADVANCE) || p.xm) {
       // the last head of the sequence: every workgroup of it has read S[b] by now
@@ -430,7 +443,7 @@ __global__ void __launch_bounds__(kD4Threads) relation_decode4_kernel(const Dec4
 }
 
 static int groups4(int D) { return (D + kGroup4 - 1) / kGroup4; }
-static int rows4(int G) { return (G <= 2 ? 64 / G : 16) * kD4Waves; }
+static int rows4(int G) { return 64 / G * kD4Waves; }
 
 static int cus4() {
   int dev = 0, cus = 0;
@@ -439,16 +452,20 @@ static int cus4() {
     return 256;
   return cus;
 }
-// Splits per head: a workgroup per CU over the whole batch, at least two steps per split at full capacity,
-// at most one split per lane of the merging wave.
+// Splits per head. One for a cache of up to four steps, which needs no merge over workgroups (batch 1, head
+// dim 48, 256 rows: 5.5 us a step, 7.0 as two splits). Else a workgroup per CU over the whole batch, each of
+// at least two steps; two per CU where each still has a dozen steps (more loads in flight: batch 16, 4700
+// rows, 17.2 -> 16.1 us; 32768 rows 106 -> 104 us; below, the merge costs more: batch 4, 10.3 and 10.9 us).
+// At most one split per lane of the merging wave.
 static int splits4(const mote_relation_decode4_args* a) {
-  const int64_t BH = int64_t(a->B) * a->H;
-  const int64_t rows = 2 * rows4(groups4(a->D));
-  int64_t n = BH > 0 ? int64_t(cus4()) / BH : 1;
-  const int64_t by_rows = (int64_t(a->capacity) + rows - 1) / rows;
-  if (n > by_rows) n = by_rows;
-  if (n > kD4MaxSplits) n = kD4MaxSplits;
-  return int(n < 1 ? 1 : n);
+  const int64_t BH = int64_t(a->B) * a->H, rows = rows4(groups4(a->D));
+  const int64_t steps = (int64_t(a->capacity) + rows - 1) / rows;
+  if (steps <= 4) return 1;
+  int64_t n = cus4() / BH;
+  if (n < 1) n = 1;
+  if (steps >= 12 * 2 * n) n *= 2;
+  if (n > (steps + 1) / 2) n = (steps + 1) / 2;
+  return int(n < kD4MaxSplits ? n : kD4MaxSplits);
 }
 
 struct Dec4Ws {
