@@ -4,7 +4,6 @@
 // acc = sum_k xq wq runs on v_mfma_i32_16x16x64_i8, exact in 32 bits; y = (acc sx) sw in fp32, rounded once.
 // One fragment convention for both operands: lane l holds 16 consecutive k of row l % 16, k group l / 16.
 // Rows of xq and wq are Kp = K rounded up to 128 bytes, xq's zero past K, so no product looks at K.
-#include <stdlib.h>
 #include "tiles.hpp"
 #include "params.hpp"
 
@@ -230,13 +229,15 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
 // ------------------------------------------------------------------------------------------------
 // Many tokens: a tile of 16 FA WN channels x 16 FB WM tokens per workgroup of WN x WM waves.
 //
-// k goes in steps of 64 through a ring of four LDS stages filled by global_load_lds (rows of 64 bytes, the
-// four 16-byte chunks of row r swizzled by (r / 2) % 4, so the eight rows that a quarter of a wave reads at
-// once cover every bank). While a wave multiplies step kb from registers it reads the fragments of step
-// kb + 1 into a second set and the steps kb + 2 to kb + 4 are in flight, so neither LDS nor memory latency
-// stands in front of a product: one barrier a step.
-// What bounds it is the LDS: per step a wave reads FA + FB KB for FA FB products of 16 cycles, and the ring
-// takes (FA WN + FB WM) KB; a 256 x 256 tile (FA, FB = 8, 4 on 2 x 4 waves) asks for 128 bytes a cycle.
+// k goes in stages of 128 (a whole cache line of every row: half lines double the L2's requests, which
+// bound 64-wide stages: 65536 x 1024 -> 4096 405 us and 384 us) through a ring of LDS stages filled by
+// global_load_lds, the eight 16-byte chunks of row r swizzled by r % 8, so the rows that a quarter of a wave
+// reads at once cover every bank. While a wave multiplies one half of a stage from registers it reads the
+// fragments of the next half into a second set, so no product waits for the LDS, and one barrier a stage
+// hands the slots over.
+// What bounds the 256 x 256 tile (8192 x 4096 -> 4096: 112 us, 2.45 POP/s): matrix cores 56 % busy at the
+// 1.9 GHz that the card runs them at; without its products it takes 90 us, without its loads and reads 90.
+// Short k (1024: 8 stages) adds the stores, which all CUs make at once: half of a tile's time.
 // ------------------------------------------------------------------------------------------------
 struct Many8Params {
   const int8_t* x;   // [M, Kp]
@@ -245,6 +246,7 @@ struct Many8Params {
   const float* sw;
   void* y; int64_t y_sr;
   int M, N, Kp, ntok, nch;
+  int gch;           // channel tiles of a group: the tiles of a group are a run, token tile by token tile
   int wide;          // y's rows start on 16-byte boundaries
 };
 
@@ -252,11 +254,11 @@ template <int FA, int FB, int WN, int WM, int RING_>
 struct Tile8 {
   static constexpr int CH = 16 * FA * WN, TOK = 16 * FB * WM, NW = WN * WM;
   static constexpr int ROWS = CH + TOK;             // rows of a stage: channels, then tokens
-  static constexpr int STAGE = 64 * ROWS;           // bytes
-  static constexpr int PER = ROWS / 16 / NW;        // transfers of a wave per stage (16 rows each)
-  static constexpr int RING = RING_;                // stages, a power of two of at least 4
+  static constexpr int STAGE = 128 * ROWS;          // bytes
+  static constexpr int PER = ROWS / 8 / NW;         // transfers of a wave per stage (8 rows each)
+  static constexpr int RING = RING_;                // stages, a power of two
   static constexpr int OUTW = 16 * FA + 8;          // a row of a wave's output tile in LDS (padded, in elements)
-  static_assert(ROWS % (16 * NW) == 0, "every wave issues as many transfers");
+  static_assert(ROWS % (8 * NW) == 0, "every wave issues as many transfers");
 };
 
 // the wave's LDS reads are done, at most N of its transfers are outstanding, and every wave is here (the
@@ -282,89 +284,87 @@ int8_many_kernel(const Many8Params p) {
   const int nwg = p.ntok * p.nch, per = (nwg + 7) / 8;
   const int seq = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (seq >= nwg) return;
-  const int m0 = seq / p.nch * S::TOK, n0 = seq % p.nch * S::CH;
+  const int g = seq / (p.ntok * p.gch), in_g = seq - g * p.ntok * p.gch;
+  const int gw = min(p.gch, p.nch - g * p.gch);  // channel tiles of this group (fewer in the last)
+  const int m0 = in_g / gw * S::TOK, n0 = (g * p.gch + in_g % gw) * S::CH;
 
   const int8_t* wb = p.w + int64_t(n0) * p.Kp;
   const int8_t* xb = p.x + int64_t(m0) * p.Kp;
   uint32_t voff[S::PER];
 #pragma unroll
   for (int i = 0; i < S::PER; ++i) {
-    const int row = (wave * S::PER + i) * 16 + (lane >> 2);
+    const int row = (wave * S::PER + i) * 8 + (lane >> 3);
     const int r = row < S::CH ? min(row, p.N - 1 - n0) : min(row - S::CH, p.M - 1 - m0);
-    voff[i] = uint32_t(r) * uint32_t(p.Kp) + 16u * ((lane & 3) ^ ((row >> 1) & 3));
+    voff[i] = uint32_t(r) * uint32_t(p.Kp) + 16u * ((lane & 7) ^ (row & 7));
   }
   const uint32_t ring = lds_addr(smem);
   auto issue = [&](int kb, int slot) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < S::PER; ++i) {
       const int g = wave * S::PER + i;
-      lds_dma16_sa((g < S::CH / 16 ? wb : xb) + 64 * kb, voff[i],
+      lds_dma16_sa((g < S::CH / 8 ? wb : xb) + 128 * kb, voff[i],
                    ring + uint32_t(slot * S::STAGE + g * 1024));
     }
   };
 
   const int wn = wave % WN, wm = wave / WN;
   const int r = lane & 15, q = lane >> 4;
-  const int foff = r * 64 + 16 * (q ^ ((r >> 1) & 3));
-  const int8_t* fa = smem + wn * FA * 1024 + foff;
-  const int8_t* fb = smem + (S::CH / 16 + wm * FB) * 1024 + foff;
+  const int foff[2] = {r * 128 + 16 * (q ^ (r & 7)), r * 128 + 16 * ((q + 4) ^ (r & 7))};
+  const int8_t* fa = smem + wn * FA * 2048;
+  const int8_t* fb = smem + (S::CH / 16 + wm * FB) * 2048;
   struct Frags {
     Chunk a[FA], b[FB];
-  };
-  auto read = [&](Frags& f, int slot) __attribute__((always_inline)) {
-    const int st = slot * S::STAGE;
-#pragma unroll
-    for (int i = 0; i < FB; ++i) f.b[i] = load_chunk(fb + st + i * 1024);
-#pragma unroll
-    for (int i = 0; i < FA; ++i) f.a[i] = load_chunk(fa + st + i * 1024);
   };
   i32x4 acc[FA][FB];
 #pragma unroll
   for (int i = 0; i < FA; ++i)
 #pragma unroll
     for (int j = 0; j < FB; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-  auto multiply = [&](const Frags& f) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < FA; ++i)
-#pragma unroll
-      for (int j = 0; j < FB; ++j) acc[i][j] = mma8(f.a[i], f.b[j], acc[i][j]);
-  };
-
-  const int nk = p.Kp / 64;  // even, at least 2
+  const int nk = p.Kp / 128;
+  constexpr int RPG = (2 * FA + FB - 1) / FA;  // reads between FB products: FA + FB in FA groups
   Frags f0, f1;
+  // the products of one half stage, the reads of the next half between them
+  auto half = [&](const Frags& cur, Frags& next, int slot, int hf) __attribute__((always_inline)) {
+    const int st = slot * S::STAGE + foff[hf];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < FA; ++i) {
+#pragma unroll
+      for (int k = RPG * i; k < RPG * i + RPG; ++k) {
+        if (k < FB) next.b[k] = load_chunk(fb + st + k * 2048);
+        else if (k < FA + FB) next.a[k - FB] = load_chunk(fa + st + (k - FB) * 2048);
+      }
+#pragma unroll
+      for (int j = 0; j < FB; ++j) acc[i][j] = mma8(cur.a[i], cur.b[j], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
 #pragma unroll
   for (int s = 0; s < S::RING; ++s)
     if (s < nk) issue(s, s);
   if (nk >= S::RING) arrive<(S::RING - 1) * S::PER>();
   else arrive<0>();
-  read(f0, 0);
-  // Step kb: this wave's part of stage kb + 1 has arrived once at most YOUNGER transfers are outstanding.
-  // Behind the barrier every wave's part has, and every wave holds step kb in registers, so stage kb's slot
-  // takes stage kb + RING. No step is conditional: at a join the compiler would wait for the reads of the
-  // next fragments before the products of the current ones (the last step reads a slot for nothing).
-  int slot = 0;  // of stage kb
-  auto step = [&](const Frags& cur, Frags& next, int kb, auto younger, auto more) __attribute__((always_inline)) {
-    arrive<decltype(younger)::value>();
-    if constexpr (decltype(more)::value) issue(kb + S::RING, slot);
-    slot = (slot + 1) & (S::RING - 1);
-    read(next, slot);
-    __builtin_amdgcn_sched_barrier(0);  // the reads ahead of the products, the products ahead of the barrier
-    multiply(cur);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  using More = std::true_type;
-  using Last = std::false_type;
+#pragma unroll
+  for (int i = 0; i < FB; ++i) f0.b[i] = load_chunk(fb + foff[0] + i * 2048);
+#pragma unroll
+  for (int i = 0; i < FA; ++i) f0.a[i] = load_chunk(fa + foff[0] + i * 2048);
+  // Stage kb in slot kb % RING: its second half is read while the first is multiplied; then stage kb + 1 has
+  // arrived (at most RING - 2 younger ones are outstanding) and every wave holds the whole of stage kb in
+  // registers, so its slot takes stage kb + RING, and the first half of kb + 1 is read while the second of
+  // kb is multiplied. The last stages issue nothing; the very last reads a slot for nothing (no condition in
+  // the loop: at a join the compiler would wait for the reads before the products that do not need them).
   int kb = 0;
-  for (; kb + S::RING < nk; kb += 2) {
-    step(f0, f1, kb, std::integral_constant<int, 2 * S::PER>{}, More{});
-    step(f1, f0, kb + 1, std::integral_constant<int, 2 * S::PER>{}, More{});
+  for (; kb + S::RING < nk; ++kb) {
+    half(f0, f1, kb & (S::RING - 1), 1);
+    arrive<(S::RING - 2) * S::PER>();
+    issue(kb + S::RING, kb & (S::RING - 1));
+    half(f1, f0, (kb + 1) & (S::RING - 1), 0);
   }
-  if (nk >= S::RING) {
-    step(f0, f1, kb, std::integral_constant<int, 2 * S::PER>{}, Last{});
-    step(f1, f0, kb + 1, std::integral_constant<int, S::PER>{}, Last{});
+  for (; kb < nk; ++kb) {
+    half(f0, f1, kb & (S::RING - 1), 1);
+    arrive<0>();
+    half(f1, f0, (kb + 1) & (S::RING - 1), 0);
   }
-  step(f0, f1, nk - 2, std::integral_constant<int, 0>{}, Last{});
-  step(f1, f0, nk - 1, std::integral_constant<int, 0>{}, Last{});
 
   // acc[i][j]: channels n0 + 16 (wn FA + i) + 4 q + e of token m0 + 16 (wm FB + j) + r. Sixteen tokens at a
   // time go through LDS (each wave its own part), so that a store instruction writes whole rows.
@@ -437,7 +437,13 @@ int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream) {
   return check_launch(what);
 }
 
-constexpr int64_t kBigTiles8 = 128;
+static int cus8() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+      cus <= 0)
+    return 256;
+  return cus;
+}
 static bool few8(const mote_int8_linear_args* a) { return a->M <= 16 && a->K <= kFewMaxK; }
 
 size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a) {
@@ -469,19 +475,31 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
   p.x = xq; p.sx = sx; p.w = a->wq; p.sw = a->w_scale; p.y = a->y; p.y_sr = a->y_sr;
   p.M = a->M; p.N = a->N; p.Kp = Kp;
   p.wide = reinterpret_cast<uintptr_t>(a->y) % 16 == 0 && (a->y_sr * int64_t(sizeof(T))) % 16 == 0;
-  const int64_t big = (int64_t(a->M) + 255) / 256 * ((a->N + 255) / 256);
   auto go = [&](auto kernel, int ch, int tok, int waves) {
     p.ntok = (a->M + tok - 1) / tok; p.nch = (a->N + ch - 1) / ch;
+    // A weight that an XCD's 4 MB L2 holds stays there whatever the order; a larger one goes in groups of
+    // up to eight channel tiles, each over all tokens (W of 4 MB: 65536 x 1024 -> 4096 392 -> 379 us, 8192
+    // rows 53 -> 51 us; of 1.8 MB: 4964 x 768 -> 2304 24 us in one group, 26 us in three).
+    const int groups = int64_t(a->N) * Kp <= (5 << 19) ? 1 : (p.nch + 7) / 8;
+    p.gch = (p.nch + groups - 1) / groups;
     const unsigned per = unsigned((int64_t(p.ntok) * p.nch + 7) / 8);
     hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * waves), 0, stream, p);
   };
-  static const int var = getenv("V8") ? atoi(getenv("V8")) : 0;
-  if (var == 5) go(int8_many_kernel<T, 4, 4, 2, 2, 4>, 128, 128, 4);
-  else if (var == 7) go(int8_many_kernel<T, 2, 2, 2, 2, 4>, 64, 64, 4);
-  else if (var == 8) go(int8_many_kernel<T, 4, 8, 4, 2, 4>, 256, 256, 8);
-  else if (var == 9) go(int8_many_kernel<T, 8, 4, 1, 4, 4>, 128, 256, 4);
-  else if (big >= kBigTiles8) go(int8_many_kernel<T, 8, 4, 2, 4, 4>, 256, 256, 8);
-  else go(int8_many_kernel<T, 4, 4, 2, 2, 4>, 128, 128, 4);
+  // The largest tile that fills the chip (tiles of ch x tok; a CU holds three workgroups of the two small
+  // ones, two of the third, one of the largest):
+  //  64 x 32 with a deep ring while one round of workgroups holds them (17 x 768 -> 2304 7.3 us, 10.2 with
+  //    128 x 128 tiles; 512 rows 9.2 and 11.7);
+  //  128 x 64 likewise (2048 x 768 -> 2304 15.1 us, 16.1 with 128 x 128; 18.9 with 64 x 32);
+  //  256 x 256 from two rounds on whose last is nearly full (8192 x 1024 -> 4096, 512 tiles: 51 us, 57 with
+  //    128 x 128; 16384 x 768 -> 2304, 576 tiles: 60 and 57 us);
+  //  128 x 128 between.
+  const int64_t cus = cus8();
+  auto tiles = [&](int ch, int tok) { return ((int64_t(a->M) + tok - 1) / tok) * ((a->N + ch - 1) / ch); };
+  const int64_t big = tiles(256, 256);
+  if (tiles(64, 32) <= 3 * cus) go(int8_many_kernel<T, 2, 1, 2, 2, 4>, 64, 32, 4);
+  else if (tiles(128, 64) <= 3 * cus) go(int8_many_kernel<T, 4, 2, 2, 2, 2>, 128, 64, 4);
+  else if (big >= 2 * cus && 20 * big >= 17 * cus * ((big + cus - 1) / cus)) go(int8_many_kernel<T, 8, 4, 2, 4, 2>, 256, 256, 8);
+  else go(int8_many_kernel<T, 4, 4, 2, 2, 2>, 128, 128, 4);
 }
 
 int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream) {
