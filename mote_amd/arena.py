@@ -35,6 +35,8 @@ import torch
 class RelationArena:
     """Cache rows of `n_layers` Relation layers for `batch` sequences (see the module docstring)."""
 
+    in_place = True  # rows are kept as they are given: views of the store may be read and written
+
     def __init__(self, n_layers: int, n_heads: int, capacity: int, d_head: int, device, dtype, batch: int = 1):
         if capacity <= 0 or batch <= 0:
             raise ValueError("an arena needs a positive capacity and batch")
@@ -87,6 +89,10 @@ class RelationArena:
     def info(self, layer: int) -> torch.Tensor:
         """[batch, H, capacity, dh] view of a layer's I~ rows."""
         return self.store[layer, 1]
+
+    def layer(self, layer: int, state: "ArenaState") -> "ArenaLayer":
+        """What layer `layer` sees of the state."""
+        return ArenaLayer(self, layer, state)
 
     def rows(self, c0: int, c1: int) -> torch.Tensor:
         """Rows [c0, c1) of every layer, kind, sequence and head, as a view of `buf`'s layout."""
@@ -227,7 +233,7 @@ class ArenaState:
             return self.mamba[layer]
         if not 0 <= layer < self.arena.n_layers:
             raise IndexError(layer)
-        return ArenaLayer(self.arena, layer, self)
+        return self.arena.layer(layer, self)
 
     def __iter__(self) -> Iterator[Any]:
         return (self[i] for i in range(self.arena.n_layers))

@@ -19,6 +19,8 @@ import torch.nn.functional as F
 
 from . import _lib as L
 from .arena import RelationArena
+from .cache4 import decode4_workspace, relation_decode4
+from .int8 import FEW_ROWS, FEW_WIDTH, int8_linear, int8_weight
 
 
 def decode_workspace(B: int, H: int, D: int, capacity: int, device, dtype=torch.bfloat16) -> torch.Tensor:
@@ -170,14 +172,21 @@ class RelationDecodeStep:
     Holds the static tensors a captured graph needs (fp32 lam/theta/inv_freq copies and the stacked
     projection weight [w1; w2; wi], refreshed by `sync_params()`, the workspace, outputs).
     `__call__(x [B,1,D], S)` returns (out [B,1,D], xm [B] = mean over heads of the exchange mass,
-    graph.py:186)."""
+    graph.py:186).
 
-    def __init__(self, mixer, arena: RelationArena, layer: int):
+    The arena may be a RelationArena4 (rows in 4 bits: relation_decode4 in the place of relation_decode).
+    int8: the projections in 8-bit integers (`int8_linear`; codes and scales are the step's own copies,
+    which `sync_params()` refreshes), for up to 16 sequences."""
+
+    def __init__(self, mixer, arena: RelationArena, layer: int, int8: bool = False):
         self.mixer, self.arena, self.layer = mixer, arena, layer
         dev = arena.device
         B, H, D = arena.batch, mixer.n_heads, mixer.d_head
         self.B = B
-        self.workspace = decode_workspace(B, H, D, arena.capacity, dev, arena.dtype)
+        if int8 and (B > FEW_ROWS or mixer.d_model > FEW_WIDTH):
+            raise ValueError(f"projections in 8 bits take up to {FEW_ROWS} sequences and a width of {FEW_WIDTH}")
+        self.int8, self.w8 = bool(int8), {}
+        self._new_workspace()
         self.y = torch.empty(B, H, D, device=dev, dtype=arena.dtype)
         self.g = torch.empty(B, H, device=dev, dtype=torch.float32)
         self.xm = torch.empty(B, device=dev, dtype=torch.float32)
@@ -188,19 +197,68 @@ class RelationDecodeStep:
         self._bufs: dict = {}
         self.sync_params()
 
+    def _new_workspace(self) -> None:
+        a, m = self.arena, self.mixer
+        make = decode_workspace if a.in_place else lambda *sizes_and_dtype: decode4_workspace(*sizes_and_dtype[:-1])
+        self.workspace = make(a.batch, m.n_heads, m.d_head, a.capacity, a.device, a.dtype)
+        self._generation = a.generation
+
     @torch.no_grad()
     def sync_params(self) -> None:
         """Refresh the step's copies of the layer's parameters (after an optimiser step; a captured
         graph keeps reading these same tensors)."""
         m = self.mixer
+        if self.int8:
+            ws = {"qkv": torch.cat([m.w1.weight, m.w2.weight, m.wi.weight], dim=0), "wo": m.wo.weight}
+            if m.out_gate:
+                ws["wg"] = m.wg.weight
+            for name, w in ws.items():
+                w8 = int8_weight(w)
+                if name in self.w8:
+                    for old, new in zip(self.w8[name][:2], w8[:2]):
+                        old.copy_(new)
+                else:
+                    self.w8[name] = w8
+            self._sync_small()
+            return
         w = torch.cat([m.w1.weight, m.w2.weight, m.wi.weight], dim=0)
         if self.w_qkv is None or self.w_qkv.shape != w.shape or self.w_qkv.dtype != w.dtype:
             self.w_qkv = w.detach().clone()
         else:
             self.w_qkv.copy_(w)
+        self._sync_small()
+
+    def _sync_small(self) -> None:
         self.lam.copy_(self.mixer.lam.detach().float())
         if self.theta is not None:
             self.theta.copy_(self.mixer.theta.detach().float())
+
+    def _core(self, qkv, S, advance, xm, run, rope_f32) -> None:
+        """The step between the projections and `_out`, into self.y and self.g."""
+        m, a = self.mixer, self.arena
+        rows = (a.p2(self.layer), a.info(self.layer)) if a.in_place else (a.cache(self.layer),)
+        step = relation_decode if a.in_place else relation_decode4
+        step(qkv[:, 0], qkv[:, 1], qkv[:, 2], S, *rows, self.lam, m.tau_s, self.inv_freq, self.theta, m.layer_idx,
+             advance, self.workspace, self.y, self.g, xm, run, rope_f32)
+
+    def _int8_step(self, x, S, advance, run, xm):
+        """The step with its projections in 8-bit integers; the launch of wo writes xm."""
+        m = self.mixer
+        B, T, Dm = x.shape
+        H, dh = m.n_heads, m.d_head
+        if T != 1 or B != self.B:
+            raise ValueError(f"the decode step takes x [{self.B}, 1, {m.d_model}], got {list(x.shape)}")
+        x2, keep = x.reshape(B, Dm), run is not None
+        buf = lambda name, n: self._static(name, (B, n), x.dtype) if keep else None
+        qkv = int8_linear(x2, self.w8["qkv"], buf("qkv", 3 * H * dh), run).view(B, 3, H, dh).to(self.arena.dtype)
+        if m.qk_norm:
+            qkv = torch.stack([m.p1_norm(qkv[:, 0]), m.p2_norm(qkv[:, 1]), qkv[:, 2]], dim=1)
+        self._core(qkv, S, advance, None, run, x.dtype == torch.float32 and self.arena.dtype != torch.float32)
+        y = self.y.to(x.dtype).reshape(B, H * dh)
+        if m.out_gate:
+            y = y * torch.sigmoid(int8_linear(x2, self.w8["wg"], buf("gate", Dm), run))
+        out = int8_linear(y, self.w8["wo"], buf("out", Dm), run, g=self.g, xm=xm)
+        return out.view(B, 1, Dm), xm
 
     def _static(self, name: str, shape, dtype) -> torch.Tensor:
         """A persistent output buffer (a predicated launch that does not run leaves it as it was)."""
@@ -225,6 +283,13 @@ class RelationDecodeStep:
         m = self.mixer
         B, T, Dm = x.shape
         H, dh = m.n_heads, m.d_head
+        if self._generation != self.arena.generation and not self.arena.in_place:
+            # a grown arena in 4 bits: its workspace belongs to its capacity
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the arena has grown: run the decode step once outside the capture first")
+            self._new_workspace()
+        if self.int8:
+            return self._int8_step(x, S, advance, run, self.xm if xm is None else xm)
         skinny = T == 1 and _skinny_ok(B, x, self.w_qkv, m.wo.weight, *([m.wg.weight] if m.out_gate else []))
         if run is not None and not skinny:
             raise ValueError("a predicated decode step needs the bf16 skinny path (B <= 16, one chunk)")
@@ -243,9 +308,7 @@ class RelationDecodeStep:
         # in the decode launch)
         # RoPE tables at x's dtype (graph.py:161): an fp32 x (serving autocast) rotates in fp32
         rope_f32 = x.dtype == torch.float32 and self.arena.dtype != torch.float32
-        relation_decode(qkv[:, 0], qkv[:, 1], qkv[:, 2], S, self.arena.p2(self.layer), self.arena.info(self.layer),
-                        self.lam, m.tau_s, self.inv_freq, self.theta, m.layer_idx, advance, self.workspace,
-                        self.y, self.g, None if skinny else xm, run, rope_f32)
+        self._core(qkv, S, advance, None if skinny else xm, run, rope_f32)
         if skinny:  # _out (relation.py:176-182) on the skinny product
             y = self.y.to(x.dtype).reshape(B, H * dh)
             if m.out_gate:

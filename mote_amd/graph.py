@@ -32,20 +32,22 @@ from .decode import RelationDecodeStep
 
 class RelationMainStep:
     def __init__(self, arena: RelationArena, S: torch.Tensor, xm_dev: Optional[torch.Tensor] = None,
-                 run: Optional[torch.Tensor] = None, advance: bool = True):
+                 run: Optional[torch.Tensor] = None, advance: bool = True, int8: bool = False):
         """arena: the decode arena (one layer per Relation layer). S: the decoder's int64 device
         position (0-d or [batch]). xm_dev: optional fp32 [n_layers] (batch 1) or [n_layers, batch]
         buffer that receives each layer's exchange mass. run: optional device flag (bool / uint8, one
-        element), the predicate of every launch. advance: the last layer's launch moves S on."""
+        element), the predicate of every launch. advance: the last layer's launch moves S on. int8: the
+        layers' projections in 8-bit integers (see RelationDecodeStep). The arena may be a RelationArena4."""
         if S.dtype != torch.int64 or S.numel() != arena.batch or not S.is_contiguous():
             raise ValueError("S must be a contiguous int64 device tensor with one position per sequence")
         self.arena, self.S, self.xm_dev, self.run, self.advance = arena, S, xm_dev, run, advance
+        self.int8 = int8
         self.steps: Dict[int, RelationDecodeStep] = {}
 
     def _step(self, mixer, li: int) -> RelationDecodeStep:
         st = self.steps.get(li)
         if st is None or st.mixer is not mixer:
-            st = RelationDecodeStep(mixer, self.arena, li)
+            st = RelationDecodeStep(mixer, self.arena, li, self.int8)
             self.steps[li] = st
         return st
 

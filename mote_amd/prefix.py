@@ -40,6 +40,11 @@ class Branch:
         self.n_chunks = 0
 
 
+def _rows_as_they_are(arena: RelationArena) -> None:
+    if not arena.in_place:
+        raise TypeError("prefix-store pages hold an arena's rows as they are: not those of an arena in 4 bits")
+
+
 def _copy_rows(arena: RelationArena, seq: int, arena_row0: int, page: torch.Tensor, page_row0: int, rows: int,
                to_page: bool) -> None:
     """Rows [arena_row0, +rows) of sequence `seq` <-> page rows [page_row0, +rows)."""
@@ -74,6 +79,7 @@ class ArenaPages:
     def store_rows(self, branch: Branch, arena: RelationArena, c0: int, c1: int, seq: int = 0) -> None:
         """Append arena rows [c0, c1) of sequence `seq` to the branch (c0 == branch.n_chunks);
         returns once the rows are on the host."""
+        _rows_as_they_are(arena)
         if c0 != branch.n_chunks:
             raise ValueError(f"store_rows appends at row {branch.n_chunks}, not {c0}")
         c = c0
@@ -106,6 +112,7 @@ class ArenaPages:
         the rows are in the arena, so the branch's pages may be freed or reused right after. A
         batch-1 arena that already holds the branch is left alone (the hot case: no copy). Growing
         a batched arena keeps every other slot's rows (the arena carries them across growth)."""
+        _rows_as_they_are(arena)
         if n_chunks > branch.n_chunks:
             raise ValueError(f"the branch holds {branch.n_chunks} rows, not {n_chunks}")
         if arena.batch == 1 and arena.owner == branch.id and arena.n_valid >= n_chunks:

@@ -747,7 +747,7 @@ class FullRelation(nn.Module):
         bf16 = x.dtype == torch.bfloat16 or (torch.is_autocast_enabled() and
                                              torch.get_autocast_dtype("cuda") == torch.bfloat16)
         if (torch.is_grad_enabled() or torch.compiler.is_compiling() or not self._fused_prologue(bf16) or T == 0
-                or arena.dtype != torch.bfloat16 or arena.batch != B or arena.n_heads != self.n_heads
+                or not arena.in_place or arena.dtype != torch.bfloat16 or arena.batch != B or arena.n_heads != self.n_heads
                 or arena.d_head != self.d_head or arena.store.device != x.device or S + T > arena.capacity):
             return None
         p2, info = (t[:, :, S: S + T] for t in (arena.p2(cache.layer), arena.info(cache.layer)))
