@@ -5,7 +5,7 @@
 // infinities and NaNs on top, so one comparison finds the groups that have no scale.
 #pragma once
 
-#include "common.hpp"
+#include "stream.hpp"
 
 namespace mote {
 
@@ -62,35 +62,40 @@ __device__ __forceinline__ void decode4(uint32_t w, float s, float (&x)[8]) {
 }
 
 // eight elements of a 16-byte aligned row
-template <typename T>
-__device__ __forceinline__ void load_octet(const T* p, float (&x)[8]);
-template <>
-__device__ __forceinline__ void load_octet<bf16_t>(const bf16_t* p, float (&x)[8]) {
-  const Chunk c = load_chunk(p);
+template <bool STREAM, typename T>
+__device__ __forceinline__ void load_octet(const T* p, float (&x)[8]) {
+  if constexpr (sizeof(T) == 2) {
+    const Chunk c = load_chunk_as<STREAM>(p);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    x[2 * j] = __uint_as_float(c.w[j] << 16);
-    x[2 * j + 1] = __uint_as_float(c.w[j] & 0xffff0000u);
+    for (int j = 0; j < 4; ++j) {
+      x[2 * j] = __uint_as_float(c.w[j] << 16);
+      x[2 * j + 1] = __uint_as_float(c.w[j] & 0xffff0000u);
+    }
+  } else {
+    const Chunk a = load_chunk_as<STREAM>(p), b = load_chunk_as<STREAM>(p + 4);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      x[j] = __uint_as_float(a.w[j]);
+      x[4 + j] = __uint_as_float(b.w[j]);
+    }
   }
 }
-template <>
-__device__ __forceinline__ void load_octet<float>(const float* p, float (&x)[8]) {
-  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-  x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
 template <typename T>
-__device__ __forceinline__ void store_octet(T* p, const float (&x)[8]);
-template <>
-__device__ __forceinline__ void store_octet<bf16_t>(bf16_t* p, const float (&x)[8]) {
-  Chunk c;
+__device__ __forceinline__ void store_octet(T* p, const float (&x)[8]) {
+  Chunk a, b;
+  if constexpr (sizeof(T) == 2) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) c.w[j] = uint32_t(f2bf(x[2 * j])) | uint32_t(f2bf(x[2 * j + 1])) << 16;
-  store_chunk(p, c);
-}
-template <>
-__device__ __forceinline__ void store_octet<float>(float* p, const float (&x)[8]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+    for (int j = 0; j < 4; ++j) a.w[j] = uint32_t(f2bf(x[2 * j])) | uint32_t(f2bf(x[2 * j + 1])) << 16;
+    store_stream(p, a);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      a.w[j] = __float_as_uint(x[j]);
+      b.w[j] = __float_as_uint(x[4 + j]);
+    }
+    store_stream(p, a);
+    store_stream(p + 4, b);
+  }
 }
 
 // what a launcher checks of a cache in 4 bits: null pointers, alignment, strides that hold a row each

@@ -6,6 +6,7 @@
 // Rows of xq and wq are Kp = K rounded up to 128 bytes, xq's zero past K, so no product looks at K.
 #include "tiles.hpp"
 #include "params.hpp"
+#include "stream.hpp"
 
 namespace mote {
 
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
 // hands the slots over.
 // What bounds the 256 x 256 tile (8192 x 4096 -> 4096: 112 us, 2.45 POP/s): matrix cores 56 % busy at the
 // 1.9 GHz that the card runs them at; without its products it takes 90 us, without its loads and reads 90.
-// Short k (1024: 8 stages) adds the stores, which all CUs make at once: half of a tile's time.
+// Short k (1024: 8 stages) adds the stores, which all CUs make at once: a third of a tile's time.
 // ------------------------------------------------------------------------------------------------
 struct Many8Params {
   const int8_t* x;   // [M, Kp]
@@ -367,7 +368,8 @@ int8_many_kernel(const Many8Params p) {
   }
 
   // acc[i][j]: channels n0 + 16 (wn FA + i) + 4 q + e of token m0 + 16 (wm FB + j) + r. Sixteen tokens at a
-  // time go through LDS (each wave its own part), so that a store instruction writes whole rows.
+  // time go through LDS (each wave its own part), so that a store instruction writes whole rows; y passes
+  // the caches by (65536 x 1024 -> 4096 381 -> 317 us, 4096 x 4096 -> 1024 34.7 -> 33.4 us, small y as before).
   lds_barrier();  // the ring is no longer read
   T* tile = reinterpret_cast<T*>(smem) + wave * 16 * S::OUTW;
   const int nw0 = n0 + wn * 16 * FA;
@@ -405,7 +407,7 @@ int8_many_kernel(const Many8Params p) {
       T* yr = reinterpret_cast<T*>(p.y) + int64_t(m) * p.y_sr + n;
       const T* src = tile + row * S::OUTW + col;
       if (p.wide && n + EPC <= p.N) {
-        store_chunk(yr, load_chunk(src));
+        store_stream(yr, load_chunk(src));
       } else {
         for (int e = 0; e < EPC && n + e < p.N; ++e) yr[e] = src[e];
       }
