@@ -438,11 +438,6 @@ def stream_of(t: torch.Tensor) -> int:
     return torch._C._cuda_getCurrentRawStream(t.device.index)
 
 
-def stream_or_null(t: torch.Tensor) -> int:
-    """stream_of for calls whose checks come with the launch: null for a tensor on the CPU, which they refuse."""
-    return torch._C._cuda_getCurrentRawStream(t.device.index) if t.is_cuda else 0
-
-
 _HERE_ALREADY = contextlib.nullcontext()
 
 

@@ -65,9 +65,10 @@ def _build_torch_launch() -> str:
     out = os.path.join(LIBDIR, TORCHNAME)
     tmp = out + ".tmp"
     cmd = [shutil.which("g++") or "g++", "-O2", "-fPIC", "-shared", "-std=c++17",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{p}" for p in inc),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-D__HIP_PLATFORM_AMD__",
+           f"-I{os.path.join(os.path.dirname(os.path.dirname(_hipcc())), 'include')}", *(f"-I{p}" for p in inc),
            os.path.join(CSRC, "torch_launch.cpp"), "-o", tmp, f"-L{LIBDIR}", f"-l:{LIBNAME}",
-           f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10",
+           f"-L{os.path.join(os.path.dirname(torch.__file__), 'lib')}", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_hip",
            "-Wl,-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

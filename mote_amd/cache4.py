@@ -56,8 +56,7 @@ def cache4_write(cache: Cache4, p2: torch.Tensor, info: torch.Tensor, start: Uni
     lens: int64 [B] on the device: sequence b writes its first lens[b] rows; the rest of a padded batch
         leaves the cache as it was."""
     n, dev = _start(start)
-    with L.device_of(p2):
-        L.native().cache4_write(*cache, p2, info, n, dev, lens, L.stream_or_null(p2))
+    L.native().cache4_write(*cache, p2, info, n, dev, lens)
 
 
 def cache4_read(cache: Cache4, d_head: int, start: Union[int, torch.Tensor] = 0, rows: Optional[int] = None,
@@ -74,8 +73,7 @@ def cache4_read(cache: Cache4, d_head: int, start: Union[int, torch.Tensor] = 0,
             raise ValueError("cache4_read: device positions need a number of rows")
         rows = cache.p2.shape[2] - n
     o2, oi = out if out is not None else (None, None)
-    with L.device_of(cache.p2):
-        return L.native().cache4_read(*cache, int(d_head), n, dev, int(rows), dtype, o2, oi, L.stream_or_null(cache.p2))
+    return L.native().cache4_read(*cache, d_head, n, dev, rows, dtype, o2, oi)
 
 
 def decode4_workspace(B: int, H: int, d_head: int, capacity: int, device) -> torch.Tensor:
@@ -103,6 +101,5 @@ def relation_decode4(p1: torch.Tensor, p2: torch.Tensor, info: torch.Tensor, S: 
         fp32; the step's arithmetic rounds to that dtype where relation_decode rounds to the cache's.
     S: int64 [B] device positions. S[b] outside [0, capacity): NaN in y[b] and g[b], nothing stored.
     Returns (y [B, H, dh], g [B, H] fp32)."""
-    with L.device_of(p1):
-        return L.native().relation_decode4(p1, p2, info, S, *cache, lam, float(tau_s), inv_freq, theta, int(layer_idx),
-                                           bool(advance), workspace, y, g, xm, run, bool(rope_f32), L.stream_or_null(p1))
+    return L.native().relation_decode4(p1, p2, info, S, *cache, lam, tau_s, inv_freq, theta, layer_idx, advance, workspace,
+                                       y, g, xm, run, rope_f32)

@@ -6,6 +6,7 @@
 // Rows of xq and wq are Kp = K rounded up to 128 bytes, xq's zero past K, so no product looks at K.
 #include "tiles.hpp"
 #include "params.hpp"
+#include "device.hpp"
 #include "stream.hpp"
 
 namespace mote {
@@ -439,13 +440,6 @@ int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream) {
   return check_launch(what);
 }
 
-static int cus8() {
-  int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-      cus <= 0)
-    return 256;
-  return cus;
-}
 static bool few8(const mote_int8_linear_args* a) { return a->M <= 16 && a->K <= kFewMaxK; }
 
 size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a) {
@@ -495,7 +489,7 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
   //  256 x 256 from two rounds on whose last is nearly full (8192 x 1024 -> 4096, 512 tiles: 51 us, 57 with
   //    128 x 128; 16384 x 768 -> 2304, 576 tiles: 60 and 57 us);
   //  128 x 128 between.
-  const int64_t cus = cus8();
+  const int64_t cus = device_cu_count();
   auto tiles = [&](int ch, int tok) { return ((int64_t(a->M) + tok - 1) / tok) * ((a->N + ch - 1) / ch); };
   const int64_t big = tiles(256, 256);
   if (tiles(64, 32) <= 3 * cus) go(int8_many_kernel<T, 2, 1, 2, 2, 4>, 64, 32, 4);

@@ -15,6 +15,7 @@
 
 #include "common.hpp"
 #include "params.hpp"
+#include "device.hpp"
 #include "fp4.hpp"
 
 namespace mote {
@@ -445,13 +446,6 @@ __global__ void __launch_bounds__(kD4Threads) relation_decode4_kernel(const Dec4
 static int groups4(int D) { return (D + kGroup4 - 1) / kGroup4; }
 static int rows4(int G) { return 64 / G * kD4Waves; }
 
-static int cus4() {
-  int dev = 0, cus = 0;
-  if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-      cus <= 0)
-    return 256;
-  return cus;
-}
 // Splits per head. One for a cache of up to four steps, which needs no merge over workgroups (batch 1, head
 // dim 48, 256 rows: 5.5 us a step, 7.0 as two splits). Else a workgroup per CU over the whole batch, each of
 // at least two steps; two per CU where each still has a dozen steps (more loads in flight: batch 16, 4700
@@ -461,7 +455,7 @@ static int splits4(const mote_relation_decode4_args* a) {
   const int64_t BH = int64_t(a->B) * a->H, rows = rows4(groups4(a->D));
   const int64_t steps = (int64_t(a->capacity) + rows - 1) / rows;
   if (steps <= 4) return 1;
-  int64_t n = cus4() / BH;
+  int64_t n = device_cu_count() / BH;
   if (n < 1) n = 1;
   if (steps >= 12 * 2 * n) n *= 2;
   if (n > (steps + 1) / 2) n = (steps + 1) / 2;
@@ -470,6 +464,7 @@ static int splits4(const mote_relation_decode4_args* a) {
 
 struct Dec4Ws {
   size_t part, cnt, cnt_seq, total;
+  int nsplit;
 };
 // the counters first: they stay where they are when another capacity changes the splits
 static Dec4Ws ws4(const mote_relation_decode4_args* a) {
@@ -478,7 +473,8 @@ static Dec4Ws ws4(const mote_relation_decode4_args* a) {
   w.cnt_seq = 0;
   w.cnt = size_t(a->B) * line;
   w.part = w.cnt + BH * line;
-  w.total = w.part + BH * size_t(splits4(a)) * size_t(a->D + 2) * sizeof(float);
+  w.nsplit = splits4(a);
+  w.total = w.part + BH * size_t(w.nsplit) * size_t(a->D + 2) * sizeof(float);
   return w;
 }
 
@@ -518,7 +514,7 @@ int launch_decode4(const mote_relation_decode4_args* a, hipStream_t stream) {
   p.cnt = reinterpret_cast<int*>(ws + w.cnt);
   p.cnt_seq = reinterpret_cast<int*>(ws + w.cnt_seq);
   p.B = a->B; p.H = a->H; p.D = a->D; p.cap = a->capacity; p.parity = a->layer_parity & 1; p.flags = a->flags;
-  p.nsplit = splits4(a);
+  p.nsplit = w.nsplit;
   p.scale = 1.0f / sqrtf((float)a->D);
   p.tau_inv = 1.0f / a->tau_s;
   const dim3 grid(unsigned(a->B * a->H * p.nsplit)), block(kD4Threads);

@@ -5,6 +5,8 @@
 // so do checks of what a call may pass, except the sizes, types and devices of operands whose extent the
 // kernel takes from another one: those are compared here. RuntimeError with the library's message
 // when a call fails. Host code only; streams come as raw handles.
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
 #include <climits>
@@ -392,12 +394,21 @@ std::tuple<Tensor, Tensor> dechunk_bwd(const Tensor& g, const Tensor& h, const T
   return {dh, dp};
 }
 
-// ---- the cache in 4 bits and the 8-bit products: checks, allocation and launch in one call ----------
+// ---- the cache in 4 bits and the 8-bit products ----------------------------------------------------------
+// Checks, allocation and launch in one call, on the operands' device and its current stream: a step of a
+// token is paced by its calls (with the stream and a device context taken in Python a call of a decode step
+// took 5.8 us of host time, 5.0 so).
 template <typename... A>
 [[noreturn]] void bad_value(A&&... a) { throw py::value_error(c10::str(std::forward<A>(a)...)); }
 void on_gpu(const Tensor& t, const char* what) {
   if (!t.is_cuda()) throw std::runtime_error(c10::str(what, " needs the HIP library and an MI355X"));
 }
+// the operands' device as the current one for the life of the object, and its current stream
+struct On {
+  c10::DeviceGuard guard;
+  void* stream;
+  explicit On(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
+};
 void no_grad(const char* what, std::initializer_list<const Tensor*> ts) {
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : ts)
@@ -462,7 +473,7 @@ void rows_of_start(mote_cache4_rows_args& a, const Cache4& c, int64_t start, con
 }
 
 void cache4_write(const Tensor& k, const Tensor& ks, const Tensor& v, const Tensor& vs, Tensor p2, Tensor info, int64_t start,
-                  const OptTensor& start_dev, const OptTensor& lens, int64_t stream) {
+                  const OptTensor& start_dev, const OptTensor& lens) {
   const char* what = "cache4_write";
   if (p2.dim() != 4 || info.sizes() != p2.sizes()) bad_value(what, ": p2 and info must both be [B, H, T, D]");
   if (info.scalar_type() != p2.scalar_type() || info.device() != p2.device())
@@ -474,15 +485,16 @@ void cache4_write(const Tensor& k, const Tensor& ks, const Tensor& v, const Tens
   rows_of_start(a, c, start, start_dev, lens, B, T, p2.device(), what);
   no_grad(what, {&p2, &info});
   on_gpu(p2, what);
+  const On on(p2);
   p2 = aligned(p2); info = aligned(info);
   a.B = int(B); a.H = int(H); a.T = int(T); a.D = int(D);
   a.p2 = view(p2); a.info = view(info);
-  check(mote_cache4_write(&a, reinterpret_cast<void*>(stream)), "mote_cache4_write");
+  check(mote_cache4_write(&a, on.stream), "mote_cache4_write");
 }
 
 std::tuple<Tensor, Tensor> cache4_read(const Tensor& k, const Tensor& ks, const Tensor& v, const Tensor& vs, int64_t D,
                                        int64_t start, const OptTensor& start_dev, int64_t rows, at::ScalarType dtype,
-                                       const OptTensor& out2, const OptTensor& outi, int64_t stream) {
+                                       const OptTensor& out2, const OptTensor& outi) {
   const char* what = "cache4_read";
   if (k.dim() != 4) bad_value(what, ": the codes of P2 must be [B, H, capacity, 16 G]");
   const int64_t B = k.size(0), H = k.size(1);
@@ -504,13 +516,14 @@ std::tuple<Tensor, Tensor> cache4_read(const Tensor& k, const Tensor& ks, const 
   }
   a.dtype = code(out2 ? p2.scalar_type() : dtype);
   on_gpu(k, what);
+  const On on(k);
   if (!out2) {
     p2 = empty({B, H, rows, D}, k, dtype);
     info = empty({B, H, rows, D}, k, dtype);
   }
   a.B = int(B); a.H = int(H); a.T = int(rows); a.D = int(D);
   a.p2 = view(p2); a.info = view(info);
-  check(mote_cache4_read(&a, reinterpret_cast<void*>(stream)), "mote_cache4_read");
+  check(mote_cache4_read(&a, on.stream), "mote_cache4_read");
   return {p2, info};
 }
 
@@ -529,7 +542,7 @@ std::tuple<Tensor, Tensor> relation_decode4(const Tensor& p1, const Tensor& p2, 
                                             const Tensor& ks, const Tensor& v, const Tensor& vs, const Tensor& lam, double tau,
                                             const OptTensor& inv_freq, const OptTensor& theta, int64_t layer_idx, bool advance,
                                             const OptTensor& workspace, const OptTensor& y_, const OptTensor& g_, const OptTensor& xm,
-                                            const OptTensor& run, bool rope_f32, int64_t stream) {
+                                            const OptTensor& run, bool rope_f32) {
   const char* what = "relation_decode4";
   if (p1.dim() != 3) bad_value(what, ": p1/p2/info must be [B, H, dh]");
   const int64_t B = p1.size(0), H = p1.size(1), D = p1.size(2);
@@ -562,6 +575,7 @@ std::tuple<Tensor, Tensor> relation_decode4(const Tensor& p1, const Tensor& p2, 
     bad_value(what, ": g must be a contiguous fp32 [B, H] tensor");
   no_grad(what, {&p1, &p2, &info});
   on_gpu(p1, what);
+  const On on(p1);
   Tensor y = y_ ? *y_ : empty({B, H, D}, p1, p1.scalar_type());
   Tensor g = g_ ? *g_ : empty({B, H}, p1, at::kFloat);
   a.B = int(B); a.H = int(H); a.D = int(D); a.capacity = int(c.capacity);
@@ -585,16 +599,17 @@ std::tuple<Tensor, Tensor> relation_decode4(const Tensor& p1, const Tensor& p2, 
   a.workspace_bytes = size_t(ws.numel()) * ws.element_size();
   a.xm = xm ? fptr(*xm) : nullptr;
   a.run = run ? static_cast<const unsigned char*>(run->data_ptr()) : nullptr;
-  check(mote_relation_decode4(&a, reinterpret_cast<void*>(stream)), "mote_relation_decode4");
+  check(mote_relation_decode4(&a, on.stream), "mote_relation_decode4");
   return {y, g};
 }
 
-std::tuple<Tensor, Tensor> quantize_rows(Tensor x, int64_t stream) {
+std::tuple<Tensor, Tensor> quantize_rows(Tensor x) {
   if (x.dim() != 2 || x.size(1) < 1) bad_value("quantize_rows: x must be [M, K]");
   mote_quantize_rows_args a{};
   a.dtype = code(x);
   no_grad("quantize_rows", {&x});
   on_gpu(x, "quantize_rows");
+  const On on(x);
   x = unit(x);
   const int64_t M = x.size(0), K = x.size(1);
   Tensor q = empty({M, (K + 127) / 128 * 128}, x, at::kChar), scale = empty({M}, x, at::kFloat);
@@ -602,12 +617,12 @@ std::tuple<Tensor, Tensor> quantize_rows(Tensor x, int64_t stream) {
   a.M = int(M); a.K = int(K);
   a.x = x.data_ptr(); a.x_sr = x.stride(0);
   a.q = static_cast<int8_t*>(q.data_ptr()); a.scale = fptr(scale);
-  check(mote_quantize_rows(&a, reinterpret_cast<void*>(stream)), "mote_quantize_rows");
+  check(mote_quantize_rows(&a, on.stream), "mote_quantize_rows");
   return {q, scale};
 }
 
 Tensor int8_linear(const Tensor& x_, const Tensor& wq, const Tensor& ws, int64_t K, const OptTensor& out, const OptTensor& run,
-                   const OptTensor& g, const OptTensor& xm, int64_t stream) {
+                   const OptTensor& g, const OptTensor& xm) {
   const char* what = "int8_linear";
   if (x_.dim() < 1 || x_.size(-1) != K || K < 1) bad_value(what, ": x must be [..., ", K, "], got ", x_.sizes());
   const int64_t Kp = (K + 127) / 128 * 128;
@@ -629,6 +644,7 @@ Tensor int8_linear(const Tensor& x_, const Tensor& wq, const Tensor& ws, int64_t
     bad_value(what, ": xm needs fp32 contiguous g [M, H] and xm [M] on x's device");
   no_grad(what, {&x_});
   on_gpu(x_, what);
+  const On on(x_);
   TORCH_CHECK(M <= INT_MAX && N <= INT_MAX && K <= INT_MAX, "int8_linear: sizes beyond 32 bits");
   const Tensor x = unit(x_.dim() == 2 ? x_ : x_.reshape({M, K}));
   Tensor y = out ? *out : empty(sizes, x_, x_.scalar_type());
@@ -648,7 +664,7 @@ Tensor int8_linear(const Tensor& x_, const Tensor& wq, const Tensor& ws, int64_t
     a.workspace = wk.data_ptr();
     a.workspace_bytes = n;
   }
-  check(mote_int8_linear(&a, reinterpret_cast<void*>(stream)), "mote_int8_linear");
+  check(mote_int8_linear(&a, on.stream), "mote_int8_linear");
   return y;
 }
 

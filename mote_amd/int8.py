@@ -31,8 +31,7 @@ class Int8Weight(NamedTuple):
 def quantize_rows(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """The rows of x [M, K] (bf16 or fp32) in 8 bits: (codes int8 [M, K rounded up to 128], zeros past K;
     scales fp32 [M])."""
-    with L.device_of(x):
-        return L.native().quantize_rows(x, L.stream_or_null(x))
+    return L.native().quantize_rows(x)
 
 
 def int8_weight(w: torch.Tensor) -> Int8Weight:
@@ -47,5 +46,4 @@ def int8_linear(x: torch.Tensor, w: Int8Weight, out: Optional[torch.Tensor] = No
 
     Up to 16 tokens of K <= 4096 are one launch, which also takes what `skinny_linear` takes: `run` (a device
     flag; 0 leaves `out` untouched), g (fp32 [M, H], contiguous) and xm (fp32 [M], the mean of g over the heads)."""
-    with L.device_of(x):
-        return L.native().int8_linear(x, w.q, w.scale, w.in_features, out, run, g, xm, L.stream_or_null(x))
+    return L.native().int8_linear(x, w.q, w.scale, w.in_features, out, run, g, xm)
