@@ -4,6 +4,8 @@
 // acc = sum_k xq wq runs on v_mfma_i32_16x16x64_i8, exact in 32 bits; y = (acc sx) sw in fp32, rounded once.
 // One fragment convention for both operands: lane l holds 16 consecutive k of row l % 16, k group l / 16.
 // Rows of xq and wq are Kp = K rounded up to 128 bytes, xq's zero past K, so no product looks at K.
+#include <algorithm>
+
 #include "tiles.hpp"
 #include "params.hpp"
 #include "device.hpp"
@@ -481,20 +483,27 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
     const unsigned per = unsigned((int64_t(p.ntok) * p.nch + 7) / 8);
     hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * waves), 0, stream, p);
   };
-  // The largest tile that fills the chip (tiles of ch x tok; a CU holds three workgroups of the two small
-  // ones, two of the third, one of the largest):
-  //  64 x 32 with a deep ring while one round of workgroups holds them (17 x 768 -> 2304 7.3 us, 10.2 with
-  //    128 x 128 tiles; 512 rows 9.2 and 11.7);
-  //  128 x 64 likewise (2048 x 768 -> 2304 15.1 us, 16.1 with 128 x 128; 18.9 with 64 x 32);
-  //  256 x 256 from two rounds on whose last is nearly full (8192 x 1024 -> 4096, 512 tiles: 51 us, 57 with
-  //    128 x 128; 16384 x 768 -> 2304, 576 tiles: 60 and 57 us);
-  //  128 x 128 between.
+  // Tiles of channels x tokens. One round of workgroups of a small tile while that holds everything (a CU
+  // holds three of either): 64 x 32 with a deep ring (17 x 768 -> 2304 7.3 us, 10.2 with 128 x 128; 512 rows
+  // 8.9 and 11.4), then 128 x 64 (2048 x 768 -> 2304 13.6 us, 14.9 with 128 x 128, 18.9 with 64 x 32).
   const int64_t cus = device_cu_count();
   auto tiles = [&](int ch, int tok) { return ((int64_t(a->M) + tok - 1) / tok) * ((a->N + ch - 1) / ch); };
-  const int64_t big = tiles(256, 256);
-  if (tiles(64, 32) <= 3 * cus) go(int8_many_kernel<T, 2, 1, 2, 2, 4>, 64, 32, 4);
-  else if (tiles(128, 64) <= 3 * cus) go(int8_many_kernel<T, 4, 2, 2, 2, 2>, 128, 64, 4);
-  else if (big >= 2 * cus && 20 * big >= 17 * cus * ((big + cus - 1) / cus)) go(int8_many_kernel<T, 8, 4, 2, 4, 2>, 256, 256, 8);
+  if (tiles(64, 32) <= 3 * cus) return go(int8_many_kernel<T, 2, 1, 2, 2, 4>, 64, 32, 4);
+  if (tiles(128, 64) <= 3 * cus) return go(int8_many_kernel<T, 4, 2, 2, 2, 2>, 128, 64, 4);
+  // Beyond, the tile whose rounds take least: a round of n stages of k takes fixed + n * stage us (fitted to
+  // k = 768, 1024 and 4096 at 4964 to 65536 rows), with one workgroup per CU of the large tiles and two of
+  // 128 x 128. 4964 x 768 -> 2304: 234 tiles of 256 x 192 in one round 20.9 us, 23.2 with 256 x 256 or 128 x
+  // 128; 16384 rows: 768 tiles of 192 x 256 in three 52.8 us, 57.7 and 57.1; 65536 x 1024 -> 4096: 256 x 256
+  // 328 us, 353 with 256 x 192, 366 with 128 x 128.
+  auto rounds_us = [&](int64_t t, int64_t slots, double fixed, double stage) {
+    return double((t + slots - 1) / slots) * (fixed + Kp / 128 * stage);
+  };
+  const double big = rounds_us(tiles(256, 256), cus, 7.3, 1.5), wide = rounds_us(tiles(256, 192), cus, 5.6, 1.15),
+               tall = rounds_us(tiles(192, 256), cus, 5.6, 1.15), mid = rounds_us(tiles(128, 128), 2 * cus, 3.5, 0.94);
+  const double best = std::min(std::min(big, wide), std::min(tall, mid));
+  if (big == best) go(int8_many_kernel<T, 8, 4, 2, 4, 2>, 256, 256, 8);
+  else if (wide == best) go(int8_many_kernel<T, 8, 3, 2, 4, 2>, 256, 192, 8);
+  else if (tall == best) go(int8_many_kernel<T, 6, 4, 2, 4, 2>, 192, 256, 8);
   else go(int8_many_kernel<T, 4, 4, 2, 2, 2>, 128, 128, 4);
 }
 

@@ -75,6 +75,19 @@ def test_linear_is_one_rounding_from_exact(cuda, dtype, M, K, N):
     _check(y, x, w)
 
 
+@pytest.mark.parametrize("M,K,N", [(700, 256, 1100), (2300, 200, 2500), (6300, 96, 2300), (16384, 64, 2304), (5000, 384, 9000)])
+def test_every_tile_size_gives_a_row_its_own_result(cuda, M, K, N):
+    """Sizes over the range of tiles (the rule picks by rounds of workgroups): rows, the last ones and those at
+    tile borders among them, equal the few-token form's bit for bit."""
+    from mote_amd.int8 import int8_linear, int8_weight
+
+    x, w8 = _x(1, M, K, BF16).to(cuda), int8_weight(_x(2, N, K, BF16).to(cuda))
+    y = int8_linear(x, w8)
+    for at in (0, 120, 185, 250, 500, M // 2, M - 16):
+        at = min(at, M - 16)
+        assert torch.equal(y[at: at + 16], int8_linear(x[at: at + 16], w8)), at
+
+
 def test_forms_agree_bit_for_bit(cuda):
     """The few-token and the many-token form give a token the same result, alone or in any batch."""
     from mote_amd.int8 import int8_linear, int8_weight
