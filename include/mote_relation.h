@@ -762,7 +762,7 @@ int mote_relation_decode4(const mote_relation_decode4_args* args, void* stream);
  * infinity stores zeros with scale NaN.
  * mote_int8_linear: y [M, N] (dtype) = ((float(acc) sx[m]) sw[n]) rounded once, acc = sum_k xq wq exact in
  * 32-bit integers (K <= 131072); x is quantised in the call, wq [N, Kp] and sw [N] come from
- * mote_quantize_rows. Up to 16 rows with K <= 4096 are one launch, which takes the decode step's predicate
+ * mote_quantize_rows. Up to 64 rows with K <= 4096 are one launch, which takes the decode step's predicate
  * and exchange mass as mote_skinny_gemm does; others quantise x into the workspace first
  * (mote_int8_linear_workspace() bytes; its contents on entry do not matter) and take neither.
  * Row strides in elements; wq on a 16-byte boundary with its rows Kp apart.

@@ -125,12 +125,15 @@ quantize_rows_kernel(const T* x, int64_t x_sr, int M, int K, int Kp, bool wide, 
 }
 
 // ------------------------------------------------------------------------------------------------
-// Few tokens (M <= 16): x is quantised where it is multiplied. One workgroup (4 waves) per 16 channels,
-// the 64-wide k steps dealt to the waves in runs; a wave issues every load of its W rows, then reads its
-// part of x, agrees on the rows' maxima with the other waves through LDS, and multiplies. The four
-// partial sums are integers: their order does not matter.
+// Few tokens: x is quantised where it is multiplied. One workgroup (4 waves) per 16 channels and 16 tokens,
+// the 64-wide k steps dealt to the waves in runs; a wave issues every load of its W rows and of its part of
+// x, agrees on the rows' maxima with the other waves through LDS, and multiplies. The four partial sums are
+// integers: their order does not matter. Every workgroup of a token tile quantises it again (24 KB at 768
+// from the L2), which costs less than a launch of its own. A launch of this size is bound by its latencies:
+// 4.4 us at 1 x 768 -> 768, 4.5 us at 1 x 768 -> 2304, whose W of 1.8 MB takes 0.4.
 // ------------------------------------------------------------------------------------------------
 constexpr int kFewWaves = 4;
+constexpr int kFewRows = 64;
 constexpr int kFewMaxK = 4096;
 
 struct Few8Params {
@@ -144,6 +147,31 @@ struct Few8Params {
   int wide;
 };
 
+// sixteen elements of a row as they lie in memory, and as numbers
+template <typename T>
+struct Row16 {
+  static constexpr int EPC = 16 / int(sizeof(T)), NC = 16 / EPC;
+  Chunk c[NC];
+  __device__ __forceinline__ void load(const T* row, int k, int K, bool wide) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+      const int k0 = k + EPC * i;
+      if (wide && k0 + EPC <= K) {
+        c[i] = load_chunk(row + k0);
+      } else {
+        T* e = reinterpret_cast<T*>(&c[i]);
+#pragma unroll
+        for (int j = 0; j < EPC; ++j) e[j] = k0 + j < K ? row[k0 + j] : T(0);
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(c[j / 4].w[j % 4]);
+    const uint32_t w = c[j / 8].w[j % 8 / 2];
+    return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+  }
+};
+
 template <typename T, int KS>
 __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Params p) {
   using E = Elem<T>;
@@ -151,35 +179,26 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
   __shared__ __align__(16) int part[kFewWaves][16][17];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, q = lane >> 4;
-  const int n0 = blockIdx.x * 16;
+  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
   const int nks = p.Kp / 64;                                 // k steps, an even number
   const int per = (nks + kFewWaves - 1) / kFewWaves;         // <= KS
   const int s0 = min(wave * per, nks), s1 = min(s0 + per, nks);
   const int8_t* wrow = p.w + int64_t(min(n0 + r, p.N - 1)) * p.Kp + 16 * q;
-  const T* xrow = reinterpret_cast<const T*>(p.x) + int64_t(min(r, p.M - 1)) * p.x_sr;
+  const T* xrow = reinterpret_cast<const T*>(p.x) + int64_t(min(m0 + r, p.M - 1)) * p.x_sr;
   Chunk a[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s)
     if (s0 + s < s1) a[s] = load_chunk(wrow + 64 * (s0 + s));
-  float x[KS][16];
-  uint32_t top = 0;
+  Row16<T> x[KS];
 #pragma unroll
-  for (int s = 0; s < KS; ++s) {
-    if (s0 + s < s1) {
-      float lo[8], hi[8];
-      row_octet<T>(xrow, 64 * (s0 + s) + 16 * q, p.K, p.wide, lo);
-      row_octet<T>(xrow, 64 * (s0 + s) + 16 * q + 8, p.K, p.wide, hi);
+  for (int s = 0; s < KS; ++s)
+    if (s0 + s < s1) x[s].load(xrow, 64 * (s0 + s) + 16 * q, p.K, p.wide);
+  float sw[4];  // of the channels that this lane stores (wave 0)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x[s][j] = lo[j];
-        x[s][8 + j] = hi[j];
-        top = max(top, max(mag_bits(lo[j]), mag_bits(hi[j])));
-      }
-    }
-  }
+  for (int i = 0; i < 4; ++i) sw[i] = p.sw[min(n0 + 4 * q + i, p.N - 1)];
   // the decode step's exchange mass on the side: workgroup 0, wave 1, lane b < M
   const int xb = int(threadIdx.x) - 64;
-  const bool xm_lane = p.xm != nullptr && blockIdx.x == 0 && xb >= 0 && xb < p.M;
+  const bool xm_lane = p.xm != nullptr && blockIdx.x == 0 && m0 == 0 && xb >= 0 && xb < p.M;
   float gsum = 0.f;
   if (xm_lane) {
     const float* gb = p.g + int64_t(xb) * p.heads;
@@ -193,6 +212,12 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
   }
   if (p.run && p.run[0] == 0) return;  // uniform: the whole workgroup leaves before its barrier
   if (xm_lane) p.xm[xb] = gsum / float(p.heads);
+  uint32_t top = 0;
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+    if (s0 + s < s1)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = max(top, mag_bits(x[s].get(j)));
   top = max(top, uint32_t(__shfl_xor(int(top), 16, 64)));
   top = max(top, uint32_t(__shfl_xor(int(top), 32, 64)));
   if (q == 0) tops[wave][r] = top;
@@ -208,8 +233,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
       Chunk b;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        b.w[j] = code8(x[s][4 * j], sc.inv) | code8(x[s][4 * j + 1], sc.inv) << 8 |
-                 code8(x[s][4 * j + 2], sc.inv) << 16 | code8(x[s][4 * j + 3], sc.inv) << 24;
+        b.w[j] = code8(x[s].get(4 * j), sc.inv) | code8(x[s].get(4 * j + 1), sc.inv) << 8 |
+                 code8(x[s].get(4 * j + 2), sc.inv) << 16 | code8(x[s].get(4 * j + 3), sc.inv) << 24;
       acc = mma8(a[s], b, acc);
     }
   }
@@ -217,7 +242,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
 #pragma unroll
   for (int i = 0; i < 4; ++i) part[wave][4 * q + i][r] = acc[i];
   __syncthreads();
-  if (wave == 0 && r < p.M) {
+  if (wave == 0 && m0 + r < p.M) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int f = 4 * q + i;
@@ -225,7 +250,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
 #pragma unroll
       for (int w = 1; w < kFewWaves; ++w) v += part[w][f][r];
       if (n0 + f < p.N)
-        reinterpret_cast<T*>(p.y)[int64_t(r) * p.y_sr + n0 + f] = E::from_f(float(v) * sc.scale * p.sw[n0 + f]);
+        reinterpret_cast<T*>(p.y)[int64_t(m0 + r) * p.y_sr + n0 + f] = E::from_f(float(v) * sc.scale * sw[i]);
     }
   }
 }
@@ -442,7 +467,15 @@ int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream) {
   return check_launch(what);
 }
 
-static bool few8(const mote_int8_linear_args* a) { return a->M <= 16 && a->K <= kFewMaxK; }
+// The one-launch form: for up to 16 tokens (16 x 768 -> 768 4.9 us, 7.2 with quantize_rows and tiles; 16 x
+// 4096 -> 4096 13.0 and 13.4), and up to 64 while the workgroups that quantise a token again are few (64 x 1024
+// -> 1024, 256 of them, 5.5 and 7.6 us; 64 x 768 -> 2304, 576, 7.2 and 7.3; 64 x 4096 -> 4096, 1024, 29 and 13);
+// the predicate and the exchange mass have it to themselves.
+static bool few8(const mote_int8_linear_args* a) {
+  if (a->M > kFewRows || a->K > kFewMaxK) return false;
+  const int64_t groups = (int64_t(a->M) + 15) / 16 * ((int64_t(a->N) + 15) / 16);
+  return a->M <= 16 || a->run || a->xm || groups * std::max(a->K, 1024) <= int64_t(2048) * device_cu_count();
+}
 
 size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a) {
   if (a->M <= 0 || a->K <= 0 || few8(a)) return 0;
@@ -457,7 +490,7 @@ static void launch_few8(const mote_int8_linear_args* a, hipStream_t stream) {
   p.M = a->M; p.N = a->N; p.K = a->K; p.Kp = int(padded_k8(a->K));
   p.wide = reinterpret_cast<uintptr_t>(a->x) % 16 == 0 && (a->x_sr * int64_t(sizeof(T))) % 16 == 0;
   const int per = (p.Kp / 64 + kFewWaves - 1) / kFewWaves;
-  const dim3 grid(unsigned((a->N + 15) / 16)), block(64 * kFewWaves);
+  const dim3 grid(unsigned((a->N + 15) / 16), unsigned((a->M + 15) / 16)), block(64 * kFewWaves);
   if (per <= 4) hipLaunchKernelGGL((int8_few_kernel<T, 4>), grid, block, 0, stream, p);
   else if (per <= 8) hipLaunchKernelGGL((int8_few_kernel<T, 8>), grid, block, 0, stream, p);
   else hipLaunchKernelGGL((int8_few_kernel<T, 16>), grid, block, 0, stream, p);
@@ -525,7 +558,7 @@ int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream) {
     else launch_few8<float>(a, stream);
     return check_launch(what);
   }
-  if (a->run || a->xm) return set_error(MOTE_ERR_SHAPE, "%s: run and xm need at most 16 rows of K <= %d", what, kFewMaxK);
+  if (a->run || a->xm) return set_error(MOTE_ERR_SHAPE, "%s: run and xm need at most %d rows of K <= %d", what, kFewRows, kFewMaxK);
   const size_t need = int8_linear_workspace_bytes(a);
   if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)
     return set_error(MOTE_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes, %zu needed", what, a->workspace_bytes, need);

@@ -176,7 +176,7 @@ class RelationDecodeStep:
 
     The arena may be a RelationArena4 (rows in 4 bits: relation_decode4 in the place of relation_decode).
     int8: the projections in 8-bit integers (`int8_linear`; codes and scales are the step's own copies,
-    which `sync_params()` refreshes), for up to 16 sequences."""
+    which `sync_params()` refreshes), for up to 64 sequences."""
 
     def __init__(self, mixer, arena: RelationArena, layer: int, int8: bool = False):
         self.mixer, self.arena, self.layer = mixer, arena, layer

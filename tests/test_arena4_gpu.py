@@ -193,8 +193,8 @@ def test_what_the_step_refuses(cuda):
     from mote_amd.decode import RelationDecodeStep
 
     m = _mixer(cuda, 192, 4)
-    with pytest.raises(ValueError, match="16 sequences"):
-        RelationDecodeStep(m, RelationArena(1, 4, 64, 48, cuda, BF16, batch=17), 0, int8=True)
+    with pytest.raises(ValueError, match="64 sequences"):
+        RelationDecodeStep(m, RelationArena(1, 4, 64, 48, cuda, BF16, batch=65), 0, int8=True)
     step = RelationDecodeStep(m, RelationArena(1, 4, 64, 48, cuda, BF16, batch=2), 0, int8=True)
     S = torch.zeros(2, dtype=torch.int64, device=cuda)
     for shape in ((2, 2, 192), (1, 1, 192)):

@@ -63,7 +63,7 @@ def test_quantize_rows_special_rows_and_strides(cuda):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("M,K,N", [(1, 768, 2304), (16, 768, 768), (5, 64, 1), (16, 4096, 48), (3, 1000, 17), (2, 1, 5),
+@pytest.mark.parametrize("M,K,N", [(1, 768, 2304), (16, 768, 768), (5, 64, 1), (16, 4096, 48), (33, 4000, 300), (64, 768, 130), (50, 700, 40), (3, 1000, 17), (2, 1, 5),
                                    (9, 2050, 271), (17, 128, 16), (64, 520, 271), (130, 768, 300), (257, 129, 129),
                                    (300, 1024, 128), (1, 5000, 40), (1000, 96, 64), (128, 4224, 256)])
 def test_linear_is_one_rounding_from_exact(cuda, dtype, M, K, N):
@@ -96,7 +96,7 @@ def test_forms_agree_bit_for_bit(cuda):
         for K, N in ((768, 2304), (520, 271), (4096, 130)):
             x, w8 = _x(1, 300, K, dtype).to(cuda), int8_weight(_x(2, N, K, BF16).to(cuda))
             y = int8_linear(x, w8)
-            for a, b in ((0, 1), (5, 21), (284, 300), (100, 117)):
+            for a, b in ((0, 1), (5, 21), (284, 300), (100, 117), (0, 64), (33, 82), (200, 265)):
                 assert torch.equal(int8_linear(x[a:b], w8), y[a:b])
 
 
@@ -149,7 +149,7 @@ def test_run_xm_and_graph(cuda):
     assert torch.equal(out, int8_linear(x, w8))
     assert torch.allclose(xm, g.double().mean(1).float(), rtol=9 * 2.0 ** -24, atol=0)  # eight additions, a division
     many = _x(11, 200, 256, BF16).to(cuda)
-    with pytest.raises(RuntimeError, match="16 rows"):
+    with pytest.raises(RuntimeError, match="64 rows"):
         int8_linear(many, w8, run=off)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
