@@ -41,27 +41,45 @@ __device__ __forceinline__ uint32_t code8(float x, float inv) {
   return inv == 0.f ? 0u : uint32_t(int(rintf(x * inv))) & 0xffu;
 }
 
-// x[k .. k + 8) of a row of K elements, zeros past its end; `wide`: the row is 16-byte aligned
-template <typename T>
-__device__ __forceinline__ void row_octet(const T* row, int k, int K, bool wide, float (&x)[8]) {
-  using E = Elem<T>;
-  if (wide && k + 8 <= K) {
-    if constexpr (sizeof(T) == 2) {
-      const Chunk c = load_chunk(row + k);
+// N elements of a row of K from k on, as they lie in memory (zeros past its end), and as numbers
+template <typename T, int N>
+struct RowPart {
+  static constexpr int EPC = 16 / int(sizeof(T)), NC = N / EPC;
+  Chunk c[NC];
+  __device__ __forceinline__ void load(const T* row, int k, int K) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[2 * j] = __uint_as_float(c.w[j] << 16);
-        x[2 * j + 1] = __uint_as_float(c.w[j] & 0xffff0000u);
+    for (int i = 0; i < NC; ++i) {
+      const int k0 = k + EPC * i;
+      if (k0 + EPC <= K) {
+        c[i] = load_any(row + k0);
+      } else {
+        T* e = reinterpret_cast<T*>(&c[i]);
+#pragma unroll
+        for (int j = 0; j < EPC; ++j) e[j] = k0 + j < K ? row[k0 + j] : T(0);
       }
-    } else {
-      const float4 a = reinterpret_cast<const float4*>(row + k)[0], b = reinterpret_cast<const float4*>(row + k)[1];
-      x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w; x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = k + j < K ? E::to_f(row[k + j]) : 0.f;
   }
-}
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) c[i] = zero_chunk();
+  }
+  __device__ __forceinline__ float get(int j) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(c[j / 4].w[j % 4]);
+    const uint32_t w = c[j / 8].w[j % 8 / 2];
+    return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
+  }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) m = max(m, mag_bits(get(j)));
+    return m;
+  }
+  // codes of elements 4 i .. 4 i + 3
+  __device__ __forceinline__ uint32_t codes(int i, float inv) const {
+    return code8(get(4 * i), inv) | code8(get(4 * i + 1), inv) << 8 | code8(get(4 * i + 2), inv) << 16 |
+           code8(get(4 * i + 3), inv) << 24;
+  }
+};
 
 __device__ __forceinline__ uint32_t wave_umax(uint32_t m) {
 #pragma unroll
@@ -76,50 +94,38 @@ constexpr int kQuantWaves = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(64 * kQuantWaves)
-quantize_rows_kernel(const T* x, int64_t x_sr, int M, int K, int Kp, bool wide, int8_t* q, float* scale) {
+quantize_rows_kernel(const T* x, int64_t x_sr, int M, int K, int Kp, int8_t* q, float* scale) {
   constexpr int NC = 4;
   const int lane = threadIdx.x & 63;
   const int m = blockIdx.x * kQuantWaves + (threadIdx.x >> 6);
   if (m >= M) return;
   const T* row = x + int64_t(m) * x_sr;
-  float v[NC][8];
+  RowPart<T, 8> v[NC];
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int k = (i * 64 + lane) * 8;
-    if (k < Kp) row_octet<T>(row, k, K, wide, v[i]);
-    else
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, mag_bits(v[i][j]));
+    if (k < Kp) v[i].load(row, k, K);
+    else v[i].zero();
   }
-  for (int k = (NC * 64 + lane) * 8; k < Kp; k += 512) {
-    float w[8];
-    row_octet<T>(row, k, K, wide, w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, mag_bits(w[j]));
+  for (int i = 0; i < NC; ++i) top = max(top, v[i].top());
+  for (int k = (NC * 64 + lane) * 8; k < Kp; k += 512) {
+    RowPart<T, 8> w;
+    w.load(row, k, K);
+    top = max(top, w.top());
   }
   const Scale8 s = scale8(wave_umax(top));
   int8_t* out = q + int64_t(m) * Kp;
-  auto put = [&](int k, const float (&w)[8]) {
-    uint2 c = make_uint2(0u, 0u);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      c.x |= code8(w[j], s.inv) << (8 * j);
-      c.y |= code8(w[4 + j], s.inv) << (8 * j);
-    }
-    *reinterpret_cast<uint2*>(out + k) = c;
-  };
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int k = (i * 64 + lane) * 8;
-    if (k < Kp) put(k, v[i]);
+    if (k < Kp) *reinterpret_cast<uint2*>(out + k) = make_uint2(v[i].codes(0, s.inv), v[i].codes(1, s.inv));
   }
   for (int k = (NC * 64 + lane) * 8; k < Kp; k += 512) {
-    float w[8];
-    row_octet<T>(row, k, K, wide, w);
-    put(k, w);
+    RowPart<T, 8> w;
+    w.load(row, k, K);
+    *reinterpret_cast<uint2*>(out + k) = make_uint2(w.codes(0, s.inv), w.codes(1, s.inv));
   }
   if (lane == 0) scale[m] = s.scale;
 }
@@ -144,32 +150,6 @@ struct Few8Params {
   const unsigned char* run;
   const float* g; float* xm;
   int M, N, K, Kp, heads;
-  int wide;
-};
-
-// sixteen elements of a row as they lie in memory, and as numbers
-template <typename T>
-struct Row16 {
-  static constexpr int EPC = 16 / int(sizeof(T)), NC = 16 / EPC;
-  Chunk c[NC];
-  __device__ __forceinline__ void load(const T* row, int k, int K, bool wide) {
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-      const int k0 = k + EPC * i;
-      if (wide && k0 + EPC <= K) {
-        c[i] = load_chunk(row + k0);
-      } else {
-        T* e = reinterpret_cast<T*>(&c[i]);
-#pragma unroll
-        for (int j = 0; j < EPC; ++j) e[j] = k0 + j < K ? row[k0 + j] : T(0);
-      }
-    }
-  }
-  __device__ __forceinline__ float get(int j) const {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(c[j / 4].w[j % 4]);
-    const uint32_t w = c[j / 8].w[j % 8 / 2];
-    return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
-  }
 };
 
 template <typename T, int KS>
@@ -189,10 +169,10 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
 #pragma unroll
   for (int s = 0; s < KS; ++s)
     if (s0 + s < s1) a[s] = load_chunk(wrow + 64 * (s0 + s));
-  Row16<T> x[KS];
+  RowPart<T, 16> x[KS];
 #pragma unroll
   for (int s = 0; s < KS; ++s)
-    if (s0 + s < s1) x[s].load(xrow, 64 * (s0 + s) + 16 * q, p.K, p.wide);
+    if (s0 + s < s1) x[s].load(xrow, 64 * (s0 + s) + 16 * q, p.K);
   float sw[4];  // of the channels that this lane stores (wave 0)
 #pragma unroll
   for (int i = 0; i < 4; ++i) sw[i] = p.sw[min(n0 + 4 * q + i, p.N - 1)];
@@ -215,9 +195,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
   uint32_t top = 0;
 #pragma unroll
   for (int s = 0; s < KS; ++s)
-    if (s0 + s < s1)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) top = max(top, mag_bits(x[s].get(j)));
+    if (s0 + s < s1) top = max(top, x[s].top());
   top = max(top, uint32_t(__shfl_xor(int(top), 16, 64)));
   top = max(top, uint32_t(__shfl_xor(int(top), 32, 64)));
   if (q == 0) tops[wave][r] = top;
@@ -232,9 +210,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
     if (s0 + s < s1) {
       Chunk b;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        b.w[j] = code8(x[s].get(4 * j), sc.inv) | code8(x[s].get(4 * j + 1), sc.inv) << 8 |
-                 code8(x[s].get(4 * j + 2), sc.inv) << 16 | code8(x[s].get(4 * j + 3), sc.inv) << 24;
+      for (int j = 0; j < 4; ++j) b.w[j] = x[s].codes(j, sc.inv);
       acc = mma8(a[s], b, acc);
     }
   }
@@ -276,7 +252,6 @@ struct Many8Params {
   void* y; int64_t y_sr;
   int M, N, Kp, ntok, nch;
   int gch;           // channel tiles of a group: the tiles of a group are a run, token tile by token tile
-  int wide;          // y's rows start on 16-byte boundaries
 };
 
 template <int FA, int FB, int WN, int WM, int RING_>
@@ -434,8 +409,8 @@ int8_many_kernel(const Many8Params p) {
       if (m >= p.M || n >= p.N) continue;
       T* yr = reinterpret_cast<T*>(p.y) + int64_t(m) * p.y_sr + n;
       const T* src = tile + row * S::OUTW + col;
-      if (p.wide && n + EPC <= p.N) {
-        store_stream(yr, load_chunk(src));
+      if (n + EPC <= p.N) {
+        store_stream_any(yr, load_chunk(src));
       } else {
         for (int e = 0; e < EPC && n + e < p.N; ++e) yr[e] = src[e];
       }
@@ -447,10 +422,9 @@ int8_many_kernel(const Many8Params p) {
 // ------------------------------------------------------------------------------------------------
 template <typename T>
 static void quantize(const void* x, int64_t x_sr, int M, int K, int8_t* q, float* scale, hipStream_t stream) {
-  const bool wide = reinterpret_cast<uintptr_t>(x) % 16 == 0 && (x_sr * int64_t(sizeof(T))) % 16 == 0;
   const dim3 grid(unsigned((int64_t(M) + kQuantWaves - 1) / kQuantWaves)), block(64 * kQuantWaves);
   hipLaunchKernelGGL(quantize_rows_kernel<T>, grid, block, 0, stream, reinterpret_cast<const T*>(x), x_sr, M, K,
-                     int(padded_k8(K)), wide, q, scale);
+                     int(padded_k8(K)), q, scale);
 }
 
 int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream) {
@@ -488,7 +462,6 @@ static void launch_few8(const mote_int8_linear_args* a, hipStream_t stream) {
   p.x = a->x; p.x_sr = a->x_sr; p.w = a->wq; p.sw = a->w_scale; p.y = a->y; p.y_sr = a->y_sr;
   p.run = a->run; p.g = a->xm ? a->g : nullptr; p.xm = a->xm; p.heads = a->xm ? a->heads : 0;
   p.M = a->M; p.N = a->N; p.K = a->K; p.Kp = int(padded_k8(a->K));
-  p.wide = reinterpret_cast<uintptr_t>(a->x) % 16 == 0 && (a->x_sr * int64_t(sizeof(T))) % 16 == 0;
   const int per = (p.Kp / 64 + kFewWaves - 1) / kFewWaves;
   const dim3 grid(unsigned((a->N + 15) / 16), unsigned((a->M + 15) / 16)), block(64 * kFewWaves);
   if (per <= 4) hipLaunchKernelGGL((int8_few_kernel<T, 4>), grid, block, 0, stream, p);
@@ -505,7 +478,6 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
   Many8Params p;
   p.x = xq; p.sx = sx; p.w = a->wq; p.sw = a->w_scale; p.y = a->y; p.y_sr = a->y_sr;
   p.M = a->M; p.N = a->N; p.Kp = Kp;
-  p.wide = reinterpret_cast<uintptr_t>(a->y) % 16 == 0 && (a->y_sr * int64_t(sizeof(T))) % 16 == 0;
   auto go = [&](auto kernel, int ch, int tok, int waves) {
     p.ntok = (a->M + tok - 1) / tok; p.nch = (a->N + ch - 1) / ch;
     // A weight that an XCD's 4 MB L2 holds stays there whatever the order; a larger one goes in groups of
