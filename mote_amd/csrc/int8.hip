@@ -252,6 +252,7 @@ struct Many8Params {
   void* y; int64_t y_sr;
   int M, N, Kp, ntok, nch;
   int gch;           // channel tiles of a group: the tiles of a group are a run, token tile by token tile
+  int stream;        // whether y passes the caches by
 };
 
 template <int FA, int FB, int WN, int WM, int RING_>
@@ -410,7 +411,14 @@ int8_many_kernel(const Many8Params p) {
       T* yr = reinterpret_cast<T*>(p.y) + int64_t(m) * p.y_sr + n;
       const T* src = tile + row * S::OUTW + col;
       if (n + EPC <= p.N) {
-        store_stream_any(yr, load_chunk(src));
+        if (p.stream) {
+          // between two of these, so that the compiler does not make one store of the two, without the hint
+          asm volatile("" ::: "memory");
+          store_stream_any(yr, load_chunk(src));
+          asm volatile("" ::: "memory");
+        } else {
+          store_any(yr, load_chunk(src));
+        }
       } else {
         for (int e = 0; e < EPC && n + e < p.N; ++e) yr[e] = src[e];
       }
@@ -478,6 +486,10 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
   Many8Params p;
   p.x = xq; p.sx = sx; p.w = a->wq; p.sw = a->w_scale; p.y = a->y; p.y_sr = a->y_sr;
   p.M = a->M; p.N = a->N; p.Kp = Kp;
+  // y passes the caches by, except where it is larger than the L2s and its rows share cache lines: those
+  // would go out in parts (30000 x 768 -> 1032 63 us, 57 through the L2s; 1056 channels 54 and 56 us)
+  const bool whole = reinterpret_cast<uintptr_t>(a->y) % 64 == 0 && (a->y_sr * int64_t(sizeof(T))) % 64 == 0;
+  p.stream = whole || double(a->M) * a->N * sizeof(T) < double(32 << 20);
   auto go = [&](auto kernel, int ch, int tok, int waves) {
     p.ntok = (a->M + tok - 1) / tok; p.nch = (a->N + ch - 1) / ch;
     // A weight that an XCD's 4 MB L2 holds stays there whatever the order; a larger one goes in groups of

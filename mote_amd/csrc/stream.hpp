@@ -21,6 +21,9 @@ typedef u32x4 __attribute__((aligned(2))) u32x4_any;
 __device__ __forceinline__ Chunk load_any(const void* p) {
   return __builtin_bit_cast(Chunk, static_cast<u32x4>(*reinterpret_cast<const u32x4_any*>(p)));
 }
+__device__ __forceinline__ void store_any(void* p, const Chunk& c) {
+  *reinterpret_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4, c);
+}
 __device__ __forceinline__ void store_stream_any(void* p, const Chunk& c) {
   __builtin_nontemporal_store(__builtin_bit_cast(u32x4, c), reinterpret_cast<u32x4_any*>(p));
 }
