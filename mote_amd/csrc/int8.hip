@@ -528,8 +528,8 @@ int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream) {
   const char* what = "int8_linear";
   if (!a) return set_error(MOTE_ERR_ARGUMENT, "%s: null args", what);
   if (a->dtype != MOTE_F32 && a->dtype != MOTE_BF16) return set_error(MOTE_ERR_ARGUMENT, "%s: bad dtype %d", what, a->dtype);
-  if (a->M < 0 || a->N <= 0 || a->K <= 0 || a->K > kMaxK8)
-    return set_error(MOTE_ERR_SHAPE, "%s: M = %d, N = %d, K = %d (K at most %d)", what, a->M, a->N, a->K, kMaxK8);
+  if (a->M < 0 || a->M > (1 << 30) || a->N <= 0 || a->N > (1 << 30) || a->K <= 0 || a->K > kMaxK8)
+    return set_error(MOTE_ERR_SHAPE, "%s: M = %d, N = %d (at most 2^30), K = %d (at most %d)", what, a->M, a->N, a->K, kMaxK8);
   if (((int64_t(a->M) + 127) / 128) * ((int64_t(a->N) + 127) / 128) >= (int64_t(1) << 30))
     return set_error(MOTE_ERR_SHAPE, "%s: too many tiles for one launch", what);
   if (a->M == 0) return MOTE_OK;

@@ -496,8 +496,9 @@ int launch_decode4(const mote_relation_decode4_args* a, hipStream_t stream) {
     return set_error(MOTE_ERR_ARGUMENT, "%s: null pointer", what);
   if (const char* bad = bad_cache4(a->cache)) return set_error(MOTE_ERR_ARGUMENT, "%s: %s", what, bad);
   const Dec4Ws w = ws4(a);
-  if (!a->workspace || a->workspace_bytes < w.total)
-    return set_error(MOTE_ERR_WORKSPACE, "%s: workspace of %zu bytes, %zu needed", what, a->workspace_bytes, w.total);
+  if (!a->workspace || a->workspace_bytes < w.total || reinterpret_cast<uintptr_t>(a->workspace) % 16)
+    return set_error(MOTE_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes, %zu needed", what, a->workspace_bytes,
+                     w.total);
   Dec4Params p;
   p.lam = a->lam; p.S = a->S;
   p.rope = a->inv_freq != nullptr;

@@ -414,6 +414,19 @@ void no_grad(const char* what, std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->requires_grad()) throw std::runtime_error(c10::str(what, " has no backward: call it under torch.no_grad()"));
 }
+// Refuses a result that lies over an operand: it would be written while another workgroup still reads there.
+// Both are rows of `width` elements back to back within, `stride` apart; columns of one buffer (the same stride,
+// the columns apart) pass.
+void apart(const Tensor& out, int64_t out_width, const Tensor& in, int64_t in_width, int64_t rows, const char* what) {
+  const int64_t e = out.element_size(), so = rows > 1 ? out.stride(0) : 0, si = rows > 1 ? in.stride(0) : 0;
+  const int64_t o = reinterpret_cast<int64_t>(out.data_ptr()) / e, i = reinterpret_cast<int64_t>(in.data_ptr()) / e;
+  if (rows == 0 || o >= i + (rows - 1) * si + in_width || i >= o + (rows - 1) * so + out_width) return;
+  if (rows > 1 && so == si) {
+    const int64_t d = ((o - i) % so + so) % so;
+    if (d >= in_width && d + out_width <= so) return;
+  }
+  bad_value(what, ": the output lies over an input");
+}
 // an int64 position per sequence (read, and with `advance` written, by the kernel as it is)
 void positions(const Tensor& t, int64_t B, c10::Device dev, const char* what, const char* name) {
   if (t.scalar_type() != at::kLong || t.device() != dev || t.numel() != B || !t.is_contiguous())
@@ -442,6 +455,8 @@ Cache4 cache4(const Tensor& p2, const Tensor& s2, const Tensor& info, const Tens
       if (writes && t.size(d) > 1 && t.stride(d) == 0) bad_value(what, ": ", name, " holds its rows for several heads at once");
     }
   };
+  if (writes && (p2.data_ptr() == info.data_ptr() || s2.data_ptr() == si.data_ptr()))
+    bad_value(what, ": P2 and I~ must not be the same rows");
   check(p2, p2, 16 * G, at::kByte, "the codes of P2");
   check(info, p2, 16 * G, at::kByte, "the codes of I~");
   check(s2, s2, G, at::kBFloat16, "the scales of P2");
@@ -573,6 +588,8 @@ std::tuple<Tensor, Tensor> relation_decode4(const Tensor& p1, const Tensor& p2, 
   if (g_ && (g_->dim() != 2 || g_->size(0) != B || g_->size(1) != H || g_->scalar_type() != at::kFloat || g_->device() != dev ||
              !g_->is_contiguous()))
     bad_value(what, ": g must be a contiguous fp32 [B, H] tensor");
+  if (y_)
+    for (const Tensor* t : {&p1, &p2, &info}) apart(*y_, H * D, *t, H * D, B, what);
   no_grad(what, {&p1, &p2, &info});
   on_gpu(p1, what);
   const On on(p1);
@@ -643,13 +660,18 @@ Tensor int8_linear(const Tensor& x_, const Tensor& wq, const Tensor& ws, int64_t
              g->dim() != 2 || g->size(0) != M || xm->numel() != M || g->device() != x_.device() || xm->device() != x_.device()))
     bad_value(what, ": xm needs fp32 contiguous g [M, H] and xm [M] on x's device");
   no_grad(what, {&x_});
-  on_gpu(x_, what);
-  const On on(x_);
   TORCH_CHECK(M <= INT_MAX && N <= INT_MAX && K <= INT_MAX, "int8_linear: sizes beyond 32 bits");
   const Tensor x = unit(x_.dim() == 2 ? x_ : x_.reshape({M, K}));
-  Tensor y = out ? *out : empty(sizes, x_, x_.scalar_type());
-  const Tensor y2 = y.dim() == 2 ? y : y.view({M, N});  // an output that is no [M, N] in memory is refused
-  if (M > 1 && y2.stride(0) < N) bad_value(what, ": the rows of out overlap");
+  Tensor y2;
+  if (out) {
+    y2 = out->dim() == 2 ? *out : out->view({M, N});  // an output that is no [M, N] in memory is refused
+    if (M > 1 && y2.stride(0) < N) bad_value(what, ": the rows of out overlap");
+    apart(y2, N, x, K, M, what);
+  }
+  on_gpu(x_, what);
+  const On on(x_);
+  const Tensor y = out ? *out : empty(sizes, x_, x_.scalar_type());
+  if (!out) y2 = y.dim() == 2 ? y : y.view({M, N});
   a.M = int(M); a.N = int(N); a.K = int(K);
   a.x = x.data_ptr(); a.x_sr = x.stride(0);
   a.wq = static_cast<const int8_t*>(wq.data_ptr()); a.w_scale = fptr(ws);

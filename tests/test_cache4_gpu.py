@@ -369,6 +369,9 @@ def test_another_stream_and_strided_stores(cuda):
         got = relation_decode4(xd[:, 0], xd[:, 1], xd[:, 2], Sd, view, lamd)
     torch.cuda.current_stream().wait_stream(side)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    four = torch.cat([xd, xd[:, :1]], 1)  # y in the rows of the projections' own buffer
+    relation_decode4(four[:, 0], four[:, 1], four[:, 2], Sd, cache, lamd, y=four[:, 3])
+    assert torch.equal(four[:, 3], want[0]) and torch.equal(four[:, :3], xd)
     for s, t in zip(store, cache):
         assert torch.equal(s[:, 1], t) and (s[:, 0] == 0).all() and (s[:, 2] == 0).all()
 

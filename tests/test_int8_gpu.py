@@ -120,6 +120,9 @@ def test_leading_dims_strides_outputs_and_empty(cuda):
         got = int8_linear(xd.reshape(-1, 100), w8, out=out[:, 7:47])
         assert got.data_ptr() == out[:, 7:].data_ptr() and torch.equal(out[:, 7:47], y.reshape(-1, 40))
         assert (out[:, :7] == 9).all() and (out[:, 47:] == 9).all()
+        both = torch.cat([xd.reshape(-1, 100), out[:, :40]], 1)  # the result in other columns of x's own rows
+        int8_linear(both[:, :100], w8, out=both[:, 100:])
+        assert torch.equal(both[:, 100:], y.reshape(-1, 40)) and torch.equal(both[:, :100], xd.reshape(-1, 100))
     assert int8_linear(torch.empty(0, 100, device=cuda, dtype=BF16), w8).shape == (0, 40)
     assert int8_linear(xd[0, 0], w8).shape == (40,)
 

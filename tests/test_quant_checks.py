@@ -78,6 +78,8 @@ def test_cache_layouts_that_are_refused():
     one = [t[:, :1].expand(t.shape) for t in c]
     with pytest.raises(ValueError, match="several heads"):
         cache4_write(Cache4(*one), k, v)
+    with pytest.raises(ValueError, match="same rows"):
+        cache4_write(c._replace(info=c.p2), k, v)
     with pytest.raises(RuntimeError, match="MI355X"):
         cache4_read(Cache4(*one), 48)  # reading shared rows is fine: only the device is missing
 
@@ -134,6 +136,9 @@ def test_decode4_refuses():
     for name, value in bad.items():
         with pytest.raises(ValueError, match=name):
             relation_decode4(x, x, x, S, c, lam, **{name: value})
+    qkv = torch.zeros(2, 3, 4, 48, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="lies over an input"):
+        relation_decode4(qkv[:, 0], qkv[:, 1], qkv[:, 2], S, c, lam, y=qkv[:, 2])
     with pytest.raises(ValueError, match="lam"):
         relation_decode4(x, x, x, S, c, torch.zeros(2))
     with pytest.raises(RuntimeError, match="no backward"):
@@ -159,6 +164,11 @@ def test_int8_refuses():
         int8_linear(x, w._replace(q=w.q.to(torch.uint8)))
     with pytest.raises(ValueError, match="out must be"):
         int8_linear(x, w, out=torch.zeros(4, 17, dtype=torch.bfloat16))
+    square = Int8Weight(torch.zeros(100, 128, dtype=torch.int8), torch.zeros(100), 100)
+    wide = torch.zeros(4, 150, dtype=torch.bfloat16)
+    for inp, out in ((x, x), (wide[:, :100], wide[:, 50:])):
+        with pytest.raises(ValueError, match="lies over an input"):
+            int8_linear(inp, square, out=out)
     with pytest.raises(ValueError, match="run"):
         int8_linear(x, w, run=torch.zeros(1))
     with pytest.raises(ValueError, match="xm"):
@@ -205,11 +215,15 @@ def test_c_entry_points_refuse_without_a_gpu():
     assert need > 0
     a.workspace, a.workspace_bytes = 16, need - 1
     assert lib.mote_relation_decode4(a, None) == 3
+    a.workspace, a.workspace_bytes = 24, need  # off a 16-byte boundary
+    assert lib.mote_relation_decode4(a, None) == 3
     w = L.Int8LinearArgs()
     assert lib.mote_int8_linear(None, None) == 1 and lib.mote_quantize_rows(None, None) == 1
     w.dtype, w.M, w.N, w.K = L.MOTE_BF16, 4, 16, 200000
     assert lib.mote_int8_linear(w, None) == 2
-    w.K, w.M = 128, 0
+    w.K, w.M = 128, (1 << 30) + 1
+    assert lib.mote_int8_linear(w, None) == 2
+    w.M = 0
     assert lib.mote_int8_linear(w, None) == 0
     w.M = 65
     assert lib.mote_int8_linear(w, None) == 1
