@@ -14,6 +14,7 @@
 namespace mote {
 
 typedef __attribute__((ext_vector_type(4))) int i32x4;
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2;
 
 constexpr float kSmall8 = 0x1p-120f;  // a row whose maximum is below stores zeros (127 / max would overflow)
 constexpr int kMaxK8 = 131072;        // sums stay below 2^31: K 127^2
@@ -36,9 +37,17 @@ __device__ __forceinline__ Scale8 scale8(uint32_t top) {
   s.scale = live ? a / 127.0f : finite ? 0.f : __builtin_nanf("");
   return s;
 }
-// the code of x, as a byte (inv 0: a row without a scale, whose infinities and NaNs must not come through)
-__device__ __forceinline__ uint32_t code8(float x, float inv) {
-  return inv == 0.f ? 0u : uint32_t(int(rintf(x * inv))) & 0xffu;
+// Four codes in a word. rint(fl(x inv)) through the 1.5 * 2^23 that leaves no fraction bits in a float: after the
+// addition (ties to even, as rint) the integer's two's complement is in the low bits, and v_perm takes its byte:
+// under three instructions a value. A row without a scale (inv 0) may hold infinities and NaNs, whose codes
+// are noise: its scale is NaN then, so every product with it is too, and quantize_rows stores zeros instead.
+__device__ __forceinline__ uint32_t codes8(float a, float b, float c, float d, float inv) {
+#pragma clang fp contract(off)
+  constexpr float kMagic = 12582912.0f;
+  const uint32_t ua = __float_as_uint(a * inv + kMagic), ub = __float_as_uint(b * inv + kMagic);
+  const uint32_t uc = __float_as_uint(c * inv + kMagic), ud = __float_as_uint(d * inv + kMagic);
+  const uint32_t lo = __builtin_amdgcn_perm(ub, ua, 0x0c0c0400u), hi = __builtin_amdgcn_perm(ud, uc, 0x0c0c0400u);
+  return lo | hi << 16;
 }
 
 // N elements of a row of K from k on, as they lie in memory (zeros past its end), and as numbers
@@ -68,7 +77,17 @@ struct RowPart {
     const uint32_t w = c[j / 8].w[j % 8 / 2];
     return __uint_as_float(j & 1 ? w & 0xffff0000u : w << 16);
   }
+  // the bits of the largest magnitude
   __device__ __forceinline__ uint32_t top() const {
+    if constexpr (sizeof(T) == 2) {
+      u16x2 m = u16x2{0, 0};
+#pragma unroll
+      for (int i = 0; i < NC; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, c[i].w[j] & 0x7fff7fffu));
+      return uint32_t(max(m.x, m.y)) << 16;
+    }
     uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < N; ++j) m = max(m, mag_bits(get(j)));
@@ -76,8 +95,7 @@ struct RowPart {
   }
   // codes of elements 4 i .. 4 i + 3
   __device__ __forceinline__ uint32_t codes(int i, float inv) const {
-    return code8(get(4 * i), inv) | code8(get(4 * i + 1), inv) << 8 | code8(get(4 * i + 2), inv) << 16 |
-           code8(get(4 * i + 3), inv) << 24;
+    return codes8(get(4 * i), get(4 * i + 1), get(4 * i + 2), get(4 * i + 3), inv);
   }
 };
 
@@ -116,16 +134,17 @@ quantize_rows_kernel(const T* x, int64_t x_sr, int M, int K, int Kp, int8_t* q, 
     top = max(top, w.top());
   }
   const Scale8 s = scale8(wave_umax(top));
+  const uint32_t keep = s.inv == 0.f ? 0u : ~0u;  // a row without a scale stores zeros
   int8_t* out = q + int64_t(m) * Kp;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int k = (i * 64 + lane) * 8;
-    if (k < Kp) *reinterpret_cast<uint2*>(out + k) = make_uint2(v[i].codes(0, s.inv), v[i].codes(1, s.inv));
+    if (k < Kp) *reinterpret_cast<uint2*>(out + k) = make_uint2(v[i].codes(0, s.inv) & keep, v[i].codes(1, s.inv) & keep);
   }
   for (int k = (NC * 64 + lane) * 8; k < Kp; k += 512) {
     RowPart<T, 8> w;
     w.load(row, k, K);
-    *reinterpret_cast<uint2*>(out + k) = make_uint2(w.codes(0, s.inv), w.codes(1, s.inv));
+    *reinterpret_cast<uint2*>(out + k) = make_uint2(w.codes(0, s.inv) & keep, w.codes(1, s.inv) & keep);
   }
   if (lane == 0) scale[m] = s.scale;
 }
