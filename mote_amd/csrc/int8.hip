@@ -68,6 +68,10 @@ struct RowPart {
       }
     }
   }
+  __device__ __forceinline__ void load_whole(const T* row, int k) {
+#pragma unroll
+    for (int i = 0; i < NC; ++i) c[i] = load_any(row + k + EPC * i);
+  }
   __device__ __forceinline__ void zero() {
 #pragma unroll
     for (int i = 0; i < NC; ++i) c[i] = zero_chunk();
@@ -99,10 +103,20 @@ struct RowPart {
   }
 };
 
+// the maximum over the lanes li, li + 16, li + 32, li + 48 (row swaps, no LDS), and over the wave
+__device__ __forceinline__ uint32_t lanegroup_umax(uint32_t m) {
+  u32x2 a = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+  m = max(a[0], a[1]);
+  a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+  return max(a[0], a[1]);
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_umax(uint32_t m) {
+  return max(m, uint32_t(__builtin_amdgcn_mov_dpp(int(m), CTRL, 0xF, 0xF, false)));
+}
 __device__ __forceinline__ uint32_t wave_umax(uint32_t m) {
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) m = max(m, uint32_t(__shfl_xor(int(m), o, 64)));
-  return m;
+  m = dpp_umax<kDppNext4>(dpp_umax<kDppRor8>(lanegroup_umax(m)));
+  return dpp_umax<kDppXor1>(dpp_umax<kDppXor2>(m));
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -123,7 +137,8 @@ quantize_rows_kernel(const T* x, int64_t x_sr, int M, int K, int Kp, int8_t* q, 
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
     const int k = (i * 64 + lane) * 8;
-    if (k < Kp) v[i].load(row, k, K);
+    if ((i + 1) * 512 <= K) v[i].load_whole(row, k);  // the whole wave's
+    else if (k < Kp) v[i].load(row, k, K);
     else v[i].zero();
   }
 #pragma unroll
@@ -176,7 +191,8 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
   using E = Elem<T>;
   __shared__ uint32_t tops[kFewWaves][16];
   __shared__ __align__(16) int part[kFewWaves][16][17];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the steps' conditions are the wave's
   const int r = lane & 15, q = lane >> 4;
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
   const int nks = p.Kp / 64;                                 // k steps, an even number
@@ -190,8 +206,10 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
     if (s0 + s < s1) a[s] = load_chunk(wrow + 64 * (s0 + s));
   RowPart<T, 16> x[KS];
 #pragma unroll
-  for (int s = 0; s < KS; ++s)
-    if (s0 + s < s1) x[s].load(xrow, 64 * (s0 + s) + 16 * q, p.K);
+  for (int s = 0; s < KS; ++s) {
+    if (64 * (s0 + s) + 64 <= min(p.K, 64 * s1)) x[s].load_whole(xrow, 64 * (s0 + s) + 16 * q);
+    else if (s0 + s < s1) x[s].load(xrow, 64 * (s0 + s) + 16 * q, p.K);
+  }
   float sw[4];  // of the channels that this lane stores (wave 0)
 #pragma unroll
   for (int i = 0; i < 4; ++i) sw[i] = p.sw[min(n0 + 4 * q + i, p.N - 1)];
@@ -215,8 +233,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
 #pragma unroll
   for (int s = 0; s < KS; ++s)
     if (s0 + s < s1) top = max(top, x[s].top());
-  top = max(top, uint32_t(__shfl_xor(int(top), 16, 64)));
-  top = max(top, uint32_t(__shfl_xor(int(top), 32, 64)));
+  top = lanegroup_umax(top);
   if (q == 0) tops[wave][r] = top;
   __syncthreads();
   top = tops[0][r];
