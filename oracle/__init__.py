@@ -15,6 +15,9 @@ noahsabaj/mote source tree):
 * `brute.py` — float64 scalar loops over (b, h, i, j) for tiny shapes, the independent pin for
   the materialized form.
 
+* `quant.py` — the 4-bit and 8-bit formats of the quantised decode path, bit for bit (no counterpart in
+  the reference).
+
 How each function is pinned (closed forms, invariants, brute force, finite differences, planted
 mistakes) is listed in the header of `relation.py`; none of them is "parity unpinned".
 """
