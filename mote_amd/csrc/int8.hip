@@ -103,7 +103,7 @@ struct RowPart {
   }
 };
 
-// the maximum over the lanes li, li + 16, li + 32, li + 48 (row swaps, no LDS), and over the wave
+// the maximum over the lanes li, li + 16, li + 32, li + 48 (row swaps, no LDS)
 __device__ __forceinline__ uint32_t lanegroup_umax(uint32_t m) {
   u32x2 a = __builtin_amdgcn_permlane32_swap(m, m, false, false);
   m = max(a[0], a[1]);
@@ -114,53 +114,62 @@ template <int CTRL>
 __device__ __forceinline__ uint32_t dpp_umax(uint32_t m) {
   return max(m, uint32_t(__builtin_amdgcn_mov_dpp(int(m), CTRL, 0xF, 0xF, false)));
 }
-__device__ __forceinline__ uint32_t wave_umax(uint32_t m) {
-  m = dpp_umax<kDppNext4>(dpp_umax<kDppRor8>(lanegroup_umax(m)));
+// the maximum over the G lanes of a row
+template <int G>
+__device__ __forceinline__ uint32_t group_umax(uint32_t m) {
+  if constexpr (G == 64) {
+    m = lanegroup_umax(m);
+  } else if constexpr (G == 32) {
+    const u32x2 a = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+    m = max(a[0], a[1]);
+  }
+  m = dpp_umax<kDppNext4>(dpp_umax<kDppRor8>(m));
   return dpp_umax<kDppXor1>(dpp_umax<kDppXor2>(m));
 }
 
 // ------------------------------------------------------------------------------------------------
-// Rows in 8 bits: a wave per row, the row in registers up to 64 * 8 * NC values (beyond, read twice)
+// Rows in 8 bits: G lanes per row, the row in registers up to 8 G NC values (beyond, read twice)
 // ------------------------------------------------------------------------------------------------
 constexpr int kQuantWaves = 4;
 
-template <typename T>
+template <typename T, int G, int NC>
 __global__ void __launch_bounds__(64 * kQuantWaves)
 quantize_rows_kernel(const T* x, int64_t x_sr, int M, int K, int Kp, int8_t* q, float* scale) {
-  constexpr int NC = 4;
-  const int lane = threadIdx.x & 63;
-  const int m = blockIdx.x * kQuantWaves + (threadIdx.x >> 6);
-  if (m >= M) return;
+  const int lane = threadIdx.x % G;
+  const int m = blockIdx.x * (64 / G * kQuantWaves) + threadIdx.x / G;
+  if (m >= M) return;  // whole groups
   const T* row = x + int64_t(m) * x_sr;
   RowPart<T, 8> v[NC];
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    const int k = (i * 64 + lane) * 8;
-    if ((i + 1) * 512 <= K) v[i].load_whole(row, k);  // the whole wave's
+    const int k = (i * G + lane) * 8;
+    if ((i + 1) * G * 8 <= K) v[i].load_whole(row, k);  // every lane's
     else if (k < Kp) v[i].load(row, k, K);
     else v[i].zero();
   }
 #pragma unroll
   for (int i = 0; i < NC; ++i) top = max(top, v[i].top());
-  for (int k = (NC * 64 + lane) * 8; k < Kp; k += 512) {
-    RowPart<T, 8> w;
-    w.load(row, k, K);
-    top = max(top, w.top());
-  }
-  const Scale8 s = scale8(wave_umax(top));
+  if constexpr (G == 64)
+    for (int k = (NC * 64 + lane) * 8; k < Kp; k += 512) {
+      RowPart<T, 8> w;
+      w.load(row, k, K);
+      top = max(top, w.top());
+    }
+  const Scale8 s = scale8(group_umax<G>(top));
   const uint32_t keep = s.inv == 0.f ? 0u : ~0u;  // a row without a scale stores zeros
   int8_t* out = q + int64_t(m) * Kp;
 #pragma unroll
   for (int i = 0; i < NC; ++i) {
-    const int k = (i * 64 + lane) * 8;
+    const int k = (i * G + lane) * 8;
     if (k < Kp) *reinterpret_cast<uint2*>(out + k) = make_uint2(v[i].codes(0, s.inv) & keep, v[i].codes(1, s.inv) & keep);
   }
-  for (int k = (NC * 64 + lane) * 8; k < Kp; k += 512) {
-    RowPart<T, 8> w;
-    w.load(row, k, K);
-    *reinterpret_cast<uint2*>(out + k) = make_uint2(w.codes(0, s.inv) & keep, w.codes(1, s.inv) & keep);
-  }
+  if constexpr (G == 64)
+    for (int k = (NC * 64 + lane) * 8; k < Kp; k += 512) {
+      RowPart<T, 8> w;
+      w.load(row, k, K);
+      *reinterpret_cast<uint2*>(out + k) = make_uint2(w.codes(0, s.inv) & keep, w.codes(1, s.inv) & keep);
+    }
   if (lane == 0) scale[m] = s.scale;
 }
 
@@ -466,9 +475,23 @@ int8_many_kernel(const Many8Params p) {
 // ------------------------------------------------------------------------------------------------
 template <typename T>
 static void quantize(const void* x, int64_t x_sr, int M, int K, int8_t* q, float* scale, hipStream_t stream) {
-  const dim3 grid(unsigned((int64_t(M) + kQuantWaves - 1) / kQuantWaves)), block(64 * kQuantWaves);
-  hipLaunchKernelGGL(quantize_rows_kernel<T>, grid, block, 0, stream, reinterpret_cast<const T*>(x), x_sr, M, K,
-                     int(padded_k8(K)), q, scale);
+  const int Kp = int(padded_k8(K));
+  auto go = [&](auto kernel, int lanes) {
+    const int rows = 64 / lanes * kQuantWaves;
+    hipLaunchKernelGGL(kernel, dim3(unsigned((int64_t(M) + rows - 1) / rows)), dim3(64 * kQuantWaves), 0, stream,
+                       reinterpret_cast<const T*>(x), x_sr, M, K, Kp, q, scale);
+  };
+  // A row's share of a wave is as wide as the row needs, so that no lane idles and a row stays in registers:
+  // 35304 x 64 11.2 -> 4.7 us and 16384 x 768 9.7 -> 8.1 us against a wave per row; 19417 x 3776 48 -> 37.6 us
+  // against half of the row read twice. 65536 x 1024 takes 32.3 us either way.
+  if (Kp <= 128) return go(quantize_rows_kernel<T, 16, 1>, 16);
+  if (Kp <= 256) return go(quantize_rows_kernel<T, 16, 2>, 16);
+  if (Kp <= 384) return go(quantize_rows_kernel<T, 16, 3>, 16);
+  if (Kp <= 512) return go(quantize_rows_kernel<T, 32, 2>, 32);
+  if (Kp <= 768) return go(quantize_rows_kernel<T, 32, 3>, 32);
+  if (Kp <= 1024) return go(quantize_rows_kernel<T, 32, 4>, 32);
+  if (Kp <= 2048) return go(quantize_rows_kernel<T, 64, 4>, 64);
+  return go(quantize_rows_kernel<T, 64, 8>, 64);
 }
 
 int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream) {
@@ -485,14 +508,15 @@ int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream) {
   return check_launch(what);
 }
 
-// The one-launch form: for up to 16 tokens (16 x 768 -> 768 4.9 us, 7.2 with quantize_rows and tiles; 16 x
-// 4096 -> 4096 13.0 and 13.4), and up to 64 while the workgroups that quantise a token again are few (64 x 1024
-// -> 1024, 256 of them, 5.5 and 7.6 us; 64 x 768 -> 2304, 576, 7.2 and 7.3; 64 x 4096 -> 4096, 1024, 29 and 13);
-// the predicate and the exchange mass have it to themselves.
+// The one-launch form: for up to 16 tokens (16 x 768 -> 768 4.8 us, 6.4 with quantize_rows and tiles; 16 x
+// 4096 -> 4096 11.2 and 11.4), and up to 64 while the workgroups that quantise a token again are few: two a CU
+// of K up to 1024 (64 x 1024 -> 1536, 384 of them, 6.4 and 6.8 us; 64 x 768 -> 2304, 576, 6.5 and 6.5), one up to
+// 2048 (32 x 2048 -> 2048, 256, 7.0 and 7.7; 48 x 1536 -> 1536, 288, 8.1 and 7.2), none beyond (32 x 4096 -> 1024
+// 10.8 and 9.8); the predicate and the exchange mass have it to themselves.
 static bool few8(const mote_int8_linear_args* a) {
   if (a->M > kFewRows || a->K > kFewMaxK) return false;
   const int64_t groups = (int64_t(a->M) + 15) / 16 * ((int64_t(a->N) + 15) / 16);
-  return a->M <= 16 || a->run || a->xm || groups * std::max(a->K, 1024) <= int64_t(2048) * device_cu_count();
+  return a->M <= 16 || a->run || a->xm || groups <= int64_t(a->K <= 1024 ? 2 : a->K <= 2048 ? 1 : 0) * device_cu_count();
 }
 
 size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a) {
@@ -537,10 +561,14 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * waves), 0, stream, p);
   };
   // Tiles of channels x tokens. One round of workgroups of a small tile while that holds everything (a CU
-  // holds three of either): 64 x 32 with a deep ring (17 x 768 -> 2304 7.3 us, 10.2 with 128 x 128; 512 rows
-  // 8.9 and 11.4), then 128 x 64 (2048 x 768 -> 2304 13.6 us, 14.9 with 128 x 128, 18.9 with 64 x 32).
+  // holds three of the small ones). Transfers into LDS reach some 47 bytes a nanosecond per CU whatever the
+  // ring's depth, so few tiles go to as many CUs as there are: 32 x 16 (258 x 3413 -> 523 10.6 us, 11.9 with
+  // 64 x 32; 128 x 768 -> 768 6.4 and 6.8; with two CUs' worth of 32 x 16 exceeded, 1000 x 520 -> 271 7.5 and
+  // 7.2); then 64 x 32 with a deep ring (512 x 768 -> 2304 8.5 us, 11.1 with 128 x 128),
+  // then 128 x 64 (2048 rows 13.1 us, 14.6 and 16.9 with 64 x 32).
   const int64_t cus = device_cu_count();
   auto tiles = [&](int ch, int tok) { return ((int64_t(a->M) + tok - 1) / tok) * ((a->N + ch - 1) / ch); };
+  if (tiles(32, 16) <= 2 * cus) return go(int8_many_kernel<T, 1, 1, 2, 1, 4>, 32, 16, 2);
   if (tiles(64, 32) <= 3 * cus) return go(int8_many_kernel<T, 2, 1, 2, 2, 4>, 64, 32, 4);
   if (tiles(128, 64) <= 3 * cus) return go(int8_many_kernel<T, 4, 2, 2, 2, 2>, 128, 64, 4);
   // Beyond, the tile whose rounds take least: a round of n stages of k takes fixed + n * stage us (fitted to

@@ -29,7 +29,8 @@ def _check(y, x, w):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("M,K", [(1, 1), (3, 127), (5, 128), (2, 129), (4, 768), (7, 2049), (1, 5000), (9, 4095)])
+@pytest.mark.parametrize("M,K", [(1, 1), (3, 127), (5, 128), (2, 129), (4, 768), (7, 2049), (1, 5000), (9, 4095), (21, 96),
+                                 (37, 200), (35, 384), (19, 385), (10, 640), (11, 1000), (6, 4097)])
 def test_quantize_rows_bit_for_bit(cuda, dtype, M, K):
     from mote_amd.int8 import quantize_rows
 
@@ -65,7 +66,7 @@ def test_quantize_rows_special_rows_and_strides(cuda):
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("M,K,N", [(1, 768, 2304), (16, 768, 768), (5, 64, 1), (16, 4096, 48), (33, 4000, 300), (64, 768, 130), (50, 700, 40), (3, 1000, 17), (2, 1, 5),
                                    (9, 2050, 271), (17, 128, 16), (64, 520, 271), (130, 768, 300), (257, 129, 129),
-                                   (300, 1024, 128), (1, 5000, 40), (1000, 96, 64), (128, 4224, 256)])
+                                   (300, 1024, 128), (1, 5000, 40), (1000, 96, 64), (128, 4224, 256), (520, 200, 1031)])
 def test_linear_is_one_rounding_from_exact(cuda, dtype, M, K, N):
     from mote_amd.int8 import int8_linear, int8_weight
 
