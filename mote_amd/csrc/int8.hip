@@ -174,14 +174,13 @@ quantize_rows_kernel(const T* x, int64_t x_sr, int M, int K, int Kp, int8_t* q, 
 }
 
 // ------------------------------------------------------------------------------------------------
-// Few tokens: x is quantised where it is multiplied. One workgroup (4 waves) per 16 channels and 16 tokens,
+// Few tokens: x is quantised where it is multiplied. One workgroup of NW waves per 16 channels and 16 tokens,
 // the 64-wide k steps dealt to the waves in runs; a wave issues every load of its W rows and of its part of
-// x, agrees on the rows' maxima with the other waves through LDS, and multiplies. The four partial sums are
+// x, agrees on the rows' maxima with the other waves through LDS, and multiplies. The partial sums are
 // integers: their order does not matter. Every workgroup of a token tile quantises it again (24 KB at 768
 // from the L2), which costs less than a launch of its own. A launch of this size is bound by its latencies:
 // 4.4 us at 1 x 768 -> 768, 4.5 us at 1 x 768 -> 2304, whose W of 1.8 MB takes 0.4.
 // ------------------------------------------------------------------------------------------------
-constexpr int kFewWaves = 4;
 constexpr int kFewRows = 64;
 constexpr int kFewMaxK = 4096;
 
@@ -195,17 +194,17 @@ struct Few8Params {
   int M, N, K, Kp, heads;
 };
 
-template <typename T, int KS>
-__global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Params p) {
+template <typename T, int NW, int KS>
+__global__ void __launch_bounds__(64 * NW) int8_few_kernel(const Few8Params p) {
   using E = Elem<T>;
-  __shared__ uint32_t tops[kFewWaves][16];
-  __shared__ __align__(16) int part[kFewWaves][16][17];
+  __shared__ uint32_t tops[NW][16];
+  __shared__ __align__(16) int part[NW][16][17];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // the steps' conditions are the wave's
   const int r = lane & 15, q = lane >> 4;
   const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
   const int nks = p.Kp / 64;                                 // k steps, an even number
-  const int per = (nks + kFewWaves - 1) / kFewWaves;         // <= KS
+  const int per = (nks + NW - 1) / NW;                       // <= KS
   const int s0 = min(wave * per, nks), s1 = min(s0 + per, nks);
   const int8_t* wrow = p.w + int64_t(min(n0 + r, p.N - 1)) * p.Kp + 16 * q;
   const T* xrow = reinterpret_cast<const T*>(p.x) + int64_t(min(m0 + r, p.M - 1)) * p.x_sr;
@@ -247,7 +246,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
   __syncthreads();
   top = tops[0][r];
 #pragma unroll
-  for (int w = 1; w < kFewWaves; ++w) top = max(top, tops[w][r]);
+  for (int w = 1; w < NW; ++w) top = max(top, tops[w][r]);
   const Scale8 sc = scale8(top);
   i32x4 acc = i32x4{0, 0, 0, 0};
 #pragma unroll
@@ -269,7 +268,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) int8_few_kernel(const Few8Para
       const int f = 4 * q + i;
       int v = part[0][f][r];
 #pragma unroll
-      for (int w = 1; w < kFewWaves; ++w) v += part[w][f][r];
+      for (int w = 1; w < NW; ++w) v += part[w][f][r];
       if (n0 + f < p.N)
         reinterpret_cast<T*>(p.y)[int64_t(m0 + r) * p.y_sr + n0 + f] = E::from_f(float(v) * sc.scale * sw[i]);
     }
@@ -509,7 +508,7 @@ int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream) {
 }
 
 // The one-launch form: for up to 16 tokens (16 x 768 -> 768 4.8 us, 6.4 with quantize_rows and tiles; 16 x
-// 4096 -> 4096 11.2 and 11.4), and up to 64 while the workgroups that quantise a token again are few: two a CU
+// 4096 -> 4096 10.4 and 11.4), and up to 64 while the workgroups that quantise a token again are few: two a CU
 // of K up to 1024 (64 x 1024 -> 1536, 384 of them, 6.4 and 6.8 us; 64 x 768 -> 2304, 576, 6.5 and 6.5), one up to
 // 2048 (32 x 2048 -> 2048, 256, 7.0 and 7.7; 48 x 1536 -> 1536, 288, 8.1 and 7.2), none beyond (32 x 4096 -> 1024
 // 10.8 and 9.8); the predicate and the exchange mass have it to themselves.
@@ -530,11 +529,15 @@ static void launch_few8(const mote_int8_linear_args* a, hipStream_t stream) {
   p.x = a->x; p.x_sr = a->x_sr; p.w = a->wq; p.sw = a->w_scale; p.y = a->y; p.y_sr = a->y_sr;
   p.run = a->run; p.g = a->xm ? a->g : nullptr; p.xm = a->xm; p.heads = a->xm ? a->heads : 0;
   p.M = a->M; p.N = a->N; p.K = a->K; p.Kp = int(padded_k8(a->K));
-  const int per = (p.Kp / 64 + kFewWaves - 1) / kFewWaves;
-  const dim3 grid(unsigned((a->N + 15) / 16), unsigned((a->M + 15) / 16)), block(64 * kFewWaves);
-  if (per <= 4) hipLaunchKernelGGL((int8_few_kernel<T, 4>), grid, block, 0, stream, p);
-  else if (per <= 8) hipLaunchKernelGGL((int8_few_kernel<T, 8>), grid, block, 0, stream, p);
-  else hipLaunchKernelGGL((int8_few_kernel<T, 16>), grid, block, 0, stream, p);
+  auto go = [&](auto kernel, int waves) {
+    const dim3 grid(unsigned((a->N + 15) / 16), unsigned((a->M + 15) / 16));
+    hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, stream, p);
+  };
+  // Beyond K = 1024 eight waves (16 x 4096 -> 4096 11.4 -> 10.4 us, 1 x 2048 -> 2048 5.5 -> 5.2), four up to there
+  // (16 x 768 -> 2304 4.7 us, 4.9 with eight).
+  if (p.Kp <= 1024) go(int8_few_kernel<T, 4, 4>, 4);
+  else if (p.Kp <= 2048) go(int8_few_kernel<T, 8, 4>, 8);
+  else go(int8_few_kernel<T, 8, 8>, 8);
 }
 
 template <typename T>

@@ -66,7 +66,8 @@ def test_quantize_rows_special_rows_and_strides(cuda):
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("M,K,N", [(1, 768, 2304), (16, 768, 768), (5, 64, 1), (16, 4096, 48), (33, 4000, 300), (64, 768, 130), (50, 700, 40), (3, 1000, 17), (2, 1, 5),
                                    (9, 2050, 271), (17, 128, 16), (64, 520, 271), (130, 768, 300), (257, 129, 129),
-                                   (300, 1024, 128), (1, 5000, 40), (1000, 96, 64), (128, 4224, 256), (520, 200, 1031)])
+                                   (300, 1024, 128), (1, 5000, 40), (1000, 96, 64), (128, 4224, 256), (520, 200, 1031),
+                                   (12, 1500, 50), (20, 2000, 33)])
 def test_linear_is_one_rounding_from_exact(cuda, dtype, M, K, N):
     from mote_amd.int8 import int8_linear, int8_weight
 
