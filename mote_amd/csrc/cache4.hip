@@ -2,9 +2,14 @@
 // attention (mote_cache4_write / mote_cache4_read; the format stands in mote_relation.h).
 //
 // Both are one pass over memory, bound by it: 2 D e bytes a row and head on the wide side, D + 4 G on the
-// narrow one. A thread holds one octet (eight values) of P2 and of I~, so a wave's wide accesses are
-// 16 bytes a lane and its code accesses 4; a group's maximum is two DPP steps over its quad. Values read
-// back pass the caches by (4407 rows, 17 MB: 6.5 -> 5.5 us; 8 x 4984 rows 26.6 -> 25.3 us).
+// narrow one. A thread holds one octet (eight values) of P2 and of I~ (fp32 rows read back: half of one, twice),
+// so a wave's wide accesses are 16 bytes a lane; a group's maximum is two DPP steps over its quad. What a value
+// costs in instructions counts beside the bytes: positions by 32-bit sums instead of divisions (8 x 4984 rows of
+// 8 x 96, bf16, 156 MB: write 35.7 -> 33.8 us), scales without divisions and no clamps (-> 31.2 us, 5.0 TB/s).
+// Values read back pass the caches by (4407 rows, 17 MB: 6.5 -> 5.5 us, 4.8 with the 32-bit positions; 8 x 4984
+// rows 26.6 -> 24.8 us, 6.3 TB/s).
+#include <algorithm>
+
 #include "common.hpp"
 #include "params.hpp"
 #include "fp4.hpp"
@@ -24,6 +29,12 @@ struct Rows4Params {
 };
 
 constexpr int kRows4Threads = 256;
+constexpr int kMaxGrid4 = 65535;  // of a grid's second and third dimensions: heads, sequences of a launch
+
+// n / G for the 1 to 4 groups of a row and n < 2^30
+__device__ __forceinline__ uint32_t over_groups4(uint32_t n, int G) {
+  return G == 3 ? __umulhi(n, 0x55555556u) : n >> (G >> 1);
+}
 
 // the (sequence, head) of the workgroup and this thread's (row, octet) in it
 struct Rows4At {
@@ -32,12 +43,11 @@ struct Rows4At {
 };
 __device__ __forceinline__ Rows4At rows4_at(const Rows4Params& p) {
   Rows4At a;
-  const int bh = blockIdx.x / p.tiles;
-  a.b = bh / p.H;
-  a.h = bh % p.H;
-  const int64_t i = int64_t(blockIdx.x % p.tiles) * kRows4Threads + threadIdx.x;
-  a.t = int(i / (4 * p.G));
-  a.o = int(i % (4 * p.G));
+  a.b = blockIdx.z;
+  a.h = blockIdx.y;
+  const uint32_t i = blockIdx.x * kRows4Threads + threadIdx.x;
+  a.t = int(over_groups4(i >> 2, p.G));
+  a.o = int(i - uint32_t(a.t) * (4 * p.G));
   a.in = a.t < p.T;
   return a;
 }
@@ -45,32 +55,27 @@ __device__ __forceinline__ Rows4At rows4_at(const Rows4Params& p) {
 template <typename T, bool STREAM>
 __global__ void __launch_bounds__(kRows4Threads) cache4_write_kernel(const Rows4Params p) {
   const Rows4At a = rows4_at(p);
-  const int64_t start = p.start_dev ? p.start_dev[a.b] : p.start;
   const int64_t len = p.lens ? p.lens[a.b] : p.T;
-  const int64_t row = start + a.t;
+  const int64_t row = (p.start_dev ? p.start_dev[a.b] : p.start) + a.t;
   // quads are whole (4 G octets a row): a row is written by all of its lanes or by none
-  const bool live = a.in && a.t < len && row >= 0 && row < p.cap;
+  if (!a.in || a.t >= len || row < 0 || row >= p.cap) return;
+  // the octets past the head dim hold its last one, of the same group, and store zeros
+  const bool pad = 8 * a.o >= p.D;
   float x[2][8];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    if (live && 8 * a.o < p.D)
-      load_octet<STREAM>(reinterpret_cast<const T*>(p.x[k]) + a.b * p.x_sb[k] + a.h * p.x_sh[k] + a.t * p.x_sr[k] + 8 * a.o, x[k]);
-    else
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[k][j] = 0.f;
-  }
+  for (int k = 0; k < 2; ++k)
+    load_octet<STREAM>(reinterpret_cast<const T*>(p.x[k]) + a.b * p.x_sb[k] + a.h * p.x_sh[k] + a.t * p.x_sr[k] +
+                       (pad ? p.D - 8 : 8 * a.o), x[k]);
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     bf16_t s;
     const uint32_t w = encode4(x[k], s);
-    if (live) {
-      *reinterpret_cast<uint32_t*>(p.code[k] + a.b * p.c_sb + a.h * p.c_sh + row * (16 * p.G) + 4 * a.o) = w;
-      if ((a.o & 3) == 0) p.scale[k][a.b * p.s_sb + a.h * p.s_sh + row * p.G + (a.o >> 2)] = s;
-    }
+    *reinterpret_cast<uint32_t*>(p.code[k] + a.b * p.c_sb + a.h * p.c_sh + row * (16 * p.G) + 4 * a.o) = pad ? 0u : w;
+    if ((a.o & 3) == 0) p.scale[k][a.b * p.s_sb + a.h * p.s_sh + row * p.G + (a.o >> 2)] = s;
   }
 }
 
-template <typename T>
+// bf16 rows
 __global__ void __launch_bounds__(kRows4Threads) cache4_read_kernel(const Rows4Params p) {
   const Rows4At a = rows4_at(p);
   if (!a.in || 8 * a.o >= p.D) return;
@@ -86,7 +91,51 @@ __global__ void __launch_bounds__(kRows4Threads) cache4_read_kernel(const Rows4P
       s = bf2f(p.scale[k][a.b * p.s_sb + a.h * p.s_sh + row * p.G + (a.o >> 2)]);
     }
     decode4(w, s, x);
-    store_octet<T>(reinterpret_cast<T*>(p.x[k]) + a.b * p.x_sb[k] + a.h * p.x_sh[k] + a.t * p.x_sr[k] + 8 * a.o, x);
+    store_octet(reinterpret_cast<bf16_t*>(p.x[k]) + a.b * p.x_sb[k] + a.h * p.x_sh[k] + a.t * p.x_sr[k] + 8 * a.o, x);
+  }
+}
+
+// fp32 rows: eight threads per group of 32 values, two groups each, so that a store writes the group's whole
+// line: stores past the caches that write half of one, and the other half with the next, cost twice their time
+// (9 x 1144 rows of head dim 128, 84 MB: 31.6 -> 17.0 us; 4 x 8193 of 96 76 -> 36 us).
+__global__ void __launch_bounds__(kRows4Threads) cache4_read_f32_kernel(const Rows4Params p) {
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int64_t start = p.start_dev ? p.start_dev[b] : p.start;
+  const int l = threadIdx.x % 8;
+  const uint32_t q0 = (blockIdx.x * kRows4Threads + threadIdx.x) / 8 * 2;
+  uint32_t w[2][2];
+  float sc[2][2];
+  int tt[2], oo[2];
+  bool in[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int t = int(over_groups4(q0 + j, p.G)), g = int(q0 + j) - t * p.G;
+    tt[j] = t; oo[j] = 32 * g + 4 * l;
+    in[j] = t < p.T && oo[j] < p.D;
+    const int64_t row = start + t;
+    const bool held = in[j] && row >= 0 && row < p.cap;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      w[j][k] = 0;
+      sc[j][k] = __builtin_nanf("");
+      if (held) {
+        w[j][k] = *reinterpret_cast<const uint16_t*>(p.code[k] + b * p.c_sb + h * p.c_sh + row * (16 * p.G) + 16 * g + 2 * l);
+        sc[j][k] = bf2f(p.scale[k][b * p.s_sb + h * p.s_sh + row * p.G + g]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    if (!in[j]) continue;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float x[8];
+      decode4(w[j][k], sc[j][k], x);
+      Chunk c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) c.w[e] = __float_as_uint(x[e]);
+      store_stream(reinterpret_cast<float*>(p.x[k]) + b * p.x_sb[k] + h * p.x_sh[k] + tt[j] * p.x_sr[k] + oo[j], c);
+    }
   }
 }
 
@@ -104,7 +153,7 @@ static int check_rows4(const mote_cache4_rows_args* a, const char* what) {
     if (reinterpret_cast<uintptr_t>(v->data) % 16 || v->stride_b % epc || v->stride_h % epc || v->stride_r % epc)
       return set_error(MOTE_ERR_ARGUMENT, "%s: rows must start on 16-byte boundaries", what);
   const int64_t octets = int64_t(a->T) * 4 * ((a->D + kGroup4 - 1) / kGroup4);
-  if ((octets / kRows4Threads + 1) * a->B * a->H >= (int64_t(1) << 31))
+  if (octets >= (int64_t(1) << 31) || a->H > kMaxGrid4 || (octets / kRows4Threads + 1) * a->B * a->H >= (int64_t(1) << 31))
     return set_error(MOTE_ERR_SHAPE, "%s: too many rows for one launch", what);
   return MOTE_OK;
 }
@@ -125,19 +174,31 @@ static int launch_rows4(const mote_cache4_rows_args* a, bool write, hipStream_t 
   p.start = a->start; p.start_dev = a->start_dev; p.lens = write ? a->lens : nullptr;
   p.H = a->H; p.T = a->T; p.D = a->D; p.G = (a->D + kGroup4 - 1) / kGroup4; p.cap = a->capacity;
   p.tiles = int((int64_t(a->T) * 4 * p.G + kRows4Threads - 1) / kRows4Threads);
-  const dim3 grid(unsigned(int64_t(p.tiles) * a->B * a->H)), block(kRows4Threads);
   // New rows that would push everything else out of the Infinity Cache (256 MB) pass it by, so that the codes
   // stay for the read behind them: write and read of 8 x 4984 rows (122 MB of them) 68 -> 61 us together; of
   // 16 x 5000 rows of head dim 48 (61 MB) 43 us, 46 so.
   const bool large = 2.0 * a->B * a->H * a->T * a->D * (a->dtype == MOTE_BF16 ? 2 : 4) >= 96e6;
-  if (a->dtype == MOTE_BF16) {
-    if (write && large) hipLaunchKernelGGL((cache4_write_kernel<bf16_t, true>), grid, block, 0, stream, p);
-    else if (write) hipLaunchKernelGGL((cache4_write_kernel<bf16_t, false>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL(cache4_read_kernel<bf16_t>, grid, block, 0, stream, p);
-  } else {
-    if (write && large) hipLaunchKernelGGL((cache4_write_kernel<float, true>), grid, block, 0, stream, p);
-    else if (write) hipLaunchKernelGGL((cache4_write_kernel<float, false>), grid, block, 0, stream, p);
-    else hipLaunchKernelGGL(cache4_read_kernel<float>, grid, block, 0, stream, p);
+  const dim3 block(kRows4Threads);
+  for (int b0 = 0; b0 < a->B; b0 += kMaxGrid4) {
+    const int nb = std::min(a->B - b0, kMaxGrid4);
+    const dim3 grid(unsigned(p.tiles), unsigned(a->H), unsigned(nb));
+    if (a->dtype == MOTE_BF16) {
+      if (write && large) hipLaunchKernelGGL((cache4_write_kernel<bf16_t, true>), grid, block, 0, stream, p);
+      else if (write) hipLaunchKernelGGL((cache4_write_kernel<bf16_t, false>), grid, block, 0, stream, p);
+      else hipLaunchKernelGGL(cache4_read_kernel, grid, block, 0, stream, p);
+    } else {
+      if (write && large) hipLaunchKernelGGL((cache4_write_kernel<float, true>), grid, block, 0, stream, p);
+      else if (write) hipLaunchKernelGGL((cache4_write_kernel<float, false>), grid, block, 0, stream, p);
+      else hipLaunchKernelGGL(cache4_read_f32_kernel, grid, block, 0, stream, p);
+    }
+    const int64_t e = a->dtype == MOTE_BF16 ? 2 : 4;
+    for (int k = 0; k < 2; ++k) {
+      p.x[k] += nb * p.x_sb[k] * e;
+      p.code[k] += nb * p.c_sb;
+      p.scale[k] += nb * p.s_sb;
+    }
+    if (p.start_dev) p.start_dev += nb;
+    if (p.lens) p.lens += nb;
   }
   return check_launch(what);
 }

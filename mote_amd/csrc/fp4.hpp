@@ -31,28 +31,40 @@ __device__ __forceinline__ uint32_t quad_umax(uint32_t m) {
   return max(m, uint32_t(__builtin_amdgcn_mov_dpp(int(m), kDppXor2, 0xF, 0xF, false)));
 }
 
+// max / 6 as a division rounds it, in three instructions for a division's ten: one step on the remainder, which
+// fma holds exactly (equal to max / 6 for every float from 2^-125 on; smaller ones have no scale).
+__device__ __forceinline__ float sixth4(float top) {
+  constexpr float r = 1.0f / 6.0f;
+  const float t = top * r;
+  return __builtin_fmaf(__builtin_fmaf(-6.0f, t, top), r, t);
+}
+// 1 / scale as a division rounds it, for normal bf16 scales up to 2^126: one Newton step on the hardware's
+// reciprocal (1 ulp; right from 2 ulps off, for every bf16)
+__device__ __forceinline__ float inverse4(float s) {
+  const float r = __builtin_amdgcn_rcpf(s);
+  return __builtin_fmaf(__builtin_fmaf(-s, r, 1.0f), r, r);
+}
+
 // The quad's group in 4 bits: this lane's eight codes, and the group's scale. All four lanes must be here
-// (lanes past the head dim with zeros). Rounding points: the scale once to bf16 (a wider one would cost
-// more than it gains: codes are 2^-2 apart), the inverse and the products in fp32.
+// (lanes past the head dim with zeros, or with values of the group, their codes dropped). Rounding points: the
+// scale once to bf16 (a wider one would cost more than it gains: codes are 2^-2 apart), the inverse and the
+// products in fp32. Products reach 6 (1 + 2^-8), where the scale was rounded down, and convert to 6.
 __device__ __forceinline__ uint32_t encode4(const float (&x)[8], bf16_t& scale) {
   uint32_t top = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(x[j]) & 0x7fffffffu);
   top = quad_umax(top);
   const bool finite = top < 0x7f800000u;
-  bf16_t sb = f2bf(__uint_as_float(finite ? top : 0u) / 6.0f);
+  bf16_t sb = f2bf(sixth4(__uint_as_float(finite ? top : 0u)));
   if (bf2f(sb) < kTiny4) sb = 0;
-  const float inv = sb ? 1.0f / bf2f(sb) : 0.f;
+  const float inv = sb ? inverse4(bf2f(sb)) : 0.f;
   scale = finite ? sb : kNanScale4;
-  float t[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) t[j] = finite ? __builtin_amdgcn_fmed3f(x[j] * inv, -6.0f, 6.0f) : 0.f;
   uint32_t w = 0;  // v_cvt_scalef32_pk_fp4_f32 rounds to nearest, ties to the even code
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[0], t[1], 1.0f, 0);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[2], t[3], 1.0f, 1);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[4], t[5], 1.0f, 2);
-  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, t[6], t[7], 1.0f, 3);
-  return w;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0] * inv, x[1] * inv, 1.0f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2] * inv, x[3] * inv, 1.0f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4] * inv, x[5] * inv, 1.0f, 2);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6] * inv, x[7] * inv, 1.0f, 3);
+  return finite ? w : 0u;
 }
 
 __device__ __forceinline__ void decode4(uint32_t w, float s, float (&x)[8]) {

@@ -93,6 +93,47 @@ def test_every_border_and_every_special_value(cuda):
     assert k[0, 1, 4, 32:].isnan().all() and (k[0, 1, 4, :32] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_scales_and_codes_of_every_magnitude(cuda, dtype):
+    """Groups whose maximum has every exponent a float has, every mantissa of a bf16 (and random ones of fp32):
+    the scale and its inverse are those of the divisions, whatever the kernel computes them with."""
+    from mote_amd.cache4 import cache4_write, cache4_zeros
+
+    e = torch.arange(-140, 128).double()[:, None]
+    m = 1.0 + torch.arange(128).double() / 128
+    if dtype == F32:
+        m = torch.cat([m, 1.0 + torch.rand(128, generator=_gen(5)).double()])
+    top = torch.ldexp(m, e.int()).reshape(-1)
+    border = (6.0 * 2.0 ** -126) * (1 + torch.arange(-64, 64).double() * (2.0 ** -23 if dtype == F32 else 2.0 ** -7))
+    top = torch.cat([top, border]).float().to(dtype)
+    top = top[top.isfinite()]
+    x = (torch.rand(1, 2, top.numel(), 32, generator=_gen(6)) * 2 - 1) * top[:, None].float()
+    x[..., 7] = top.float()
+    x = x.to(dtype)
+    cache = cache4_zeros(1, 2, top.numel(), 32, cuda)
+    cache4_write(cache, x.to(cuda), (-x).to(cuda))
+    for codes, scales, t in ((cache.p2, cache.p2_scale, x), (cache.info, cache.info_scale, -x)):
+        vals, s = Q.encode4(t)
+        assert torch.equal(scales.cpu(), s)
+        assert torch.equal(Q.unpack_codes(codes.cpu(), 32), vals)
+
+
+def test_more_sequences_than_one_launch_takes(cuda):
+    from mote_amd.cache4 import cache4_read, cache4_write, cache4_zeros
+
+    B, D = 70001, 8
+    cache = cache4_zeros(B, 1, 3, D, cuda)
+    x = _rows(11, B, 1, 1, D, BF16)
+    start, lens = (torch.arange(B) % 3), (torch.arange(B) % 5 > 0).long()
+    cache4_write(cache, x.to(cuda), (-x).to(cuda), start.to(cuda), lens.to(cuda))
+    vals, s = Q.encode4(x)
+    want = torch.zeros(B, 1, 3, D, dtype=torch.double)
+    want[torch.arange(B), 0, start] = (Q.values4(vals, s) * lens[:, None, None, None])[:, 0, 0]
+    for dtype in (BF16, F32):
+        k, v = cache4_read(cache, D, 0, dtype=dtype)
+        assert torch.equal(k.cpu(), want.float().to(dtype)) and torch.equal(v.cpu(), -want.float().to(dtype))
+
+
 def test_positions_lengths_and_strides(cuda):
     """Device positions, padded batches, rows outside the capacity, transposed and misaligned inputs,
     caches that are slices of a larger store, views as outputs."""

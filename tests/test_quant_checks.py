@@ -203,6 +203,9 @@ def test_c_entry_points_refuse_without_a_gpu():
         assert call(r, None) == 1 and b"16-byte" in lib.mote_last_error()
         r.p2.stride_r, r.cache.codes_sh = 48, 24
         assert call(r, None) == 1 and b"codes" in lib.mote_last_error()
+        r.cache.codes_sh = 32
+        for r.H, r.T in ((65536, 4), (2, 1 << 28)):
+            assert call(r, None) == 2 and b"too many" in lib.mote_last_error()
     a = L.Decode4Args()
     assert lib.mote_relation_decode4(None, None) == 1
     a.dtype, a.B, a.H, a.D, a.capacity = L.MOTE_BF16, 1, 3, 96, 256
