@@ -707,7 +707,7 @@ typedef struct mote_cache4 {
  * (dtype; rows on 16-byte boundaries). start is `start`, or start_dev[b] (device) when start_dev is not
  * NULL; with lens (device, [B], or NULL) sequence b writes its first lens[b] rows only. Rows outside
  * [0, capacity) are skipped. Replaces: ArenaLayer.write (mote/model/arena.py:133-139). H is at most 65535,
- * T below 2^27.
+ * T below 2^26.
  * mote_cache4_read: rows start + t, t < T, into the views p2 / info (dtype), each value rounded once;
  * rows outside [0, capacity) read as NaN; lens is not used. */
 typedef struct mote_cache4_rows_args {

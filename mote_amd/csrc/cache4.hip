@@ -2,13 +2,14 @@
 // attention (mote_cache4_write / mote_cache4_read; the format stands in mote_relation.h).
 //
 // Both are one pass over memory, bound by it: 2 D e bytes a row and head on the wide side, D + 4 G on the
-// narrow one. A thread holds one octet (eight values) of P2 and of I~ (fp32 rows read back: half of one, twice),
-// so a wave's wide accesses are 16 bytes a lane; a group's maximum is two DPP steps over its quad. What a value
+// narrow one. Wide accesses are 16 bytes a lane. A writing thread holds one octet (eight values) of P2 and of
+// I~, and a group's maximum is two DPP steps over its quad; a reading one a 16-byte chunk of either. What a value
 // costs in instructions counts beside the bytes: positions by 32-bit sums instead of divisions (8 x 4984 rows of
 // 8 x 96, bf16, 156 MB: write 35.7 -> 33.8 us), scales without divisions and no clamps (-> 31.2 us, 5.0 TB/s).
 // Values read back pass the caches by (4407 rows, 17 MB: 6.5 -> 5.5 us, 4.8 with the 32-bit positions; 8 x 4984
 // rows 26.6 -> 24.8 us, 6.3 TB/s).
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "params.hpp"
@@ -25,7 +26,8 @@ struct Rows4Params {
   int64_t start;
   const int64_t* start_dev;
   const int64_t* lens;
-  int H, T, D, G, cap, tiles;
+  int T, D, G, cap;
+  uint32_t over_mul, over_shift;  // n over_mul / 2^over_shift = n / (chunks of a row), n < 2^31 (reads)
 };
 
 constexpr int kRows4Threads = 256;
@@ -75,67 +77,38 @@ __global__ void __launch_bounds__(kRows4Threads) cache4_write_kernel(const Rows4
   }
 }
 
-// bf16 rows
+// A thread per 16-byte chunk of the rows, in memory order, so that a store writes whole lines where rows follow each
+// other. Past the caches, lines written in parts cost twice their time:
+// with an octet of fp32 a thread, stored in halves, 9 x 1144 rows of head dim 128 (84 MB) took 31.6 us, now 15.9;
+// with whole groups and idle threads past the head dim 4 x 3001 rows of 120 24.1, now 15.0.
+template <typename T>
 __global__ void __launch_bounds__(kRows4Threads) cache4_read_kernel(const Rows4Params p) {
-  const Rows4At a = rows4_at(p);
-  if (!a.in || 8 * a.o >= p.D) return;
-  const int64_t row = (p.start_dev ? p.start_dev[a.b] : p.start) + a.t;
+  constexpr int EPC = 16 / int(sizeof(T));
+  const uint32_t i = blockIdx.x * kRows4Threads + threadIdx.x;
+  const int t = int(uint64_t(i) * p.over_mul >> p.over_shift);
+  const int c = int(i) - t * (p.D / EPC);
+  const int b = blockIdx.z, h = blockIdx.y;
+  if (t >= p.T) return;
+  const int64_t row = (p.start_dev ? p.start_dev[b] : p.start) + t;
   const bool held = row >= 0 && row < p.cap;
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    float x[8];
     uint32_t w = 0;
     float s = __builtin_nanf("");
     if (held) {
-      w = *reinterpret_cast<const uint32_t*>(p.code[k] + a.b * p.c_sb + a.h * p.c_sh + row * (16 * p.G) + 4 * a.o);
-      s = bf2f(p.scale[k][a.b * p.s_sb + a.h * p.s_sh + row * p.G + (a.o >> 2)]);
+      using Codes = std::conditional_t<EPC == 8, uint32_t, uint16_t>;
+      w = *reinterpret_cast<const Codes*>(p.code[k] + b * p.c_sb + h * p.c_sh + row * (16 * p.G) + EPC / 2 * c);
+      s = bf2f(p.scale[k][b * p.s_sb + h * p.s_sh + row * p.G + c / (kGroup4 / EPC)]);
     }
+    float x[8];
     decode4(w, s, x);
-    store_octet(reinterpret_cast<bf16_t*>(p.x[k]) + a.b * p.x_sb[k] + a.h * p.x_sh[k] + a.t * p.x_sr[k] + 8 * a.o, x);
-  }
-}
-
-// fp32 rows: eight threads per group of 32 values, two groups each, so that a store writes the group's whole
-// line: stores past the caches that write half of one, and the other half with the next, cost twice their time
-// (9 x 1144 rows of head dim 128, 84 MB: 31.6 -> 17.0 us; 4 x 8193 of 96 76 -> 36 us).
-__global__ void __launch_bounds__(kRows4Threads) cache4_read_f32_kernel(const Rows4Params p) {
-  const int b = blockIdx.z, h = blockIdx.y;
-  const int64_t start = p.start_dev ? p.start_dev[b] : p.start;
-  const int l = threadIdx.x % 8;
-  const uint32_t q0 = (blockIdx.x * kRows4Threads + threadIdx.x) / 8 * 2;
-  uint32_t w[2][2];
-  float sc[2][2];
-  int tt[2], oo[2];
-  bool in[2];
+    Chunk v;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int t = int(over_groups4(q0 + j, p.G)), g = int(q0 + j) - t * p.G;
-    tt[j] = t; oo[j] = 32 * g + 4 * l;
-    in[j] = t < p.T && oo[j] < p.D;
-    const int64_t row = start + t;
-    const bool held = in[j] && row >= 0 && row < p.cap;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      w[j][k] = 0;
-      sc[j][k] = __builtin_nanf("");
-      if (held) {
-        w[j][k] = *reinterpret_cast<const uint16_t*>(p.code[k] + b * p.c_sb + h * p.c_sh + row * (16 * p.G) + 16 * g + 2 * l);
-        sc[j][k] = bf2f(p.scale[k][b * p.s_sb + h * p.s_sh + row * p.G + g]);
-      }
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (EPC == 8) v.w[j] = uint32_t(f2bf(x[2 * j])) | uint32_t(f2bf(x[2 * j + 1])) << 16;
+      else v.w[j] = __float_as_uint(x[j]);
     }
-  }
-#pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if (!in[j]) continue;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      float x[8];
-      decode4(w[j][k], sc[j][k], x);
-      Chunk c;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) c.w[e] = __float_as_uint(x[e]);
-      store_stream(reinterpret_cast<float*>(p.x[k]) + b * p.x_sb[k] + h * p.x_sh[k] + tt[j] * p.x_sr[k] + oo[j], c);
-    }
+    store_stream(reinterpret_cast<T*>(p.x[k]) + b * p.x_sb[k] + h * p.x_sh[k] + t * p.x_sr[k] + EPC * c, v);
   }
 }
 
@@ -153,7 +126,7 @@ static int check_rows4(const mote_cache4_rows_args* a, const char* what) {
     if (reinterpret_cast<uintptr_t>(v->data) % 16 || v->stride_b % epc || v->stride_h % epc || v->stride_r % epc)
       return set_error(MOTE_ERR_ARGUMENT, "%s: rows must start on 16-byte boundaries", what);
   const int64_t octets = int64_t(a->T) * 4 * ((a->D + kGroup4 - 1) / kGroup4);
-  if (octets >= (int64_t(1) << 31) || a->H > kMaxGrid4 || (octets / kRows4Threads + 1) * a->B * a->H >= (int64_t(1) << 31))
+  if (octets >= (int64_t(1) << 30) || a->H > kMaxGrid4 || (octets / kRows4Threads + 1) * a->B * a->H >= (int64_t(1) << 31))
     return set_error(MOTE_ERR_SHAPE, "%s: too many rows for one launch", what);
   return MOTE_OK;
 }
@@ -172,8 +145,13 @@ static int launch_rows4(const mote_cache4_rows_args* a, bool write, hipStream_t 
   p.scale[0] = reinterpret_cast<bf16_t*>(a->cache.p2_scale); p.scale[1] = reinterpret_cast<bf16_t*>(a->cache.info_scale);
   p.c_sb = a->cache.codes_sb; p.c_sh = a->cache.codes_sh; p.s_sb = a->cache.scale_sb; p.s_sh = a->cache.scale_sh;
   p.start = a->start; p.start_dev = a->start_dev; p.lens = write ? a->lens : nullptr;
-  p.H = a->H; p.T = a->T; p.D = a->D; p.G = (a->D + kGroup4 - 1) / kGroup4; p.cap = a->capacity;
-  p.tiles = int((int64_t(a->T) * 4 * p.G + kRows4Threads - 1) / kRows4Threads);
+  p.T = a->T; p.D = a->D; p.G = (a->D + kGroup4 - 1) / kGroup4; p.cap = a->capacity;
+  const int chunks = a->D * (a->dtype == MOTE_BF16 ? 2 : 4) / 16;
+  uint32_t bits = 0;
+  while ((1 << bits) < chunks) ++bits;
+  p.over_shift = 31 + bits;
+  p.over_mul = uint32_t((uint64_t(1) << p.over_shift) / chunks) + 1;
+  const int64_t tiles = (int64_t(a->T) * (write ? 4 * p.G : chunks) + kRows4Threads - 1) / kRows4Threads;
   // New rows that would push everything else out of the Infinity Cache (256 MB) pass it by, so that the codes
   // stay for the read behind them: write and read of 8 x 4984 rows (122 MB of them) 68 -> 61 us together; of
   // 16 x 5000 rows of head dim 48 (61 MB) 43 us, 46 so.
@@ -181,15 +159,15 @@ static int launch_rows4(const mote_cache4_rows_args* a, bool write, hipStream_t 
   const dim3 block(kRows4Threads);
   for (int b0 = 0; b0 < a->B; b0 += kMaxGrid4) {
     const int nb = std::min(a->B - b0, kMaxGrid4);
-    const dim3 grid(unsigned(p.tiles), unsigned(a->H), unsigned(nb));
+    const dim3 grid(unsigned(tiles), unsigned(a->H), unsigned(nb));
     if (a->dtype == MOTE_BF16) {
       if (write && large) hipLaunchKernelGGL((cache4_write_kernel<bf16_t, true>), grid, block, 0, stream, p);
       else if (write) hipLaunchKernelGGL((cache4_write_kernel<bf16_t, false>), grid, block, 0, stream, p);
-      else hipLaunchKernelGGL(cache4_read_kernel, grid, block, 0, stream, p);
+      else hipLaunchKernelGGL(cache4_read_kernel<bf16_t>, grid, block, 0, stream, p);
     } else {
       if (write && large) hipLaunchKernelGGL((cache4_write_kernel<float, true>), grid, block, 0, stream, p);
       else if (write) hipLaunchKernelGGL((cache4_write_kernel<float, false>), grid, block, 0, stream, p);
-      else hipLaunchKernelGGL(cache4_read_f32_kernel, grid, block, 0, stream, p);
+      else hipLaunchKernelGGL(cache4_read_kernel<float>, grid, block, 0, stream, p);
     }
     const int64_t e = a->dtype == MOTE_BF16 ? 2 : 4;
     for (int k = 0; k < 2; ++k) {

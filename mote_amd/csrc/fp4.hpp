@@ -92,24 +92,6 @@ __device__ __forceinline__ void load_octet(const T* p, float (&x)[8]) {
     }
   }
 }
-template <typename T>
-__device__ __forceinline__ void store_octet(T* p, const float (&x)[8]) {
-  Chunk a, b;
-  if constexpr (sizeof(T) == 2) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) a.w[j] = uint32_t(f2bf(x[2 * j])) | uint32_t(f2bf(x[2 * j + 1])) << 16;
-    store_stream(p, a);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      a.w[j] = __float_as_uint(x[j]);
-      b.w[j] = __float_as_uint(x[4 + j]);
-    }
-    store_stream(p, a);
-    store_stream(p + 4, b);
-  }
-}
-
 // what a launcher checks of a cache in 4 bits: null pointers, alignment, strides that hold a row each
 inline const char* bad_cache4(const mote_cache4& c) {
   if (!c.p2 || !c.p2_scale || !c.info || !c.info_scale) return "null pointer";
