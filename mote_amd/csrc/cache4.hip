@@ -77,10 +77,11 @@ __global__ void __launch_bounds__(kRows4Threads) cache4_write_kernel(const Rows4
   }
 }
 
-// A thread per 16-byte chunk of the rows, in memory order, so that a store writes whole lines where rows follow each
-// other. Past the caches, lines written in parts cost twice their time:
-// with an octet of fp32 a thread, stored in halves, 9 x 1144 rows of head dim 128 (84 MB) took 31.6 us, now 15.9;
-// with whole groups and idle threads past the head dim 4 x 3001 rows of 120 24.1, now 15.0.
+// A thread per 16-byte chunk of the rows, in memory order, so that a store writes whole lines where rows follow
+// each other. Past the caches, lines written in parts cost twice their time: with an octet of fp32 a thread, stored
+// in halves, 9 x 1144 rows of head dim 128 (84 MB) took 31.6 us, now 15.9; with whole groups and idle threads past
+// the head dim 4 x 3001 rows of 120 24.1, now 15.0. (Writing fp32 rows so as well, eight lanes a group: 118 MB
+// 31.0 -> 29.8 us, but 3 MB 3.6 -> 3.9.)
 template <typename T>
 __global__ void __launch_bounds__(kRows4Threads) cache4_read_kernel(const Rows4Params p) {
   constexpr int EPC = 16 / int(sizeof(T));

@@ -136,8 +136,8 @@ template <typename T, int G, int NC>
 __global__ void __launch_bounds__(64 * kQuantWaves)
 quantize_rows_kernel(const T* x, int64_t x_sr, int M, int K, int Kp, int8_t* q, float* scale) {
   const int lane = threadIdx.x % G;
-  const int m = blockIdx.x * (64 / G * kQuantWaves) + threadIdx.x / G;
-  if (m >= M) return;  // whole groups
+  const uint32_t m = blockIdx.x * (64 / G * kQuantWaves) + threadIdx.x / G;
+  if (m >= uint32_t(M)) return;  // whole groups
   const T* row = x + int64_t(m) * x_sr;
   RowPart<T, 8> v[NC];
   uint32_t top = 0;
@@ -563,12 +563,11 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
     const unsigned per = unsigned((int64_t(p.ntok) * p.nch + 7) / 8);
     hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * waves), 0, stream, p);
   };
-  // Tiles of channels x tokens. One round of workgroups of a small tile while that holds everything (a CU
-  // holds three of the small ones). Transfers into LDS reach some 47 bytes a nanosecond per CU whatever the
-  // ring's depth, so few tiles go to as many CUs as there are: 32 x 16 (258 x 3413 -> 523 10.6 us, 11.9 with
-  // 64 x 32; 128 x 768 -> 768 6.4 and 6.8; with two CUs' worth of 32 x 16 exceeded, 1000 x 520 -> 271 7.5 and
-  // 7.2); then 64 x 32 with a deep ring (512 x 768 -> 2304 8.5 us, 11.1 with 128 x 128),
-  // then 128 x 64 (2048 rows 13.1 us, 14.6 and 16.9 with 64 x 32).
+  // Tiles of channels x tokens. One round of workgroups of a small tile while that holds everything (a CU holds
+  // three of the small ones). Transfers into LDS reach some 47 bytes a nanosecond per CU whatever the ring's depth,
+  // so few tiles go to as many CUs as there are: 32 x 16 (258 x 3413 -> 523 10.6 us, 11.9 with 64 x 32; 128 x 768
+  // -> 768 6.4 and 6.8; past two a CU 1000 x 520 -> 271 7.5 and 7.2). Then 64 x 32 with a deep ring (512 x 768 ->
+  // 2304 8.5 us, 11.1 with 128 x 128), then 128 x 64 (2048 rows 13.1 us, 14.6, and 16.9 with 64 x 32).
   const int64_t cus = device_cu_count();
   auto tiles = [&](int ch, int tok) { return ((int64_t(a->M) + tok - 1) / tok) * ((a->N + ch - 1) / ch); };
   if (tiles(32, 16) <= 2 * cus) return go(int8_many_kernel<T, 1, 1, 2, 1, 4>, 32, 16, 2);
