@@ -564,19 +564,21 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
     hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * waves), 0, stream, p);
   };
   // Tiles of channels x tokens. One round of workgroups of a small tile while that holds everything. Transfers into
-  // LDS reach some 47 bytes a nanosecond per CU, so few tiles go to as many CUs as there are: 32 x 16 (258 x 3413 ->
-  // 523 10.6 us, 11.9 with 64 x 32; 128 x 768 -> 768 6.4 and 6.8; past two a CU 1000 x 520 -> 271 7.5 and 7.2). Then
-  // 64 x 32, up to three a CU (512 x 768 -> 2304 8.5 us, 11.1 with 128 x 128), or two where k is long and one of
-  // 128 x 64 a CU does, with fewer bytes a product and a ring of four (600 x 2048 -> 2048 12.2, 12.8 with 64 x 32; 700 x
-  // 1024 -> 1600 9.4 and 9.2); that one (512 x 4096 -> 4096 19.5 us, 25.2 with a ring of two, 24.5 with 64 x 32; 2048 x
-  // 1024 -> 1024 10.1, 11.2 and 11.6); then 128 x 64 with a ring of two, three a CU (2048 x 768 -> 2304 12.8, 13.0 with
-  // 128 x 128, 17.1 with the ring of four, 16.3 with 64 x 32).
+  // LDS reach some 47 bytes a nanosecond per CU, so few tiles go to as many CUs as there are: 32 x 16 (258 x 3413
+  // -> 523 10.6 us, 11.9 with 64 x 32; 128 x 768 -> 768 6.4 and 6.8; past two a CU 1000 x 520 -> 271 7.5 and 7.2).
+  // Then 64 x 32, up to three a CU (512 x 768 -> 2304 8.5 us, 11.1 with 128 x 128), or two where k is long and one
+  // of 128 x 64 a CU does, with fewer bytes a product and a ring of four (600 x 2048 -> 2048 12.2, 12.8 with 64 x
+  // 32; 700 x 1024 -> 1600 9.4 and 9.2); that one (512 x 4096 -> 4096 19.5 us, 25.2 with a ring of two, 24.5 with
+  // 64 x 32; 2048 x 1024 -> 1024 10.1, 11.2 and 11.6); one of 128 x 128 a CU with a ring of four where k is long
+  // (4096 x 4096 -> 1024 31.0, 33.3 with the next; 2000 x 300 -> 2048 9.7 and 9.4); then 128 x 64 with a ring of
+  // two, three a CU (2048 x 768 -> 2304 12.8, 13.0 with 128 x 128, 16.3 with 64 x 32).
   const int64_t cus = device_cu_count();
   auto tiles = [&](int ch, int tok) { return ((int64_t(a->M) + tok - 1) / tok) * ((a->N + ch - 1) / ch); };
   if (tiles(32, 16) <= 2 * cus) return go(int8_many_kernel<T, 1, 1, 2, 1, 4>, 32, 16, 2);
   const bool one_each = tiles(128, 64) <= cus;
   if (tiles(64, 32) <= (one_each && Kp > 1024 ? 2 : 3) * cus) return go(int8_many_kernel<T, 2, 1, 2, 2, 4>, 64, 32, 4);
   if (one_each) return go(int8_many_kernel<T, 2, 2, 4, 2, 4>, 128, 64, 8);
+  if (tiles(128, 128) <= cus && Kp >= 1024) return go(int8_many_kernel<T, 4, 2, 2, 4, 4>, 128, 128, 8);
   if (tiles(128, 64) <= 3 * cus) return go(int8_many_kernel<T, 4, 2, 2, 2, 2>, 128, 64, 4);
   // Beyond, the tile whose rounds take least: a round of n stages of k takes fixed + n * stage us (fitted to
   // k = 768, 1024 and 4096 at 4964 to 65536 rows), with one workgroup per CU of the large tiles and two of

@@ -67,7 +67,8 @@ def test_quantize_rows_special_rows_and_strides(cuda):
 @pytest.mark.parametrize("M,K,N", [(1, 768, 2304), (16, 768, 768), (5, 64, 1), (16, 4096, 48), (33, 4000, 300), (64, 768, 130), (50, 700, 40), (3, 1000, 17), (2, 1, 5),
                                    (9, 2050, 271), (17, 128, 16), (64, 520, 271), (130, 768, 300), (257, 129, 129),
                                    (300, 1024, 128), (1, 5000, 40), (1000, 96, 64), (128, 4224, 256), (520, 200, 1031),
-                                   (12, 1500, 50), (20, 2000, 33), (700, 1200, 1700), (2000, 100, 999)])
+                                   (12, 1500, 50), (20, 2000, 33), (700, 1200, 1700), (2000, 100, 999),
+                                   (1100, 1100, 2470)])
 def test_linear_is_one_rounding_from_exact(cuda, dtype, M, K, N):
     from mote_amd.int8 import int8_linear, int8_weight
 
@@ -77,7 +78,7 @@ def test_linear_is_one_rounding_from_exact(cuda, dtype, M, K, N):
     _check(y, x, w)
 
 
-@pytest.mark.parametrize("M,K,N", [(700, 256, 1100), (700, 1200, 1700), (2000, 256, 999), (2300, 200, 2500), (6300, 96, 2300), (16384, 64, 2304), (5000, 384, 9000)])
+@pytest.mark.parametrize("M,K,N", [(700, 256, 1100), (700, 1200, 1700), (2000, 256, 999), (1100, 1100, 2500), (2300, 200, 2500), (6300, 96, 2300), (16384, 64, 2304), (5000, 384, 9000)])
 def test_every_tile_size_gives_a_row_its_own_result(cuda, M, K, N):
     """Sizes over the range of tiles (the rule picks by rounds of workgroups): rows, the last ones and those at
     tile borders among them, equal the few-token form's bit for bit."""
