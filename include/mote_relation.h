@@ -726,9 +726,10 @@ int mote_cache4_read(const mote_cache4_rows_args* args, void* stream);
 /* One decode step over that cache: mote_relation_decode (see there for every argument they share) with
  * the past rows j < S at their 4-bit values. The Self term and the new chunk's share of y take the new
  * rows as they are; they are then stored in 4 bits at row S. S[b] outside [0, capacity) writes NaN into
- * y[b] and g[b] and stores nothing. The workspace (mote_relation_decode4_workspace() bytes, zeroed once
- * before its first call) is left with its counters at zero; it serves calls of one B and H (the counters'
- * places follow from them), one after the other. */
+ * y[b] and g[b] and stores nothing. The workspace (at least mote_relation_decode4_workspace() bytes,
+ * zeroed once before its first call) is left with its counters at zero and serves calls one after the other:
+ * of any sizes that it has the bytes for, given with the same workspace_bytes each time (counters lie in its
+ * first half, partials in its second), or of one B and H with any. */
 typedef struct mote_relation_decode4_args {
   int dtype;
   int B, H, D, capacity, layer_parity, flags;

@@ -78,8 +78,9 @@ def cache4_read(cache: Cache4, d_head: int, start: Union[int, torch.Tensor] = 0,
 
 def decode4_workspace(B: int, H: int, d_head: int, capacity: int, device) -> torch.Tensor:
     """A workspace for `relation_decode4` at these sizes: completion counters and per-split partials, zeroed
-    here once; every call leaves the counters at zero again. Calls of these sizes may share it one after the
-    other (the layers of a step, captured graphs that are replayed in turn); they must not overlap."""
+    here once; every call leaves the counters at zero again. Calls whose workspace has as many bytes may share
+    it one after the other (the layers of a step, captured graphs that are replayed in turn); they must not
+    overlap. It is passed whole: a part of one is no workspace for smaller sizes."""
     a = L.Decode4Args()
     a.B, a.H, a.D, a.capacity = B, H, d_head, capacity
     with L.device_of(device):

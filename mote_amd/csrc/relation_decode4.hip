@@ -17,6 +17,7 @@
 //
 // Grid, rings, splits, predicate and the publish / count / merge protocol are those of relation_decode.hip;
 // its comments give the reasons.
+#include <algorithm>
 #include <type_traits>
 
 #include "common.hpp"
@@ -469,18 +470,20 @@ static int splits4(const mote_relation_decode4_args* a) {
 }
 
 struct Dec4Ws {
-  size_t part, cnt, cnt_seq, total;
+  size_t cnt, total;
   int nsplit;
 };
-// the counters first: they stay where they are when another capacity changes the splits
+// Counters in the first half of a workspace, partials in the second, whatever the sizes: a call of other sizes on
+// the same bytes finds its counters at zero, never where an earlier one left partials. (With the partials right
+// behind the counters, B = 1, H = 4, D = 40 with 5120 rows and B = H = 4, D = 48 with 768 shared their 14720 bytes,
+// and the second call counted on the first one's floats: no workgroup was the last, nothing was written.)
 static Dec4Ws ws4(const mote_relation_decode4_args* a) {
   const size_t BH = size_t(a->B) * a->H, line = kD4CntStride * sizeof(int);
   Dec4Ws w;
-  w.cnt_seq = 0;
   w.cnt = size_t(a->B) * line;
-  w.part = w.cnt + BH * line;
   w.nsplit = splits4(a);
-  w.total = w.part + BH * size_t(w.nsplit) * size_t(a->D + 2) * sizeof(float);
+  const size_t counters = w.cnt + BH * line, partials = BH * size_t(w.nsplit) * size_t(a->D + 2) * sizeof(float);
+  w.total = 2 * ((std::max(counters, partials) + 15) / 16 * 16);
   return w;
 }
 
@@ -517,9 +520,9 @@ int launch_decode4(const mote_relation_decode4_args* a, hipStream_t stream) {
   p.c_sb = a->cache.codes_sb; p.c_sh = a->cache.codes_sh; p.s_sb = a->cache.scale_sb; p.s_sh = a->cache.scale_sh;
   p.y = a->y; p.y_sb = a->y_sb; p.g = a->g; p.xm = a->xm; p.run = a->run;
   char* ws = reinterpret_cast<char*>(a->workspace);
-  p.part = reinterpret_cast<float*>(ws + w.part);
+  p.part = reinterpret_cast<float*>(ws + a->workspace_bytes / 32 * 16);
   p.cnt = reinterpret_cast<int*>(ws + w.cnt);
-  p.cnt_seq = reinterpret_cast<int*>(ws + w.cnt_seq);
+  p.cnt_seq = reinterpret_cast<int*>(ws);
   p.B = a->B; p.H = a->H; p.D = a->D; p.cap = a->capacity; p.parity = a->layer_parity & 1; p.flags = a->flags;
   p.nsplit = w.nsplit;
   p.scale = 1.0f / sqrtf((float)a->D);

@@ -607,7 +607,7 @@ std::tuple<Tensor, Tensor> relation_decode4(const Tensor& p1, const Tensor& p2, 
   a.cache = c.c;
   a.y = y.data_ptr(); a.y_sb = y.stride(0); a.g = fptr(g);
   const int64_t need = int64_t(mote_relation_decode4_workspace(&a));
-  // another shape's counters lie elsewhere: its workspace would not be zero where this call counts
+  // the halves that counters and partials lie in follow from the bytes: one workspace, one number of them
   if (workspace && workspace->numel() * workspace->element_size() != need)
     bad_value(what, ": a workspace of ", workspace->numel() * workspace->element_size(), " bytes, ", need,
               " needed (decode4_workspace makes one for these sizes)");

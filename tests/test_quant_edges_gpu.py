@@ -1,0 +1,83 @@
+"""The quantised operators on the GPU at the edges of what a call may pass: workspaces and layers' objects that
+several calls share, sizes at a launch's limit, every kernel form that a rule on sizes selects."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def _step_inputs(cuda, seed, B, H, D, cap):
+    """(new chunk [B, 3, H, D], S, a cache of ordinary random rows) with every position in the cache's second half."""
+    from mote_amd.cache4 import Cache4, groups
+
+    g, G = _gen(seed), groups(D)
+    codes = lambda: torch.randint(0, 256, (B, H, cap, 16 * G), generator=g, dtype=torch.uint8).to(cuda)
+    scales = lambda: (0.2 + 0.3 * torch.rand(B, H, cap, G, generator=g)).to(BF16).to(cuda)
+    x = torch.randn(B, 3, H, D, generator=g).to(BF16).to(cuda)
+    return x, torch.randint(cap // 2, cap, (B,), generator=g).to(cuda), Cache4(codes(), scales(), codes(), scales())
+
+
+def _raw_step(x, S, cache, lam, ws):
+    """relation_decode4 through the C entry point, on the workspace as it is; y, g and the S that it advanced."""
+    from mote_amd import _lib as L
+
+    B, _, H, D = x.shape
+    y = torch.full((B, H, D), 7.0, device=x.device, dtype=BF16)
+    g, S = torch.full((B, H), 7.0, device=x.device), S.clone()
+    a = L.Decode4Args()
+    a.dtype, a.B, a.H, a.D, a.capacity, a.flags, a.tau_s = L.MOTE_BF16, B, H, D, cache.p2.shape[2], L.MOTE_DECODE_ADVANCE, 2.0
+    a.lam, a.S, a.in_sb = lam.data_ptr(), S.data_ptr(), x.stride(0)
+    a.p1, a.p2, a.info = (x[:, i].data_ptr() for i in range(3))
+    a.cache.p2, a.cache.p2_scale, a.cache.info, a.cache.info_scale = (t.data_ptr() for t in cache)
+    a.cache.codes_sb, a.cache.codes_sh, a.cache.scale_sb, a.cache.scale_sh = (*cache.p2.stride()[:2], *cache.p2_scale.stride()[:2])
+    a.y, a.y_sb, a.g = y.data_ptr(), H * D, g.data_ptr()
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    assert ws.numel() >= int(L.lib().mote_relation_decode4_workspace(a))
+    L.check(L.lib().mote_relation_decode4(a, L.stream_of(x)), "mote_relation_decode4")
+    return y, g, S
+
+
+@pytest.mark.parametrize("first,second", [
+    ((1, 4, 40, 5120), (4, 4, 48, 768)), ((1, 8, 64, 4096), (3, 4, 40, 4096)), ((1, 8, 64, 8192), (16, 8, 64, 768)),
+    ((1, 8, 96, 5376), (16, 8, 96, 512)), ((16, 8, 128, 512), (1, 8, 128, 4096)), ((2, 4, 48, 2560), (4, 4, 40, 1280))])
+def test_calls_of_other_sizes_on_one_workspace(cuda, first, second):
+    """A workspace that calls of several batches and heads take in turn: each finds its counters at zero, so y, g
+    and S are those of a workspace of its own, bit for bit."""
+    from mote_amd.cache4 import decode4_workspace, relation_decode4
+
+    n = max(decode4_workspace(*sizes, cuda).numel() for sizes in (first, second))
+    ws, lam = torch.zeros(n, dtype=torch.uint8, device=cuda), torch.tensor(0.5, device=cuda)
+    for turn in range(3):
+        for sizes in (first, second):
+            x, S, cache = _step_inputs(cuda, 31 + turn, *sizes)
+            y, g, advanced = _raw_step(x, S, cache, lam, ws)
+            want = relation_decode4(x[:, 0], x[:, 1], x[:, 2], S, cache, lam)
+            assert torch.equal(y, want[0]) and torch.equal(g, want[1]) and torch.equal(advanced, S + 1), (turn, sizes)
+            if decode4_workspace(*sizes, cuda).numel() == n:
+                got = relation_decode4(x[:, 0], x[:, 1], x[:, 2], S, cache, lam, workspace=ws)
+                assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (turn, sizes)
+
+
+@pytest.mark.parametrize("capacities", [(512, 5376, 1024), (5376, 300)])
+def test_one_batch_on_a_workspace_of_any_bytes(cuda, capacities):
+    """Calls of one B and H may be given another number of a workspace's bytes each time (a cache that grows)."""
+    from mote_amd.cache4 import decode4_workspace, relation_decode4
+
+    B, H, D = 2, 8, 96
+    need = {cap: decode4_workspace(B, H, D, cap, cuda).numel() for cap in capacities}
+    ws, lam = torch.zeros(max(need.values()), dtype=torch.uint8, device=cuda), torch.tensor(0.5, device=cuda)
+    for turn in range(2):
+        for cap in capacities:
+            x, S, cache = _step_inputs(cuda, 41 + turn, B, H, D, cap)
+            y, g, _ = _raw_step(x, S, cache, lam, ws[:need[cap]])
+            want = relation_decode4(x[:, 0], x[:, 1], x[:, 2], S, cache, lam)
+            assert torch.equal(y, want[0]) and torch.equal(g, want[1]), (turn, cap)
