@@ -189,6 +189,11 @@ class ArenaLayer:
         """(P2, I~) rows [0, upto) as [batch, H, upto, dh] views (head stride capacity * dh)."""
         return self.arena.p2(self.layer)[:, :, :upto], self.arena.info(self.layer)[:, :, :upto]
 
+    def extend(self, p2: torch.Tensor, info: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """`write`, and rows [0, n + T) as the new rows' own queries read them."""
+        self.write(p2, info)
+        return self.views(self.state.n + p2.shape[2])
+
 
 def _map_tensors(o: Any, fn: Callable[[torch.Tensor], Any]) -> Any:
     """`o` rebuilt with `fn` applied to every tensor inside it (lists, tuples, named tuples and

@@ -7,7 +7,7 @@
 
 `dtype` is the dtype that rows come in and are read back in (the model's); a row and head take 18 bytes per
 32 dims instead of 64 in bf16. What a window or a step adds takes part in it as it is: a prompt window's own
-rows are read unrounded by its own queries (ArenaLayer4.views), as relation_decode4's new chunk is; the rows
+rows are read unrounded by its own queries (ArenaLayer4.extend), as relation_decode4's new chunk is; the rows
 before it are read at their 4-bit values. A prompt in two windows therefore differs from one window by the
 rounding of the first window's rows, as it differs from the same arena in bf16.
 
@@ -92,37 +92,32 @@ class RelationArena4(RelationArena):
 class ArenaLayer4(ArenaLayer):
     """A layer of the state: `write` stores rows in 4 bits, `views` reads rows back."""
 
-    __slots__ = ("_fresh",)
+    __slots__ = ()
 
-    def __init__(self, arena: RelationArena4, layer: int, state: ArenaState):
-        super().__init__(arena, layer, state)
-        self._fresh: Optional[Tuple[int, torch.Tensor, torch.Tensor]] = None
+    def _cast(self, p2: torch.Tensor, info: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        return p2.to(self.arena.dtype), info.to(self.arena.dtype)
 
     def write(self, p2: torch.Tensor, info: torch.Tensor) -> None:
-        """Store T new rows [n, n + T) of every sequence; p2 / info are [batch, H, T, dh]. They are kept, as
-        they are, until the state moves on, for `views`."""
+        """Store T new rows [n, n + T) of every sequence; p2 / info are [batch, H, T, dh]."""
         n, T = self.state.n, p2.shape[2]
         if n + T > self.arena.capacity:
             raise RuntimeError(f"arena overflow: rows up to {n + T} in a capacity of {self.arena.capacity}")
-        dtype = self.arena.dtype
-        p2, info = p2.to(dtype), info.to(dtype)
-        cache4_write(self.arena.cache(self.layer), p2, info, n)
-        self._fresh = (n, p2, info)
+        cache4_write(self.arena.cache(self.layer), *self._cast(p2, info), n)
 
     def views(self, upto: int) -> Tuple[torch.Tensor, torch.Tensor]:
-        """(P2, I~) rows [0, upto) as new [batch, H, upto, dh] tensors in the arena's dtype: the rows written
-        through this object since the state last moved as they were given, the others at their 4-bit values."""
-        a, n = self.arena, self.state.n
-        held, take = upto, 0
-        if self._fresh is not None and self._fresh[0] == n < upto <= n + self._fresh[1].shape[2]:
-            held, take = n, upto - n
-        if not take:
-            return cache4_read(a.cache(self.layer), a.d_head, 0, upto, dtype=a.dtype)
-        new = tuple(t[:, :, :take] for t in self._fresh[1:])
-        if not held:
+        """(P2, I~) rows [0, upto) at their 4-bit values, as new [batch, H, upto, dh] tensors in the arena's dtype."""
+        return cache4_read(self.arena.cache(self.layer), self.arena.d_head, 0, upto, dtype=self.arena.dtype)
+
+    def extend(self, p2: torch.Tensor, info: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Store T new rows as `write` does; rows [0, n + T) for their own queries: the stored ones at their 4-bit
+        values, the new ones as they are. Nothing of them is kept beside the arena's rows."""
+        a, n, T = self.arena, self.state.n, p2.shape[2]
+        new = self._cast(p2, info)
+        self.write(*new)
+        if n == 0:
             return new
-        out = tuple(torch.empty(a.batch, a.n_heads, upto, a.d_head, device=a.device, dtype=a.dtype) for _ in range(2))
-        cache4_read(a.cache(self.layer), a.d_head, 0, held, out=tuple(t[:, :, :held] for t in out))
+        out = tuple(torch.empty(a.batch, a.n_heads, n + T, a.d_head, device=a.device, dtype=a.dtype) for _ in range(2))
+        cache4_read(a.cache(self.layer), a.d_head, 0, n, out=tuple(t[:, :, :n] for t in out))
         for t, rows in zip(out, new):
-            t[:, :, held:].copy_(rows)
+            t[:, :, n:].copy_(rows)
         return out

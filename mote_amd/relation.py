@@ -784,17 +784,17 @@ class FullRelation(nn.Module):
         arena = isinstance(cache, ArenaLayer)
         S = cache.n if arena else (0 if cache is None else cache[0].shape[2])
         p1 = self._heads_into(x, S, cache) if arena else None
-        if p1 is None:
+        if p1 is not None:
+            p2_all, info_all = cache.views(S + T)
+        else:
             p1, p2, info = self.heads(x, S)
             if arena:
-                cache.write(p2, info)
-        if arena:
-            p2_all, info_all = cache.views(S + T)
-        elif cache is not None:
-            p2_all = torch.cat([cache[0], p2], dim=2)
-            info_all = torch.cat([cache[1], info], dim=2)
-        else:
-            p2_all, info_all = p2, info
+                p2_all, info_all = cache.extend(p2, info)
+            elif cache is not None:
+                p2_all = torch.cat([cache[0], p2], dim=2)
+                info_all = torch.cat([cache[1], info], dim=2)
+            else:
+                p2_all, info_all = p2, info
         new_cache = cache if arena else (p2_all, info_all)
         if p2_all.dtype != p1.dtype:  # an arena kept in another dtype than the activations
             p1 = p1.to(p2_all.dtype)

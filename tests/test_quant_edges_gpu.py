@@ -81,3 +81,59 @@ def test_one_batch_on_a_workspace_of_any_bytes(cuda, capacities):
             y, g, _ = _raw_step(x, S, cache, lam, ws[:need[cap]])
             want = relation_decode4(x[:, 0], x[:, 1], x[:, 2], S, cache, lam)
             assert torch.equal(y, want[0]) and torch.equal(g, want[1]), (turn, cap)
+
+
+# ---- the arena's layers ----------------------------------------------------------------------------
+def test_a_layer_that_is_kept_reads_what_the_arena_holds(cuda):
+    """An ArenaLayer4 object gives the rows that are stored, whoever stored them last: another object of the layer,
+    a decode step, or itself from tensors that have changed since."""
+    from mote_amd.arena import ArenaState
+    from mote_amd.arena4 import RelationArena4
+    from mote_amd.cache4 import cache4_read, relation_decode4
+
+    B, H, D, T = 2, 4, 48, 20
+    state = ArenaState(RelationArena4(1, H, 64, D, cuda, BF16, batch=B), 5)
+    cache = state.arena.cache(0)
+    k, v, k2, v2 = (torch.randn(B, H, T, D, generator=_gen(50 + i)).to(BF16).to(cuda) for i in range(4))
+    layer = state[0]
+    held = lambda: cache4_read(cache, D, 0, 5 + T)
+    same = lambda: all(torch.equal(a, b) for a, b in zip(layer.views(5 + T), held()))
+    layer.write(k, v)
+    assert same() and same()
+    k.mul_(2.0)
+    assert same()
+    state[0].write(k2, v2)
+    assert same()
+    x = torch.randn(B, 3, H, D, generator=_gen(60)).to(BF16).to(cuda)
+    relation_decode4(x[:, 0], x[:, 1], x[:, 2], torch.full((B,), 5, device=cuda), cache, torch.tensor(0.5, device=cuda))
+    assert same()
+    state.advance(T)
+    state.n -= T
+    assert same()
+
+
+def test_a_window_reads_its_own_rows_as_they_are(cuda):
+    """What `extend` gives a window: the rows before it as they are stored, its own as they were given; the layer
+    that a forward hands back holds no rows of its own."""
+    from mote_amd.arena import ArenaState, RelationArena
+    from mote_amd.arena4 import RelationArena4
+    from mote_amd.cache4 import cache4_read
+    from mote_amd.relation import FullRelation
+
+    B, H, D = 2, 4, 48
+    for arena in (RelationArena4(1, H, 64, D, cuda, BF16, batch=B), RelationArena(1, H, 64, D, cuda, BF16, batch=B)):
+        state = ArenaState(arena)
+        for T in (11, 1, 30):
+            k, v = (torch.randn(B, H, T, D, generator=_gen(T + i)).to(cuda) for i in range(2))
+            before = [t.clone() for t in state[0].views(state.n)]
+            rows = state[0].extend(k, v)
+            for r, old, new in zip(rows, before, (k, v)):
+                assert r.shape == (B, H, state.n + T, D) and r.dtype == BF16
+                assert torch.equal(r[:, :, : state.n], old) and torch.equal(r[:, :, state.n:], new.to(BF16))
+            state.advance(T)
+    mixer = FullRelation(H * D, H, 0, device=cuda).to(BF16)
+    state = ArenaState(RelationArena4(1, H, 64, D, cuda, BF16, batch=B))
+    with torch.no_grad():
+        _, layer = mixer(torch.randn(B, 9, H * D, generator=_gen(70)).to(BF16).to(cuda), cache=state[0], return_cache=True)
+    assert not any(torch.is_tensor(getattr(layer, n, None)) for c in type(layer).__mro__ for n in getattr(c, "__slots__", ()))
+    assert all(torch.equal(a, b) for a, b in zip(layer.views(9), cache4_read(state.arena.cache(0), D, 0, 9)))
