@@ -690,7 +690,8 @@ int mote_dechunk_step(const mote_dechunk_step_args* args, void* stream);
  * byte i, dim 2 i + 1 the high half; a row's codes are padded to whole groups (16 G bytes).
  * mote_cache4: codes [B, H, capacity, 16 G] bytes and scales [B, H, capacity, G] bf16 of P2 and I~,
  * rows of one head back to back; batch and head strides in bytes for the codes (codes on 16-byte
- * boundaries), in elements for the scales.
+ * boundaries), in elements for the scales. Calls that write refuse strides by which sequences or heads share
+ * rows; P2's and I~'s must not lie over one another.
  * ------------------------------------------------------------------------------------------------ */
 typedef struct mote_cache4 {
   void* p2;

@@ -66,7 +66,8 @@ def cache4_read(cache: Cache4, d_head: int, start: Union[int, torch.Tensor] = 0,
 
     start: an int, or int64 [B] on the device (rows that it takes out of [0, capacity) read as NaN).
     rows: all from an int start on by default.
-    out: two views to write instead of new tensors (their dtype counts; any strides of whole 16-byte chunks)."""
+    out: two views to write instead of new tensors (their dtype counts; any strides of whole 16-byte chunks),
+        every row at a place of its own and none in the cache."""
     n, dev = _start(start)
     if rows is None:
         if dev is not None:

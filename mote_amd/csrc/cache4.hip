@@ -136,6 +136,9 @@ static int launch_rows4(const mote_cache4_rows_args* a, bool write, hipStream_t 
   const char* what = write ? "cache4_write" : "cache4_read";
   if (const int rc = check_rows4(a, what)) return rc;
   if (a->B == 0 || a->H == 0 || a->T == 0) return MOTE_OK;
+  if (write)
+    if (const char* bad = shared_cache4(a->cache, a->B, a->H, a->capacity, (a->D + kGroup4 - 1) / kGroup4))
+      return set_error(MOTE_ERR_ARGUMENT, "%s: %s", what, bad);
   Rows4Params p;
   const mote_view* v[2] = {&a->p2, &a->info};
   for (int k = 0; k < 2; ++k) {

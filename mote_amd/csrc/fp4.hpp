@@ -5,6 +5,10 @@
 // infinities and NaNs on top, so one comparison finds the groups that have no scale.
 #pragma once
 
+#include <algorithm>
+#include <cstdlib>
+#include <limits>
+
 #include "stream.hpp"
 
 namespace mote {
@@ -92,12 +96,27 @@ __device__ __forceinline__ void load_octet(const T* p, float (&x)[8]) {
     }
   }
 }
-// what a launcher checks of a cache in 4 bits: null pointers, alignment, strides that hold a row each
+// what a launcher checks of a cache in 4 bits: null pointers, alignment
 inline const char* bad_cache4(const mote_cache4& c) {
   if (!c.p2 || !c.p2_scale || !c.info || !c.info_scale) return "null pointer";
   const uintptr_t codes = reinterpret_cast<uintptr_t>(c.p2) | reinterpret_cast<uintptr_t>(c.info);
   const uintptr_t scales = reinterpret_cast<uintptr_t>(c.p2_scale) | reinterpret_cast<uintptr_t>(c.info_scale);
   if (codes % 16 || c.codes_sb % 16 || c.codes_sh % 16 || scales % 2) return "codes must start on 16-byte boundaries";
+  return nullptr;
+}
+// and of one that it writes: every sequence and head has rows of its own
+inline const char* shared_cache4(const mote_cache4& c, int64_t B, int64_t H, int64_t capacity, int64_t groups) {
+  auto apart = [&](int64_t sb, int64_t sh, int64_t block) {
+    sb = B > 1 ? std::abs(sb) : std::numeric_limits<int64_t>::max();
+    sh = H > 1 ? std::abs(sh) : std::numeric_limits<int64_t>::max();
+    const bool by_head = sh < sb;
+    const int64_t low = std::min(sb, sh), high = std::max(sb, sh), n = by_head ? H : B;
+    if (B <= 1 && H <= 1) return true;
+    if (low < block) return false;
+    return B <= 1 || H <= 1 || (high - block) / low >= n - 1;
+  };
+  if (!apart(c.codes_sb, c.codes_sh, capacity * 16 * groups) || !apart(c.scale_sb, c.scale_sh, capacity * groups))
+    return "sequences or heads share rows";
   return nullptr;
 }
 

@@ -508,6 +508,8 @@ int launch_decode4(const mote_relation_decode4_args* a, hipStream_t stream) {
   if (!a->workspace || a->workspace_bytes < w.total || reinterpret_cast<uintptr_t>(a->workspace) % 16)
     return set_error(MOTE_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes, %zu needed", what, a->workspace_bytes,
                      w.total);
+  if (const char* bad = shared_cache4(a->cache, a->B, a->H, a->capacity, groups4(a->D)))
+    return set_error(MOTE_ERR_ARGUMENT, "%s: %s", what, bad);
   Dec4Params p;
   p.lam = a->lam; p.S = a->S;
   p.rope = a->inv_freq != nullptr;

@@ -9,10 +9,13 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <array>
 #include <climits>
 #include <initializer_list>
 #include <string>
 #include <tuple>
+#include <utility>
 #include <vector>
 
 #include "../../include/mote_relation.h"
@@ -427,6 +430,49 @@ void apart(const Tensor& out, int64_t out_width, const Tensor& in, int64_t in_wi
   }
   bad_value(what, ": the output lies over an input");
 }
+// Whether every element of a view has an address of its own: taken by stride, a step passes all that the smaller
+// ones reach. With `other`, a view of as many dims and the same sizes, the two taken together (as one view with a
+// dim of two more where their strides agree, by the ranges that they span where not).
+bool separate(const Tensor& t, const Tensor* other = nullptr) {
+  if (t.numel() == 0) return true;
+  constexpr int kMost = 8;
+  std::array<std::pair<int64_t, int64_t>, kMost + 1> dim;  // stride, size
+  int n = 0;
+  bool alike = true;
+  int64_t span = 1, span2 = 1;
+  for (int64_t i = 0; i < t.dim() && n < kMost; ++i) {
+    if (t.size(i) == 1) continue;
+    dim[n++] = {t.stride(i), t.size(i)};
+    span += (t.size(i) - 1) * t.stride(i);
+    if (other) {
+      alike = alike && other->stride(i) == t.stride(i);
+      span2 += (other->size(i) - 1) * other->stride(i);
+    }
+  }
+  if (other) {
+    const int64_t e = t.element_size(), a = reinterpret_cast<int64_t>(t.data_ptr()), b = reinterpret_cast<int64_t>(other->data_ptr());
+    if (b >= a + span * e || a >= b + span2 * e) return separate(t) && separate(*other);
+    if (!alike || (b - a) % e) return false;
+    dim[n++] = {b > a ? (b - a) / e : (a - b) / e, 2};
+  }
+  std::sort(dim.begin(), dim.begin() + n);
+  int64_t reach = 1;
+  for (int i = 0; i < n; ++i) {
+    if (dim[i].first < reach) return false;
+    reach += dim[i].first * (dim[i].second - 1);
+  }
+  return true;
+}
+// whether the ranges of memory that two views span are apart
+bool ranges_apart(const Tensor& a, const Tensor& b) {
+  auto end = [](const Tensor& t) {
+    int64_t span = 1;
+    for (int64_t i = 0; i < t.dim(); ++i) span += (t.size(i) - 1) * t.stride(i);
+    return reinterpret_cast<int64_t>(t.data_ptr()) + span * t.element_size();
+  };
+  if (a.numel() == 0 || b.numel() == 0) return true;
+  return reinterpret_cast<int64_t>(a.data_ptr()) >= end(b) || reinterpret_cast<int64_t>(b.data_ptr()) >= end(a);
+}
 // an int64 position per sequence (read, and with `advance` written, by the kernel as it is)
 void positions(const Tensor& t, int64_t B, c10::Device dev, const char* what, const char* name) {
   if (t.scalar_type() != at::kLong || t.device() != dev || t.numel() != B || !t.is_contiguous())
@@ -451,16 +497,15 @@ Cache4 cache4(const Tensor& p2, const Tensor& s2, const Tensor& info, const Tens
       bad_value(what, ": the rows of a head must lie back to back (", name, ")");
     for (int d = 0; d < 2; ++d) {
       if (t.size(d) > 1 && t.stride(d) != like.stride(d)) bad_value(what, ": P2 and I~ must have the same strides");
-      // heads (or sequences) that share rows would be written over one another
-      if (writes && t.size(d) > 1 && t.stride(d) == 0) bad_value(what, ": ", name, " holds its rows for several heads at once");
     }
+    // heads (or sequences) that share rows would be written over one another
+    if (writes && !separate(t)) bad_value(what, ": ", name, " holds its rows for several heads at once");
   };
-  if (writes && (p2.data_ptr() == info.data_ptr() || s2.data_ptr() == si.data_ptr()))
-    bad_value(what, ": P2 and I~ must not be the same rows");
   check(p2, p2, 16 * G, at::kByte, "the codes of P2");
   check(info, p2, 16 * G, at::kByte, "the codes of I~");
   check(s2, s2, G, at::kBFloat16, "the scales of P2");
   check(si, s2, G, at::kBFloat16, "the scales of I~");
+  if (writes && (!separate(p2, &info) || !separate(s2, &si))) bad_value(what, ": P2 and I~ must not be the same rows");
   Cache4 r;
   r.c = mote_cache4{p2.data_ptr(), s2.data_ptr(), info.data_ptr(), si.data_ptr(),
                     p2.size(0) > 1 ? p2.stride(0) : 0, p2.size(1) > 1 ? p2.stride(1) : 0,
@@ -523,9 +568,11 @@ std::tuple<Tensor, Tensor> cache4_read(const Tensor& k, const Tensor& ks, const 
     for (const Tensor* t : {&p2, &info}) {
       if (t->dim() != 4 || t->size(0) != B || t->size(1) != H || t->size(2) != rows || t->size(3) != D || t->device() != k.device())
         bad_value(what, ": out must be two [B, H, rows, D] tensors on the cache's device");
-      for (int d = 0; d < 3; ++d)
-        if (t->size(d) > 1 && t->stride(d) == 0) bad_value(what, ": out holds its rows for several places at once");
+      if (!separate(*t)) bad_value(what, ": out holds its rows for several places at once");
+      for (const Tensor* held : {&k, &ks, &v, &vs})
+        if (!ranges_apart(*t, *held)) bad_value(what, ": out lies over the cache");
     }
+    if (!separate(p2, &info)) bad_value(what, ": the two tensors of out lie over one another");
     if (info.scalar_type() != p2.scalar_type()) throw py::type_error("cache4_read: out must be two tensors of one dtype");
     if (p2.requires_grad() || info.requires_grad()) throw std::runtime_error("cache4_read: out must not require a gradient");
   }
