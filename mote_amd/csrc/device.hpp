@@ -1,4 +1,4 @@
-// The current device's CU count, asked once per device (host code).
+// The current device's CU count, asked once per device, and what a launch can hold (host code).
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -18,5 +18,8 @@ inline int device_cu_count() {
   known[dev].store(cus, std::memory_order_relaxed);
   return cus;
 }
+
+// whether a grid's first dimension of so many workgroups can be launched: below 2^32 threads
+inline bool grid_fits(int64_t workgroups, int threads) { return workgroups * threads < (int64_t(1) << 32); }
 
 }  // namespace mote

@@ -472,13 +472,19 @@ int8_many_kernel(const Many8Params p) {
 }
 
 // ------------------------------------------------------------------------------------------------
+constexpr int kQuantMost = 1 << 25;  // rows of a launch: up to 64 threads each, and a grid holds fewer than 2^32
+
 template <typename T>
-static void quantize(const void* x, int64_t x_sr, int M, int K, int8_t* q, float* scale, hipStream_t stream) {
+static int quantize(const void* x, int64_t x_sr, int M, int K, int8_t* q, float* scale, hipStream_t stream, const char* what) {
   const int Kp = int(padded_k8(K));
   auto go = [&](auto kernel, int lanes) {
     const int rows = 64 / lanes * kQuantWaves;
-    hipLaunchKernelGGL(kernel, dim3(unsigned((int64_t(M) + rows - 1) / rows)), dim3(64 * kQuantWaves), 0, stream,
-                       reinterpret_cast<const T*>(x), x_sr, M, K, Kp, q, scale);
+    for (int64_t m0 = 0; m0 < M; m0 += kQuantMost) {
+      const int part = int(std::min<int64_t>(M - m0, kQuantMost));
+      hipLaunchKernelGGL(kernel, dim3(unsigned((part + rows - 1) / rows)), dim3(64 * kQuantWaves), 0, stream,
+                         reinterpret_cast<const T*>(x) + m0 * x_sr, x_sr, part, K, Kp, q + m0 * Kp, scale + m0);
+    }
+    return check_launch(what);
   };
   // A row's share of a wave is as wide as the row needs, so that no lane idles and a row stays in registers:
   // 35304 x 64 11.2 -> 4.7 us and 16384 x 768 9.7 -> 8.1 us against a wave per row; 19417 x 3776 48 -> 37.6 us
@@ -502,9 +508,8 @@ int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream) {
   if (!a->x || !a->q || !a->scale) return set_error(MOTE_ERR_ARGUMENT, "%s: null pointer", what);
   if (a->M > 1 && a->x_sr < 0) return set_error(MOTE_ERR_ARGUMENT, "%s: negative row stride", what);
   if (reinterpret_cast<uintptr_t>(a->q) % 16) return set_error(MOTE_ERR_ARGUMENT, "%s: q must start on a 16-byte boundary", what);
-  if (a->dtype == MOTE_BF16) quantize<bf16_t>(a->x, a->x_sr, a->M, a->K, a->q, a->scale, stream);
-  else quantize<float>(a->x, a->x_sr, a->M, a->K, a->q, a->scale, stream);
-  return check_launch(what);
+  return a->dtype == MOTE_BF16 ? quantize<bf16_t>(a->x, a->x_sr, a->M, a->K, a->q, a->scale, stream, what)
+                               : quantize<float>(a->x, a->x_sr, a->M, a->K, a->q, a->scale, stream, what);
 }
 
 // The one-launch form: for up to 16 tokens (16 x 768 -> 768 4.8 us, 6.4 with quantize_rows and tiles; 16 x
@@ -524,28 +529,29 @@ size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a) {
 }
 
 template <typename T>
-static void launch_few8(const mote_int8_linear_args* a, hipStream_t stream) {
+static int launch_few8(const mote_int8_linear_args* a, hipStream_t stream, const char* what) {
   Few8Params p;
   p.x = a->x; p.x_sr = a->x_sr; p.w = a->wq; p.sw = a->w_scale; p.y = a->y; p.y_sr = a->y_sr;
   p.run = a->run; p.g = a->xm ? a->g : nullptr; p.xm = a->xm; p.heads = a->xm ? a->heads : 0;
   p.M = a->M; p.N = a->N; p.K = a->K; p.Kp = int(padded_k8(a->K));
   auto go = [&](auto kernel, int waves) {
     const dim3 grid(unsigned((a->N + 15) / 16), unsigned((a->M + 15) / 16));
+    if (!grid_fits(grid.x, 64 * waves)) return set_error(MOTE_ERR_SHAPE, "%s: N = %d is too many channels for one launch", what, a->N);
     hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, stream, p);
+    return check_launch(what);
   };
   // Beyond K = 1024 eight waves (16 x 4096 -> 4096 11.4 -> 10.4 us, 1 x 2048 -> 2048 5.5 -> 5.2), four up to there
   // (16 x 768 -> 2304 4.7 us, 4.9 with eight).
-  if (p.Kp <= 1024) go(int8_few_kernel<T, 4, 4>, 4);
-  else if (p.Kp <= 2048) go(int8_few_kernel<T, 8, 4>, 8);
-  else go(int8_few_kernel<T, 8, 8>, 8);
+  if (p.Kp <= 1024) return go(int8_few_kernel<T, 4, 4>, 4);
+  if (p.Kp <= 2048) return go(int8_few_kernel<T, 8, 4>, 8);
+  return go(int8_few_kernel<T, 8, 8>, 8);
 }
 
 template <typename T>
-static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
+static int launch_many8(const mote_int8_linear_args* a, hipStream_t stream, const char* what) {
   const int Kp = int(padded_k8(a->K));
   int8_t* xq = reinterpret_cast<int8_t*>(a->workspace);
   float* sx = reinterpret_cast<float*>(xq + size_t(a->M) * Kp);
-  quantize<T>(a->x, a->x_sr, a->M, a->K, xq, sx, stream);
   Many8Params p;
   p.x = xq; p.sx = sx; p.w = a->wq; p.sw = a->w_scale; p.y = a->y; p.y_sr = a->y_sr;
   p.M = a->M; p.N = a->N; p.Kp = Kp;
@@ -560,8 +566,11 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
     // rows 53 -> 51 us; of 1.8 MB: 4964 x 768 -> 2304 24 us in one group, 26 us in three).
     const int groups = int64_t(a->N) * Kp <= (5 << 19) ? 1 : (p.nch + 7) / 8;
     p.gch = (p.nch + groups - 1) / groups;
-    const unsigned per = unsigned((int64_t(p.ntok) * p.nch + 7) / 8);
-    hipLaunchKernelGGL(kernel, dim3(8 * per), dim3(64 * waves), 0, stream, p);
+    const int64_t grid = (int64_t(p.ntok) * p.nch + 7) / 8 * 8;
+    if (!grid_fits(grid, 64 * waves)) return set_error(MOTE_ERR_SHAPE, "%s: M = %d, N = %d are too many tiles for one launch", what, a->M, a->N);
+    if (const int rc = quantize<T>(a->x, a->x_sr, a->M, a->K, xq, sx, stream, what)) return rc;
+    hipLaunchKernelGGL(kernel, dim3(unsigned(grid)), dim3(64 * waves), 0, stream, p);
+    return check_launch(what);
   };
   // Tiles of channels x tokens. One round of workgroups of a small tile while that holds everything. Transfers into
   // LDS reach some 47 bytes a nanosecond per CU, so few tiles go to as many CUs as there are: 32 x 16 (258 x 3413
@@ -591,10 +600,10 @@ static void launch_many8(const mote_int8_linear_args* a, hipStream_t stream) {
   const double big = rounds_us(tiles(256, 256), cus, 7.3, 1.5), wide = rounds_us(tiles(256, 192), cus, 5.6, 1.15),
                tall = rounds_us(tiles(192, 256), cus, 5.6, 1.15), mid = rounds_us(tiles(128, 128), 2 * cus, 3.5, 0.94);
   const double best = std::min(std::min(big, wide), std::min(tall, mid));
-  if (big == best) go(int8_many_kernel<T, 8, 4, 2, 4, 2>, 256, 256, 8);
-  else if (wide == best) go(int8_many_kernel<T, 8, 3, 2, 4, 2>, 256, 192, 8);
-  else if (tall == best) go(int8_many_kernel<T, 6, 4, 2, 4, 2>, 192, 256, 8);
-  else go(int8_many_kernel<T, 4, 4, 2, 2, 2>, 128, 128, 4);
+  if (big == best) return go(int8_many_kernel<T, 8, 4, 2, 4, 2>, 256, 256, 8);
+  if (wide == best) return go(int8_many_kernel<T, 8, 3, 2, 4, 2>, 256, 192, 8);
+  if (tall == best) return go(int8_many_kernel<T, 6, 4, 2, 4, 2>, 192, 256, 8);
+  return go(int8_many_kernel<T, 4, 4, 2, 2, 2>, 128, 128, 4);
 }
 
 int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream) {
@@ -610,18 +619,12 @@ int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream) {
   if (a->M > 1 && (a->x_sr < 0 || a->y_sr < a->N)) return set_error(MOTE_ERR_ARGUMENT, "%s: row strides shorter than the rows", what);
   if (reinterpret_cast<uintptr_t>(a->wq) % 16) return set_error(MOTE_ERR_ARGUMENT, "%s: wq must start on a 16-byte boundary", what);
   if (a->xm && (!a->g || a->heads <= 0)) return set_error(MOTE_ERR_ARGUMENT, "%s: xm needs g and heads > 0", what);
-  if (few8(a)) {
-    if (a->dtype == MOTE_BF16) launch_few8<bf16_t>(a, stream);
-    else launch_few8<float>(a, stream);
-    return check_launch(what);
-  }
+  if (few8(a)) return a->dtype == MOTE_BF16 ? launch_few8<bf16_t>(a, stream, what) : launch_few8<float>(a, stream, what);
   if (a->run || a->xm) return set_error(MOTE_ERR_SHAPE, "%s: run and xm need at most %d rows of K <= %d", what, kFewRows, kFewMaxK);
   const size_t need = int8_linear_workspace_bytes(a);
   if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)
     return set_error(MOTE_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes, %zu needed", what, a->workspace_bytes, need);
-  if (a->dtype == MOTE_BF16) launch_many8<bf16_t>(a, stream);
-  else launch_many8<float>(a, stream);
-  return check_launch(what);
+  return a->dtype == MOTE_BF16 ? launch_many8<bf16_t>(a, stream, what) : launch_many8<float>(a, stream, what);
 }
 
 }  // namespace mote

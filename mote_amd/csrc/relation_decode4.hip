@@ -510,6 +510,8 @@ int launch_decode4(const mote_relation_decode4_args* a, hipStream_t stream) {
                      w.total);
   if (const char* bad = shared_cache4(a->cache, a->B, a->H, a->capacity, groups4(a->D)))
     return set_error(MOTE_ERR_ARGUMENT, "%s: %s", what, bad);
+  if (!grid_fits(int64_t(a->B) * a->H * w.nsplit, kD4Threads))
+    return set_error(MOTE_ERR_SHAPE, "%s: %d sequences of %d heads are too many for one launch", what, a->B, a->H);
   Dec4Params p;
   p.lam = a->lam; p.S = a->S;
   p.rope = a->inv_freq != nullptr;

@@ -122,3 +122,20 @@ def test_c_entry_points_refuse_caches_that_share_rows():
             c.scale_sb, c.scale_sh = (H * head, head) if codes else (sb // 16, sh // 16)
             for call in (rows, step):
                 assert call(c) == 1 and b"share rows" in lib.mote_last_error(), (sb, sh, codes, call)
+
+
+def test_sizes_beyond_a_launch_are_refused():
+    """A grid holds fewer than 2^32 threads: what needs more is refused before anything is launched."""
+    lib = L.lib()
+    w = L.Int8LinearArgs()
+    w.dtype, w.x, w.wq, w.w_scale, w.y, w.workspace, w.workspace_bytes = L.MOTE_BF16, *(16,) * 5, 1 << 62
+    for M, N, K in ((1, 1 << 28, 128), (16, 1 << 27, 2048), (1 << 20, 1 << 19, 64), (1 << 30, 1 << 13, 1)):
+        w.M, w.N, w.K, w.x_sr, w.y_sr = M, N, K, K, N
+        assert lib.mote_int8_linear(w, None) == 2 and b"for one launch" in lib.mote_last_error(), (M, N, K)
+    a = L.Decode4Args()
+    a.dtype, a.B, a.H, a.D, a.capacity = L.MOTE_BF16, 1 << 23, 2, 8, 1
+    a.lam = a.S = a.p1 = a.p2 = a.info = a.y = a.g = a.workspace = 16
+    a.workspace_bytes = int(lib.mote_relation_decode4_workspace(a))
+    a.cache.p2 = a.cache.info = a.cache.p2_scale = a.cache.info_scale = 16
+    a.cache.codes_sb, a.cache.codes_sh, a.cache.scale_sb, a.cache.scale_sh = 32, 16, 2, 1
+    assert lib.mote_relation_decode4(a, None) == 2 and b"for one launch" in lib.mote_last_error()

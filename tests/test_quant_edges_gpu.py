@@ -137,3 +137,27 @@ def test_a_window_reads_its_own_rows_as_they_are(cuda):
         _, layer = mixer(torch.randn(B, 9, H * D, generator=_gen(70)).to(BF16).to(cuda), cache=state[0], return_cache=True)
     assert not any(torch.is_tensor(getattr(layer, n, None)) for c in type(layer).__mro__ for n in getattr(c, "__slots__", ()))
     assert all(torch.equal(a, b) for a, b in zip(layer.views(9), cache4_read(state.arena.cache(0), D, 0, 9)))
+
+
+# ---- sizes at a launch's limit -----------------------------------------------------------------------
+def test_more_rows_than_one_launch_quantises(cuda):
+    """Past 2^28 rows: the codes and scales of every row, and products of the first rows, the last ones and those
+    beside the borders between launches."""
+    from mote_amd.int8 import int8_linear, int8_weight, quantize_rows
+
+    M = (1 << 28) + 5
+    x = torch.empty(M, 1, device=cuda, dtype=BF16)
+    for a in range(0, M, 1 << 25):  # whole numbers up to 125: exact in bf16
+        n = min(1 << 25, M - a)
+        x[a: a + n, 0] = (torch.arange(a, a + n, device=cuda) % 251 - 125).to(BF16)
+    q, s = quantize_rows(x)
+    for a in range(0, M, 1 << 25):
+        part, b = x[a: a + (1 << 25), 0].float(), min(a + (1 << 25), M)
+        assert torch.equal(q[a:b, 0].float(), 127 * part.sign()), a
+        assert torch.equal(s[a:b], torch.div(part.abs(), torch.full_like(part, 127.0))), a
+        assert (q[a: a + 1000, 1:] == 0).all() and (q[b - 1000: b, 1:] == 0).all()
+    del q, s
+    w8 = int8_weight(torch.tensor([[3.0]], device=cuda))
+    y = int8_linear(x, w8)
+    for a in (0, *range((1 << 25) - 8, M, 1 << 25), M - 16):
+        assert torch.equal(y[a: a + 16], int8_linear(x[a: a + 16], w8)), a
