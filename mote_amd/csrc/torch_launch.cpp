@@ -486,6 +486,7 @@ struct Cache4 {
 Cache4 cache4(const Tensor& p2, const Tensor& s2, const Tensor& info, const Tensor& si, int64_t B, int64_t H, int64_t D,
               c10::Device dev, bool writes, const char* what) {
   if (D <= 0 || D > 128 || D % 8) bad_value(what, ": head dim ", D, " unsupported (need 8 <= D <= 128, D % 8 == 0)");
+  if (B > INT_MAX || H > INT_MAX) bad_value(what, ": ", B, " sequences of ", H, " heads (sizes beyond 32 bits)");
   const int64_t G = (D + 31) / 32;
   const int64_t cap = p2.dim() == 4 ? p2.size(2) : 0;
   auto check = [&](const Tensor& t, const Tensor& like, int64_t width, at::ScalarType dt, const char* name) {
@@ -517,6 +518,7 @@ Cache4 cache4(const Tensor& p2, const Tensor& s2, const Tensor& info, const Tens
 
 void rows_of_start(mote_cache4_rows_args& a, const Cache4& c, int64_t start, const OptTensor& start_dev, const OptTensor& lens,
                    int64_t B, int64_t T, c10::Device dev, const char* what) {
+  if (T > INT_MAX) bad_value(what, ": ", T, " rows (sizes beyond 32 bits)");
   if (start_dev) {
     positions(*start_dev, B, dev, what, "start");
     a.start_dev = static_cast<const int64_t*>(start_dev->data_ptr());

@@ -139,3 +139,20 @@ def test_sizes_beyond_a_launch_are_refused():
     a.cache.p2 = a.cache.info = a.cache.p2_scale = a.cache.info_scale = 16
     a.cache.codes_sb, a.cache.codes_sh, a.cache.scale_sb, a.cache.scale_sh = 32, 16, 2, 1
     assert lib.mote_relation_decode4(a, None) == 2 and b"for one launch" in lib.mote_last_error()
+
+
+def test_more_rows_than_32_bits_count_are_refused():
+    """With device positions the capacity does not bound the number of rows: one that 32 bits cannot hold is
+    refused, not cut."""
+    from mote_amd.cache4 import cache4_read, cache4_write
+
+    c, start = _cache(1, 2, 64, 48), torch.zeros(1, dtype=torch.int64)
+    for T in (1 << 31, (1 << 32) + 4):
+        rows = torch.zeros(1, 2, 1, 48, dtype=BF16).expand(1, 2, T, 48)
+        with pytest.raises(ValueError, match="32 bits"):
+            cache4_write(c, rows, rows, start)
+        with pytest.raises(ValueError, match="32 bits"):
+            cache4_read(c, 48, start, T)
+    one = [t[:1, :1, :1, :].expand(1 << 32, 1, 1, t.shape[3]) for t in c]
+    with pytest.raises(ValueError, match="32 bits"):
+        cache4_read(type(c)(*one), 48)
