@@ -5,6 +5,7 @@
 // so do checks of what a call may pass, except the sizes, types and devices of operands whose extent the
 // kernel takes from another one: those are compared here. RuntimeError with the library's message
 // when a call fails. Host code only; streams come as raw handles.
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
@@ -412,7 +413,15 @@ struct On {
   void* stream;
   explicit On(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
+// Refuses tensors whose derivative would be lost: tangents of forward mode (which no_grad leaves on), gradients
+// under grad mode.
+void no_tangent(const char* what, std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts)
+    if (t->_fw_grad(0).defined()) throw std::runtime_error(c10::str(what, " has no forward-mode derivative: it takes no dual tensors"));
+}
 void no_grad(const char* what, std::initializer_list<const Tensor*> ts) {
+  no_tangent(what, ts);
   if (!at::GradMode::is_enabled()) return;
   for (const Tensor* t : ts)
     if (t->requires_grad()) throw std::runtime_error(c10::str(what, " has no backward: call it under torch.no_grad()"));
@@ -577,6 +586,7 @@ std::tuple<Tensor, Tensor> cache4_read(const Tensor& k, const Tensor& ks, const 
     if (!separate(p2, &info)) bad_value(what, ": the two tensors of out lie over one another");
     if (info.scalar_type() != p2.scalar_type()) throw py::type_error("cache4_read: out must be two tensors of one dtype");
     if (p2.requires_grad() || info.requires_grad()) throw std::runtime_error("cache4_read: out must not require a gradient");
+    no_tangent(what, {&p2, &info});
   }
   a.dtype = code(out2 ? p2.scalar_type() : dtype);
   on_gpu(k, what);

@@ -156,3 +156,28 @@ def test_more_rows_than_32_bits_count_are_refused():
     one = [t[:1, :1, :1, :].expand(1 << 32, 1, 1, t.shape[3]) for t in c]
     with pytest.raises(ValueError, match="32 bits"):
         cache4_read(type(c)(*one), 48)
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives are not dropped in silence, under no_grad neither (which leaves forward mode on)."""
+    from mote_amd.cache4 import cache4_read, cache4_write, relation_decode4
+    from mote_amd.int8 import Int8Weight, int8_linear, quantize_rows
+
+    fwd = torch.autograd.forward_ad
+    c, S, lam = _cache(), torch.zeros(2, dtype=torch.int64), torch.tensor(0.5)
+    rows, x = torch.zeros(2, 4, 8, 48, dtype=BF16), torch.zeros(2, 4, 48, dtype=BF16)
+    w, t = Int8Weight(torch.zeros(16, 128, dtype=torch.int8), torch.zeros(16), 48), torch.zeros(4, 48)
+    with fwd.dual_level():
+        dual = lambda v: fwd.make_dual(v, torch.ones_like(v))
+        calls = [lambda: cache4_write(c, dual(rows), rows), lambda: cache4_write(c, rows, dual(rows)),
+                 lambda: relation_decode4(dual(x), x, x, S, c, lam), lambda: relation_decode4(x, x, dual(x), S, c, lam),
+                 lambda: cache4_read(c, 48, 0, 8, out=(dual(rows), rows.clone())),
+                 lambda: quantize_rows(dual(t)), lambda: int8_linear(dual(t), w)]
+        for grad in (True, False):
+            for call in calls:
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+        with pytest.raises(RuntimeError, match="MI355X"):
+            int8_linear(t, w)
+        with fwd._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="MI355X"):
+            int8_linear(dual(t), w)
