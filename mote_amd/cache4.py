@@ -6,7 +6,8 @@ has every rounding point): 18 bytes a group, 3.6 times fewer than bf16. Scales f
 own 32 values, so channels of unlike size and single outliers cost their own group only. A group that holds a
 NaN or an infinity reads back as NaN.
 
-Nothing here has a backward: calls whose rows require a gradient are refused under grad mode.
+Nothing here has a derivative: calls with rows, parameters or outputs that require a gradient are refused under
+grad mode, those with dual tensors always.
 """
 
 from __future__ import annotations
@@ -102,6 +103,7 @@ def relation_decode4(p1: torch.Tensor, p2: torch.Tensor, info: torch.Tensor, S: 
     p1, p2, info: raw projections of the new chunk, [B, H, dh] (head stride dh, any batch stride), bf16 or
         fp32; the step's arithmetic rounds to that dtype where relation_decode rounds to the cache's.
     S: int64 [B] device positions. S[b] outside [0, capacity): NaN in y[b] and g[b], nothing stored.
+    lam, inv_freq, theta: a layer's own parameters are taken under torch.no_grad() (they have no backward here).
     Returns (y [B, H, dh], g [B, H] fp32)."""
     return L.native().relation_decode4(p1, p2, info, S, *cache, lam, tau_s, inv_freq, theta, layer_idx, advance, workspace,
                                        y, g, xm, run, rope_f32)

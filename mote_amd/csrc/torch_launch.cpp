@@ -413,8 +413,8 @@ struct On {
   void* stream;
   explicit On(const Tensor& t) : guard(t.device()), stream(c10::hip::getCurrentHIPStream(t.device().index()).stream()) {}
 };
-// Refuses tensors whose derivative would be lost: tangents of forward mode (which no_grad leaves on), gradients
-// under grad mode.
+// Refuses tensors, parameters and given outputs among them, whose derivative would be lost: tangents of forward
+// mode (which no_grad leaves on), gradients under grad mode.
 void no_tangent(const char* what, std::initializer_list<const Tensor*> ts) {
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
   for (const Tensor* t : ts)
@@ -649,7 +649,9 @@ std::tuple<Tensor, Tensor> relation_decode4(const Tensor& p1, const Tensor& p2, 
     bad_value(what, ": g must be a contiguous fp32 [B, H] tensor");
   if (y_)
     for (const Tensor* t : {&p1, &p2, &info}) apart(*y_, H * D, *t, H * D, B, what);
-  no_grad(what, {&p1, &p2, &info});
+  no_grad(what, {&p1, &p2, &info, &lam});
+  for (const OptTensor* t : {&inv_freq, &theta, &y_, &g_, &xm})
+    if (*t) no_grad(what, {&**t});
   on_gpu(p1, what);
   const On on(p1);
   Tensor y = y_ ? *y_ : empty({B, H, D}, p1, p1.scalar_type());
@@ -718,7 +720,9 @@ Tensor int8_linear(const Tensor& x_, const Tensor& wq, const Tensor& ws, int64_t
   if (xm && (!g || g->scalar_type() != at::kFloat || xm->scalar_type() != at::kFloat || !g->is_contiguous() || !xm->is_contiguous() ||
              g->dim() != 2 || g->size(0) != M || xm->numel() != M || g->device() != x_.device() || xm->device() != x_.device()))
     bad_value(what, ": xm needs fp32 contiguous g [M, H] and xm [M] on x's device");
-  no_grad(what, {&x_});
+  no_grad(what, {&x_, &ws});
+  for (const OptTensor* t : {&out, &xm, &g})
+    if (*t) no_grad(what, {&**t});
   TORCH_CHECK(M <= INT_MAX && N <= INT_MAX && K <= INT_MAX, "int8_linear: sizes beyond 32 bits");
   const Tensor x = unit(x_.dim() == 2 ? x_ : x_.reshape({M, K}));
   Tensor y2;

@@ -5,8 +5,9 @@
 
 A row's scale is max|row| / 127 and its codes are rint(x (127 / max|row|)); the products are summed exactly in
 32-bit integers, so y = (acc sx) sw depends on nothing but the codes and scales (no order of summation, no
-split). A token with a NaN or an infinity gives a row of NaN. Serving only: there is no backward, and calls
-whose x requires a gradient are refused under grad mode.
+split). A token with a NaN or an infinity gives a row of NaN. Serving only: there is no derivative, and calls
+with tensors that require a gradient are refused under grad mode, those with dual tensors always (`int8_weight`
+takes a parameter as the constant that it is at the time).
 """
 
 from __future__ import annotations

@@ -181,3 +181,25 @@ def test_tangents_are_refused():
             int8_linear(t, w)
         with fwd._set_fwd_grad_enabled(False), pytest.raises(RuntimeError, match="MI355X"):
             int8_linear(dual(t), w)
+
+
+def test_parameters_and_outputs_that_want_a_gradient_are_refused():
+    from mote_amd.cache4 import relation_decode4
+    from mote_amd.int8 import Int8Weight, int8_linear
+
+    c, S = _cache(), torch.zeros(2, dtype=torch.int64)
+    x, want = torch.zeros(2, 4, 48, dtype=BF16), lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, requires_grad=True)
+    args = dict(lam=torch.tensor(0.5))
+    w, t = Int8Weight(torch.zeros(16, 128, dtype=torch.int8), torch.zeros(16), 48), torch.zeros(2, 48)
+    calls = [(lambda **kw: relation_decode4(x, x, x, S, c, **{**args, **kw}), name, value) for name, value in
+             (("lam", want(())), ("inv_freq", want(24)), ("theta", want(2)), ("y", want(2, 4, 48, dt=BF16)),
+              ("g", want(2, 4)), ("xm", want(2)))]
+    calls += [(lambda **kw: int8_linear(t, **{"w": w, **kw}), name, value) for name, value in
+              (("w", w._replace(scale=want(16))), ("out", want(2, 16)))]
+    calls += [(lambda **kw: int8_linear(t, w, **{"g": torch.zeros(2, 4), "xm": torch.zeros(2), **kw}), name, value) for name, value in
+              (("g", want(2, 4)), ("xm", want(2)))]
+    for call, name, value in calls:
+        with pytest.raises(RuntimeError, match="no backward"):
+            call(**{name: value})
+        with torch.no_grad(), pytest.raises(RuntimeError, match="MI355X"):
+            call(**{name: value})
