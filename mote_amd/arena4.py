@@ -38,8 +38,10 @@ class RelationArena4(RelationArena):
 
     def _zeros(self, capacity: int) -> torch.Tensor:
         shape = (self.n_layers, 2, self.batch, self.n_heads, capacity)
-        self.scales = torch.zeros((*shape, self.groups), device=self.device, dtype=torch.bfloat16)
-        return torch.zeros((*shape, 16 * self.groups), device=self.device, dtype=torch.uint8)
+        scales = torch.zeros((*shape, self.groups), device=self.device, dtype=torch.bfloat16)
+        codes = torch.zeros((*shape, 16 * self.groups), device=self.device, dtype=torch.uint8)
+        self.scales = scales  # once both are there: a growth that fails leaves the arena as it was
+        return codes
 
     @property
     def bytes_per_chunk(self) -> int:

@@ -203,3 +203,30 @@ def test_parameters_and_outputs_that_want_a_gradient_are_refused():
             call(**{name: value})
         with torch.no_grad(), pytest.raises(RuntimeError, match="MI355X"):
             call(**{name: value})
+
+
+@pytest.mark.parametrize("batch", [1, 2])
+@pytest.mark.parametrize("fails", [torch.uint8, torch.bfloat16])
+def test_a_growth_that_fails_leaves_the_arena_as_it_was(monkeypatch, batch, fails):
+    from mote_amd import arena4
+
+    a = arena4.RelationArena4(2, 2, 16, 32, "cpu", batch=batch)
+    a.store.random_(0, 256)
+    a.scales.copy_(torch.rand(a.scales.shape))
+    a.claim(9, 10) if batch == 1 else None
+    before = [t.clone() for t in (*a.cache(0), *a.cache(1))]
+    zeros = torch.zeros
+
+    def no_memory(*size, **kw):
+        if kw.get("dtype") == fails:
+            raise torch.OutOfMemoryError("out of memory")
+        return zeros(*size, **kw)
+
+    with monkeypatch.context() as m:
+        m.setattr(torch, "zeros", no_memory)
+        with pytest.raises(torch.OutOfMemoryError):
+            a.ensure(17)
+    assert a.capacity == 16 and a.generation == 0
+    assert all(torch.equal(x, y) for x, y in zip((*a.cache(0), *a.cache(1)), before))
+    assert a.ensure(17) and a.capacity == 32 and a.scales.shape[4] == 32
+    assert all(torch.equal(x[:, :, :10], y[:, :, :10]) for x, y in zip((*a.cache(0), *a.cache(1)), before))
