@@ -161,3 +161,173 @@ def test_more_rows_than_one_launch_quantises(cuda):
     y = int8_linear(x, w8)
     for a in (0, *range((1 << 25) - 8, M, 1 << 25), M - 16):
         assert torch.equal(y[a: a + 16], int8_linear(x[a: a + 16], w8)), a
+
+
+# ---- every form that a rule on sizes selects ------------------------------------------------------------
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M,N,K", [
+    (200, 300, 900),     # 32 x 16 tiles, a ring of four
+    (515, 1111, 1000),   # 64 x 32, four
+    (1010, 1990, 1500),  # 128 x 64, four
+    (2000, 2000, 1100),  # 128 x 128, four
+    (2040, 2300, 520),   # 128 x 64, two
+    (2890, 2290, 600),   # 128 x 128, two
+    (4961, 2290, 700),   # 256 x 192
+    (16370, 2300, 640),  # 192 x 256
+    (16384, 2304, 768),  # 192 x 256, no tail
+    (8100, 4090, 1000),  # 256 x 256
+])
+def test_every_tile_in_its_steady_state(cuda, dtype, M, N, K):
+    """Each tile that the rule picks (at 256 CUs), with more stages than its ring has, so that slots are filled
+    again, and with tails of tokens and channels. y is the exact sum of the codes' products, converted to fp32,
+    times the two scales, each step rounded once: nothing is left open, so every value is compared bit for bit."""
+    from mote_amd.int8 import int8_linear, int8_weight, quantize_rows
+
+    x = (torch.randn(M, K, generator=_gen(M)) * (1 + 5 * (torch.arange(K) % 97 == 0))).to(dtype).to(cuda)
+    w = int8_weight((torch.randn(N, K, generator=_gen(N)) * 0.05).to(cuda))
+    q, s = quantize_rows(x)
+    y = int8_linear(x, w)
+    wd = w.q.double().t().contiguous()
+    for a in range(0, M, 4096):
+        acc = torch.mm(q[a: a + 4096].double(), wd).float()
+        assert torch.equal(y[a: a + 4096], (acc * s[a: a + 4096, None] * w.scale).to(dtype)), a
+    buf = torch.full((M, N + 33), 9.0, device=cuda, dtype=dtype)  # rows that share cache lines
+    int8_linear(x, w, out=buf[:, 5: N + 5])
+    assert torch.equal(buf[:, 5: N + 5], y) and (buf[:, :5] == 9).all() and (buf[:, N + 5:] == 9).all()
+
+
+@pytest.mark.parametrize("dtype,T", [(BF16, 4300), (F32, 2200)])
+def test_rows_that_pass_the_caches_by(cuda, dtype, T):
+    """100 MB and more of rows in one call (read past the caches) store what smaller calls store, bit for bit."""
+    from mote_amd.cache4 import cache4_write, cache4_zeros
+
+    B, H, D = 8, 8, 96
+    assert 2 * B * H * T * D * (2 if dtype == BF16 else 4) >= 100e6
+    k, v = (torch.randn(B, T, H, D, generator=torch.Generator(device=cuda).manual_seed(i), device=cuda).to(dtype).transpose(1, 2)
+            for i in range(2))
+    v[3, 2, 7, 11] = float("inf")
+    once, parts = cache4_zeros(B, H, T + 9, D, cuda), cache4_zeros(B, H, T + 9, D, cuda)
+    start, lens = torch.arange(B, device=cuda), T - 100 * torch.arange(B, device=cuda)
+    cache4_write(once, k, v, start, lens)
+    for a in range(0, T, 1000):
+        cache4_write(parts, k[:, :, a: a + 1000], v[:, :, a: a + 1000], start + a, lens - a)
+    for x, y in zip(once, parts):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8)) and x.view(torch.uint8).any()
+
+
+# ---- the decode step over an arena in 4 bits with its projections as they are --------------------------------
+def _mixer(cuda, d, H, layer, dtype, **kw):
+    from mote_amd.relation import FullRelation
+
+    torch.manual_seed(d + layer)
+    m = FullRelation(d, H, layer, device=cuda, **kw).to(dtype)
+    with torch.no_grad():
+        m.lam.fill_(0.4)
+        m.theta.copy_(torch.rand(H // 2) * 0.6 - 0.3)
+    return m
+
+
+def _token_by_hand(m, x, S, cache, arena_dtype):
+    """One step from the public operators: the skinny product where it applies, else F.linear."""
+    import torch.nn.functional as F
+
+    from mote_amd.cache4 import relation_decode4
+    from mote_amd.decode import skinny_linear
+
+    B, _, d = x.shape
+    H, dh = m.n_heads, m.d_head
+    w = torch.cat([m.w1.weight, m.w2.weight, m.wi.weight])
+    skinny = x.dtype == BF16 and B <= 16 and d % 128 == 0
+    qkv = (skinny_linear(x.reshape(B, d), w) if skinny else F.linear(x, w)).view(B, 3, H, dh).to(arena_dtype)
+    if m.qk_norm:
+        qkv = torch.stack([m.p1_norm(qkv[:, 0]), m.p2_norm(qkv[:, 1]), qkv[:, 2]], 1)
+    y, g = relation_decode4(qkv[:, 0], qkv[:, 1], qkv[:, 2], S, cache, m.lam, m.tau_s, m.inv_freq, m.theta, m.layer_idx,
+                            rope_f32=x.dtype == F32 and arena_dtype != F32)
+    y = y.to(x.dtype)
+    if not skinny:
+        return m._out(y.view(B, H, 1, dh), x), g
+    y = y.reshape(B, H * dh)
+    if m.out_gate:
+        y = y * torch.sigmoid(skinny_linear(x.reshape(B, d), m.wg.weight))
+    return skinny_linear(y, m.wo.weight).view(B, 1, d), g
+
+
+@pytest.mark.parametrize("d,H,B,x_dtype,arena_dtype,kw", [
+    (512, 8, 2, BF16, BF16, dict(qk_norm=True, out_gate=True)), (768, 8, 16, BF16, BF16, {}), (192, 4, 3, BF16, BF16, {}),
+    (512, 8, 20, BF16, BF16, dict(out_gate=True)), (192, 4, 1, F32, F32, {}), (512, 8, 2, F32, BF16, {})])
+def test_steps_over_four_bits_with_the_layers_own_projections(cuda, d, H, B, x_dtype, arena_dtype, kw):
+    """Prompts of two layers, then steps through RelationMainStep, the arena growing on the way: the tokens, the
+    exchange masses and the arena are those of the operators put together by hand."""
+    from mote_amd.arena import ArenaState
+    from mote_amd.arena4 import RelationArena4
+    from mote_amd.cache4 import Cache4
+    from mote_amd.graph import RelationMainStep
+
+    mixers = [_mixer(cuda, d, H, i, x_dtype, **kw) for i in range(2)]
+    arena = RelationArena4(2, H, 64, d // H, cuda, arena_dtype, batch=B)
+    state = ArenaState(arena)
+    with torch.no_grad():
+        h = torch.randn(B, 60, d, generator=_gen(1)).to(x_dtype).to(cuda)
+        for i, m in enumerate(mixers):
+            h = m(h, cache=state[i])
+        state.advance(60)
+        arena.claim(1, 60) if B == 1 else None
+        S = torch.full((B,), 60, device=cuda)
+        twin, St, xm = [Cache4(*(t.clone() for t in arena.cache(i))) for i in range(2)], S.clone(), torch.empty(2, B, device=cuda)
+        step = RelationMainStep(arena, S, xm)
+        for t in range(5):
+            if t == 2:
+                arena.claim(1, 62) if B == 1 else None
+                arena.ensure(100)
+                grow = lambda c: torch.cat([c, torch.zeros_like(c)], 2)
+                twin = [Cache4(*(grow(c) for c in layer)) for layer in twin]
+            x = xt = torch.randn(B, 1, d, generator=_gen(100 + t)).to(x_dtype).to(cuda)
+            for i, m in enumerate(mixers):
+                x = step(m, x, li=i)
+                xt, g = _token_by_hand(m, xt, St, twin[i], arena_dtype)
+                assert torch.equal(x, xt), (t, i)
+                # H additions and a division of numbers up to 1
+                assert torch.allclose(xm[i], g.mean(1), rtol=2 * (H + 1) * 2.0 ** -24, atol=0)
+            St += 1
+            assert torch.equal(S, St)
+    for i in range(2):
+        assert all(torch.equal(a, b) for a, b in zip(arena.cache(i), twin[i]))
+
+
+def test_captured_token_over_four_bits(cuda):
+    """One graph of a two-layer token with bf16 projections, replayed with the router's bit on and off and other work
+    in between, against eager steps."""
+    from mote_amd.arena4 import RelationArena4
+    from mote_amd.graph import RelationMainStep
+
+    d, H, B = 512, 8, 2
+    mixers = [_mixer(cuda, d, H, i, BF16, out_gate=True) for i in range(2)]
+    a, b = (RelationArena4(2, H, 128, d // H, cuda, BF16, batch=B) for _ in range(2))
+    Sa, Sb = torch.tensor([0, 5], device=cuda), torch.tensor([0, 5], device=cuda)
+    run, x = torch.ones(1, dtype=torch.bool, device=cuda), torch.randn(B, 1, d, generator=_gen(0)).to(BF16).to(cuda)
+    sa, sb = RelationMainStep(a, Sa, run=run), RelationMainStep(b, Sb)
+
+    def token(step, h):
+        for i, m in enumerate(mixers):
+            h = step(m, h, li=i)
+        return h
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        token(sa, x)
+    torch.cuda.current_stream().wait_stream(side)
+    a.store.zero_(), a.scales.zero_(), Sa.copy_(Sb)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = token(sa, x)
+    want = None
+    for t in range(8):
+        x.copy_(torch.randn(B, 1, d, generator=_gen(50 + t)).to(BF16))
+        run.fill_(t % 3 != 1)
+        graph.replay()
+        if t % 3 != 1:
+            want = token(sb, x)
+        torch.cuda.synchronize()
+        assert torch.equal(Sa, Sb) and torch.equal(a.store, b.store) and torch.equal(a.scales, b.scales)
+        assert torch.equal(out, want)
