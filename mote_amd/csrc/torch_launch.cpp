@@ -10,7 +10,6 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/extension.h>
 
-#include <algorithm>
 #include <array>
 #include <climits>
 #include <initializer_list>
@@ -440,10 +439,10 @@ void apart(const Tensor& out, int64_t out_width, const Tensor& in, int64_t in_wi
   bad_value(what, ": the output lies over an input");
 }
 // Whether every element of a view has an address of its own: taken by stride, a step passes all that the smaller
-// ones reach. With `other`, a view of as many dims and the same sizes, the two taken together (as one view with a
-// dim of two more where their strides agree, by the ranges that they span where not).
+// ones reach. With `other`, a view of as many dims and the same sizes, whether two views that are separate each are
+// so together (as one view with a dim of two more where their strides agree, by the ranges that they span where not).
 bool separate(const Tensor& t, const Tensor* other = nullptr) {
-  if (t.numel() == 0) return true;
+  if (t.numel() == 0 || (!other && t.is_contiguous())) return true;
   constexpr int kMost = 8;
   std::array<std::pair<int64_t, int64_t>, kMost + 1> dim;  // stride, size
   int n = 0;
@@ -460,11 +459,12 @@ bool separate(const Tensor& t, const Tensor* other = nullptr) {
   }
   if (other) {
     const int64_t e = t.element_size(), a = reinterpret_cast<int64_t>(t.data_ptr()), b = reinterpret_cast<int64_t>(other->data_ptr());
-    if (b >= a + span * e || a >= b + span2 * e) return separate(t) && separate(*other);
+    if (b >= a + span * e || a >= b + span2 * e) return true;
     if (!alike || (b - a) % e) return false;
     dim[n++] = {b > a ? (b - a) / e : (a - b) / e, 2};
   }
-  std::sort(dim.begin(), dim.begin() + n);
+  for (int i = 1; i < n; ++i)
+    for (int j = i; j > 0 && dim[j] < dim[j - 1]; --j) std::swap(dim[j], dim[j - 1]);
   int64_t reach = 1;
   for (int i = 0; i < n; ++i) {
     if (dim[i].first < reach) return false;
