@@ -765,9 +765,10 @@ int mote_relation_decode4(const mote_relation_decode4_args* args, void* stream);
  * infinity stores zeros with scale NaN.
  * mote_int8_linear: y [M, N] (dtype) = ((float(acc) sx[m]) sw[n]) rounded once, acc = sum_k xq wq exact in
  * 32-bit integers (K <= 131072); x is quantised in the call, wq [N, Kp] and sw [N] come from
- * mote_quantize_rows. Up to 64 rows with K <= 4096 are one launch, which takes the decode step's predicate
- * and exchange mass as mote_skinny_gemm does; others quantise x into the workspace first
- * (mote_int8_linear_workspace() bytes; its contents on entry do not matter) and take neither.
+ * mote_quantize_rows. Up to 64 rows with K <= 4096 may come with the decode step's predicate and exchange
+ * mass, as mote_skinny_gemm takes them, and are one launch then, as are up to 16 rows and those of up to 64 that
+ * few workgroups hold; others quantise x into the workspace first (mote_int8_linear_workspace() bytes, 0 where
+ * none is needed; its contents on entry do not matter) and take neither.
  * Row strides in elements; wq on a 16-byte boundary with its rows Kp apart.
  * ------------------------------------------------------------------------------------------------ */
 typedef struct mote_quantize_rows_args {

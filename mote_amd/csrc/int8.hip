@@ -179,7 +179,7 @@ quantize_rows_kernel(const T* x, int64_t x_sr, int M, int K, int Kp, int8_t* q, 
 // x, agrees on the rows' maxima with the other waves through LDS, and multiplies. The partial sums are
 // integers: their order does not matter. Every workgroup of a token tile quantises it again (24 KB at 768
 // from the L2), which costs less than a launch of its own. A launch of this size is bound by its latencies:
-// 4.4 us at 1 x 768 -> 768, 4.5 us at 1 x 768 -> 2304, whose W of 1.8 MB takes 0.4.
+// 3.5 us at 1 x 768 -> 768, 3.6 us at 1 x 768 -> 2304, whose W of 1.8 MB takes 0.4.
 // ------------------------------------------------------------------------------------------------
 constexpr int kFewRows = 64;
 constexpr int kFewMaxK = 4096;
@@ -516,7 +516,8 @@ int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream) {
 // 4096 -> 4096 10.4 and 11.4), and up to 64 while the workgroups that quantise a token again are few: two a CU
 // of K up to 1024 (64 x 1024 -> 1536, 384 of them, 6.4 and 6.8 us; 64 x 768 -> 2304, 576, 6.5 and 6.5), one up to
 // 2048 (32 x 2048 -> 2048, 256, 7.0 and 7.7; 48 x 1536 -> 1536, 288, 8.1 and 7.2), none beyond (32 x 4096 -> 1024
-// 10.8 and 9.8); the predicate and the exchange mass have it to themselves.
+// 9.4 and 9.2, fp32 12.6 and 9.2); the predicate and the exchange mass exist in it alone, so calls with them take it at
+// every size (64 x 4096 -> 4096 26.0 us, 10.0 with tiles).
 static bool few8(const mote_int8_linear_args* a) {
   if (a->M > kFewRows || a->K > kFewMaxK) return false;
   const int64_t groups = (int64_t(a->M) + 15) / 16 * ((int64_t(a->N) + 15) / 16);
@@ -593,7 +594,9 @@ static int launch_many8(const mote_int8_linear_args* a, hipStream_t stream, cons
   // k = 768, 1024 and 4096 at 4964 to 65536 rows), with one workgroup per CU of the large tiles and two of
   // 128 x 128. 4964 x 768 -> 2304: 234 tiles of 256 x 192 in one round 20.9 us, 23.2 with 256 x 256 or 128 x
   // 128; 16384 rows: 768 tiles of 192 x 256 in three 52.8 us, 57.7 and 57.1; 65536 x 1024 -> 4096: 256 x 256
-  // 328 us, 353 with 256 x 192, 366 with 128 x 128.
+  // 328 us, 353 with 256 x 192, 366 with 128 x 128. The costs are those of bf16 results; fp32 ones store twice the
+  // bytes and take the same rule (23.8, 60.2 and 391 us at these sizes, x quantised included; bf16 18.6, 46.6, 325),
+  // their other tiles not measured.
   auto rounds_us = [&](int64_t t, int64_t slots, double fixed, double stage) {
     return double((t + slots - 1) / slots) * (fixed + Kp / 128 * stage);
   };

@@ -18,7 +18,7 @@ import torch
 
 from . import _lib as L
 
-FEW_ROWS, FEW_WIDTH = 64, 4096  # one launch, with the decode step's predicate and exchange mass
+FEW_ROWS, FEW_WIDTH = 64, 4096  # most tokens and inputs of a call with the decode step's predicate or exchange mass
 
 
 class Int8Weight(NamedTuple):
@@ -45,6 +45,7 @@ def int8_linear(x: torch.Tensor, w: Int8Weight, out: Optional[torch.Tensor] = No
                 g: Optional[torch.Tensor] = None, xm: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y [..., N] = x [..., K] W^T in x's dtype (bf16 or fp32), x quantised per token in the call.
 
-    Up to 64 tokens of K <= 4096 are one launch, which also takes what `skinny_linear` takes: `run` (a device
-    flag; 0 leaves `out` untouched), g (fp32 [M, H], contiguous) and xm (fp32 [M], the mean of g over the heads)."""
+    Up to 64 tokens of K <= 4096 may take what `skinny_linear` takes: `run` (a device flag; 0 leaves `out`
+    untouched), g (fp32 [M, H], contiguous) and xm (fp32 [M], the mean of g over the heads). Such calls are one
+    launch, as are those of up to 16 tokens and those of up to 64 that few workgroups hold; others are two."""
     return L.native().int8_linear(x, w.q, w.scale, w.in_features, out, run, g, xm)
