@@ -37,6 +37,13 @@ def _check_run(run: Optional[torch.Tensor], dev) -> None:
         raise ValueError("run must be a one-element bool or uint8 tensor on the inputs' device")
 
 
+def _no_tangent(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses dual tensors: the kernels would drop their tangents (no_grad leaves forward mode on)."""
+    ad = torch.autograd.forward_ad
+    if ad._current_level >= 0 and any(t is not None and ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: it takes no dual tensors")
+
+
 def _f32_param(t: torch.Tensor, n: int, name: str, dev) -> torch.Tensor:
     if not torch.is_tensor(t) or t.numel() != n or t.device != dev:
         raise ValueError(f"{name} must be a tensor of {n} element(s) on the inputs' device")
@@ -68,6 +75,7 @@ def relation_decode(p1: torch.Tensor, p2: torch.Tensor, info: torch.Tensor, S: t
     """
     if p1.dim() != 3:
         raise ValueError("p1/p2/info must be [B, H, dh]")
+    _no_tangent("relation_decode", p1, p2, info, lam, inv_freq, theta, y, g, xm)
     B, H, D = p1.shape
     dev = p1.device
     for t in (p1, p2, info):
@@ -137,6 +145,7 @@ def skinny_linear(x: torch.Tensor, w: torch.Tensor, out: Optional[torch.Tensor] 
     xm (fp32 [B]) the same launch writes xm[b] = mean of g[b] in head order (graph.py:186)."""
     B, K = x.shape
     N = w.shape[0]
+    _no_tangent("skinny_linear", x, w, out, g, xm)
     if x.dtype != torch.bfloat16 or w.dtype != torch.bfloat16:
         raise TypeError("skinny_linear: bf16 x and w")
     if x.stride(-1) != 1 or w.stride(-1) != 1 or w.shape[1] != K:

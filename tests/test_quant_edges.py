@@ -230,3 +230,19 @@ def test_a_growth_that_fails_leaves_the_arena_as_it_was(monkeypatch, batch, fail
     assert all(torch.equal(x, y) for x, y in zip((*a.cache(0), *a.cache(1)), before))
     assert a.ensure(17) and a.capacity == 32 and a.scales.shape[4] == 32
     assert all(torch.equal(x[:, :, :10], y[:, :, :10]) for x, y in zip((*a.cache(0), *a.cache(1)), before))
+
+
+def test_the_steps_of_the_model_type_refuse_tangents_too():
+    from mote_amd.decode import relation_decode, skinny_linear
+
+    fwd = torch.autograd.forward_ad
+    x, S, lam = torch.zeros(2, 4, 48, dtype=BF16), torch.zeros(2, dtype=torch.int64), torch.tensor(0.5)
+    rows, w = torch.zeros(2, 4, 64, 48, dtype=BF16), torch.zeros(16, 128, dtype=BF16)
+    with fwd.dual_level(), torch.no_grad():
+        dual = lambda v: fwd.make_dual(v, torch.ones_like(v))
+        for call in (lambda: relation_decode(dual(x), x, x, S, rows, rows, lam), lambda: relation_decode(x, x, x, S, rows, rows, dual(lam)),
+                     lambda: skinny_linear(dual(w[:4]), w), lambda: skinny_linear(w[:4], dual(w))):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="MI355X"):
+            relation_decode(x, x, x, S, rows, rows, lam)
