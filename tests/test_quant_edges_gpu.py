@@ -331,3 +331,42 @@ def test_captured_token_over_four_bits(cuda):
         torch.cuda.synchronize()
         assert torch.equal(Sa, Sb) and torch.equal(a.store, b.store) and torch.equal(a.scales, b.scales)
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_both_outputs_in_one_buffer(cuda, dtype):
+    """The two outputs of a read as columns, as alternate rows and as halves of one buffer."""
+    from mote_amd.cache4 import cache4_read
+
+    B, H, T, D = 2, 4, 10, 48
+    _, _, cache = _step_inputs(cuda, 80, B, H, D, 64)
+    want = cache4_read(cache, D, 3, T, dtype=dtype)
+    new = lambda *s: torch.full(s, 9.0, device=cuda, dtype=dtype)
+    side, turned, long, inner = new(B, H, T, 2 * D), new(B, T, H, 2 * D).transpose(1, 2), new(B, H, 2 * T, D), new(B, 3, H, T, D)
+    for out in ((side[..., :D], side[..., D:]), (turned[..., D:], turned[..., :D]), (long[:, :, ::2], long[:, :, 1::2]),
+                (inner[:, 0], inner[:, 2])):
+        got = cache4_read(cache, D, 3, T, out=out)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(torch.equal(a, b) for a, b in zip(out, want))
+    assert (inner[:, 1] == 9).all()
+
+
+def test_windows_of_another_type_than_the_arena(cuda):
+    """An fp32 layer over an arena of bf16 rows in 4 bits: two windows, against the operators put together by hand."""
+    from mote_amd.arena import ArenaState
+    from mote_amd.arena4 import RelationArena4
+    from mote_amd.cache4 import cache4_read
+    from mote_amd.flash_relation import flash_relation
+
+    d, H, B = 192, 4, 2
+    m = _mixer(cuda, d, H, 1, F32)
+    arena = RelationArena4(1, H, 128, d // H, cuda, BF16, batch=B)
+    state = ArenaState(arena)
+    with torch.no_grad():
+        for T in (50, 1, 30):
+            x, n = torch.randn(B, T, d, generator=_gen(T)).to(cuda), state.n
+            held = cache4_read(arena.cache(0), d // H, 0, n)
+            q, k, v = (t.to(BF16) for t in m.heads(x, n))
+            y, g = flash_relation(q, torch.cat([held[0], k], 2), torch.cat([held[1], v], 2), m.lam, m.tau_s, q_start=n)
+            out, gates = m(x, cache=state[0], return_gates=True)
+            assert torch.equal(out, m._out(y.to(F32), x)) and torch.equal(gates, g)
+            state.advance(T)
