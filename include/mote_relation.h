@@ -797,6 +797,92 @@ typedef struct mote_int8_linear_args {
 size_t mote_int8_linear_workspace(const mote_int8_linear_args* args);
 int mote_int8_linear(const mote_int8_linear_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The {P2, I~} cache in pages of 8-bit values. No counterpart in the reference, whose arena holds its rows
+ * in the model's dtype, contiguous per sequence (mote/model/arena.py:30-51).
+ * A sequence's rows form blocks of 64; whole blocks are held in 8 bits, each in a page of a pool that its
+ * table row names, and are never written again, so sequences may share them. Its newest rows, fewer than 64,
+ * are held in the model's dtype in its tail.
+ * Format of a block of one head, P2 and I~ apart: the fp32 scale s = max|x| / 448 and one e4m3 code per value,
+ * nearest to x (448 / max|x|) (fp32 quotient and product, ties to even); the value is code * s in fp32. A block
+ * whose maximum is below 2^-112 stores zeros with scale 0; one with a NaN or an infinity stores zeros with scale
+ * NaN, so every value read from it is NaN. With D padded to Dp = 16 ceil(D / 16), a page of P2 holds its bytes
+ * as [Dp / 16][64 rows][16 dims], one of I~ as [Dp dims][64 rows], padded dims zero.
+ * mote_cache8: codes of page p and head h at p codes_sp + h 64 Dp bytes (16-byte boundaries), scales at
+ * p scale_sp + h; tails [B, H, 64, D] with the rows of a sequence back to back, tail_sb elements apart, on
+ * 16-byte boundaries; table [B, blocks] of page numbers, rows table_sb apart. A number outside [0, pages) is no
+ * page: blocks written there are dropped, and rows read from there are NaN.
+ * ------------------------------------------------------------------------------------------------ */
+typedef struct mote_cache8 {
+  void* p2;
+  float* p2_scale;
+  void* info;
+  float* info_scale;
+  void* p2_tail;
+  void* info_tail;
+  const int32_t* table;
+  int64_t codes_sp;
+  int64_t scale_sp;
+  int64_t tail_sb;
+  int64_t table_sb;
+  int pages;
+  int blocks;
+} mote_cache8;
+
+/* mote_cache8_write: T new rows of every sequence and head from p2 / info [B, H, T, D] (dtype, the tails'; rows on
+ * 16-byte boundaries) behind the rows that the sequence holds: `start`, or start_dev[b] (device) when start_dev
+ * is not NULL, is their number. With lens (device, [B], or NULL) sequence b takes its first lens[b] rows only.
+ * Blocks that the new rows complete go to their pages, with the tail's older rows where they began there; the rows
+ * behind them to the tail. A start outside [0, 64 blocks], and rows from 64 blocks on, store nothing.
+ * mote_cache8_read: rows start + t, t < T, of sequences that hold `held` (or held_dev[b]) rows into the views
+ * p2 / info (dtype), each value rounded once; positions outside [0, held) read as zeros, those that the table has
+ * no page for as NaN; lens is not used; tail_dtype is the tails' type. */
+typedef struct mote_cache8_rows_args {
+  int dtype;
+  int tail_dtype;
+  int B, H, T, D;
+  mote_view p2, info;
+  mote_cache8 cache;
+  int64_t start;
+  const int64_t* start_dev;
+  const int64_t* lens;
+  int64_t held;
+  const int64_t* held_dev;
+} mote_cache8_rows_args;
+
+int mote_cache8_write(const mote_cache8_rows_args* args, void* stream);
+int mote_cache8_read(const mote_cache8_rows_args* args, void* stream);
+
+/* One decode step over that cache: mote_relation_decode (see there for every argument they share) with the past
+ * rows j < S at their 8-bit values, those of the tail as they are. The new rows take part as they are and are then
+ * stored at position S: into the tail, and with S % 64 == 63 the block into its page. S[b] outside
+ * [0, 64 blocks) writes NaN into y[b] and g[b] and stores nothing; so does, but for the append, a whole block
+ * without a page. The workspace rule is mote_relation_decode4's. */
+typedef struct mote_relation_decode8_args {
+  int dtype;
+  int B, H, D, layer_parity, flags;
+  float tau_s;
+  const float* lam;
+  const float* inv_freq;
+  const float* theta;
+  int64_t* S;
+  const void* p1;
+  const void* p2;
+  const void* info;
+  int64_t in_sb;
+  mote_cache8 cache;
+  void* y;
+  int64_t y_sb;
+  float* g;
+  void* workspace;
+  size_t workspace_bytes;
+  float* xm;
+  const unsigned char* run;
+} mote_relation_decode8_args;
+
+size_t mote_relation_decode8_workspace(const mote_relation_decode8_args* args);
+int mote_relation_decode8(const mote_relation_decode8_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -290,6 +290,33 @@ class Int8LinearArgs(C.Structure):
     ]
 
 
+class Cache8View(C.Structure):
+    _fields_ = [
+        ("p2", C.c_void_p), ("p2_scale", C.c_void_p), ("info", C.c_void_p), ("info_scale", C.c_void_p),
+        ("p2_tail", C.c_void_p), ("info_tail", C.c_void_p), ("table", C.c_void_p), ("codes_sp", C.c_int64),
+        ("scale_sp", C.c_int64), ("tail_sb", C.c_int64), ("table_sb", C.c_int64), ("pages", C.c_int),
+        ("blocks", C.c_int),
+    ]
+
+
+class Cache8RowsArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("tail_dtype", C.c_int), ("B", C.c_int), ("H", C.c_int), ("T", C.c_int), ("D", C.c_int),
+        ("p2", View), ("info", View), ("cache", Cache8View), ("start", C.c_int64), ("start_dev", C.c_void_p),
+        ("lens", C.c_void_p), ("held", C.c_int64), ("held_dev", C.c_void_p),
+    ]
+
+
+class Decode8Args(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("B", C.c_int), ("H", C.c_int), ("D", C.c_int), ("layer_parity", C.c_int),
+        ("flags", C.c_int), ("tau_s", C.c_float), ("lam", C.c_void_p), ("inv_freq", C.c_void_p),
+        ("theta", C.c_void_p), ("S", C.c_void_p), ("p1", C.c_void_p), ("p2", C.c_void_p), ("info", C.c_void_p),
+        ("in_sb", C.c_int64), ("cache", Cache8View), ("y", C.c_void_p), ("y_sb", C.c_int64), ("g", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("xm", C.c_void_p), ("run", C.c_void_p),
+    ]
+
+
 # every symbol the header declares, with its argument types
 EXPORTS = {
     "mote_last_error": ([], C.c_char_p),
@@ -337,6 +364,10 @@ EXPORTS = {
     "mote_quantize_rows": ([C.POINTER(QuantizeRowsArgs), C.c_void_p], C.c_int),
     "mote_int8_linear_workspace": ([C.POINTER(Int8LinearArgs)], C.c_size_t),
     "mote_int8_linear": ([C.POINTER(Int8LinearArgs), C.c_void_p], C.c_int),
+    "mote_cache8_write": ([C.POINTER(Cache8RowsArgs), C.c_void_p], C.c_int),
+    "mote_cache8_read": ([C.POINTER(Cache8RowsArgs), C.c_void_p], C.c_int),
+    "mote_relation_decode8_workspace": ([C.POINTER(Decode8Args)], C.c_size_t),
+    "mote_relation_decode8": ([C.POINTER(Decode8Args), C.c_void_p], C.c_int),
     "mote_abi_layout": ([], C.c_char_p),
     "mote_clock_probe": ([C.c_void_p, C.c_int, C.c_int, C.c_void_p], C.c_int),
 }
@@ -356,6 +387,9 @@ STRUCTS = {
     "mote_dechunk_step_args": DechunkStepArgs, "mote_cache4": Cache4View, "mote_cache4_rows_args": Cache4RowsArgs,
     "mote_relation_decode4_args": Decode4Args, "mote_quantize_rows_args": QuantizeRowsArgs,
     "mote_int8_linear_args": Int8LinearArgs,
+    "mote_cache8": Cache8View,
+    "mote_cache8_rows_args": Cache8RowsArgs,
+    "mote_relation_decode8_args": Decode8Args,
 }
 
 

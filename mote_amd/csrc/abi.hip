@@ -40,6 +40,10 @@ int launch_decode4(const mote_relation_decode4_args* a, hipStream_t stream);
 int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream);
 size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a);
 int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream);
+int launch_cache8_write(const mote_cache8_rows_args* a, hipStream_t stream);
+int launch_cache8_read(const mote_cache8_rows_args* a, hipStream_t stream);
+size_t decode8_workspace_bytes(const mote_relation_decode8_args* a);
+int launch_decode8(const mote_relation_decode8_args* a, hipStream_t stream);
 
 }  // namespace mote
 
@@ -227,6 +231,23 @@ size_t mote_int8_linear_workspace(const mote_int8_linear_args* args) {
 int mote_int8_linear(const mote_int8_linear_args* args, void* stream) {
   mote::g_err[0] = 0;
   return mote::launch_int8_linear(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+int mote_cache8_write(const mote_cache8_rows_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_cache8_write(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+int mote_cache8_read(const mote_cache8_rows_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_cache8_read(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t mote_relation_decode8_workspace(const mote_relation_decode8_args* args) { return args ? mote::decode8_workspace_bytes(args) : 0; }
+
+int mote_relation_decode8(const mote_relation_decode8_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_decode8(args, reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

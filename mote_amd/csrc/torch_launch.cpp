@@ -681,6 +681,217 @@ std::tuple<Tensor, Tensor> relation_decode4(const Tensor& p1, const Tensor& p2, 
   return {y, g};
 }
 
+// ---- the cache in pages of 8-bit values ------------------------------------------------------------------
+struct Cache8 {
+  mote_cache8 c;
+  int64_t rows;  // that the table reaches
+};
+// A layer's pool, tails and table for sequences and heads [B, H] of head dim D; `writes`: every place once.
+Cache8 cache8(const std::vector<Tensor>& t, int64_t B, int64_t H, int64_t D, c10::Device dev, bool writes, const char* what) {
+  if (t.size() != 7) bad_value(what, ": a cache has seven tensors");
+  if (D <= 0 || D > 128 || D % 8) bad_value(what, ": head dim ", D, " unsupported (need 8 <= D <= 128, D % 8 == 0)");
+  if (B > INT_MAX || H > INT_MAX) bad_value(what, ": ", B, " sequences of ", H, " heads (sizes beyond 32 bits)");
+  const Tensor &p2 = t[0], &s2 = t[1], &info = t[2], &si = t[3], &t2 = t[4], &ti = t[5], &table = t[6];
+  const int64_t C = (D + 15) / 16, P = p2.dim() == 5 ? p2.size(0) : 0, M = table.dim() == 2 ? table.size(1) : 0;
+  auto check = [&](const Tensor& x, at::IntArrayRef sizes, at::ScalarType dt, int packed, const char* name) {
+    if (x.sizes() != sizes || x.numel() == 0) bad_value(what, ": ", name, " must be ", sizes, ", got ", x.sizes());
+    if (x.scalar_type() != dt || x.device() != dev)
+      throw py::type_error(c10::str(what, ": ", name, " must be ", c10::toString(dt), " on the rows' device"));
+    int64_t s = 1;  // dims from `packed` on lie back to back
+    for (int64_t d = x.dim() - 1; d >= packed; --d) {
+      if (x.size(d) > 1 && x.stride(d) != s) bad_value(what, ": ", name, " must lie back to back from dim ", packed, " on");
+      s *= x.size(d);
+    }
+  };
+  check(p2, {P, H, C, 64, 16}, at::kByte, 1, "the pages of P2");
+  check(info, {P, H, 16 * C, 64}, at::kByte, 1, "the pages of I~");
+  check(s2, {P, H}, at::kFloat, 1, "the scales of P2");
+  check(si, {P, H}, at::kFloat, 1, "the scales of I~");
+  const at::ScalarType tt = t2.scalar_type();
+  code(tt);
+  check(t2, {B, H, 64, D}, tt, 1, "the tails of P2");
+  check(ti, {B, H, 64, D}, tt, 1, "the tails of I~");
+  check(table, {B, M}, at::kInt, 1, "the table");
+  if (P > 1 && (p2.stride(0) != info.stride(0) || s2.stride(0) != si.stride(0)))
+    bad_value(what, ": P2 and I~ must have the same strides");
+  if (B > 1 && t2.stride(0) != ti.stride(0)) bad_value(what, ": the tails must have the same strides");
+  if (P > INT_MAX || M > (int64_t(1) << 24)) bad_value(what, ": ", P, " pages, ", M, " blocks (at most 2^31 and 2^24)");
+  if (writes) {
+    for (const Tensor* x : {&p2, &info, &s2, &si, &t2, &ti})
+      if (!separate(*x)) bad_value(what, ": pages or sequences lie over one another");
+    if (!ranges_apart(t2, ti) && !separate(t2, &ti)) bad_value(what, ": P2 and I~ must not be the same rows");
+    if (p2.data_ptr() == info.data_ptr() || s2.data_ptr() == si.data_ptr() || t2.data_ptr() == ti.data_ptr())
+      bad_value(what, ": P2 and I~ must not be the same rows");
+  }
+  Cache8 r;
+  r.c = mote_cache8{p2.data_ptr(), fptr(s2), info.data_ptr(), fptr(si), t2.data_ptr(), ti.data_ptr(), iptr(table),
+                    P > 1 ? p2.stride(0) : 0, P > 1 ? s2.stride(0) : 0, B > 1 ? t2.stride(0) : 0, B > 1 ? table.stride(0) : 0,
+                    int(P), int(M)};
+  r.rows = 64 * M;
+  return r;
+}
+
+void cache8_write(const std::vector<Tensor>& c_, Tensor p2, Tensor info, int64_t start, const OptTensor& start_dev,
+                  const OptTensor& lens) {
+  const char* what = "cache8_write";
+  if (p2.dim() != 4 || info.sizes() != p2.sizes()) bad_value(what, ": p2 and info must both be [B, H, T, D]");
+  if (info.scalar_type() != p2.scalar_type() || info.device() != p2.device())
+    throw py::type_error("cache8_write: p2 and info must share a dtype and a device");
+  const int64_t B = p2.size(0), H = p2.size(1), T = p2.size(2), D = p2.size(3);
+  mote_cache8_rows_args a{};
+  a.dtype = a.tail_dtype = code(p2);
+  const Cache8 c = cache8(c_, B, H, D, p2.device(), true, what);
+  if (c_[4].scalar_type() != p2.scalar_type()) throw py::type_error("cache8_write: rows and tails must share a dtype");
+  if (T > (int64_t(1) << 30) - 1) bad_value(what, ": ", T, " rows (at most 2^30 - 1)");
+  if (start_dev) {
+    positions(*start_dev, B, p2.device(), what, "start");
+    a.start_dev = static_cast<const int64_t*>(start_dev->data_ptr());
+  } else if (start < 0 || start > c.rows - T) {
+    throw std::runtime_error(c10::str(what, ": rows ", start, " to ", start + T, " in a table of ", c.rows));
+  }
+  a.start = start;
+  if (lens) {
+    positions(*lens, B, p2.device(), what, "lens");
+    a.lens = static_cast<const int64_t*>(lens->data_ptr());
+  }
+  no_grad(what, {&p2, &info});
+  for (const Tensor* x : {&p2, &info})
+    for (const Tensor& held : c_)
+      if (!ranges_apart(*x, held)) bad_value(what, ": the rows lie over the cache");
+  on_gpu(p2, what);
+  const On on(p2);
+  p2 = aligned(p2); info = aligned(info);
+  a.B = int(B); a.H = int(H); a.T = int(T); a.D = int(D);
+  a.p2 = view(p2); a.info = view(info);
+  a.cache = c.c;
+  check(mote_cache8_write(&a, on.stream), "mote_cache8_write");
+}
+
+std::tuple<Tensor, Tensor> cache8_read(const std::vector<Tensor>& c_, int64_t held, const OptTensor& held_dev, int64_t start,
+                                       const OptTensor& start_dev, int64_t rows, at::ScalarType dtype, const OptTensor& out2,
+                                       const OptTensor& outi) {
+  const char* what = "cache8_read";
+  if (c_.size() != 7 || c_[4].dim() != 4) bad_value(what, ": the tails of P2 must be [B, H, 64, D]");
+  const Tensor& like = c_[4];
+  const int64_t B = like.size(0), H = like.size(1), D = like.size(3);
+  const Cache8 c = cache8(c_, B, H, D, like.device(), false, what);
+  mote_cache8_rows_args a{};
+  if (rows < 0 || rows > (int64_t(1) << 30) - 1) bad_value(what, ": ", rows, " rows (0 to 2^30 - 1)");
+  if (start_dev) {
+    positions(*start_dev, B, like.device(), what, "start");
+    a.start_dev = static_cast<const int64_t*>(start_dev->data_ptr());
+  } else if (start < 0) {
+    throw std::runtime_error(c10::str(what, ": rows from ", start));
+  }
+  if (held_dev) {
+    positions(*held_dev, B, like.device(), what, "held");
+    a.held_dev = static_cast<const int64_t*>(held_dev->data_ptr());
+  } else if (held < 0 || held > c.rows) {
+    throw std::runtime_error(c10::str(what, ": ", held, " rows held in a table of ", c.rows));
+  }
+  a.start = start;
+  a.held = held;
+  Tensor p2, info;
+  if (out2) {
+    p2 = *out2; info = *outi;
+    for (const Tensor* t : {&p2, &info}) {
+      if (t->sizes() != at::IntArrayRef({B, H, rows, D}) || t->device() != like.device())
+        bad_value(what, ": out must be two [B, H, rows, D] tensors on the cache's device");
+      if (!separate(*t)) bad_value(what, ": out holds its rows for several places at once");
+      for (const Tensor& x : c_)
+        if (!ranges_apart(*t, x)) bad_value(what, ": out lies over the cache");
+    }
+    if (!separate(p2, &info)) bad_value(what, ": the two tensors of out lie over one another");
+    if (info.scalar_type() != p2.scalar_type()) throw py::type_error("cache8_read: out must be two tensors of one dtype");
+    if (p2.requires_grad() || info.requires_grad()) throw std::runtime_error("cache8_read: out must not require a gradient");
+    no_tangent(what, {&p2, &info});
+  }
+  no_grad(what, {&c_[1], &c_[3], &c_[4], &c_[5]});
+  a.dtype = code(out2 ? p2.scalar_type() : dtype);
+  a.tail_dtype = code(like);
+  on_gpu(like, what);
+  const On on(like);
+  if (!out2) {
+    p2 = empty({B, H, rows, D}, like, dtype);
+    info = empty({B, H, rows, D}, like, dtype);
+  }
+  a.B = int(B); a.H = int(H); a.T = int(rows); a.D = int(D);
+  a.p2 = view(p2); a.info = view(info);
+  a.cache = c.c;
+  check(mote_cache8_read(&a, on.stream), "mote_cache8_read");
+  return {p2, info};
+}
+
+std::tuple<Tensor, Tensor> relation_decode8(const Tensor& p1, const Tensor& p2, const Tensor& info, const Tensor& S,
+                                            const std::vector<Tensor>& c_, const Tensor& lam, double tau, const OptTensor& inv_freq,
+                                            const OptTensor& theta, int64_t layer_idx, bool advance, const OptTensor& workspace,
+                                            const OptTensor& y_, const OptTensor& g_, const OptTensor& xm, const OptTensor& run,
+                                            bool rope_f32) {
+  const char* what = "relation_decode8";
+  if (p1.dim() != 3) bad_value(what, ": p1/p2/info must be [B, H, dh]");
+  const int64_t B = p1.size(0), H = p1.size(1), D = p1.size(2);
+  const c10::Device dev = p1.device();
+  for (const Tensor* t : {&p1, &p2, &info}) {
+    if (t->sizes() != p1.sizes() || t->stride(2) != 1 || t->stride(1) != D || (B > 1 && t->stride(0) != p1.stride(0)))
+      bad_value(what, ": p1/p2/info must be [B, H, dh] with head stride dh and one batch stride");
+    if (t->scalar_type() != p1.scalar_type() || t->device() != dev)
+      throw py::type_error("relation_decode8: p1, p2 and info must share a dtype and a device");
+  }
+  if (B < 1 || H < 1 || H % 2) bad_value(what, ": B = ", B, " sequences of H = ", H, " heads (an even number)");
+  mote_relation_decode8_args a{};
+  a.dtype = code(p1);
+  const Cache8 c = cache8(c_, B, H, D, dev, true, what);
+  if (c_[4].scalar_type() != p1.scalar_type()) throw py::type_error("relation_decode8: the step and the tails must share a dtype");
+  positions(S, B, dev, what, "S");
+  const Tensor lam32 = small_f32(lam, 1, p1, what, "lam");
+  Tensor inv, th;
+  if (inv_freq) inv = small_f32(*inv_freq, D / 2, p1, what, "inv_freq");
+  if (theta) th = small_f32(*theta, H / 2, p1, what, "theta");
+  if (xm && (xm->scalar_type() != at::kFloat || xm->numel() != B || !xm->is_contiguous() || xm->device() != dev))
+    bad_value(what, ": xm must be a contiguous fp32 tensor of B elements");
+  check_run(run, p1, what);
+  if (workspace && (workspace->device() != dev || !workspace->is_contiguous()))
+    bad_value(what, ": workspace must be a contiguous tensor on the inputs' device");
+  if (y_ && (y_->sizes() != p1.sizes() || y_->scalar_type() != p1.scalar_type() || y_->device() != dev || y_->stride(2) != 1 ||
+             y_->stride(1) != D || (B > 1 && y_->stride(0) < H * D)))
+    bad_value(what, ": y must be [B, H, dh] in the inputs' dtype with head stride dh");
+  if (g_ && (g_->dim() != 2 || g_->size(0) != B || g_->size(1) != H || g_->scalar_type() != at::kFloat || g_->device() != dev ||
+             !g_->is_contiguous()))
+    bad_value(what, ": g must be a contiguous fp32 [B, H] tensor");
+  if (y_)
+    for (const Tensor* t : {&p1, &p2, &info}) apart(*y_, H * D, *t, H * D, B, what);
+  no_grad(what, {&p1, &p2, &info, &lam});
+  for (const OptTensor* t : {&inv_freq, &theta, &y_, &g_, &xm})
+    if (*t) no_grad(what, {&**t});
+  on_gpu(p1, what);
+  const On on(p1);
+  Tensor y = y_ ? *y_ : empty({B, H, D}, p1, p1.scalar_type());
+  Tensor g = g_ ? *g_ : empty({B, H}, p1, at::kFloat);
+  a.B = int(B); a.H = int(H); a.D = int(D);
+  a.layer_parity = int(((layer_idx % 2) + 2) % 2);
+  a.flags = (advance ? MOTE_DECODE_ADVANCE : 0) | (rope_f32 ? MOTE_DECODE_ROPE_F32 : 0);
+  a.tau_s = float(tau);
+  a.lam = fptr(lam32);
+  a.inv_freq = inv_freq ? fptr(inv) : nullptr;
+  a.theta = theta ? fptr(th) : nullptr;
+  a.S = static_cast<int64_t*>(S.data_ptr());
+  a.p1 = p1.data_ptr(); a.p2 = p2.data_ptr(); a.info = info.data_ptr(); a.in_sb = p1.stride(0);
+  a.cache = c.c;
+  a.y = y.data_ptr(); a.y_sb = y.stride(0); a.g = fptr(g);
+  const int64_t need = int64_t(mote_relation_decode8_workspace(&a));
+  // the halves that counters and partials lie in follow from the bytes: one workspace, one number of them
+  if (workspace && workspace->numel() * workspace->element_size() != need)
+    bad_value(what, ": a workspace of ", workspace->numel() * workspace->element_size(), " bytes, ", need,
+              " needed (decode8_workspace makes one for these sizes)");
+  const Tensor ws = workspace ? *workspace : at::zeros({need}, p1.options().dtype(at::kByte));
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = size_t(ws.numel()) * ws.element_size();
+  a.xm = xm ? fptr(*xm) : nullptr;
+  a.run = run ? static_cast<const unsigned char*>(run->data_ptr()) : nullptr;
+  check(mote_relation_decode8(&a, on.stream), "mote_relation_decode8");
+  return {y, g};
+}
+
 std::tuple<Tensor, Tensor> quantize_rows(Tensor x) {
   if (x.dim() != 2 || x.size(1) < 1) bad_value("quantize_rows: x must be [M, K]");
   mote_quantize_rows_args a{};
@@ -772,6 +983,9 @@ PYBIND11_MODULE(_torch_launch, m) {
   m.def("cache4_write", &cache4_write, nogil());
   m.def("cache4_read", &cache4_read, nogil());
   m.def("relation_decode4", &relation_decode4, nogil());
+  m.def("cache8_write", &cache8_write, nogil());
+  m.def("cache8_read", &cache8_read, nogil());
+  m.def("relation_decode8", &relation_decode8, nogil());
   m.def("quantize_rows", &quantize_rows, nogil());
   m.def("int8_linear", &int8_linear, nogil());
 }

@@ -1,7 +1,7 @@
 """Plain forms of the quantised formats, on the CPU in 64 bits with the formats' own rounding points.
 
-4 bits: groups of 32 values share a bf16 scale, codes are e2m1. 8 bits: a row shares an fp32 scale. Every
-32-bit quotient and product of the definition is taken in fp64 and rounded (a quotient or product of two fp32
+4 bits: groups of 32 values share a bf16 scale, codes are e2m1. 8 bits: a row shares an fp32 scale, and in the
+paged cache a block of 64 rows of a head does, whose codes are e4m3. Every 32-bit quotient and product of the definition is taken in fp64 and rounded (a quotient or product of two fp32
 values is rounded correctly that way), so codes and scales are the definition's bit for bit.
 """
 
@@ -60,6 +60,44 @@ def unpack_codes(codes: torch.Tensor, D: int) -> torch.Tensor:
     """Stored bytes [..., 16 G] -> signed code values [..., D] fp64."""
     nib = torch.stack([codes & 15, codes >> 4], -1).flatten(-2)[..., :D].long()
     return torch.where(nib >= 8, -1.0, 1.0).double() * MAGNITUDES[nib % 8]
+
+
+def nearest_e4m3(t: torch.Tensor) -> torch.Tensor:
+    """The e4m3 value nearest to each fp64 value (ties to the even mantissa, 448 at most)."""
+    n = torch.arange(127)
+    mag = torch.where(n < 8, (n % 8).double() * 2.0 ** -9, (1.0 + (n % 8).double() / 8.0) * torch.pow(2.0, (n // 8 - 7).double()))
+    a = t.abs().clamp(max=448.0)
+    hi = torch.searchsorted(mag, a.contiguous()).clamp(max=126)   # the first value >= a
+    lo = (hi - 1).clamp(min=0)
+    up, down = mag[hi] - a, a - mag[lo]
+    pick = torch.where(up < down, hi, torch.where(down < up, lo, torch.where(hi % 2 == 0, hi, lo)))
+    return torch.where(t < 0, -1.0, 1.0).double() * mag[pick]
+
+
+def block8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Blocks [..., 64, D] -> (codes as values fp64, scales fp64 [...], NaN for blocks with a NaN or an infinity)."""
+    x = x.double()
+    finite = torch.isfinite(x).flatten(-2).all(-1)
+    top = torch.where(finite[..., None, None], x, 0.0).abs().amax((-1, -2))
+    live = finite & (top >= 2.0 ** -112)
+    safe = torch.where(live, top, 1.0)
+    t = _f32(torch.where(live[..., None, None], x, 0.0) * _f32(448.0 / safe)[..., None, None])
+    scale = torch.where(live, _f32(safe / 448.0), 0.0)
+    return nearest_e4m3(t), torch.where(finite, scale, float("nan"))
+
+
+def values8(x: torch.Tensor) -> torch.Tensor:
+    """fp64 values that blocks [..., 64, D] have in 8 bits (32-bit numbers)."""
+    codes, scale = block8(x)
+    return _f32(codes * scale[..., None, None])
+
+
+def held8(rows: torch.Tensor) -> torch.Tensor:
+    """fp64 values of the rows [H, n, D] of one sequence as the paged cache holds them: whole blocks in 8 bits, the
+    rest as it is."""
+    n = rows.shape[1] // 64 * 64
+    whole = values8(rows[:, :n].unflatten(1, (-1, 64))).flatten(1, 2) if n else rows[:, :0].double()
+    return torch.cat([whole, rows[:, n:].double()], 1)
 
 
 def quantize8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
