@@ -883,6 +883,69 @@ typedef struct mote_relation_decode8_args {
 size_t mote_relation_decode8_workspace(const mote_relation_decode8_args* args);
 int mote_relation_decode8(const mote_relation_decode8_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The pages of that cache: table [B, blocks] (int32, rows table_sb apart) names the page of block j of sequence b,
+ * -1 where there is none; refs [pages] counts the entries that name a page (0: free). Every call is on the device
+ * and in stream order. No counterpart in the reference, whose prefix store keeps its pages on the host
+ * (mote/infer/prefix_cache.py:122-176).
+ * mote_pages_free: the entries of the n sequences seqs[] (host memory, each once) release their pages.
+ * mote_pages_fork: the n sequences seqs[] release theirs, then share src's first S[src] / 64 entries; S[dst] = S[src],
+ * and the S[src] % 64 rows of src's tail are copied in every plane of tails [planes][B][H][64][D] (elem_bytes a
+ * value; planes tails_sp, sequences tails_sb elements apart; NULL for none). src is none of seqs.
+ * mote_pages_reserve: every sequence gets pages for the blocks j < rows / 64 (rows, or rows_dev[b]) that have none:
+ * free pages from the lowest number on, in the order of (b, j). *missing (device) is the number of entries left
+ * without one.
+ * ------------------------------------------------------------------------------------------------ */
+typedef struct mote_pages_args {
+  int B, blocks, pages, n;
+  int32_t* table;
+  int64_t table_sb;
+  int32_t* refs;
+  const int32_t* seqs;
+  int src;
+  int64_t* S;
+  int elem_bytes, planes, H, D;
+  void* tails;
+  int64_t tails_sp, tails_sb;
+  int64_t rows;
+  const int64_t* rows_dev;
+  int32_t* missing;
+} mote_pages_args;
+
+int mote_pages_free(const mote_pages_args* args, void* stream);
+int mote_pages_fork(const mote_pages_args* args, void* stream);
+int mote_pages_reserve(const mote_pages_args* args, void* stream);
+
+/* mote_pages_compact: the pages in use (refs > 0) of a pool copied into another, in the order of their numbers from
+ * 0 on: codes [planes][pages][page_bytes] (planes codes_sp bytes apart; 16-byte multiples), scales
+ * [planes][pages][H] (planes scale_sp elements apart), refs; refs2 past them zero, codes2 and scales2 left as they
+ * were. table2 [B, blocks] (dense) is the table in the new numbers. Pages beyond the new pool are dropped, their
+ * entries -1 and counted in *missing (device). Workspace: mote_pages_compact_workspace() bytes, contents on entry
+ * do not matter. */
+typedef struct mote_pages_compact_args {
+  int planes, pages, pages2, H, B, blocks;
+  int64_t page_bytes;
+  const void* codes;
+  int64_t codes_sp;
+  const float* scales;
+  int64_t scale_sp;
+  const int32_t* refs;
+  const int32_t* table;
+  int64_t table_sb;
+  void* codes2;
+  int64_t codes2_sp;
+  float* scales2;
+  int64_t scale2_sp;
+  int32_t* refs2;
+  int32_t* table2;
+  int32_t* missing;
+  void* workspace;
+  size_t workspace_bytes;
+} mote_pages_compact_args;
+
+size_t mote_pages_compact_workspace(const mote_pages_compact_args* args);
+int mote_pages_compact(const mote_pages_compact_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -317,6 +317,27 @@ class Decode8Args(C.Structure):
     ]
 
 
+class PagesArgs(C.Structure):
+    _fields_ = [
+        ("B", C.c_int), ("blocks", C.c_int), ("pages", C.c_int), ("n", C.c_int), ("table", C.c_void_p),
+        ("table_sb", C.c_int64), ("refs", C.c_void_p), ("seqs", C.c_void_p), ("src", C.c_int), ("S", C.c_void_p),
+        ("elem_bytes", C.c_int), ("planes", C.c_int), ("H", C.c_int), ("D", C.c_int), ("tails", C.c_void_p),
+        ("tails_sp", C.c_int64), ("tails_sb", C.c_int64), ("rows", C.c_int64), ("rows_dev", C.c_void_p),
+        ("missing", C.c_void_p),
+    ]
+
+
+class PagesCompactArgs(C.Structure):
+    _fields_ = [
+        ("planes", C.c_int), ("pages", C.c_int), ("pages2", C.c_int), ("H", C.c_int), ("B", C.c_int),
+        ("blocks", C.c_int), ("page_bytes", C.c_int64), ("codes", C.c_void_p), ("codes_sp", C.c_int64),
+        ("scales", C.c_void_p), ("scale_sp", C.c_int64), ("refs", C.c_void_p), ("table", C.c_void_p),
+        ("table_sb", C.c_int64), ("codes2", C.c_void_p), ("codes2_sp", C.c_int64), ("scales2", C.c_void_p),
+        ("scale2_sp", C.c_int64), ("refs2", C.c_void_p), ("table2", C.c_void_p), ("missing", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+    ]
+
+
 # every symbol the header declares, with its argument types
 EXPORTS = {
     "mote_last_error": ([], C.c_char_p),
@@ -368,6 +389,11 @@ EXPORTS = {
     "mote_cache8_read": ([C.POINTER(Cache8RowsArgs), C.c_void_p], C.c_int),
     "mote_relation_decode8_workspace": ([C.POINTER(Decode8Args)], C.c_size_t),
     "mote_relation_decode8": ([C.POINTER(Decode8Args), C.c_void_p], C.c_int),
+    "mote_pages_free": ([C.POINTER(PagesArgs), C.c_void_p], C.c_int),
+    "mote_pages_fork": ([C.POINTER(PagesArgs), C.c_void_p], C.c_int),
+    "mote_pages_reserve": ([C.POINTER(PagesArgs), C.c_void_p], C.c_int),
+    "mote_pages_compact_workspace": ([C.POINTER(PagesCompactArgs)], C.c_size_t),
+    "mote_pages_compact": ([C.POINTER(PagesCompactArgs), C.c_void_p], C.c_int),
     "mote_abi_layout": ([], C.c_char_p),
     "mote_clock_probe": ([C.c_void_p, C.c_int, C.c_int, C.c_void_p], C.c_int),
 }
@@ -387,6 +413,8 @@ STRUCTS = {
     "mote_dechunk_step_args": DechunkStepArgs, "mote_cache4": Cache4View, "mote_cache4_rows_args": Cache4RowsArgs,
     "mote_relation_decode4_args": Decode4Args, "mote_quantize_rows_args": QuantizeRowsArgs,
     "mote_int8_linear_args": Int8LinearArgs,
+    "mote_pages_args": PagesArgs,
+    "mote_pages_compact_args": PagesCompactArgs,
     "mote_cache8": Cache8View,
     "mote_cache8_rows_args": Cache8RowsArgs,
     "mote_relation_decode8_args": Decode8Args,

@@ -40,6 +40,11 @@ int launch_decode4(const mote_relation_decode4_args* a, hipStream_t stream);
 int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream);
 size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a);
 int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream);
+int launch_pages_free(const mote_pages_args* a, hipStream_t stream);
+int launch_pages_fork(const mote_pages_args* a, hipStream_t stream);
+int launch_pages_reserve(const mote_pages_args* a, hipStream_t stream);
+size_t pages_compact_workspace_bytes(const mote_pages_compact_args* a);
+int launch_pages_compact(const mote_pages_compact_args* a, hipStream_t stream);
 int launch_cache8_write(const mote_cache8_rows_args* a, hipStream_t stream);
 int launch_cache8_read(const mote_cache8_rows_args* a, hipStream_t stream);
 size_t decode8_workspace_bytes(const mote_relation_decode8_args* a);
@@ -248,6 +253,28 @@ size_t mote_relation_decode8_workspace(const mote_relation_decode8_args* args) {
 int mote_relation_decode8(const mote_relation_decode8_args* args, void* stream) {
   mote::g_err[0] = 0;
   return mote::launch_decode8(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+int mote_pages_free(const mote_pages_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_pages_free(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+int mote_pages_fork(const mote_pages_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_pages_fork(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+int mote_pages_reserve(const mote_pages_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_pages_reserve(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+size_t mote_pages_compact_workspace(const mote_pages_compact_args* args) { return args ? mote::pages_compact_workspace_bytes(args) : 0; }
+
+int mote_pages_compact(const mote_pages_compact_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_pages_compact(args, reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

@@ -892,6 +892,143 @@ std::tuple<Tensor, Tensor> relation_decode8(const Tensor& p1, const Tensor& p2, 
   return {y, g};
 }
 
+// ---- the pages of that cache ------------------------------------------------------------------------------
+// table [B, blocks] and refs [pages] as a call's arguments
+mote_pages_args page_table(const Tensor& refs, const Tensor& table, const char* what) {
+  if (refs.dim() != 1 || refs.numel() < 1 || !refs.is_contiguous()) bad_value(what, ": refs must be contiguous, a count per page");
+  if (table.dim() != 2 || table.numel() < 1 || (table.size(1) > 1 && table.stride(1) != 1) || !separate(table))
+    bad_value(what, ": the table must be [B, blocks] with unit stride, every entry at a place of its own");
+  if (refs.scalar_type() != at::kInt || table.scalar_type() != at::kInt || refs.device() != table.device())
+    throw py::type_error(c10::str(what, ": refs and the table must be int32 on one device"));
+  if (!ranges_apart(refs, table)) bad_value(what, ": refs lies over the table");
+  if (table.size(0) > INT_MAX || table.size(1) > (int64_t(1) << 24) || refs.numel() > (int64_t(1) << 30))
+    bad_value(what, ": at most 2^24 blocks and 2^30 pages");
+  mote_pages_args a{};
+  a.B = int(table.size(0)); a.blocks = int(table.size(1)); a.pages = int(refs.numel());
+  a.table = iptr(table); a.table_sb = a.B > 1 ? table.stride(0) : 0;
+  a.refs = iptr(refs);
+  return a;
+}
+std::vector<int32_t> sequences(const std::vector<int64_t>& seqs, int64_t B, int64_t src, const char* what) {
+  std::vector<int32_t> r;
+  std::vector<bool> seen(size_t(B), false);
+  for (const int64_t s : seqs) {
+    if (s < 0 || s >= B) bad_value(what, ": no sequence ", s, " of ", B);
+    if (s == src) bad_value(what, ": sequence ", s, " is the source");
+    if (seen[size_t(s)]) bad_value(what, ": sequence ", s, " twice");
+    seen[size_t(s)] = true;
+    r.push_back(int32_t(s));
+  }
+  return r;
+}
+
+void pages_free(const Tensor& refs, const Tensor& table, const std::vector<int64_t>& seqs) {
+  const char* what = "pages_free";
+  mote_pages_args a = page_table(refs, table, what);
+  const std::vector<int32_t> list = sequences(seqs, a.B, -1, what);
+  on_gpu(table, what);
+  const On on(table);
+  a.seqs = list.data(); a.n = int(list.size());
+  check(mote_pages_free(&a, on.stream), "mote_pages_free");
+}
+
+void pages_fork(const Tensor& refs, const Tensor& table, const Tensor& S, int64_t src, const std::vector<int64_t>& dst,
+                const OptTensor& tails) {
+  const char* what = "pages_fork";
+  mote_pages_args a = page_table(refs, table, what);
+  positions(S, a.B, table.device(), what, "S");
+  if (src < 0 || src >= a.B) bad_value(what, ": no sequence ", src, " of ", a.B);
+  const std::vector<int32_t> list = sequences(dst, a.B, src, what);
+  if (tails) {
+    const Tensor& t = *tails;
+    if (t.dim() != 5 || t.size(1) != a.B || t.size(3) != 64 || t.numel() == 0 || t.device() != table.device())
+      bad_value(what, ": tails must be [planes, B, H, 64, D] on the table's device, got ", t.sizes());
+    const int64_t H = t.size(2), D = t.size(4);
+    code(t);
+    if (D > 128 || D % 8) bad_value(what, ": head dim ", D, " unsupported (need 8 <= D <= 128, D % 8 == 0)");
+    if (t.stride(4) != 1 || t.stride(3) != D || (H > 1 && t.stride(2) != 64 * D) || !separate(t))
+      bad_value(what, ": the tails of a sequence must lie back to back, each at a place of its own");
+    if (t.size(0) > INT_MAX || H > INT_MAX) bad_value(what, ": sizes beyond 32 bits");
+    if (!ranges_apart(t, table) || !ranges_apart(t, refs) || !ranges_apart(t, S)) bad_value(what, ": tails lies over the table");
+    no_grad(what, {&t});
+    a.elem_bytes = int(t.element_size()); a.planes = int(t.size(0)); a.H = int(H); a.D = int(D);
+    a.tails = t.data_ptr();
+    a.tails_sp = a.planes > 1 ? t.stride(0) : 0; a.tails_sb = a.B > 1 ? t.stride(1) : 0;
+  }
+  on_gpu(table, what);
+  const On on(table);
+  a.S = static_cast<int64_t*>(S.data_ptr());
+  a.src = int(src); a.seqs = list.data(); a.n = int(list.size());
+  check(mote_pages_fork(&a, on.stream), "mote_pages_fork");
+}
+
+Tensor pages_reserve(const Tensor& refs, const Tensor& table, int64_t rows, const OptTensor& rows_dev) {
+  const char* what = "pages_reserve";
+  mote_pages_args a = page_table(refs, table, what);
+  if (rows_dev) {
+    positions(*rows_dev, a.B, table.device(), what, "rows");
+    a.rows_dev = static_cast<const int64_t*>(rows_dev->data_ptr());
+  } else if (rows < 0 || rows / 64 > a.blocks) {
+    throw std::runtime_error(c10::str(what, ": ", rows, " rows in a table of ", int64_t(a.blocks) * 64));
+  }
+  a.rows = rows;
+  on_gpu(table, what);
+  const On on(table);
+  Tensor missing = empty({1}, table, at::kInt);
+  a.missing = iptr(missing);
+  check(mote_pages_reserve(&a, on.stream), "mote_pages_reserve");
+  return missing;
+}
+
+std::tuple<Tensor, Tensor> pages_compact(const std::vector<Tensor>& pool, const Tensor& table, const std::vector<Tensor>& into) {
+  const char* what = "pages_compact";
+  if (pool.size() != 3 || into.size() != 3) bad_value(what, ": a pool has three tensors");
+  const mote_pages_args t = page_table(pool[2], table, what);
+  mote_pages_compact_args a{};
+  const Tensor& like = pool[0];
+  auto check_pool = [&](const std::vector<Tensor>& p) {
+    const Tensor &codes = p[0], &scales = p[1], &refs = p[2];
+    if (codes.dim() != 3 || scales.dim() != 3 || refs.dim() != 1 || codes.size(0) != like.size(0) || codes.size(2) != like.size(2) ||
+        scales.size(0) != codes.size(0) || scales.size(1) != codes.size(1) || scales.size(2) != pool[1].size(2) ||
+        refs.size(0) != codes.size(1) || codes.numel() == 0 || scales.numel() == 0)
+      bad_value(what, ": a pool is codes [planes, pages, bytes], scales [planes, pages, H], refs [pages], alike but for their pages");
+    if (codes.size(2) % 16) bad_value(what, ": pages of ", codes.size(2), " bytes (a multiple of 16)");
+    if (codes.scalar_type() != at::kByte || scales.scalar_type() != at::kFloat || refs.scalar_type() != at::kInt ||
+        codes.device() != table.device() || scales.device() != table.device() || refs.device() != table.device())
+      throw py::type_error("pages_compact: codes must be uint8, scales fp32 and refs int32, on the table's device");
+    for (const Tensor* x : {&codes, &scales})
+      if ((x->size(2) > 1 && x->stride(2) != 1) || (x->size(1) > 1 && x->stride(1) != x->size(2)) || !separate(*x))
+        bad_value(what, ": the pages of a plane must lie back to back, each at a place of its own");
+    if (!refs.is_contiguous()) bad_value(what, ": refs must be contiguous");
+    if (reinterpret_cast<uintptr_t>(codes.data_ptr()) % 16 || (codes.size(0) > 1 && codes.stride(0) % 16))
+      bad_value(what, ": pages must start on 16-byte boundaries");
+    if (codes.size(0) > INT_MAX || codes.size(1) > (int64_t(1) << 30) || scales.size(2) > INT_MAX) bad_value(what, ": sizes beyond 32 bits");
+    no_grad(what, {&scales});
+  };
+  check_pool(pool);
+  check_pool(into);
+  std::vector<const Tensor*> all{&pool[0], &pool[1], &pool[2], &table, &into[0], &into[1], &into[2]};
+  for (size_t i = 4; i < all.size(); ++i)
+    for (size_t k = 0; k < i; ++k)
+      if (!ranges_apart(*all[i], *all[k])) bad_value(what, ": the new pool lies over the old one");
+  on_gpu(table, what);
+  const On on(table);
+  Tensor table2 = empty(table.sizes(), table, at::kInt), missing = empty({1}, table, at::kInt);
+  a.planes = int(like.size(0)); a.pages = int(like.size(1)); a.pages2 = int(into[0].size(1)); a.H = int(pool[1].size(2));
+  a.B = t.B; a.blocks = t.blocks; a.page_bytes = like.size(2);
+  a.codes = like.data_ptr(); a.codes_sp = a.planes > 1 ? like.stride(0) : 0;
+  a.scales = fptr(pool[1]); a.scale_sp = a.planes > 1 ? pool[1].stride(0) : 0;
+  a.refs = t.refs; a.table = t.table; a.table_sb = t.table_sb;
+  a.codes2 = into[0].data_ptr(); a.codes2_sp = a.planes > 1 ? into[0].stride(0) : 0;
+  a.scales2 = fptr(into[1]); a.scale2_sp = a.planes > 1 ? into[1].stride(0) : 0;
+  a.refs2 = iptr(into[2]); a.table2 = iptr(table2); a.missing = iptr(missing);
+  const Tensor ws = bytes(mote_pages_compact_workspace(&a), table);
+  a.workspace = ws.data_ptr();
+  a.workspace_bytes = size_t(ws.numel());
+  check(mote_pages_compact(&a, on.stream), "mote_pages_compact");
+  return {table2, missing};
+}
+
 std::tuple<Tensor, Tensor> quantize_rows(Tensor x) {
   if (x.dim() != 2 || x.size(1) < 1) bad_value("quantize_rows: x must be [M, K]");
   mote_quantize_rows_args a{};
@@ -986,6 +1123,10 @@ PYBIND11_MODULE(_torch_launch, m) {
   m.def("cache8_write", &cache8_write, nogil());
   m.def("cache8_read", &cache8_read, nogil());
   m.def("relation_decode8", &relation_decode8, nogil());
+  m.def("pages_free", &pages_free, nogil());
+  m.def("pages_fork", &pages_fork, nogil());
+  m.def("pages_reserve", &pages_reserve, nogil());
+  m.def("pages_compact", &pages_compact, nogil());
   m.def("quantize_rows", &quantize_rows, nogil());
   m.def("int8_linear", &int8_linear, nogil());
 }
