@@ -946,6 +946,36 @@ typedef struct mote_pages_compact_args {
 size_t mote_pages_compact_workspace(const mote_pages_compact_args* args);
 int mote_pages_compact(const mote_pages_compact_args* args, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * mote_sample: the next token of every row of logits [B, V] (dtype, unit element stride, rows l_sr apart, V <= 2^20)
+ * from one random number u[b] in [0, 1).
+ * Weights w = exp((x - max) / temperature); order: by logit, ties to the lowest index first. Kept are the first
+ * top_k (0: all), of these the shortest run from the first on that holds at least top_p of their weight (1: all),
+ * and of those the ones with w >= min_p; the first is always kept. The token is the first in that order whose
+ * running weight exceeds u times the weight kept. A temperature of 0 takes the first of the order. Each setting is
+ * one number, or a device array of one per row where its _dev is not NULL.
+ * A row whose logits are all -inf, one with a NaN, and one with a NaN among u and its settings give -1. Of several
+ * logits +inf each has the same weight. Weights are sums of fixed-point numbers (2^-43): no order of summation.
+ * With run (device flag) 0 nothing is written.
+ * Replaces: GraphDecoder._sample (mote/infer/graph.py:243), for one sequence with the reference's own settings.
+ * ------------------------------------------------------------------------------------------------ */
+typedef struct mote_sample_args {
+  int dtype;
+  int B, V;
+  const void* logits; int64_t l_sr;
+  const float* u;
+  float temperature, top_p, min_p;
+  int64_t top_k;
+  const float* temperature_dev;
+  const float* top_p_dev;
+  const float* min_p_dev;
+  const int64_t* top_k_dev;
+  int64_t* tokens;
+  const unsigned char* run;
+} mote_sample_args;
+
+int mote_sample(const mote_sample_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

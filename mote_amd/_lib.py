@@ -338,6 +338,15 @@ class PagesCompactArgs(C.Structure):
     ]
 
 
+class SampleArgs(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int), ("B", C.c_int), ("V", C.c_int), ("logits", C.c_void_p), ("l_sr", C.c_int64),
+        ("u", C.c_void_p), ("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float),
+        ("top_k", C.c_int64), ("temperature_dev", C.c_void_p), ("top_p_dev", C.c_void_p), ("min_p_dev", C.c_void_p),
+        ("top_k_dev", C.c_void_p), ("tokens", C.c_void_p), ("run", C.c_void_p),
+    ]
+
+
 # every symbol the header declares, with its argument types
 EXPORTS = {
     "mote_last_error": ([], C.c_char_p),
@@ -394,6 +403,7 @@ EXPORTS = {
     "mote_pages_reserve": ([C.POINTER(PagesArgs), C.c_void_p], C.c_int),
     "mote_pages_compact_workspace": ([C.POINTER(PagesCompactArgs)], C.c_size_t),
     "mote_pages_compact": ([C.POINTER(PagesCompactArgs), C.c_void_p], C.c_int),
+    "mote_sample": ([C.POINTER(SampleArgs), C.c_void_p], C.c_int),
     "mote_abi_layout": ([], C.c_char_p),
     "mote_clock_probe": ([C.c_void_p, C.c_int, C.c_int, C.c_void_p], C.c_int),
 }
@@ -413,6 +423,7 @@ STRUCTS = {
     "mote_dechunk_step_args": DechunkStepArgs, "mote_cache4": Cache4View, "mote_cache4_rows_args": Cache4RowsArgs,
     "mote_relation_decode4_args": Decode4Args, "mote_quantize_rows_args": QuantizeRowsArgs,
     "mote_int8_linear_args": Int8LinearArgs,
+    "mote_sample_args": SampleArgs,
     "mote_pages_args": PagesArgs,
     "mote_pages_compact_args": PagesCompactArgs,
     "mote_cache8": Cache8View,

@@ -40,6 +40,7 @@ int launch_decode4(const mote_relation_decode4_args* a, hipStream_t stream);
 int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream);
 size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a);
 int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream);
+int launch_sample(const mote_sample_args* a, hipStream_t stream);
 int launch_pages_free(const mote_pages_args* a, hipStream_t stream);
 int launch_pages_fork(const mote_pages_args* a, hipStream_t stream);
 int launch_pages_reserve(const mote_pages_args* a, hipStream_t stream);
@@ -275,6 +276,11 @@ size_t mote_pages_compact_workspace(const mote_pages_compact_args* args) { retur
 int mote_pages_compact(const mote_pages_compact_args* args, void* stream) {
   mote::g_err[0] = 0;
   return mote::launch_pages_compact(args, reinterpret_cast<hipStream_t>(stream));
+}
+
+int mote_sample(const mote_sample_args* args, void* stream) {
+  mote::g_err[0] = 0;
+  return mote::launch_sample(args, reinterpret_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

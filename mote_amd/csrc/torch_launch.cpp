@@ -1101,6 +1101,64 @@ Tensor int8_linear(const Tensor& x_, const Tensor& wq, const Tensor& ws, int64_t
   return y;
 }
 
+// ---- the next token ---------------------------------------------------------------------------------------
+// a setting: one number, or a device tensor of one per row
+template <typename N, typename D>
+void setting(const py::object& x, at::ScalarType dt, int64_t B, const Tensor& like, N& number, const D*& dev, const char* name) {
+  const char* what = "sample_tokens";
+  if (!THPVariable_Check(x.ptr())) {
+    try {
+      number = x.cast<N>();
+    } catch (const py::cast_error&) {
+      throw py::type_error(c10::str(what, ": ", name, " must be ", c10::toString(dt), ": a number, or one per row"));
+    }
+    return;
+  }
+  const Tensor t = THPVariable_Unpack(x.ptr());
+  if (t.dim() != 1 || t.numel() != B || !t.is_contiguous() || t.device() != like.device())
+    bad_value(what, ": ", name, " must be a number, or a contiguous tensor of B = ", B, " on the logits' device");
+  if (t.scalar_type() != dt) throw py::type_error(c10::str(what, ": ", name, " must be ", c10::toString(dt), ", one per row"));
+  no_grad(what, {&t});
+  dev = static_cast<const D*>(t.data_ptr());
+}
+
+Tensor sample_tokens(const Tensor& x_, const Tensor& u, const py::object& temperature, const py::object& top_k,
+                     const py::object& top_p, const py::object& min_p, const OptTensor& out, const OptTensor& run) {
+  const char* what = "sample_tokens";
+  if (x_.dim() != 2) bad_value(what, ": logits must be [B, V], got ", x_.sizes());
+  const int64_t B = x_.size(0), V = x_.size(1);
+  if (V < 1 || V > (int64_t(1) << 20) || B > INT_MAX) bad_value(what, ": ", B, " rows of ", V, " logits (1 to 2^20 a row)");
+  mote_sample_args a{};
+  a.dtype = code(x_);
+  if (u.dim() != 1 || u.numel() != B || !u.is_contiguous() || u.device() != x_.device())
+    bad_value(what, ": u must be a contiguous tensor of B = ", B, " on the logits' device");
+  if (u.scalar_type() != at::kFloat) throw py::type_error("sample_tokens: u must be float32");
+  setting(temperature, at::kFloat, B, x_, a.temperature, a.temperature_dev, "temperature");
+  setting(top_k, at::kLong, B, x_, a.top_k, a.top_k_dev, "top_k");
+  setting(top_p, at::kFloat, B, x_, a.top_p, a.top_p_dev, "top_p");
+  setting(min_p, at::kFloat, B, x_, a.min_p, a.min_p_dev, "min_p");
+  if (!a.temperature_dev && !(a.temperature >= 0.f)) bad_value(what, ": temperature ", a.temperature, " (0 or more)");
+  if (!a.top_k_dev && a.top_k < 0) bad_value(what, ": top_k ", a.top_k, " (0 for all, or more)");
+  if (!a.top_p_dev && !(a.top_p >= 0.f)) bad_value(what, ": top_p ", a.top_p, " (0 or more)");
+  if (!a.min_p_dev && !(a.min_p >= 0.f)) bad_value(what, ": min_p ", a.min_p, " (0 or more)");
+  check_run(run, x_, what);
+  if (out && (out->dim() != 1 || out->numel() != B || out->scalar_type() != at::kLong || out->device() != x_.device() ||
+              !out->is_contiguous()))
+    bad_value(what, ": out must be a contiguous int64 tensor of B = ", B, " on the logits' device");
+  no_grad(what, {&x_, &u});
+  on_gpu(x_, what);
+  const On on(x_);
+  const Tensor x = x_.size(1) > 1 ? unit(x_) : x_;
+  const Tensor tokens = out ? *out : empty({B}, x_, at::kLong);
+  a.B = int(B); a.V = int(V);
+  a.logits = x.data_ptr(); a.l_sr = B > 1 ? x.stride(0) : 0;
+  a.u = fptr(u);
+  a.tokens = static_cast<int64_t*>(tokens.data_ptr());
+  a.run = run ? static_cast<const unsigned char*>(run->data_ptr()) : nullptr;
+  check(mote_sample(&a, on.stream), "mote_sample");
+  return tokens;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_torch_launch, m) {
@@ -1129,4 +1187,5 @@ PYBIND11_MODULE(_torch_launch, m) {
   m.def("pages_compact", &pages_compact, nogil());
   m.def("quantize_rows", &quantize_rows, nogil());
   m.def("int8_linear", &int8_linear, nogil());
+  m.def("sample_tokens", &sample_tokens);  // takes numbers or tensors: with the interpreter's lock
 }
