@@ -956,7 +956,8 @@ int mote_pages_compact(const mote_pages_compact_args* args, void* stream);
  * one number, or a device array of one per row where its _dev is not NULL.
  * A row whose logits are all -inf, one with a NaN, and one with a NaN among u and its settings give -1. Of several
  * logits +inf each has the same weight. Weights are sums of fixed-point numbers (2^-43): no order of summation.
- * With run (device flag) 0 nothing is written.
+ * With run (device flag) 0 no token is written. Workspace: mote_sample_workspace() bytes (0 where none is needed),
+ * contents on entry do not matter.
  * Replaces: GraphDecoder._sample (mote/infer/graph.py:243), for one sequence with the reference's own settings.
  * ------------------------------------------------------------------------------------------------ */
 typedef struct mote_sample_args {
@@ -971,9 +972,12 @@ typedef struct mote_sample_args {
   const float* min_p_dev;
   const int64_t* top_k_dev;
   int64_t* tokens;
+  void* workspace;
+  size_t workspace_bytes;
   const unsigned char* run;
 } mote_sample_args;
 
+size_t mote_sample_workspace(const mote_sample_args* args);
 int mote_sample(const mote_sample_args* args, void* stream);
 
 #ifdef __cplusplus

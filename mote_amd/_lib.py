@@ -343,7 +343,8 @@ class SampleArgs(C.Structure):
         ("dtype", C.c_int), ("B", C.c_int), ("V", C.c_int), ("logits", C.c_void_p), ("l_sr", C.c_int64),
         ("u", C.c_void_p), ("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float),
         ("top_k", C.c_int64), ("temperature_dev", C.c_void_p), ("top_p_dev", C.c_void_p), ("min_p_dev", C.c_void_p),
-        ("top_k_dev", C.c_void_p), ("tokens", C.c_void_p), ("run", C.c_void_p),
+        ("top_k_dev", C.c_void_p), ("tokens", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t),
+        ("run", C.c_void_p),
     ]
 
 
@@ -403,6 +404,7 @@ EXPORTS = {
     "mote_pages_reserve": ([C.POINTER(PagesArgs), C.c_void_p], C.c_int),
     "mote_pages_compact_workspace": ([C.POINTER(PagesCompactArgs)], C.c_size_t),
     "mote_pages_compact": ([C.POINTER(PagesCompactArgs), C.c_void_p], C.c_int),
+    "mote_sample_workspace": ([C.POINTER(SampleArgs)], C.c_size_t),
     "mote_sample": ([C.POINTER(SampleArgs), C.c_void_p], C.c_int),
     "mote_abi_layout": ([], C.c_char_p),
     "mote_clock_probe": ([C.c_void_p, C.c_int, C.c_int, C.c_void_p], C.c_int),

@@ -40,6 +40,7 @@ int launch_decode4(const mote_relation_decode4_args* a, hipStream_t stream);
 int launch_quantize_rows(const mote_quantize_rows_args* a, hipStream_t stream);
 size_t int8_linear_workspace_bytes(const mote_int8_linear_args* a);
 int launch_int8_linear(const mote_int8_linear_args* a, hipStream_t stream);
+size_t sample_workspace_bytes(const mote_sample_args* a);
 int launch_sample(const mote_sample_args* a, hipStream_t stream);
 int launch_pages_free(const mote_pages_args* a, hipStream_t stream);
 int launch_pages_fork(const mote_pages_args* a, hipStream_t stream);
@@ -277,6 +278,8 @@ int mote_pages_compact(const mote_pages_compact_args* args, void* stream) {
   mote::g_err[0] = 0;
   return mote::launch_pages_compact(args, reinterpret_cast<hipStream_t>(stream));
 }
+
+size_t mote_sample_workspace(const mote_sample_args* args) { return args ? mote::sample_workspace_bytes(args) : 0; }
 
 int mote_sample(const mote_sample_args* args, void* stream) {
   mote::g_err[0] = 0;

@@ -5,12 +5,17 @@
 // weight up to the token at which p of that is reached, the draw for the token at which u of the weight kept is
 // passed; min-p is a sum over the row. Nothing is sorted. Weights are fixed-point numbers of 2^-43 of the largest,
 // rounded from an fp64 exponential, in 64 bits: sums of up to 2^20 of them are exact, so their order does not matter
-// and atomics may make them, and a border differs from the real one by 2^-33 of the largest weight at most.
+// and atomics may make them, and a border differs from the real one by V 2^-44 of the largest weight at most.
 //
-// A row: its maximum; a histogram over 2048 intervals of the logit (an interval's count and weight); its prefix
-// sums, in which a search finds an interval; the interval's tokens gathered in LDS, where each counts the ones before
-// it. An interval of more tokens than LDS holds (many equal logits) is searched by the digits of its keys instead.
+// A row: its maximum; a histogram over intervals of the logit (an interval's count and weight); its prefix sums, in
+// which a search finds an interval; then the digits of the keys, and for equal logits of the indices, of that
+// interval's tokens, which are gathered in LDS unless they are too many (many equal logits).
+//
+// Up to 32768 logits a workgroup has a row, in registers. Longer rows go in pieces over three launches (maximum;
+// histogram; the tokens of the intervals that a search can end in, and by the last piece of a row the searches),
+// since one CU alone reads a row of 131072 logits in 5 us and makes its exponentials in 30.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.hpp"
 #include "device.hpp"
@@ -18,6 +23,8 @@
 #include "stream.hpp"
 
 namespace mote {
+
+typedef unsigned long long u64;
 
 struct SampleParams {
   const void* logits;
@@ -32,58 +39,78 @@ struct SampleParams {
   int64_t* tokens;
   const unsigned char* run;
   int V;
+  // rows in pieces
+  char* ws;
+  int pieces, piece;  // logits of a piece: whole 16-byte chunks
 };
 
-typedef unsigned long long u64;
-constexpr int kBins = 2048;
+constexpr int kBins = 2048;                      // intervals of a long row
 constexpr int kList = 1024;                      // tokens of an interval that are searched in LDS
 constexpr double kOne = 8796093022208.0;         // 2^43: the largest weight
 constexpr float kReach = 31.0f;                  // exp(-31) < 2^-44: no weight from there on
+constexpr double kReach2 = 45.0;                 // 2^-45: nor from there
+constexpr int kMaxPieces = 64;
 
 // order of logits: a larger key comes first (the sum with +0 makes one zero of two)
 __device__ __forceinline__ uint32_t key_of(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return b ^ (uint32_t(int32_t(b) >> 31) | 0x80000000u);
 }
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
-template <int NT>
+struct Digits {
+  u64 mass[256];
+  uint32_t cnt[256];
+};
+template <int BINS, int LIST>
 struct Lds {
-  u64 mass[kBins];  // prefix sums once scanned
-  uint32_t cnt[kBins];
-  u64 lw[kList];
-  uint32_t lkey[kList], lidx[kList];
+  u64 mass[BINS];  // prefix sums once scanned
+  uint32_t cnt[BINS];
+  u64 lw[LIST];  // the tokens of an interval
+  uint32_t lkey[LIST], lidx[LIST];
+  Digits dig[3];
   u64 red64[16];
   uint32_t red32[16];
   float redf[16], redm[16];
-  int redi[16];
-  u64 out_before, out_w;
-  uint32_t out_idx, n;
-  int nan;
+  u64 high;
+  uint32_t bin[2], idx, n, first;
+  int last;
 };
 
+// wave prefix sums by DPP moves within and across rows of 16 lanes (a shuffle through LDS costs several times more)
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_or0(uint32_t x) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(x), CTRL, ROWS, 0xF, false));
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_or0(u64 x) {
+  return (u64(dpp_or0<CTRL, ROWS>(uint32_t(x >> 32))) << 32) | dpp_or0<CTRL, ROWS>(uint32_t(x));
+}
+template <typename N>
+__device__ __forceinline__ N wave_scan(N x) {  // inclusive
+  x += dpp_or0<0x111, 0xF>(x);  // row_shr:1
+  x += dpp_or0<0x112, 0xF>(x);
+  x += dpp_or0<0x114, 0xF>(x);
+  x += dpp_or0<0x118, 0xF>(x);
+  x += dpp_or0<0x142, 0xA>(x);  // row_bcast:15 into rows 1 and 3
+  x += dpp_or0<0x143, 0xC>(x);  // row_bcast:31 into rows 2 and 3
+  return x;
+}
+
 // exclusive prefix over the workgroup's threads
-template <int NT>
-__device__ __forceinline__ void scan_block(u64& m, uint32_t& c, Lds<NT>& s) {
+template <int NT, typename S>
+__device__ __forceinline__ void scan_block(u64& m, uint32_t& c, S& s) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const u64 m0 = m;
-  const uint32_t c0 = c;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const u64 mm = __shfl_up(m, d);
-    const uint32_t cc = __shfl_up(c, d);
-    if (lane >= d) {
-      m += mm;
-      c += cc;
-    }
-  }
+  const u64 m1 = wave_scan(m);
+  const uint32_t c1 = wave_scan(c);
   __syncthreads();
   if (lane == 63) {
-    s.red64[wave] = m;
-    s.red32[wave] = c;
+    s.red64[wave] = m1;
+    s.red32[wave] = c1;
   }
   __syncthreads();
-  m -= m0;
-  c -= c0;
+  m = m1 - m;
+  c = c1 - c;
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) {
     if (w < wave) {
@@ -93,20 +120,21 @@ __device__ __forceinline__ void scan_block(u64& m, uint32_t& c, Lds<NT>& s) {
   }
 }
 
-// R > 0: a thread holds elements tid + r NT of the row; R == 0: the row is read again each time
+// R > 0: a thread holds elements tid + r NT of the row; R == 0: the row is read each time, 16 bytes a thread
 template <typename T, int NT, int R>
 struct Row {
   const T* p;
-  int V;
+  int from, to;
   float x[R > 0 ? R : 1];
-  __device__ __forceinline__ void open(const T* row, int v) {
+  __device__ __forceinline__ void open(const T* row, int f, int t) {
     p = row;
-    V = v;
+    from = f;
+    to = t;
     if constexpr (R > 0) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const int i = int(threadIdx.x) + r * NT;
-        x[r] = i < V ? Elem<T>::to_f(p[i]) : 0.f;
+        const int i = from + int(threadIdx.x) + r * NT;
+        x[r] = i < to ? Elem<T>::to_f(p[i]) : 0.f;
       }
     }
   }
@@ -115,274 +143,648 @@ struct Row {
     if constexpr (R > 0) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
-        const int i = int(threadIdx.x) + r * NT;
-        if (i < V) f(x[r], i);
+        const int i = from + int(threadIdx.x) + r * NT;
+        if (i < to) f(x[r], i);
       }
     } else {
       constexpr int PER = 16 / int(sizeof(T));
-      const int whole = V / PER;
+      const int whole = (to - from) / PER;
       for (int c = threadIdx.x; c < whole; c += NT) {
-        const Chunk q = load_any(p + c * PER);
+        const int i0 = from + c * PER;
+        const Chunk q = load_any(p + i0);
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
           float v;
           if constexpr (sizeof(T) == 2) v = __uint_as_float(k % 2 ? q.w[k / 2] & 0xffff0000u : q.w[k / 2] << 16);
           else v = __uint_as_float(q.w[k]);
-          f(v, c * PER + k);
+          f(v, i0 + k);
         }
       }
-      for (int i = whole * PER + int(threadIdx.x); i < V; i += NT) f(Elem<T>::to_f(p[i]), i);
+      for (int i = from + whole * PER + int(threadIdx.x); i < to; i += NT) f(Elem<T>::to_f(p[i]), i);
     }
   }
 };
 
+// a row's settings
+struct Setting {
+  float temperature, top_p, min_p, u;
+  int64_t top_k;
+  __device__ __forceinline__ Setting(const SampleParams& p, int b)
+      : temperature(p.temperature_dev ? p.temperature_dev[b] : p.temperature), top_p(p.top_p_dev ? p.top_p_dev[b] : p.top_p),
+        min_p(p.min_p_dev ? p.min_p_dev[b] : p.min_p), u(p.u[b]), top_k(p.top_k_dev ? p.top_k_dev[b] : p.top_k) {}
+  __device__ __forceinline__ bool nan() const {
+    return u != u || temperature != temperature || top_p != top_p || min_p != min_p;
+  }
+  __device__ __forceinline__ bool greedy() const { return !(temperature > 0.f); }
+};
+
+// intervals and weights of a row
+template <int BINS>
 struct Scale {
-  float top;       // the largest logit
-  float per;       // intervals per unit of the logit
-  double inv_t;
-  __device__ __forceinline__ int bin(float x) const {
+  float top;     // the largest logit
+  float per;     // intervals per unit of the logit
+  double rate;   // log2(e) / temperature
+  __device__ __forceinline__ Scale(const Setting& o, float top_, float low) : top(top_) {
+    rate = 1.44269504088896340736 / double(o.temperature);
+    const float span = fminf(kReach * o.temperature, top - low);  // at most as far as weights reach
+    per = span > 0.f ? float(BINS) / span : 0.f;
+    if (!(per < __builtin_inff())) per = 3e38f;  // a span below the normal numbers
+  }
+  __device__ __forceinline__ int bin(float x) const {  // never smaller for a smaller logit
     if (x == top) return 0;
-    const float t = (top - x) * per;  // inf where the logit or the largest one is infinite
-    return t < float(kBins - 1) ? int(t) : kBins - 1;
+    const float t = (top - x) * per;  // infinite or NaN where a logit is infinite: the last interval
+    return t < float(BINS - 1) ? int(t) : BINS - 1;
   }
-  __device__ __forceinline__ double weight(float x) const {
-    const double d = double(x) - double(top);
-    return x == top ? 1.0 : d > -__builtin_inf() ? exp(d * inv_t) : 0.0;
+  // The weight in units of 2^-43, from 2^f on |f| <= 1/2 by its power series up to f^11 (what follows is below 2^-47 of
+  // it) in fp64: seventeen instructions, a library exponential to the last place takes three times as many (64 rows of
+  // 131072 logits: 64 -> 37 us over all).
+  __device__ __forceinline__ u64 weight(float x) const {
+    const double y = (double(x) - double(top)) * rate;  // 0 for the largest logit, NaN where both are infinite
+    if (!(y > -kReach2)) return x == top ? u64(kOne) : 0;
+    const double n = __builtin_rint(y), f = y - n;
+    constexpr double l = 0.693147180559945309417;
+    constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7,
+                     c8 = c7 * l / 8, c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11;
+    double e = fma(c11, f, c10);
+    e = fma(e, f, c9);
+    e = fma(e, f, c8);
+    e = fma(e, f, c7);
+    e = fma(e, f, c6);
+    e = fma(e, f, c5);
+    e = fma(e, f, c4);
+    e = fma(e, f, c3);
+    e = fma(e, f, c2);
+    e = fma(e, f, l);
+    e = fma(e, f, 1.0);
+    // the sum with 2^52 holds the nearest whole number in its low bits
+    return u64(__double_as_longlong(ldexp(e, int(n) + 43) + 4503599627370496.0)) & ((u64(1) << 52) - 1);
   }
-  __device__ __forceinline__ u64 fixed(double w) const { return u64(w * kOne + 0.5); }
+  // keys that an interval's logits lie between (bin() is off by less than 2^-10 of an interval)
+  __device__ __forceinline__ void keys(int bin, uint32_t& lo, uint32_t& hi) const {
+    const float a = float(double(top) - (bin - 0.05) / double(per)), b = float(double(top) - (bin + 1.05) / double(per));
+    hi = bin == 0 || a != a ? key_of(top) : min(key_of(a) + 1, key_of(top));
+    lo = bin == BINS - 1 || b != b ? 0 : max(key_of(b), 1u) - 1;
+  }
 };
 
-// The first token at which the running count (COUNT) or weight passes `target`: its index, its weight and the weight
-// before it into s.out_*. The prefix sums stand in s; every thread is here, and a barrier ends it.
-template <bool COUNT, typename T, int NT, int R>
-__device__ void cross(const Row<T, NT, R>& row, const Scale& sc, u64 target, Lds<NT>& s) {
-  const int tid = threadIdx.x;
-  // the interval
-  if (tid == 0) s.n = 0;
-#pragma unroll
-  for (int i = 0; i < kBins / NT; ++i) {
-    const int b = tid + i * NT;
-    const u64 hi = COUNT ? u64(s.cnt[b]) : s.mass[b];
-    const u64 lo = b == 0 ? 0 : COUNT ? u64(s.cnt[b - 1]) : s.mass[b - 1];
-    if (lo <= target && target < hi) s.out_idx = b;
-  }
-  __syncthreads();
-  const int bin = int(s.out_idx);
-  u64 mass0 = bin == 0 ? 0 : s.mass[bin - 1];
-  u64 cnt0 = bin == 0 ? 0 : s.cnt[bin - 1];
-  const int n = int(s.cnt[bin] - cnt0);
-  if (n <= kList) {
-    row.each([&](float x, int i) {
-      if (sc.bin(x) != bin) return;
-      const int at = atomicAdd(&s.n, 1u);
-      s.lkey[at] = key_of(x);
-      s.lidx[at] = i;
-      s.lw[at] = sc.fixed(sc.weight(x));
-    });
-    __syncthreads();
-    for (int i = tid; i < n; i += NT) {
-      const uint32_t k = s.lkey[i], id = s.lidx[i];
-      u64 mass = mass0, cnt = cnt0;
-      for (int j = 0; j < n; ++j) {
-        const uint32_t kj = s.lkey[j];
-        if (kj > k || (kj == k && s.lidx[j] < id)) {
-          mass += s.lw[j];
-          ++cnt;
-        }
-      }
-      const u64 before = COUNT ? cnt : mass;
-      if (before <= target && target < before + (COUNT ? 1 : s.lw[i])) {
-        s.out_before = mass;
-        s.out_w = s.lw[i];
-        s.out_idx = id;
-      }
+// the smallest weight that min_p keeps: the exact product is a whole number or lies between two
+__device__ __forceinline__ u64 floor_of(float min_p) {
+  return u64(__builtin_ceil(double(fminf(fmaxf(min_p, 0.f), 1.f)) * kOne));
+}
+// u and p as targets of the running weight
+__device__ __forceinline__ u64 target_of_u(float u, u64 kept) {
+  return __umul64hi(u64(double(fminf(fmaxf(u, 0.f), 0x1.fffffep-1f)) * 18446744073709551616.0), kept);
+}
+__device__ __forceinline__ u64 target_of_p(float p, u64 kept) {  // passed by the first token that reaches p kept
+  const u64 f = u64(fmaxf(p, 0.f) * 18446744073709551616.0), want = __umul64hi(f, kept) + (f * kept != 0);
+  return want > 0 ? want - 1 : 0;
+}
+
+// Adds to a histogram in LDS, a wave whose lanes all add to one place (masked or equal logits) in one addition.
+__device__ __forceinline__ void add_to(u64* mass, uint32_t* cnt, int at, u64 w) {
+  if (__ballot(at == __builtin_amdgcn_readfirstlane(at)) == ~u64(0)) {
+    const u64 sum = wave_scan(w);
+    if ((threadIdx.x & 63) == 63) {
+      if (sum) atomicAdd(&mass[at], sum);
+      atomicAdd(&cnt[at], 64u);
     }
-    __syncthreads();
     return;
   }
-  // by digits of 8 bits of the key, the list's memory as their histogram (256 digits, the largest first)
-  uint32_t prefix = 0;
-  for (int shift = 24; shift >= 0; shift -= 8) {
+  if (w) atomicAdd(&mass[at], w);
+  atomicAdd(&cnt[at], 1u);
+}
+
+// What a workgroup keeps between its searches: which of the buffers come next (one is cleared while the last one may
+// still be read, so a search costs one barrier a step).
+struct Turn {
+  int digits = 0, bins = 0;
+};
+
+struct Found {
+  u64 before, w;  // the weight before the token, and its own
+  uint32_t idx;
+};
+__device__ __forceinline__ uint32_t lane_u32(uint32_t x, int lane) { return uint32_t(__builtin_amdgcn_readlane(int(x), lane)); }
+__device__ __forceinline__ u64 lane_u64(u64 x, int lane) {
+  return (u64(lane_u32(uint32_t(x >> 32), lane)) << 32) | lane_u32(uint32_t(x), lane);
+}
+
+// The first of the tokens that each(f) gives f(key, index, weight) of, at which the running count (COUNT) or weight,
+// `cnt0` and `mass0` before the first, passes `target`: by digits of 8 bits of the key, the largest first, until one token is
+// left, then of the index, the smallest first. There are `c` of them of the weight `m`; their keys lie between `klo` and
+// `khi` and differ from bit LOW on, indices are below `V`. Every thread is here; every wave has the result.
+template <bool COUNT, bool INDEX, int LOW, int NT, typename S, typename Each>
+__device__ __forceinline__ Found select(const Each& each, u64 target, u64 mass0, u64 cnt0, u64 m, uint32_t c, uint32_t klo,
+                                        uint32_t khi, int V, S& s, Turn& turn) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  auto above = [](int bit) { return bit >= 32 ? 0u : ~0u << bit; };
+  int kbits = klo == khi ? LOW : max(32 - __builtin_clz(klo ^ khi), LOW), ibits = V > 1 ? 32 - __builtin_clz(uint32_t(V - 1)) : 0;
+  const uint32_t last = (1u << ibits) - 1;  // the inverse of index 0
+  uint32_t kmask = above(kbits), kp = khi & kmask, ip = 0, imask = 0;
+  auto mine = [&](uint32_t key, uint32_t inv) { return ((key ^ kp) & kmask) == 0 && ((inv ^ ip) & imask) == 0; };
+  while (c > 1 && (kbits > LOW || (INDEX && ibits > 0))) {
+    const bool on_key = kbits > LOW;
+    const int shift = on_key ? max(kbits - 8, LOW) : max(ibits - 8, 0), width = (on_key ? kbits : ibits) - shift;
+    const uint32_t digits = (1u << width) - 1;
+    Digits& now = s.dig[turn.digits % 3];
+    Digits& next = s.dig[(turn.digits + 1) % 3];
+    ++turn.digits;
     for (int i = tid; i < 256; i += NT) {
-      s.lw[i] = 0;
-      s.lidx[i] = 0;
+      next.mass[i] = 0;
+      next.cnt[i] = 0;
     }
-    __syncthreads();
-    row.each([&](float x, int) {
-      const uint32_t k = key_of(x);
-      if (sc.bin(x) != bin || (shift < 24 && (k ^ prefix) >> (shift + 8))) return;
-      const int d = int((k >> shift) & 255u);
-      atomicAdd(&s.lw[d], sc.fixed(sc.weight(x)));
-      atomicAdd(&s.lidx[d], 1u);
+    each([&](uint32_t key, uint32_t idx, auto weight) {
+      const uint32_t inv = last - idx;
+      if (!mine(key, inv)) return;
+      add_to(now.mass, now.cnt, int(((on_key ? key : inv) >> shift) & digits), weight());
     });
     __syncthreads();
-    if (tid == 0) {
-      for (int d = 255; d >= 0; --d) {
-        const u64 m = s.lw[d], c = s.lidx[d];
-        if (target < (COUNT ? cnt0 + c : mass0 + m)) {
-          s.out_before = mass0;
-          s.out_w = cnt0;
-          s.out_idx = uint32_t(d);
-          break;
-        }
-        mass0 += m;
-        cnt0 += c;
-      }
+    // lane l has digits 255 - 4 l and the three below it
+    u64 dm[4], tm = 0;
+    uint32_t dc[4], tc = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      dm[k] = now.mass[255 - 4 * lane - k];
+      dc[k] = now.cnt[255 - 4 * lane - k];
+      tm += dm[k];
+      tc += dc[k];
     }
-    __syncthreads();
-    mass0 = s.out_before;
-    cnt0 = s.out_w;
-    prefix |= s.out_idx << shift;
-    __syncthreads();
+    u64 bm = mass0 + wave_scan(tm) - tm, bc = cnt0 + wave_scan(tc) - tc, hm = 0, hbm = 0, hbc = 0;
+    uint32_t hc = 0, digit = 0;
+    bool hit = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const u64 lo = COUNT ? bc : bm, hi = lo + (COUNT ? u64(dc[k]) : dm[k]);
+      if (lo <= target && target < hi) {
+        hit = true;
+        digit = uint32_t(255 - 4 * lane - k);
+        hm = dm[k]; hc = dc[k]; hbm = bm; hbc = bc;
+      }
+      bm += dm[k];
+      bc += dc[k];
+    }
+    const int src = __ffsll(static_cast<u64>(__ballot(hit))) - 1;
+    digit = lane_u32(digit, src);
+    m = lane_u64(hm, src);
+    c = lane_u32(hc, src);
+    mass0 = lane_u64(hbm, src);
+    cnt0 = lane_u64(hbc, src);
+    if (on_key) {
+      kbits = shift;
+      kp |= digit << shift;
+      kmask = above(kbits);
+    } else {
+      ibits = shift;
+      ip |= digit << shift;
+      imask = above(ibits) & last;
+    }
   }
-  // tokens of one logit: the one that many places on, in the order of their indices
-  const float x = __uint_as_float(prefix & 0x80000000u ? prefix ^ 0x80000000u : ~prefix);
-  const u64 w = sc.fixed(sc.weight(x));
-  const u64 place = COUNT ? target - cnt0 : (target - mass0) / w;
-  const int per = (row.V + NT - 1) / NT, i0 = min(tid * per, row.V), i1 = min(i0 + per, row.V);
-  uint32_t mine = 0;
-  for (int i = i0; i < i1; ++i) mine += key_of(Elem<T>::to_f(row.p[i])) == prefix;
-  u64 unused = 0;
-  uint32_t before = mine;
-  scan_block<NT>(unused, before, s);
-  if (before <= place && place < before + mine) {
-    uint32_t at = before;
-    for (int i = i0; i < i1; ++i) {
-      if (key_of(Elem<T>::to_f(row.p[i])) != prefix) continue;
-      if (at++ == place) {
-        s.out_before = mass0 + place * w;
-        s.out_w = w;
-        s.out_idx = uint32_t(i);
-        break;
-      }
-    }
+  if (!INDEX) {  // of equal logits each has the same weight
+    const u64 w = c == 1 ? m : m / c, place = c == 1 ? 0 : COUNT ? target - cnt0 : (target - mass0) / w;
+    return {mass0 + place * w, w, 0};
+  }
+  each([&](uint32_t key, uint32_t idx, auto) {
+    if (mine(key, last - idx)) s.idx = idx;
+  });
+  __syncthreads();
+  return {mass0, m, s.idx};
+}
+
+// the interval in which the running count or weight passes `target` (below their sum)
+template <bool COUNT, int NT, int BINS, typename S>
+__device__ __forceinline__ int find_bin(u64 target, S& s, Turn& turn) {
+  uint32_t& slot = s.bin[turn.bins++ & 1];
+#pragma unroll
+  for (int i = 0; i < BINS / NT; ++i) {
+    const int b = threadIdx.x + i * NT;
+    const u64 hi = COUNT ? u64(s.cnt[b]) : s.mass[b];
+    const u64 lo = b == 0 ? 0 : COUNT ? u64(s.cnt[b - 1]) : s.mass[b - 1];
+    if (lo <= target && target < hi) slot = b;
+  }
+  __syncthreads();
+  return int(slot);
+}
+
+// The first token of the row at which the running count (COUNT) or weight passes `target`, its index with INDEX. The
+// prefix sums stand in s; every thread is here.
+template <bool COUNT, bool INDEX, typename T, int NT, int R, int BINS, int LIST>
+__device__ Found cross(const Row<T, NT, R>& row, const Scale<BINS>& sc, u64 target, Lds<BINS, LIST>& s, Turn& turn) {
+  if (threadIdx.x == 0) s.n = 0;
+  const int bin = find_bin<COUNT, NT, BINS>(target, s, turn);
+  const u64 mass0 = bin == 0 ? 0 : s.mass[bin - 1];
+  const u64 cnt0 = bin == 0 ? 0 : s.cnt[bin - 1];
+  const int n = int(s.cnt[bin] - cnt0);
+  constexpr int LOW = sizeof(T) == 2 ? 16 : 0;
+  uint32_t klo, khi;
+  sc.keys(bin, klo, khi);
+  if (!INDEX && n == 1) return {mass0, s.mass[bin] - mass0, 0};  // the token is the interval
+  if (n > LIST) {
+    Row<T, NT, 0> whole;  // from memory each time: rare, and a step over registers is unrolled
+    whole.open(row.p, row.from, row.to);
+    auto each = [&](auto f) {
+      whole.each([&](float x, int i) {
+        if (sc.bin(x) == bin) f(key_of(x), uint32_t(i), [&] { return sc.weight(x); });
+      });
+    };
+    return select<COUNT, INDEX, LOW, NT>(each, target, mass0, cnt0, s.mass[bin] - mass0, n, klo, khi, row.to, s, turn);
+  }
+  row.each([&](float x, int i) {
+    if (sc.bin(x) != bin) return;
+    const int at = atomicAdd(&s.n, 1u);
+    s.lkey[at] = key_of(x);
+    s.lidx[at] = i;
+    s.lw[at] = sc.weight(x);
+  });
+  __syncthreads();
+  if (n == 1) return {mass0, s.lw[0], s.lidx[0]};
+  auto each = [&](auto f) {
+    for (int i = threadIdx.x; i < n; i += NT) f(s.lkey[i], s.lidx[i], [&] { return s.lw[i]; });
+  };
+  return select<COUNT, INDEX, LOW, NT>(each, target, mass0, cnt0, s.mass[bin] - mass0, n, klo, khi, row.to, s, turn);
+}
+
+// counts and weights of the intervals to their prefix sums, in place; a barrier ends it
+template <int NT, int BINS, typename S>
+__device__ __forceinline__ void scan_bins(S& s) {
+  constexpr int N = BINS / NT;
+  const int tid = threadIdx.x;
+  u64 m[N], tm = 0;
+  uint32_t c[N], tc = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    tm += s.mass[tid * N + i];
+    tc += s.cnt[tid * N + i];
+    m[i] = tm;
+    c[i] = tc;
+  }
+  scan_block<NT>(tm, tc, s);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s.mass[tid * N + i] = m[i] + tm;
+    s.cnt[tid * N + i] = c[i] + tc;
   }
   __syncthreads();
 }
 
-template <typename T, int NT, int R>
-__global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
-  __shared__ Lds<NT> s;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
-  if (p.run && *p.run == 0) return;
-  Row<T, NT, R> row;
-  row.open(reinterpret_cast<const T*>(p.logits) + b * p.l_sr, p.V);
-  const float temperature = p.temperature_dev ? p.temperature_dev[b] : p.temperature;
-  const float top_p = p.top_p_dev ? p.top_p_dev[b] : p.top_p;
-  const float min_p = p.min_p_dev ? p.min_p_dev[b] : p.min_p;
-  const int64_t top_k = p.top_k_dev ? p.top_k_dev[b] : p.top_k;
-  const float u = p.u[b];
-
-  // the largest logit, the first token that has it, the smallest finite one
-  float top = kNegInf, low = __builtin_inff();
-  int first = p.V;
-  bool nan = false;
-  row.each([&](float x, int i) {
-    nan = nan || x != x;
-    if (x > top || (x == top && i < first)) {
-      top = x;
-      first = i;
-    }
-    if (x > kNegInf) low = fminf(low, x);
-  });
-  auto best = [&](float t, int f) {
-    if (t > top || (t == top && f < first)) {
-      top = t;
-      first = f;
-    }
-  };
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const float t = __shfl_xor(top, d);
-    const int f = __shfl_xor(first, d);
-    best(t, f);
-    low = fminf(low, __shfl_xor(low, d));
+// the searches of a row whose intervals are summed and whose weight above min_p is `high`
+template <typename T, int NT, int R, int BINS, int LIST>
+__device__ __forceinline__ void draw(const Row<T, NT, R>& row, const Scale<BINS>& sc, const Setting& o, u64 high,
+                                     Lds<BINS, LIST>& s, int64_t* token) {
+  Turn turn;
+  for (int i = threadIdx.x; i < 256; i += NT) {
+    s.dig[0].mass[i] = 0;
+    s.dig[0].cnt[i] = 0;
   }
-  if (tid == 0) s.nan = 0;
-  __syncthreads();
-  if (__ballot(nan) && lane == 0) s.nan = 1;
+  u64 kept = s.mass[BINS - 1];
+  if (o.top_k > 0 && o.top_k < row.to) {
+    const Found f = cross<true, false>(row, sc, u64(o.top_k - 1), s, turn);
+    kept = f.before + f.w;
+  }
+  if (o.top_p < 1.f) {
+    const Found f = cross<false, false>(row, sc, target_of_p(o.top_p, kept), s, turn);
+    kept = f.before + f.w;
+  }
+  kept = min(kept, high);
+  const Found f = cross<false, true>(row, sc, target_of_u(o.u, kept), s, turn);
+  if (threadIdx.x == 0) *token = f.idx;
+}
+
+// the largest logit, the smallest finite one and whether there is a NaN, over the workgroup
+template <int NT, typename S, typename Rows>
+__device__ __forceinline__ void extremes(const Rows& row, float& top, float& low, bool& nan, S& s) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  top = kNegInf;
+  low = __builtin_inff();
+  nan = false;
+  row.each([&](float x, int) {
+    nan = nan || x != x;
+    top = fmaxf(top, x);
+    low = x > kNegInf ? fminf(low, x) : low;
+  });
+  top = wave_max(top);
+  low = -wave_max(-low);
+  nan = __ballot(nan) != 0;
   if (lane == 0) {
     s.redf[wave] = top;
-    s.redi[wave] = first;
     s.redm[wave] = low;
-  }
-#pragma unroll
-  for (int i = 0; i < kBins / NT; ++i) {
-    s.mass[tid + i * NT] = 0;
-    s.cnt[tid + i * NT] = 0;
+    s.red32[wave] = nan;
   }
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) {
-    best(s.redf[w], s.redi[w]);
+    top = fmaxf(top, s.redf[w]);
     low = fminf(low, s.redm[w]);
+    nan = nan || s.red32[w];
   }
-  const bool bad = s.nan || top == kNegInf || u != u || temperature != temperature || top_p != top_p || min_p != min_p;
-  if (bad || !(temperature > 0.f)) {  // nothing to draw from, or the first of the order
-    if (tid == 0) p.tokens[b] = bad ? -1 : first;
+}
+
+// ---- a workgroup a row -------------------------------------------------------------------------------------
+template <typename T, int NT, int R, int BINS>
+__global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
+  constexpr int LIST = BINS < kList ? BINS : kList;
+  __shared__ Lds<BINS, LIST> s;
+  const int tid = threadIdx.x, b = blockIdx.x;
+  const Setting o(p, b);
+  Row<T, NT, R> row;
+  row.open(reinterpret_cast<const T*>(p.logits) + b * p.l_sr, 0, p.V);
+  if (p.run && *p.run == 0) return;
+#pragma unroll
+  for (int i = 0; i < BINS / NT; ++i) {
+    s.mass[tid + i * NT] = 0;
+    s.cnt[tid + i * NT] = 0;
+  }
+  if (tid == 0) {
+    s.high = 0;
+    s.first = p.V;
+  }
+  float top, low;
+  bool nan;
+  extremes<NT>(row, top, low, nan, s);
+  if (nan || top == kNegInf || o.nan()) {
+    if (tid == 0) p.tokens[b] = -1;
     return;
   }
-
-  Scale sc;
-  sc.top = top;
-  sc.inv_t = 1.0 / double(temperature);
-  const float span = fminf(kReach * temperature, top - low);  // at most as far as weights reach
-  sc.per = span > 0.f ? float(kBins) / span : 0.f;
-  if (!(sc.per < __builtin_inff())) sc.per = 3e38f;  // a span below the normal numbers
-  const double floor_p = fminf(min_p, 1.f);
+  if (o.greedy()) {
+    row.each([&](float x, int i) {
+      if (x == top) atomicMin(&s.first, uint32_t(i));
+    });
+    __syncthreads();
+    if (tid == 0) p.tokens[b] = s.first;
+    return;
+  }
+  const Scale<BINS> sc(o, top, low);
+  const bool cut = o.min_p > 0.f;
+  const u64 least = floor_of(o.min_p);
   u64 high = 0;
   row.each([&](float x, int) {
-    const double w = sc.weight(x);
-    const u64 f = sc.fixed(w);
-    const int bin = sc.bin(x);
-    if (f) atomicAdd(&s.mass[bin], f);
-    atomicAdd(&s.cnt[bin], 1u);
-    if (w >= floor_p) high += f;
+    const u64 w = sc.weight(x);
+    add_to(s.mass, s.cnt, sc.bin(x), w);
+    if (w >= least) high += w;
   });
+  if (cut) {
+    high = wave_scan(high);
+    if ((tid & 63) == 63) atomicAdd(&s.high, high);
+  }
   __syncthreads();
-  {  // prefix sums, in place
-    constexpr int N = kBins / NT;
-    u64 m[N], tm = 0;
-    uint32_t c[N], tc = 0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      tm += s.mass[tid * N + i];
-      tc += s.cnt[tid * N + i];
-      m[i] = tm;
-      c[i] = tc;
-    }
-    scan_block<NT>(tm, tc, s);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      s.mass[tid * N + i] = m[i] + tm;
-      s.cnt[tid * N + i] = c[i] + tc;
-    }
-    u64 all = high;
-    uint32_t unused = 0;
-    scan_block<NT>(all, unused, s);
-    if (tid == NT - 1) s.lw[0] = all + high;
+  scan_bins<NT, BINS>(s);
+  draw(row, sc, o, cut ? s.high : s.mass[BINS - 1], s, p.tokens + b);
+}
+
+// ---- a row in pieces ---------------------------------------------------------------------------------------
+constexpr int kPieceThreads = 512;
+constexpr int kRowList = 2048;  // tokens of the intervals that a row's searches can end in
+struct RowWs {                  // in the workspace, written and read at agent scope or launches apart
+  u64 mass[kBins];
+  u64 high;
+  float top[kMaxPieces], low[kMaxPieces];
+  uint32_t nan[kMaxPieces], first[kMaxPieces];
+  uint32_t cnt[kBins];
+  uint32_t done, n;
+  uint32_t key[kRowList], idx[kRowList];
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kPieceThreads) sample_top_kernel(const SampleParams p) {
+  constexpr int NT = kPieceThreads;
+  __shared__ struct {
+    float redf[16], redm[16];
+    uint32_t red32[16], first;
+  } s;
+  const int tid = threadIdx.x, b = blockIdx.x / p.pieces, g = blockIdx.x % p.pieces;
+  RowWs& w = reinterpret_cast<RowWs*>(p.ws)[b];
+  Row<T, NT, 0> row;
+  row.open(reinterpret_cast<const T*>(p.logits) + b * p.l_sr, g * p.piece, min(p.V, (g + 1) * p.piece));
+  if (p.run && *p.run == 0) return;
+  for (int i = g * NT + tid; i < kBins; i += p.pieces * NT) {
+    w.mass[i] = 0;
+    w.cnt[i] = 0;
+  }
+  if (tid == 0) s.first = p.V;
+  float top, low;
+  bool nan;
+  extremes<NT>(row, top, low, nan, s);
+  const Setting o(p, b);
+  if (o.greedy()) {
+    row.each([&](float x, int i) {
+      if (x == top) atomicMin(&s.first, uint32_t(i));
+    });
     __syncthreads();
-    high = s.lw[0];
+  }
+  if (tid == 0) {
+    w.top[g] = top;
+    w.low[g] = low;
+    w.nan[g] = nan;
+    w.first[g] = s.first;
+    if (g == 0) {
+      w.high = 0;
+      w.done = 0;
+      w.n = 0;
+    }
+  }
+}
+
+// a row's extremes from its pieces' (every lane of every wave), and the token where there is nothing to search
+struct Whole {
+  float top, low;
+  bool over;
+  int64_t token;
+};
+__device__ __forceinline__ Whole whole_row(const RowWs& w, const SampleParams& p, const Setting& o) {
+  const int lane = threadIdx.x & 63;
+  const bool in = lane < p.pieces;
+  Whole r;
+  const float mine = in ? w.top[lane] : kNegInf;
+  r.top = wave_max(mine);
+  r.low = -wave_max(in ? -w.low[lane] : kNegInf);
+  const bool nan = __ballot(in && w.nan[lane]) != 0 || r.top == kNegInf || o.nan();
+  r.over = nan || o.greedy();
+  r.token = -1;
+  if (!nan && o.greedy()) {
+    const uint64_t has = __ballot(in && mine == r.top);
+    r.token = w.first[__ffsll(static_cast<unsigned long long>(has)) - 1];
+  }
+  return r;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(const SampleParams p) {
+  constexpr int NT = kPieceThreads;
+  __shared__ u64 mass[kBins];
+  __shared__ uint32_t cnt[kBins];
+  const int tid = threadIdx.x, b = blockIdx.x / p.pieces, g = blockIdx.x % p.pieces;
+  if (p.run && *p.run == 0) return;
+  RowWs& w = reinterpret_cast<RowWs*>(p.ws)[b];
+  const Setting o(p, b);
+  const Whole all = whole_row(w, p, o);
+  if (all.over) {
+    if (g == 0 && tid == 0) p.tokens[b] = all.token;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kBins / NT; ++i) {
+    mass[tid + i * NT] = 0;
+    cnt[tid + i * NT] = 0;
+  }
+  __syncthreads();
+  Row<T, NT, 0> row;
+  row.open(reinterpret_cast<const T*>(p.logits) + b * p.l_sr, g * p.piece, min(p.V, (g + 1) * p.piece));
+  const Scale<kBins> sc(o, all.top, all.low);
+  const u64 least = floor_of(o.min_p);
+  u64 high = 0;
+  row.each([&](float x, int) {
+    const u64 wt = sc.weight(x);
+    add_to(mass, cnt, sc.bin(x), wt);
+    if (wt >= least) high += wt;
+  });
+  if (o.min_p > 0.f) {
+    high = wave_scan(high);
+    if ((tid & 63) == 63 && high) __hip_atomic_fetch_add(&w.high, high, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kBins / NT; ++i) {
+    const int k = tid + i * NT;
+    if (cnt[k]) __hip_atomic_fetch_add(&w.cnt[k], cnt[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (mass[k]) __hip_atomic_fetch_add(&w.mass[k], mass[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+}
+
+// Every piece finds the intervals that a search can end in (the weight that top-k and top-p leave is only known to
+// within an interval) and appends its tokens of those to the row's list; the row's last piece has all of them.
+template <typename T>
+__global__ void __launch_bounds__(kPieceThreads) sample_pick_kernel(const SampleParams p) {
+  constexpr int NT = kPieceThreads;
+  __shared__ Lds<kBins, kRowList> s;
+  __shared__ int lbin[kRowList];
+  const int tid = threadIdx.x, b = blockIdx.x / p.pieces, g = blockIdx.x % p.pieces;
+  if (p.run && *p.run == 0) return;
+  RowWs& w = reinterpret_cast<RowWs*>(p.ws)[b];
+  const Setting o(p, b);
+  const Whole all = whole_row(w, p, o);
+  if (all.over) return;
+#pragma unroll
+  for (int i = 0; i < kBins / NT; ++i) {
+    s.mass[tid + i * NT] = w.mass[tid + i * NT];
+    s.cnt[tid + i * NT] = w.cnt[tid + i * NT];
+  }
+  if (tid == 0) s.n = 0;
+  const u64 high = o.min_p > 0.f ? w.high : ~u64(0);
+  __syncthreads();
+  scan_bins<NT, kBins>(s);
+  const Scale<kBins> sc(o, all.top, all.low);
+  const bool by_k = o.top_k > 0 && o.top_k < p.V, by_p = o.top_p < 1.f;
+  auto before = [&](int bin) { return bin == 0 ? u64(0) : s.mass[bin - 1]; };
+  auto count = [&](int lo, int hi) { return s.cnt[hi] - (lo == 0 ? 0u : s.cnt[lo - 1]); };
+  Turn turn;
+  auto find = [&](u64 target) { return find_bin<false, NT, kBins>(target, s, turn); };
+  // the weight kept lies in [lo, hi]
+  u64 lo = s.mass[kBins - 1], hi = lo;
+  int kb = -1, p0 = -1, p1 = -2;
+  if (by_k) {
+    kb = find_bin<true, NT, kBins>(u64(o.top_k - 1), s, turn);
+    lo = before(kb);
+    hi = s.mass[kb];
+  }
+  if (by_p) {
+    p0 = find(target_of_p(o.top_p, lo));
+    p1 = find(target_of_p(o.top_p, hi));
+    lo = before(p0);
+    hi = s.mass[p1];
+  }
+  lo = min(lo, high);
+  hi = min(hi, high);
+  const int u0 = find(target_of_u(o.u, lo)), u1 = find(target_of_u(o.u, hi));
+  const u64 total = u64(kb >= 0 ? count(kb, kb) : 0) + (by_p ? count(p0, p1) : 0) + count(u0, u1);
+  auto in = [&](int bin) { return bin == kb || (bin >= p0 && bin <= p1) || (bin >= u0 && bin <= u1); };
+  const T* logits = reinterpret_cast<const T*>(p.logits) + b * p.l_sr;
+  const bool fits = total <= kRowList;  // the same for every piece of the row
+  if (fits) {
+    Row<T, NT, 0> row;
+    row.open(logits, g * p.piece, min(p.V, (g + 1) * p.piece));
+    row.each([&](float x, int i) {
+      if (!in(sc.bin(x))) return;
+      const int at = atomicAdd(&s.n, 1u);
+      s.lkey[at] = key_of(x);
+      s.lidx[at] = i;
+    });
     __syncthreads();
+    const uint32_t n = s.n;
+    if (tid == 0 && n) s.first = __hip_atomic_fetch_add(&w.n, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    for (uint32_t i = tid; i < n; i += NT) {
+      __hip_atomic_store(&w.key[s.first + i], s.lkey[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(&w.idx[s.first + i], s.lidx[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  // publish, then count: agent-scope stores are acknowledged at the device-coherent level before the barrier, the
+  // count's add is issued after it, and the workgroup that sees the last count reads with agent-scope loads
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (tid == 0) s.last = __hip_atomic_fetch_add(&w.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == uint32_t(p.pieces - 1);
+  __syncthreads();
+  if (!s.last) return;
+
+  if (!fits) {
+    // one of the intervals holds too many: the searches over the whole row, by the digits of the keys there
+    Row<T, NT, 0> row;
+    row.open(logits, 0, p.V);
+    draw(row, sc, o, high, s, p.tokens + b);
+    return;
+  }
+  const int n = int(__hip_atomic_load(&w.n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  for (int i = tid; i < n; i += NT) {
+    const uint32_t k = __hip_atomic_load(&w.key[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const float x = of_key(k);
+    s.lkey[i] = k;
+    s.lidx[i] = __hip_atomic_load(&w.idx[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s.lw[i] = sc.weight(x);
+    lbin[i] = sc.bin(x);
+  }
+  __syncthreads();
+  for (int i = tid; i < 256; i += NT) {
+    s.dig[0].mass[i] = 0;
+    s.dig[0].cnt[i] = 0;
   }
   u64 kept = s.mass[kBins - 1];
-  if (top_k > 0 && top_k < p.V) {
-    cross<true>(row, sc, u64(top_k - 1), s);
-    kept = s.out_before + s.out_w;
-    __syncthreads();
+  auto search = [&](auto by_count, auto index, u64 target) {
+    constexpr bool COUNT = decltype(by_count)::value;
+    const int bin = find_bin<COUNT, NT, kBins>(target, s, turn);
+    auto each = [&](auto f) {
+      for (int i = tid; i < n; i += NT)
+        if (lbin[i] == bin) f(s.lkey[i], s.lidx[i], [&] { return s.lw[i]; });
+    };
+    uint32_t klo, khi;
+    sc.keys(bin, klo, khi);
+    return select<COUNT, decltype(index)::value, sizeof(T) == 2 ? 16 : 0, NT>(
+        each, target, before(bin), bin == 0 ? 0 : s.cnt[bin - 1], s.mass[bin] - before(bin), count(bin, bin), klo, khi, p.V, s, turn);
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (by_k) {
+    const Found f = search(Yes{}, No{}, u64(o.top_k - 1));
+    kept = f.before + f.w;
   }
-  if (top_p < 1.f) {
-    // the first token at which the running weight reaches p kept, a whole number at or above it
-    const u64 pf = u64(fmaxf(top_p, 0.f) * 18446744073709551616.0);  // exact: p in units of 2^-64
-    const u64 want = __umul64hi(pf, kept) + (pf * kept != 0);
-    cross<false>(row, sc, want > 0 ? want - 1 : 0, s);
-    kept = s.out_before + s.out_w;
-    __syncthreads();
+  if (by_p) {
+    const Found f = search(No{}, No{}, target_of_p(o.top_p, kept));
+    kept = f.before + f.w;
   }
   kept = min(kept, high);
-  const float uc = fminf(fmaxf(u, 0.f), 0x1.fffffep-1f);
-  cross<false>(row, sc, __umul64hi(u64(double(uc) * 18446744073709551616.0), kept), s);
-  if (tid == 0) p.tokens[b] = s.out_idx;
+  const Found f = search(No{}, Yes{}, target_of_u(o.u, kept));
+  if (tid == 0) p.tokens[b] = f.idx;
+}
+
+constexpr int kWholeRow = 32768;  // longer rows go in pieces
+
+// Pieces of a row: two workgroups a CU over the batch, of at least 4096 logits.
+static int pieces_of(int B, int V) {
+  if (V <= kWholeRow) return 1;
+  int64_t n = 2 * int64_t(device_cu_count()) / B;
+  n = std::min<int64_t>(n, V / 4096);
+  return int(std::max<int64_t>(2, std::min<int64_t>(n, kMaxPieces)));
+}
+
+size_t sample_workspace_bytes(const mote_sample_args* a) {
+  return a->B > 0 && a->V > kWholeRow ? size_t(a->B) * sizeof(RowWs) : 0;
 }
 
 int launch_sample(const mote_sample_args* a, hipStream_t stream) {
@@ -393,19 +795,37 @@ int launch_sample(const mote_sample_args* a, hipStream_t stream) {
     return set_error(MOTE_ERR_SHAPE, "%s: %d rows of %d logits (1 to 2^20 a row)", what, a->B, a->V);
   if (a->B == 0) return MOTE_OK;
   if (!a->logits || !a->u || !a->tokens) return set_error(MOTE_ERR_ARGUMENT, "%s: null pointer", what);
-  if (!grid_fits(a->B, 1024)) return set_error(MOTE_ERR_SHAPE, "%s: %d rows are too many for one launch", what, a->B);
-  SampleParams p;
+  SampleParams p{};
   p.logits = a->logits; p.l_sr = a->l_sr; p.u = a->u;
   p.temperature = a->temperature; p.top_p = a->top_p; p.min_p = a->min_p; p.top_k = a->top_k;
   p.temperature_dev = a->temperature_dev; p.top_p_dev = a->top_p_dev; p.min_p_dev = a->min_p_dev; p.top_k_dev = a->top_k_dev;
   p.tokens = a->tokens; p.run = a->run; p.V = a->V;
-#define MOTE_SAMPLE(NT_, R_) hipLaunchKernelGGL((sample_kernel<T, NT_, R_>), dim3(a->B), dim3(NT_), 0, stream, p)
-#define MOTE_SAMPLE_V                            \
-  if (a->V <= 512) MOTE_SAMPLE(512, 1);          \
-  else if (a->V <= 1024) MOTE_SAMPLE(1024, 1);   \
-  else if (a->V <= 8192) MOTE_SAMPLE(1024, 8);   \
-  else if (a->V <= 32768) MOTE_SAMPLE(1024, 32); \
-  else MOTE_SAMPLE(1024, 0);
+  p.pieces = pieces_of(a->B, a->V);
+  if (!grid_fits(int64_t(a->B) * p.pieces, 1024)) return set_error(MOTE_ERR_SHAPE, "%s: %d rows are too many for one launch", what, a->B);
+  if (p.pieces > 1) {
+    const size_t need = sample_workspace_bytes(a);
+    if (!a->workspace || a->workspace_bytes < need || reinterpret_cast<uintptr_t>(a->workspace) % 16)
+      return set_error(MOTE_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes, %zu needed", what, a->workspace_bytes, need);
+    p.ws = reinterpret_cast<char*>(a->workspace);
+    p.piece = ((a->V + p.pieces - 1) / p.pieces + 7) / 8 * 8;
+    p.pieces = (a->V + p.piece - 1) / p.piece;
+    const dim3 grid(unsigned(a->B) * p.pieces), block(kPieceThreads);
+    auto launch = [&](auto t) {
+      using T = decltype(t);
+      hipLaunchKernelGGL((sample_top_kernel<T>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((sample_hist_kernel<T>), grid, block, 0, stream, p);
+      hipLaunchKernelGGL((sample_pick_kernel<T>), grid, block, 0, stream, p);
+    };
+    if (a->dtype == MOTE_BF16) launch(bf16_t{});
+    else launch(0.f);
+    return check_launch(what);
+  }
+#define MOTE_SAMPLE(NT_, R_, BINS_) hipLaunchKernelGGL((sample_kernel<T, NT_, R_, BINS_>), dim3(a->B), dim3(NT_), 0, stream, p)
+#define MOTE_SAMPLE_V                                   \
+  if (a->V <= 512) MOTE_SAMPLE(256, 2, 512);            \
+  else if (a->V <= 1024) MOTE_SAMPLE(512, 2, 1024);     \
+  else if (a->V <= 8192) MOTE_SAMPLE(1024, 8, 2048);    \
+  else MOTE_SAMPLE(1024, 32, 2048);
   if (a->dtype == MOTE_BF16) {
     using T = bf16_t;
     MOTE_SAMPLE_V

@@ -1155,6 +1155,12 @@ Tensor sample_tokens(const Tensor& x_, const Tensor& u, const py::object& temper
   a.u = fptr(u);
   a.tokens = static_cast<int64_t*>(tokens.data_ptr());
   a.run = run ? static_cast<const unsigned char*>(run->data_ptr()) : nullptr;
+  Tensor ws;
+  if (const size_t n = mote_sample_workspace(&a)) {
+    ws = bytes(n, x);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = n;
+  }
   check(mote_sample(&a, on.stream), "mote_sample");
   return tokens;
 }
