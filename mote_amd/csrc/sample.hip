@@ -8,12 +8,13 @@
 // and atomics may make them, and a border differs from the real one by V 2^-44 of the largest weight at most.
 //
 // A row: its maximum; a histogram over intervals of the logit (an interval's count and weight); its prefix sums, in
-// which a search finds an interval; then the digits of the keys, and for equal logits of the indices, of that
-// interval's tokens, which are gathered in LDS unless they are too many (many equal logits).
+// which a search finds an interval; then that interval's tokens, which are gathered in LDS unless they are too many
+// (many equal logits): up to 64 each count the ones before them, more are told apart by the digits of their keys, and
+// equal ones by those of their indices.
 //
-// Up to 32768 logits a workgroup has a row, in registers. Longer rows go in pieces over three launches (maximum;
-// histogram; the tokens of the intervals that a search can end in, and by the last piece of a row the searches),
-// since one CU alone reads a row of 131072 logits in 5 us and makes its exponentials in 30.
+// Up to 8192 logits a workgroup has a row, in registers. Longer rows go in pieces over three launches: the maximum; the
+// histogram, and by a row's last piece its prefix sums and the intervals that a search can end in; the tokens of
+// those, and by the row's last piece the searches.
 #include <algorithm>
 #include <type_traits>
 
@@ -48,7 +49,7 @@ constexpr int kBins = 2048;                      // intervals of a long row
 constexpr int kList = 1024;                      // tokens of an interval that are searched in LDS
 constexpr double kOne = 8796093022208.0;         // 2^43: the largest weight
 constexpr float kReach = 31.0f;                  // exp(-31) < 2^-44: no weight from there on
-constexpr double kReach2 = 45.0;                 // 2^-45: nor from there
+constexpr double kReach2 = 46.0;                 // nor at 2^-46
 constexpr int kMaxPieces = 64;
 
 // order of logits: a larger key comes first (the sum with +0 makes one zero of two)
@@ -66,14 +67,16 @@ template <int BINS, int LIST>
 struct Lds {
   u64 mass[BINS];  // prefix sums once scanned
   uint32_t cnt[BINS];
-  u64 lw[LIST];  // the tokens of an interval
+  u64 lw[LIST];  // the tokens of the intervals that a search can end in
   uint32_t lkey[LIST], lidx[LIST];
+  int lbin[LIST];
+  uint16_t slot[16][64];
   Digits dig[3];
   u64 red64[16];
   uint32_t red32[16];
   float redf[16], redm[16];
   u64 high;
-  uint32_t bin[2], idx, n, first;
+  uint32_t idx, n, first;
   int last;
 };
 
@@ -138,30 +141,38 @@ struct Row {
       }
     }
   }
-  template <typename F>
-  __device__ __forceinline__ void each(F f) const {
+  // many(v, i) for PER logits from i on, one(v, i) for single ones
+  static constexpr int PER = 16 / int(sizeof(T));
+  template <typename Many, typename One>
+  __device__ __forceinline__ void each(Many many, One one) const {
     if constexpr (R > 0) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         const int i = from + int(threadIdx.x) + r * NT;
-        if (i < to) f(x[r], i);
+        if (i < to) one(x[r], i);
       }
     } else {
-      constexpr int PER = 16 / int(sizeof(T));
       const int whole = (to - from) / PER;
       for (int c = threadIdx.x; c < whole; c += NT) {
         const int i0 = from + c * PER;
         const Chunk q = load_any(p + i0);
+        float v[PER];
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
-          float v;
-          if constexpr (sizeof(T) == 2) v = __uint_as_float(k % 2 ? q.w[k / 2] & 0xffff0000u : q.w[k / 2] << 16);
-          else v = __uint_as_float(q.w[k]);
-          f(v, i0 + k);
+          if constexpr (sizeof(T) == 2) v[k] = __uint_as_float(k % 2 ? q.w[k / 2] & 0xffff0000u : q.w[k / 2] << 16);
+          else v[k] = __uint_as_float(q.w[k]);
         }
+        many(v, i0);
       }
-      for (int i = from + whole * PER + int(threadIdx.x); i < to; i += NT) f(Elem<T>::to_f(p[i]), i);
+      for (int i = from + whole * PER + int(threadIdx.x); i < to; i += NT) one(Elem<T>::to_f(p[i]), i);
     }
+  }
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    each([&](const float (&v)[PER], int i) {
+#pragma unroll
+      for (int k = 0; k < PER; ++k) f(v[k], i + k);
+    }, f);
   }
 };
 
@@ -196,11 +207,11 @@ struct Scale {
     return t < float(BINS - 1) ? int(t) : BINS - 1;
   }
   // The weight in units of 2^-43, from 2^f on |f| <= 1/2 by its power series up to f^11 (what follows is below 2^-47 of
-  // it) in fp64: seventeen instructions, a library exponential to the last place takes three times as many (64 rows of
-  // 131072 logits: 64 -> 37 us over all).
+  // it) in fp64, without a branch: seventeen instructions, where an exponential to the last place takes three times as
+  // many.
   __device__ __forceinline__ u64 weight(float x) const {
-    const double y = (double(x) - double(top)) * rate;  // 0 for the largest logit, NaN where both are infinite
-    if (!(y > -kReach2)) return x == top ? u64(kOne) : 0;
+    // 0 for the largest logit; NaN where it is infinite goes as far down as any
+    const double y = fmax((double(x) - double(top)) * rate, -kReach2);
     const double n = __builtin_rint(y), f = y - n;
     constexpr double l = 0.693147180559945309417;
     constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7,
@@ -217,7 +228,8 @@ struct Scale {
     e = fma(e, f, l);
     e = fma(e, f, 1.0);
     // the sum with 2^52 holds the nearest whole number in its low bits
-    return u64(__double_as_longlong(ldexp(e, int(n) + 43) + 4503599627370496.0)) & ((u64(1) << 52) - 1);
+    const u64 w = u64(__double_as_longlong(ldexp(e, int(n) + 43) + 4503599627370496.0)) & ((u64(1) << 52) - 1);
+    return x == top ? u64(kOne) : w;
   }
   // keys that an interval's logits lie between (bin() is off by less than 2^-10 of an interval)
   __device__ __forceinline__ void keys(int bin, uint32_t& lo, uint32_t& hi) const {
@@ -231,33 +243,96 @@ struct Scale {
 __device__ __forceinline__ u64 floor_of(float min_p) {
   return u64(__builtin_ceil(double(fminf(fmaxf(min_p, 0.f), 1.f)) * kOne));
 }
-// u and p as targets of the running weight
-__device__ __forceinline__ u64 target_of_u(float u, u64 kept) {
-  return __umul64hi(u64(double(fminf(fmaxf(u, 0.f), 0x1.fffffep-1f)) * 18446744073709551616.0), kept);
-}
-__device__ __forceinline__ u64 target_of_p(float p, u64 kept) {  // passed by the first token that reaches p kept
-  const u64 f = u64(fmaxf(p, 0.f) * 18446744073709551616.0), want = __umul64hi(f, kept) + (f * kept != 0);
-  return want > 0 ? want - 1 : 0;
-}
+// What a row's three searches are for: the last token that top-k keeps (of the running count), the last that top-p keeps,
+// the draw. They are stages of one loop, and its body is small: a row comes through it once, and instructions that no
+// wave has run before cost more than their execution (unrolled and specialised for each stage the searches of 77 tokens
+// took 8 us).
+struct Goals {
+  u64 fp, fu;  // top_p and u in units of 2^-64
+  int64_t last;
+  bool by_k, by_p;
+  __device__ __forceinline__ Goals(const Setting& o, int V)
+      : fp(u64(fmaxf(o.top_p, 0.f) * 18446744073709551616.0)),
+        fu(u64(double(fminf(fmaxf(o.u, 0.f), 0x1.fffffep-1f)) * 18446744073709551616.0)), last(o.top_k - 1),
+        by_k(o.top_k > 0 && o.top_k < V), by_p(o.top_p < 1.f) {}
+  __device__ __forceinline__ bool has(int stage) const { return stage == 0 ? by_k : stage == 1 ? by_p : true; }
+  // passed by the token that the stage is for, when the weight `kept` is left before it
+  __device__ __forceinline__ u64 target(int stage, u64 kept) const {
+    if (stage == 0) return u64(last);
+    const u64 f = stage == 1 ? fp : fu, up = __umul64hi(f, kept);
+    if (stage == 2) return up;
+    const u64 want = up + (f * kept != 0);  // top-p: the first token that reaches p kept
+    return want > 0 ? want - 1 : 0;
+  }
+};
 
-// Adds to a histogram in LDS, a wave whose lanes all add to one place (masked or equal logits) in one addition.
-__device__ __forceinline__ void add_to(u64* mass, uint32_t* cnt, int at, u64 w) {
+// A row's (or a piece's) histogram in LDS. Where every logit that a wave holds is in the first or the last interval (equal
+// or masked ones) it adds them at once: 64 additions to one place take their turns.
+template <int BINS, typename Rows, typename S>
+__device__ __forceinline__ u64 histogram(const Rows& row, const Scale<BINS>& sc, float min_p, S& s) {
+  constexpr int PER = Rows::PER;
+  const bool cut = min_p > 0.f;
+  const u64 least = floor_of(min_p);
+  u64 high = 0;  // the weight that min_p keeps
+  auto above = [&](u64 w) {
+    if (cut) high += w >= least ? w : 0;
+  };
+  row.each(
+      [&](const float (&v)[PER], int) {
+        u64 w[PER];
+        int bin[PER], any = 0, all = BINS - 1;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          w[k] = sc.weight(v[k]);
+          bin[k] = sc.bin(v[k]);
+          any |= bin[k];
+          all &= bin[k];
+          above(w[k]);
+        }
+        if (__ballot(any == 0) == ~u64(0) || __ballot(all == BINS - 1) == ~u64(0)) {
+          u64 sum = w[0];
+#pragma unroll
+          for (int k = 1; k < PER; ++k) sum += w[k];
+          sum = wave_scan(sum);
+          if ((threadIdx.x & 63) == 63) {
+            atomicAdd(&s.mass[bin[0]], sum);
+            atomicAdd(&s.cnt[bin[0]], uint32_t(64 * PER));
+          }
+          return;
+        }
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          atomicAdd(&s.mass[bin[k]], w[k]);
+          atomicAdd(&s.cnt[bin[k]], 1u);
+        }
+      },
+      [&](float x, int) {
+        const u64 w = sc.weight(x);
+        const int bin = sc.bin(x);
+        atomicAdd(&s.mass[bin], w);
+        atomicAdd(&s.cnt[bin], 1u);
+        above(w);
+      });
+  return high;
+}
+// An addition to a histogram of digits; a wave whose lanes all have one digit makes one.
+__device__ __forceinline__ void add_to(Digits& d, int at, u64 w) {
   if (__ballot(at == __builtin_amdgcn_readfirstlane(at)) == ~u64(0)) {
     const u64 sum = wave_scan(w);
     if ((threadIdx.x & 63) == 63) {
-      if (sum) atomicAdd(&mass[at], sum);
-      atomicAdd(&cnt[at], 64u);
+      atomicAdd(&d.mass[at], sum);
+      atomicAdd(&d.cnt[at], 64u);
     }
     return;
   }
-  if (w) atomicAdd(&mass[at], w);
-  atomicAdd(&cnt[at], 1u);
+  atomicAdd(&d.mass[at], w);
+  atomicAdd(&d.cnt[at], 1u);
 }
 
-// What a workgroup keeps between its searches: which of the buffers come next (one is cleared while the last one may
+// What a workgroup keeps between its searches: which of the buffers comes next (one is cleared while the last one may
 // still be read, so a search costs one barrier a step).
 struct Turn {
-  int digits = 0, bins = 0;
+  int digits = 0;
 };
 
 struct Found {
@@ -269,12 +344,12 @@ __device__ __forceinline__ u64 lane_u64(u64 x, int lane) {
   return (u64(lane_u32(uint32_t(x >> 32), lane)) << 32) | lane_u32(uint32_t(x), lane);
 }
 
-// The first of the tokens that each(f) gives f(key, index, weight) of, at which the running count (COUNT) or weight,
+// The first of the tokens that each(f) gives f(key, index, weight) of, at which the running count (by_count) or weight,
 // `cnt0` and `mass0` before the first, passes `target`: by digits of 8 bits of the key, the largest first, until one token is
 // left, then of the index, the smallest first. There are `c` of them of the weight `m`; their keys lie between `klo` and
 // `khi` and differ from bit LOW on, indices are below `V`. Every thread is here; every wave has the result.
-template <bool COUNT, bool INDEX, int LOW, int NT, typename S, typename Each>
-__device__ __forceinline__ Found select(const Each& each, u64 target, u64 mass0, u64 cnt0, u64 m, uint32_t c, uint32_t klo,
+template <int LOW, int NT, typename S, typename Each>
+__device__ __forceinline__ Found select(bool by_count, bool index, const Each& each, u64 target, u64 mass0, u64 cnt0, u64 m, uint32_t c, uint32_t klo,
                                         uint32_t khi, int V, S& s, Turn& turn) {
   const int tid = threadIdx.x, lane = tid & 63;
   auto above = [](int bit) { return bit >= 32 ? 0u : ~0u << bit; };
@@ -282,7 +357,7 @@ __device__ __forceinline__ Found select(const Each& each, u64 target, u64 mass0,
   const uint32_t last = (1u << ibits) - 1;  // the inverse of index 0
   uint32_t kmask = above(kbits), kp = khi & kmask, ip = 0, imask = 0;
   auto mine = [&](uint32_t key, uint32_t inv) { return ((key ^ kp) & kmask) == 0 && ((inv ^ ip) & imask) == 0; };
-  while (c > 1 && (kbits > LOW || (INDEX && ibits > 0))) {
+  while (c > 1 && (kbits > LOW || (index && ibits > 0))) {
     const bool on_key = kbits > LOW;
     const int shift = on_key ? max(kbits - 8, LOW) : max(ibits - 8, 0), width = (on_key ? kbits : ibits) - shift;
     const uint32_t digits = (1u << width) - 1;
@@ -296,7 +371,7 @@ __device__ __forceinline__ Found select(const Each& each, u64 target, u64 mass0,
     each([&](uint32_t key, uint32_t idx, auto weight) {
       const uint32_t inv = last - idx;
       if (!mine(key, inv)) return;
-      add_to(now.mass, now.cnt, int(((on_key ? key : inv) >> shift) & digits), weight());
+      add_to(now, int(((on_key ? key : inv) >> shift) & digits), weight());
     });
     __syncthreads();
     // lane l has digits 255 - 4 l and the three below it
@@ -314,7 +389,7 @@ __device__ __forceinline__ Found select(const Each& each, u64 target, u64 mass0,
     bool hit = false;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const u64 lo = COUNT ? bc : bm, hi = lo + (COUNT ? u64(dc[k]) : dm[k]);
+      const u64 lo = by_count ? bc : bm, hi = lo + (by_count ? u64(dc[k]) : dm[k]);
       if (lo <= target && target < hi) {
         hit = true;
         digit = uint32_t(255 - 4 * lane - k);
@@ -339,8 +414,8 @@ __device__ __forceinline__ Found select(const Each& each, u64 target, u64 mass0,
       imask = above(ibits) & last;
     }
   }
-  if (!INDEX) {  // of equal logits each has the same weight
-    const u64 w = c == 1 ? m : m / c, place = c == 1 ? 0 : COUNT ? target - cnt0 : (target - mass0) / w;
+  if (!index) {  // of equal logits each has the same weight
+    const u64 w = c == 1 ? m : m / c, place = c == 1 ? 0 : by_count ? target - cnt0 : (target - mass0) / w;
     return {mass0 + place * w, w, 0};
   }
   each([&](uint32_t key, uint32_t idx, auto) {
@@ -350,57 +425,160 @@ __device__ __forceinline__ Found select(const Each& each, u64 target, u64 mass0,
   return {mass0, m, s.idx};
 }
 
-// the interval in which the running count or weight passes `target` (below their sum)
-template <bool COUNT, int NT, int BINS, typename S>
-__device__ __forceinline__ int find_bin(u64 target, S& s, Turn& turn) {
-  uint32_t& slot = s.bin[turn.bins++ & 1];
-#pragma unroll
-  for (int i = 0; i < BINS / NT; ++i) {
-    const int b = threadIdx.x + i * NT;
-    const u64 hi = COUNT ? u64(s.cnt[b]) : s.mass[b];
-    const u64 lo = b == 0 ? 0 : COUNT ? u64(s.cnt[b - 1]) : s.mass[b - 1];
-    if (lo <= target && target < hi) slot = b;
+// The same where there are at most 64 tokens, the lane's own being (key, idx, w) where `in`: each counts the ones before
+// it. Every wave does it for itself: no barrier.
+__device__ __forceinline__ Found select_wave(bool by_count, bool in, uint32_t key, uint32_t idx, u64 w, u64 target, u64 mass0,
+                                             u64 cnt0) {
+  u64 mass = mass0;
+  uint32_t cnt = uint32_t(cnt0);
+  const uint32_t n = __popcll(__ballot(in));  // lanes 0 to n - 1
+#pragma unroll 1
+  for (uint32_t j = 0; j < n; ++j) {
+    const uint32_t kj = lane_u32(key, j), ij = lane_u32(idx, j);
+    const u64 wj = lane_u64(w, j);
+    const bool before = kj > key || (kj == key && ij < idx);
+    mass += before ? wj : 0;
+    cnt += before ? 1u : 0u;
   }
-  __syncthreads();
-  return int(slot);
+  const u64 lo = by_count ? u64(cnt) : mass;
+  const int src = __ffsll(static_cast<u64>(__ballot(in && lo <= target && target < lo + (by_count ? 1 : w)))) - 1;
+  return {lane_u64(mass, src), lane_u64(w, src), lane_u32(idx, src)};
 }
 
-// The first token of the row at which the running count (COUNT) or weight passes `target`, its index with INDEX. The
-// prefix sums stand in s; every thread is here.
-template <bool COUNT, bool INDEX, typename T, int NT, int R, int BINS, int LIST>
-__device__ Found cross(const Row<T, NT, R>& row, const Scale<BINS>& sc, u64 target, Lds<BINS, LIST>& s, Turn& turn) {
-  if (threadIdx.x == 0) s.n = 0;
-  const int bin = find_bin<COUNT, NT, BINS>(target, s, turn);
-  const u64 mass0 = bin == 0 ? 0 : s.mass[bin - 1];
-  const u64 cnt0 = bin == 0 ? 0 : s.cnt[bin - 1];
-  const int n = int(s.cnt[bin] - cnt0);
-  constexpr int LOW = sizeof(T) == 2 ? 16 : 0;
-  uint32_t klo, khi;
-  sc.keys(bin, klo, khi);
-  if (!INDEX && n == 1) return {mass0, s.mass[bin] - mass0, 0};  // the token is the interval
-  if (n > LIST) {
-    Row<T, NT, 0> whole;  // from memory each time: rare, and a step over registers is unrolled
-    whole.open(row.p, row.from, row.to);
-    auto each = [&](auto f) {
-      whole.each([&](float x, int i) {
-        if (sc.bin(x) == bin) f(key_of(x), uint32_t(i), [&] { return sc.weight(x); });
-      });
-    };
-    return select<COUNT, INDEX, LOW, NT>(each, target, mass0, cnt0, s.mass[bin] - mass0, n, klo, khi, row.to, s, turn);
+// Prefix sums of the intervals in LDS, every BINS / 64-th of them in a wave's registers.
+struct Interval {
+  int bin;
+  u64 mass0, mass1;  // the weight before it and up to its end
+  uint32_t cnt0, cnt1;
+};
+template <int BINS>
+struct Prefix {
+  static constexpr int STEP = BINS / 64;
+  const u64* mass;
+  const uint32_t* cnt;
+  u64 m;
+  uint32_t c;
+  __device__ __forceinline__ Prefix(const u64* mass_, const uint32_t* cnt_) : mass(mass_), cnt(cnt_) {
+    const int i = int(threadIdx.x & 63) * STEP + STEP - 1;
+    m = mass[i];
+    c = cnt[i];
   }
-  row.each([&](float x, int i) {
-    if (sc.bin(x) != bin) return;
-    const int at = atomicAdd(&s.n, 1u);
-    s.lkey[at] = key_of(x);
-    s.lidx[at] = i;
-    s.lw[at] = sc.weight(x);
+  __device__ __forceinline__ u64 all() const { return lane_u64(m, 63); }
+  // The interval in which the running count or weight passes `target` (below their sum): the first whose prefix sum is
+  // larger, by two steps of 64. Every wave for itself, in scalar registers but for the comparisons.
+  __device__ __forceinline__ Interval find(bool by_count, u64 target) const {
+    const int lane = threadIdx.x & 63;
+    const int a = __ffsll(static_cast<u64>(__ballot(target < (by_count ? u64(c) : m)))) - 1;
+    const int k = a * STEP + min(lane, STEP - 1);
+    const u64 fm = mass[k];
+    const uint32_t fc = cnt[k];
+    const int f = __ffsll(static_cast<u64>(__ballot(target < (by_count ? u64(fc) : fm)))) - 1;
+    Interval r;
+    r.bin = a * STEP + f;
+    r.mass1 = lane_u64(fm, f);
+    r.cnt1 = lane_u32(fc, f);
+    const int before = f > 0 ? f - 1 : a > 0 ? a - 1 : 0;
+    r.mass0 = f > 0 ? lane_u64(fm, before) : a > 0 ? lane_u64(m, before) : 0;
+    r.cnt0 = f > 0 ? lane_u32(fc, before) : a > 0 ? lane_u32(c, before) : 0;
+    return r;
+  }
+};
+
+// The intervals that each stage can end in (the weight that the ones before it leave is only known to within an interval
+// until they are searched), and how many tokens are in them.
+struct Plan {
+  int from[3], to[3];
+  uint32_t total;
+  __device__ __forceinline__ bool has(int bin) const {
+    return (bin >= from[0] && bin <= to[0]) || (bin >= from[1] && bin <= to[1]) || (bin >= from[2] && bin <= to[2]);
+  }
+};
+template <int BINS>
+__device__ __forceinline__ Plan plan_row(const Goals& goals, u64 high, const Prefix<BINS>& prefix) {
+  Plan r{{0, 0, 0}, {-1, -1, -1}, 0};
+  u64 lo = prefix.all(), hi = lo;  // the weight kept lies in [lo, hi]
+#pragma unroll
+  for (int stage = 0; stage < 3; ++stage) {
+    if (!goals.has(stage)) continue;
+    if (stage == 2) {
+      lo = min(lo, high);
+      hi = min(hi, high);
+    }
+    const u64 t0 = goals.target(stage, lo), t1 = goals.target(stage, hi);
+    const Interval a = prefix.find(stage == 0, t0), b = t1 == t0 ? a : prefix.find(stage == 0, t1);
+    lo = a.mass0;
+    hi = b.mass1;
+    r.total += b.cnt1 - a.cnt0;
+    r.from[stage] = a.bin;
+    r.to[stage] = b.bin;
+  }
+  return r;
+}
+
+// The searches of a row: prefix sums in s, the tokens of its plan's intervals in the list (n of them), or FROM_ROW when
+// they do not fit, then each(f) gives f(key, index, interval, weight) of every token of the row. dig[0] is clear.
+template <bool FROM_ROW, int LOW, int NT, int BINS, typename S, typename Each>
+__device__ __forceinline__ uint32_t resolve(const Goals& goals, const Prefix<BINS>& prefix, const Scale<BINS>& sc, u64 high, int n, int V,
+                                            S& s, const Each& each) {
+  const int lane = threadIdx.x & 63;
+  Turn turn;
+  u64 kept = prefix.all();
+  uint32_t token = 0;
+#pragma unroll 1
+  for (int stage = 0; stage < 3; ++stage) {
+    if (!goals.has(stage)) continue;
+    if (stage == 2) kept = min(kept, high);
+    const u64 target = goals.target(stage, kept);
+    const Interval at = prefix.find(stage == 0, target);
+    const uint32_t c = at.cnt1 - at.cnt0;
+    if (stage < 2 && c == 1) {  // the token is the interval
+      kept = at.mass1;
+      continue;
+    }
+    Found f;
+    if (!FROM_ROW && c <= 64) {
+      uint16_t* slot = s.slot[threadIdx.x >> 6];  // the wave's: where in the list the interval's tokens are
+      int have = 0;
+#pragma unroll 1
+      for (int i0 = 0; i0 < n; i0 += 64) {
+        const bool in = i0 + lane < n && s.lbin[min(i0 + lane, n - 1)] == at.bin;
+        const u64 mask = __ballot(in);
+        if (in) slot[have + __popcll(mask & ((u64(1) << lane) - 1))] = uint16_t(i0 + lane);
+        have += __popcll(mask);
+      }
+      __builtin_amdgcn_wave_barrier();
+      const int mine = lane < int(c) ? slot[lane] : 0;
+      __builtin_amdgcn_wave_barrier();
+      f = select_wave(stage == 0, lane < int(c), s.lkey[mine], s.lidx[mine], s.lw[mine], target, at.mass0, at.cnt0);
+    } else {
+      uint32_t klo, khi;
+      sc.keys(at.bin, klo, khi);
+      auto of_bin = [&](auto g) {
+        each([&](uint32_t k, uint32_t i, int bin, auto weight) {
+          if (bin == at.bin) g(k, i, weight);
+        });
+      };
+      f = select<LOW, NT>(stage == 0, stage == 2, of_bin, target, at.mass0, at.cnt0, at.mass1 - at.mass0, c, klo, khi, V, s, turn);
+    }
+    kept = f.before + f.w;
+    token = f.idx;
+  }
+  return token;
+}
+template <typename T, int NT, int BINS, typename S>
+__device__ __forceinline__ uint32_t resolve_list(const Goals& goals, const Prefix<BINS>& prefix, const Scale<BINS>& sc, u64 high, int n, int V, S& s) {
+  return resolve<false, sizeof(T) == 2 ? 16 : 0, NT>(goals, prefix, sc, high, n, V, s, [&](auto f) {
+    for (int i = threadIdx.x; i < n; i += NT) f(s.lkey[i], s.lidx[i], s.lbin[i], [&] { return s.lw[i]; });
   });
-  __syncthreads();
-  if (n == 1) return {mass0, s.lw[0], s.lidx[0]};
-  auto each = [&](auto f) {
-    for (int i = threadIdx.x; i < n; i += NT) f(s.lkey[i], s.lidx[i], [&] { return s.lw[i]; });
-  };
-  return select<COUNT, INDEX, LOW, NT>(each, target, mass0, cnt0, s.mass[bin] - mass0, n, klo, khi, row.to, s, turn);
+}
+// (from memory each time: rare, and a step over registers is unrolled)
+template <typename T, int NT, int BINS, typename S>
+__device__ __forceinline__ uint32_t resolve_row(const Goals& goals, const Prefix<BINS>& prefix, const Scale<BINS>& sc, u64 high, const T* logits, int V, S& s) {
+  Row<T, NT, 0> row;
+  row.open(logits, 0, V);
+  return resolve<true, sizeof(T) == 2 ? 16 : 0, NT>(goals, prefix, sc, high, 0, V, s, [&](auto f) {
+    row.each([&](float x, int i) { f(key_of(x), uint32_t(i), sc.bin(x), [&] { return sc.weight(x); }); });
+  });
 }
 
 // counts and weights of the intervals to their prefix sums, in place; a barrier ends it
@@ -424,29 +602,6 @@ __device__ __forceinline__ void scan_bins(S& s) {
     s.cnt[tid * N + i] = c[i] + tc;
   }
   __syncthreads();
-}
-
-// the searches of a row whose intervals are summed and whose weight above min_p is `high`
-template <typename T, int NT, int R, int BINS, int LIST>
-__device__ __forceinline__ void draw(const Row<T, NT, R>& row, const Scale<BINS>& sc, const Setting& o, u64 high,
-                                     Lds<BINS, LIST>& s, int64_t* token) {
-  Turn turn;
-  for (int i = threadIdx.x; i < 256; i += NT) {
-    s.dig[0].mass[i] = 0;
-    s.dig[0].cnt[i] = 0;
-  }
-  u64 kept = s.mass[BINS - 1];
-  if (o.top_k > 0 && o.top_k < row.to) {
-    const Found f = cross<true, false>(row, sc, u64(o.top_k - 1), s, turn);
-    kept = f.before + f.w;
-  }
-  if (o.top_p < 1.f) {
-    const Found f = cross<false, false>(row, sc, target_of_p(o.top_p, kept), s, turn);
-    kept = f.before + f.w;
-  }
-  kept = min(kept, high);
-  const Found f = cross<false, true>(row, sc, target_of_u(o.u, kept), s, turn);
-  if (threadIdx.x == 0) *token = f.idx;
 }
 
 // the largest logit, the smallest finite one and whether there is a NaN, over the workgroup
@@ -514,34 +669,68 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
   }
   const Scale<BINS> sc(o, top, low);
   const bool cut = o.min_p > 0.f;
-  const u64 least = floor_of(o.min_p);
-  u64 high = 0;
-  row.each([&](float x, int) {
-    const u64 w = sc.weight(x);
-    add_to(s.mass, s.cnt, sc.bin(x), w);
-    if (w >= least) high += w;
-  });
+  u64 high = histogram<BINS>(row, sc, o.min_p, s);
   if (cut) {
     high = wave_scan(high);
     if ((tid & 63) == 63) atomicAdd(&s.high, high);
   }
   __syncthreads();
+  if (tid == 0) s.n = 0;
+  for (int i = tid; i < 256; i += NT) {
+    s.dig[0].mass[i] = 0;
+    s.dig[0].cnt[i] = 0;
+  }
   scan_bins<NT, BINS>(s);
-  draw(row, sc, o, cut ? s.high : s.mass[BINS - 1], s, p.tokens + b);
+  high = cut ? s.high : ~u64(0);
+  const Goals goals(o, p.V);
+  const Prefix<BINS> prefix(s.mass, s.cnt);
+  const Plan plan = plan_row(goals, high, prefix);
+  uint32_t token;
+  if (plan.total <= LIST) {
+    row.each([&](float x, int i) {
+      const int bin = sc.bin(x);
+      if (!plan.has(bin)) return;
+      const int at = atomicAdd(&s.n, 1u);
+      s.lkey[at] = key_of(x);
+      s.lidx[at] = i;
+      s.lw[at] = sc.weight(x);
+      s.lbin[at] = bin;
+    });
+    __syncthreads();
+    token = resolve_list<T, NT>(goals, prefix, sc, high, int(s.n), p.V, s);
+  } else {
+    token = resolve_row<T, NT>(goals, prefix, sc, high, row.p, p.V, s);
+  }
+  if (tid == 0) p.tokens[b] = token;
 }
 
 // ---- a row in pieces ---------------------------------------------------------------------------------------
 constexpr int kPieceThreads = 512;
 constexpr int kRowList = 2048;  // tokens of the intervals that a row's searches can end in
-struct RowWs {                  // in the workspace, written and read at agent scope or launches apart
-  u64 mass[kBins];
+struct RowWs {                  // in the workspace: what a launch leaves for the next, and pieces for their row's last
+  u64 mass[kBins];              // prefix sums when the second launch has ended
   u64 high;
+  uint32_t cnt[kBins];
   float top[kMaxPieces], low[kMaxPieces];
   uint32_t nan[kMaxPieces], first[kMaxPieces];
-  uint32_t cnt[kBins];
+  Plan plan;
   uint32_t done, n;
   uint32_t key[kRowList], idx[kRowList];
 };
+// publish, then count: agent-scope stores and additions are acknowledged at the device-coherent level before the
+// barrier, the count's addition is issued after it, and the workgroup that sees the last count reads with agent-scope
+// loads. Every thread is here; the same answer for all.
+__device__ __forceinline__ bool last_piece(RowWs& w, int pieces, int& flag) {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (threadIdx.x == 0) flag = __hip_atomic_fetch_add(&w.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == uint32_t(pieces - 1);
+  __syncthreads();
+  return flag != 0;
+}
+template <typename N>
+__device__ __forceinline__ N agent_load(const N* p) {
+  return __hip_atomic_load(const_cast<N*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kPieceThreads) sample_top_kernel(const SampleParams p) {
@@ -609,8 +798,13 @@ __device__ __forceinline__ Whole whole_row(const RowWs& w, const SampleParams& p
 template <typename T>
 __global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(const SampleParams p) {
   constexpr int NT = kPieceThreads;
-  __shared__ u64 mass[kBins];
-  __shared__ uint32_t cnt[kBins];
+  __shared__ struct {
+    u64 mass[kBins];
+    uint32_t cnt[kBins];
+    u64 red64[16];
+    uint32_t red32[16];
+    int last;
+  } s;
   const int tid = threadIdx.x, b = blockIdx.x / p.pieces, g = blockIdx.x % p.pieces;
   if (p.run && *p.run == 0) return;
   RowWs& w = reinterpret_cast<RowWs*>(p.ws)[b];
@@ -622,20 +816,14 @@ __global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(const Sample
   }
 #pragma unroll
   for (int i = 0; i < kBins / NT; ++i) {
-    mass[tid + i * NT] = 0;
-    cnt[tid + i * NT] = 0;
+    s.mass[tid + i * NT] = 0;
+    s.cnt[tid + i * NT] = 0;
   }
   __syncthreads();
   Row<T, NT, 0> row;
   row.open(reinterpret_cast<const T*>(p.logits) + b * p.l_sr, g * p.piece, min(p.V, (g + 1) * p.piece));
   const Scale<kBins> sc(o, all.top, all.low);
-  const u64 least = floor_of(o.min_p);
-  u64 high = 0;
-  row.each([&](float x, int) {
-    const u64 wt = sc.weight(x);
-    add_to(mass, cnt, sc.bin(x), wt);
-    if (wt >= least) high += wt;
-  });
+  u64 high = histogram<kBins>(row, sc, o.min_p, s);
   if (o.min_p > 0.f) {
     high = wave_scan(high);
     if ((tid & 63) == 63 && high) __hip_atomic_fetch_add(&w.high, high, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -644,65 +832,62 @@ __global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(const Sample
 #pragma unroll
   for (int i = 0; i < kBins / NT; ++i) {
     const int k = tid + i * NT;
-    if (cnt[k]) __hip_atomic_fetch_add(&w.cnt[k], cnt[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (mass[k]) __hip_atomic_fetch_add(&w.mass[k], mass[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (s.cnt[k]) __hip_atomic_fetch_add(&w.cnt[k], s.cnt[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (s.mass[k]) __hip_atomic_fetch_add(&w.mass[k], s.mass[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (!last_piece(w, p.pieces, s.last)) return;
+
+  // ---- the row's last piece: prefix sums, and the intervals that a search can end in ----
+  {
+    u64 m[kBins / NT];
+    uint32_t c[kBins / NT];
+#pragma unroll
+    for (int i = 0; i < kBins / NT; ++i) {
+      m[i] = agent_load(&w.mass[tid + i * NT]);
+      c[i] = agent_load(&w.cnt[tid + i * NT]);
+    }
+#pragma unroll
+    for (int i = 0; i < kBins / NT; ++i) {
+      s.mass[tid + i * NT] = m[i];
+      s.cnt[tid + i * NT] = c[i];
+    }
+  }
+  high = o.min_p > 0.f ? agent_load(&w.high) : ~u64(0);
+  __syncthreads();
+  scan_bins<NT, kBins>(s);
+#pragma unroll
+  for (int i = 0; i < kBins / NT; ++i) {
+    w.mass[tid + i * NT] = s.mass[tid + i * NT];
+    w.cnt[tid + i * NT] = s.cnt[tid + i * NT];
+  }
+  const Plan plan = plan_row(Goals(o, p.V), high, Prefix<kBins>(s.mass, s.cnt));
+  if (tid == 0) {
+    w.plan = plan;
+    w.done = 0;
   }
 }
 
-// Every piece finds the intervals that a search can end in (the weight that top-k and top-p leave is only known to
-// within an interval) and appends its tokens of those to the row's list; the row's last piece has all of them.
 template <typename T>
 __global__ void __launch_bounds__(kPieceThreads) sample_pick_kernel(const SampleParams p) {
   constexpr int NT = kPieceThreads;
   __shared__ Lds<kBins, kRowList> s;
-  __shared__ int lbin[kRowList];
   const int tid = threadIdx.x, b = blockIdx.x / p.pieces, g = blockIdx.x % p.pieces;
   if (p.run && *p.run == 0) return;
   RowWs& w = reinterpret_cast<RowWs*>(p.ws)[b];
   const Setting o(p, b);
   const Whole all = whole_row(w, p, o);
   if (all.over) return;
-#pragma unroll
-  for (int i = 0; i < kBins / NT; ++i) {
-    s.mass[tid + i * NT] = w.mass[tid + i * NT];
-    s.cnt[tid + i * NT] = w.cnt[tid + i * NT];
-  }
   if (tid == 0) s.n = 0;
-  const u64 high = o.min_p > 0.f ? w.high : ~u64(0);
-  __syncthreads();
-  scan_bins<NT, kBins>(s);
+  const Plan plan = w.plan;
+  const bool fits = plan.total <= kRowList;
   const Scale<kBins> sc(o, all.top, all.low);
-  const bool by_k = o.top_k > 0 && o.top_k < p.V, by_p = o.top_p < 1.f;
-  auto before = [&](int bin) { return bin == 0 ? u64(0) : s.mass[bin - 1]; };
-  auto count = [&](int lo, int hi) { return s.cnt[hi] - (lo == 0 ? 0u : s.cnt[lo - 1]); };
-  Turn turn;
-  auto find = [&](u64 target) { return find_bin<false, NT, kBins>(target, s, turn); };
-  // the weight kept lies in [lo, hi]
-  u64 lo = s.mass[kBins - 1], hi = lo;
-  int kb = -1, p0 = -1, p1 = -2;
-  if (by_k) {
-    kb = find_bin<true, NT, kBins>(u64(o.top_k - 1), s, turn);
-    lo = before(kb);
-    hi = s.mass[kb];
-  }
-  if (by_p) {
-    p0 = find(target_of_p(o.top_p, lo));
-    p1 = find(target_of_p(o.top_p, hi));
-    lo = before(p0);
-    hi = s.mass[p1];
-  }
-  lo = min(lo, high);
-  hi = min(hi, high);
-  const int u0 = find(target_of_u(o.u, lo)), u1 = find(target_of_u(o.u, hi));
-  const u64 total = u64(kb >= 0 ? count(kb, kb) : 0) + (by_p ? count(p0, p1) : 0) + count(u0, u1);
-  auto in = [&](int bin) { return bin == kb || (bin >= p0 && bin <= p1) || (bin >= u0 && bin <= u1); };
   const T* logits = reinterpret_cast<const T*>(p.logits) + b * p.l_sr;
-  const bool fits = total <= kRowList;  // the same for every piece of the row
+  __syncthreads();
   if (fits) {
     Row<T, NT, 0> row;
     row.open(logits, g * p.piece, min(p.V, (g + 1) * p.piece));
     row.each([&](float x, int i) {
-      if (!in(sc.bin(x))) return;
+      if (!plan.has(sc.bin(x))) return;
       const int at = atomicAdd(&s.n, 1u);
       s.lkey[at] = key_of(x);
       s.lidx[at] = i;
@@ -716,69 +901,48 @@ __global__ void __launch_bounds__(kPieceThreads) sample_pick_kernel(const Sample
       __hip_atomic_store(&w.idx[s.first + i], s.lidx[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
-  // publish, then count: agent-scope stores are acknowledged at the device-coherent level before the barrier, the
-  // count's add is issued after it, and the workgroup that sees the last count reads with agent-scope loads
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (tid == 0) s.last = __hip_atomic_fetch_add(&w.done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == uint32_t(p.pieces - 1);
-  __syncthreads();
-  if (!s.last) return;
+  if (!last_piece(w, p.pieces, s.last)) return;
 
-  if (!fits) {
-    // one of the intervals holds too many: the searches over the whole row, by the digits of the keys there
-    Row<T, NT, 0> row;
-    row.open(logits, 0, p.V);
-    draw(row, sc, o, high, s, p.tokens + b);
-    return;
+  // ---- the row's last piece: the searches ----
+#pragma unroll
+  for (int i = 0; i < kBins / NT; ++i) {
+    s.mass[tid + i * NT] = w.mass[tid + i * NT];
+    s.cnt[tid + i * NT] = w.cnt[tid + i * NT];
   }
-  const int n = int(__hip_atomic_load(&w.n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-  for (int i = tid; i < n; i += NT) {
-    const uint32_t k = __hip_atomic_load(&w.key[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const float x = of_key(k);
-    s.lkey[i] = k;
-    s.lidx[i] = __hip_atomic_load(&w.idx[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    s.lw[i] = sc.weight(x);
-    lbin[i] = sc.bin(x);
-  }
-  __syncthreads();
   for (int i = tid; i < 256; i += NT) {
     s.dig[0].mass[i] = 0;
     s.dig[0].cnt[i] = 0;
   }
-  u64 kept = s.mass[kBins - 1];
-  auto search = [&](auto by_count, auto index, u64 target) {
-    constexpr bool COUNT = decltype(by_count)::value;
-    const int bin = find_bin<COUNT, NT, kBins>(target, s, turn);
-    auto each = [&](auto f) {
-      for (int i = tid; i < n; i += NT)
-        if (lbin[i] == bin) f(s.lkey[i], s.lidx[i], [&] { return s.lw[i]; });
-    };
-    uint32_t klo, khi;
-    sc.keys(bin, klo, khi);
-    return select<COUNT, decltype(index)::value, sizeof(T) == 2 ? 16 : 0, NT>(
-        each, target, before(bin), bin == 0 ? 0 : s.cnt[bin - 1], s.mass[bin] - before(bin), count(bin, bin), klo, khi, p.V, s, turn);
-  };
-  using Yes = std::true_type;
-  using No = std::false_type;
-  if (by_k) {
-    const Found f = search(Yes{}, No{}, u64(o.top_k - 1));
-    kept = f.before + f.w;
+  const u64 high = o.min_p > 0.f ? w.high : ~u64(0);
+  const Goals goals(o, p.V);
+  uint32_t token;
+  if (fits) {
+    const int n = int(agent_load(&w.n));
+    for (int i = tid; i < n; i += NT) {
+      const uint32_t k = agent_load(&w.key[i]), idx = agent_load(&w.idx[i]);
+      const float x = of_key(k);
+      s.lkey[i] = k;
+      s.lidx[i] = idx;
+      s.lw[i] = sc.weight(x);
+      s.lbin[i] = sc.bin(x);
+    }
+    __syncthreads();
+    token = resolve_list<T, NT>(goals, Prefix<kBins>(s.mass, s.cnt), sc, high, n, p.V, s);
+  } else {
+    __syncthreads();
+    token = resolve_row<T, NT>(goals, Prefix<kBins>(s.mass, s.cnt), sc, high, logits, p.V, s);
   }
-  if (by_p) {
-    const Found f = search(No{}, No{}, target_of_p(o.top_p, kept));
-    kept = f.before + f.w;
-  }
-  kept = min(kept, high);
-  const Found f = search(No{}, Yes{}, target_of_u(o.u, kept));
-  if (tid == 0) p.tokens[b] = f.idx;
+  if (tid == 0) p.tokens[b] = token;
 }
 
-constexpr int kWholeRow = 32768;  // longer rows go in pieces
+constexpr int kWholeRow = 8192;  // longer rows go in pieces
 
-// Pieces of a row: two workgroups a CU over the batch, of at least 4096 logits.
+// Pieces of a row: a workgroup a CU over the batch, two where a piece would be over 16384 logits, of at least 4096 (64 x
+// 131072 fp32 in 4, 8 pieces 56, 52 us; 16 x 131072 in 16, 32 pieces 33.8, 36.9; 1 x 32000 in 7, 3 pieces 24.5, 28).
 static int pieces_of(int B, int V) {
   if (V <= kWholeRow) return 1;
-  int64_t n = 2 * int64_t(device_cu_count()) / B;
+  int64_t n = std::max<int64_t>(device_cu_count() / B, 1);
+  if (V / n > 16384) n *= 2;
   n = std::min<int64_t>(n, V / 4096);
   return int(std::max<int64_t>(2, std::min<int64_t>(n, kMaxPieces)));
 }
@@ -821,11 +985,10 @@ int launch_sample(const mote_sample_args* a, hipStream_t stream) {
     return check_launch(what);
   }
 #define MOTE_SAMPLE(NT_, R_, BINS_) hipLaunchKernelGGL((sample_kernel<T, NT_, R_, BINS_>), dim3(a->B), dim3(NT_), 0, stream, p)
-#define MOTE_SAMPLE_V                                   \
-  if (a->V <= 512) MOTE_SAMPLE(256, 2, 512);            \
-  else if (a->V <= 1024) MOTE_SAMPLE(512, 2, 1024);     \
-  else if (a->V <= 8192) MOTE_SAMPLE(1024, 8, 2048);    \
-  else MOTE_SAMPLE(1024, 32, 2048);
+#define MOTE_SAMPLE_V                               \
+  if (a->V <= 512) MOTE_SAMPLE(256, 2, 512);        \
+  else if (a->V <= 1024) MOTE_SAMPLE(512, 2, 1024); \
+  else MOTE_SAMPLE(1024, 8, 2048);
   if (a->dtype == MOTE_BF16) {
     using T = bf16_t;
     MOTE_SAMPLE_V
