@@ -5,7 +5,7 @@
 // Per past row j: U_j = s_page <q, c_j> / sqrt(D), e_j = SiLU(U_j), running max m and sum l,
 // z += exp(e_j - m) s'_page c'_j. A row is D bytes of P2 and of I~ and a page's two scales, half of bf16's bytes, so a
 // sweep is bound by memory; a wave has a page at a time. P2: lane r holds row r, whose score is a sum of its own
-// (codes as bf16 pairs, exact, for v_dot2_f32_bf16 with the query in scalar registers; fp32 queries in fp32). The
+// (codes as bf16 pairs, exact, for v_dot2_f32_bf16; fp32 queries in fp32). The
 // weights go round in LDS (64 floats of the wave's own), and for I~ a lane holds 16 rows of one dim of each
 // 16-dim chunk, so a sweep keeps D / 16 sums a lane and its end is two steps within a quad. The running maximum is
 // the wave's: a rescale multiplies D / 16 sums and is taken when the maximum has grown by 2^8. Page numbers and
@@ -67,41 +67,30 @@ __device__ __forceinline__ float lane_f32(float x, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
-// <q, codes> over the 16 dims of chunk c
-template <typename T, int C>
-struct Query8;
-template <int C>
-struct Query8<bf16_t, C> {
-  uint32_t v[8 * C];  // pairs, the same in every lane
-  __device__ __forceinline__ void set(const float* sq) {
-#pragma unroll
-    for (int j = 0; j < 8 * C; ++j)
-      v[j] = uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(f2bf(sq[2 * j])) | (uint32_t(f2bf(sq[2 * j + 1])) << 16))));
-  }
-  __device__ __forceinline__ void dot(int c, const Chunk& k, float& a, float& b) const {
+// <q, codes> over the 16 dims of chunk c; the query in LDS, read by all lanes at once (bf16 pairs in scalar registers
+// spilled from head dim 96 on: batch 1, 4130 rows 10.6 us, 9.6 so)
+template <typename T>
+__device__ __forceinline__ void dot8(const T* q, int c, const Chunk& k, float& a, float& b) {
+  if constexpr (sizeof(T) == 2) {
+    const Chunk q0 = load_chunk(q + 16 * c), q1 = load_chunk(q + 16 * c + 8);
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      a = __builtin_amdgcn_fdot2_f32_bf16(codes8_bf16<false>(k.w[w]), __builtin_bit_cast(bf16x2, v[8 * c + 2 * w]), a, false);
-      b = __builtin_amdgcn_fdot2_f32_bf16(codes8_bf16<true>(k.w[w]), __builtin_bit_cast(bf16x2, v[8 * c + 2 * w + 1]), b, false);
+      const Chunk& h = w < 2 ? q0 : q1;
+      a = __builtin_amdgcn_fdot2_f32_bf16(codes8_bf16<false>(k.w[w]), __builtin_bit_cast(bf16x2, h.w[2 * w % 4]), a, false);
+      b = __builtin_amdgcn_fdot2_f32_bf16(codes8_bf16<true>(k.w[w]), __builtin_bit_cast(bf16x2, h.w[2 * w % 4 + 1]), b, false);
     }
-  }
-};
-template <int C>
-struct Query8<float, C> {
-  const float* v;  // in LDS
-  __device__ __forceinline__ void set(const float* sq) { v = sq; }
-  __device__ __forceinline__ void dot(int c, const Chunk& k, float& a, float& b) const {
+  } else {
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float4 q = *reinterpret_cast<const float4*>(v + 16 * c + 4 * w);
+      const float4 f = *reinterpret_cast<const float4*>(q + 16 * c + 4 * w);
       const f32x2 x = codes8_f32<false>(k.w[w]), y = codes8_f32<true>(k.w[w]);
-      a = fmaf(x.x, q.x, a);
-      b = fmaf(x.y, q.y, b);
-      a = fmaf(y.x, q.z, a);
-      b = fmaf(y.y, q.w, b);
+      a = fmaf(x.x, f.x, a);
+      b = fmaf(x.y, f.y, b);
+      a = fmaf(y.x, f.z, a);
+      b = fmaf(y.y, f.w, b);
     }
   }
-};
+}
 
 template <typename T, int C, bool STREAM>
 __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8Params p) {
@@ -112,6 +101,7 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
   constexpr int PIECES = DP / PER;            // pieces of a padded tail row
   __shared__ __align__(16) float zred[kD8MaxSplits * (DP + 2)];
   __shared__ __align__(16) float sq[DP], knew[DP], inew[DP];
+  __shared__ __align__(16) T sqt[DP];  // the query as it is
   __shared__ __align__(16) float sp[kD8Waves][kPage8];
   __shared__ float sm[kD8Waves], sl[kD8Waves];
   __shared__ float wsp[kD8MaxSplits];
@@ -187,6 +177,23 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
     resolve(0);
     fetch(0, I0{});
   }
+  // the tail, by the last split (it has the fewest pages): 16 rows a wave, a quad of lanes a row of P2, and for I~ a lane
+  // the dims that it has of a page
+  const int r0 = 16 * wave, quad = lane >> 2, part4 = lane & 3;
+  const bool tailed = split == nsp - 1 && rest > r0;
+  Chunk tk[(PIECES + 3) / 4];
+  T tv[4][C];
+  if (tailed) {
+    const int64_t off = b * p.tail_sb + int64_t(h) * (kPage8 * D);
+    const T* kt = reinterpret_cast<const T*>(p.kt) + off + (r0 + quad) * D;
+    const T* vt = reinterpret_cast<const T*>(p.vt) + off + (r0 + part4) * D;
+#pragma unroll
+    for (int i = 0; i < (PIECES + 3) / 4; ++i) tk[i] = load_chunk(kt + min((part4 + 4 * i) * PER, D - PER));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int c = 0; c < C; ++c) tv[i][c] = vt[4 * i * D + min(16 * c + quad, D - 1)];
+  }
 
   float cs, sn;
   sincosf((float)S * invf, &sn, &cs);
@@ -206,6 +213,8 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
   if (tid < half) {
     sq[tid] = rq0;
     sq[tid + half] = rq1;
+    sqt[tid] = E::from_f(rq0);
+    sqt[tid + half] = E::from_f(rq1);
     knew[tid] = rk0;
     knew[tid + half] = rk1;
   } else if (tid >= 128 && tid < 128 + D) {
@@ -213,19 +222,17 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
   }
   if (tid < DP - D) {  // padded dims hold zeros
     sq[D + tid] = 0.f;
+    sqt[D + tid] = E::from_f(0.f);
     knew[D + tid] = 0.f;
     inew[D + tid] = 0.f;
   }
   __syncthreads();
 
-  Query8<T, C> q;
-  q.set(sq);
   float m = kNegInf, l = 0.f;
   float z[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) z[c] = 0.f;
   float* spw = sp[wave];
-  const int quad = lane >> 2, part4 = lane & 3;
   const float c2 = p.scale * kLog2e;
 
   // a row's weight from its score in log2 units; the maximum over the wave moves m
@@ -241,27 +248,19 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
     }
   };
 
-  // the tail, by the last split (it has the fewest pages): 16 rows a wave, a quad of lanes a row
-  const int r0 = 16 * wave;
-  if (split == nsp - 1 && rest > r0) {
-    const int64_t off = b * p.tail_sb + int64_t(h) * (kPage8 * D);
-    const T* kt = reinterpret_cast<const T*>(p.kt) + off;
-    const T* vt = reinterpret_cast<const T*>(p.vt) + off;
+  if (tailed) {
     const int row = r0 + quad;
-    float vv[4][C];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int c = 0; c < C; ++c) vv[i][c] = E::to_f(vt[(r0 + part4 + 4 * i) * D + min(16 * c + quad, D - 1)]);
     float u = 0.f;
 #pragma unroll
     for (int i = 0; i < (PIECES + 3) / 4; ++i) {
       const int d = (part4 + 4 * i) * PER;
-      float x[PER];
-      load_values<PER>(kt + row * D + min(d, D - PER), x);
 #pragma unroll
-      for (int k = 0; k < PER; ++k)
-        if (d < D) u = fmaf(x[k], sq[d + k], u);
+      for (int k = 0; k < PER; ++k) {
+        float x;
+        if constexpr (sizeof(T) == 2) x = __uint_as_float(k % 2 ? tk[i].w[k / 2] & 0xffff0000u : tk[i].w[k / 2] << 16);
+        else x = __uint_as_float(tk[i].w[k]);
+        if (d < D) u = fmaf(x, sq[d + k], u);
+      }
     }
     u += dpp<kDppXor1>(u);
     u += dpp<kDppXor2>(u);
@@ -278,7 +277,7 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
       const float w = spw[part4 + 4 * i];
       const bool in = r0 + part4 + 4 * i < rest;  // rows behind may hold anything
 #pragma unroll
-      for (int c = 0; c < C; ++c) z[c] = in ? fmaf(w, vv[i][c], z[c]) : z[c];
+      for (int c = 0; c < C; ++c) z[c] = in ? fmaf(w, E::to_f(tv[i][c]), z[c]) : z[c];
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -287,7 +286,7 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
     constexpr int U = decltype(u)::value;
     float d0 = 0.f, d1 = 0.f;
 #pragma unroll
-    for (int c = 0; c < C; ++c) q.dot(c, kr[U][c], d0, d1);
+    for (int c = 0; c < C; ++c) dot8(sqt, c, kr[U][c], d0, d1);
     const float ev = silu2((d0 + d1) * (lane_f32(ksl, j & 63) * c2));
     raise(ev);
     const float pr = fexp2(ev - m);
@@ -482,13 +481,16 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
   }
 }
 
-// Splits per head: a workgroup per CU over the whole batch, each with a page for every wave; at most one split per
-// lane of the merging wave.
+// Splits per head: a workgroup per CU over the whole batch, each with a page for every wave; two per CU where every wave
+// still has two pages (more loads in flight, and sequences of unlike lengths even out: 16 x 4700 rows of 4 x 48, fp32
+// 11.1 -> 10.1 us, 2 x 32768 of 8 x 128 27.3 -> 26.7; below, the merge costs more: 1 x 1000 rows 9.4 and 9.7). At most
+// one split per lane of the merging wave.
 static int splits8(const mote_relation_decode8_args* a) {
-  const int64_t BH = int64_t(a->B) * a->H, most = (int64_t(a->cache.blocks) + kD8Waves - 1) / kD8Waves;
+  const int64_t BH = int64_t(a->B) * a->H, blocks = a->cache.blocks;
   int64_t n = device_cu_count() / BH;
   if (n < 1) n = 1;
-  if (n > most) n = most;
+  if (blocks >= 2 * kD8Waves * 2 * n) n *= 2;
+  n = std::min(n, (blocks + kD8Waves - 1) / kD8Waves);
   return int(n < kD8MaxSplits ? n : kD8MaxSplits);
 }
 
@@ -553,7 +555,9 @@ int launch_decode8(const mote_relation_decode8_args* a, hipStream_t stream) {
   p.scale = 1.0f / sqrtf((float)a->D);
   p.tau_inv = 1.0f / a->tau_s;
   const dim3 grid(unsigned(a->B * a->H * p.nsplit)), block(kD8Threads);
-  const bool stream_rows = false;
+  // pages are read past the caches once a layer's pool outgrows the L2s, though the Infinity Cache may hold it: 87 MB of
+  // rows in 117 MB 22.0 -> 19.8 us, 805 MB in 1.07 GB 159 -> 140; 53 MB in 53 MB 10.8 either way
+  const bool stream_rows = 2.0 * c.pages * a->H * kPage8 * 16 * chunks8(a->D) > 64e6;
 #define MOTE_D8(C_)                                                                                                    \
   if (stream_rows) hipLaunchKernelGGL((relation_decode8_kernel<T, C_, true>), grid, block, 0, stream, p);              \
   else hipLaunchKernelGGL((relation_decode8_kernel<T, C_, false>), grid, block, 0, stream, p);

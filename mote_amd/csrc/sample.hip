@@ -974,11 +974,12 @@ int launch_sample(const mote_sample_args* a, hipStream_t stream) {
     p.piece = ((a->V + p.pieces - 1) / p.pieces + 7) / 8 * 8;
     p.pieces = (a->V + p.piece - 1) / p.piece;
     const dim3 grid(unsigned(a->B) * p.pieces), block(kPieceThreads);
+    const bool draws = a->temperature_dev || a->temperature > 0.f;  // else the second launch has every token
     auto launch = [&](auto t) {
       using T = decltype(t);
       hipLaunchKernelGGL((sample_top_kernel<T>), grid, block, 0, stream, p);
       hipLaunchKernelGGL((sample_hist_kernel<T>), grid, block, 0, stream, p);
-      hipLaunchKernelGGL((sample_pick_kernel<T>), grid, block, 0, stream, p);
+      if (draws) hipLaunchKernelGGL((sample_pick_kernel<T>), grid, block, 0, stream, p);
     };
     if (a->dtype == MOTE_BF16) launch(bf16_t{});
     else launch(0.f);
