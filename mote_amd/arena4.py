@@ -28,6 +28,7 @@ class RelationArena4(RelationArena):
     """`store` holds the codes, uint8 [n_layers, 2, batch, H, capacity, 16 G], `scales` bf16 [..., G]."""
 
     in_place = False
+    kind = "cache4"
 
     def __init__(self, n_layers: int, n_heads: int, capacity: int, d_head: int, device, dtype=torch.bfloat16, batch: int = 1):
         if dtype not in (torch.bfloat16, torch.float32):

@@ -20,6 +20,7 @@ import torch.nn.functional as F
 from . import _lib as L
 from .arena import RelationArena
 from .cache4 import decode4_workspace, relation_decode4
+from .cache8 import decode8_workspace, relation_decode8
 from .int8 import FEW_ROWS, FEW_WIDTH, int8_linear, int8_weight
 
 
@@ -183,7 +184,8 @@ class RelationDecodeStep:
     `__call__(x [B,1,D], S)` returns (out [B,1,D], xm [B] = mean over heads of the exchange mass,
     graph.py:186).
 
-    The arena may be a RelationArena4 (rows in 4 bits: relation_decode4 in the place of relation_decode).
+    The arena may be a RelationArena4 or a RelationArena8 (rows in 4 bits, or pages of 8: relation_decode4 or
+    relation_decode8 in the place of relation_decode).
     int8: the projections in 8-bit integers (`int8_linear`; codes and scales are the step's own copies,
     which `sync_params()` refreshes), for up to 64 sequences. The launch of wo writes xm, so it is one launch at
     every size, also where int8_linear would take tiles for it: 64 sequences of width 4096 26.0 us, 10.0 with tiles
@@ -210,8 +212,11 @@ class RelationDecodeStep:
 
     def _new_workspace(self) -> None:
         a, m = self.arena, self.mixer
-        make = decode_workspace if a.in_place else lambda *sizes_and_dtype: decode4_workspace(*sizes_and_dtype[:-1])
-        self.workspace = make(a.batch, m.n_heads, m.d_head, a.capacity, a.device, a.dtype)
+        sizes = (a.batch, m.n_heads, m.d_head, a.capacity, a.device)
+        if a.in_place:
+            self.workspace = decode_workspace(*sizes, a.dtype)
+        else:
+            self.workspace = (decode4_workspace if a.kind == "cache4" else decode8_workspace)(*sizes)
         self._generation = a.generation
 
     @torch.no_grad()
@@ -248,7 +253,7 @@ class RelationDecodeStep:
         """The step between the projections and `_out`, into self.y and self.g."""
         m, a = self.mixer, self.arena
         rows = (a.p2(self.layer), a.info(self.layer)) if a.in_place else (a.cache(self.layer),)
-        step = relation_decode if a.in_place else relation_decode4
+        step = relation_decode if a.in_place else relation_decode4 if a.kind == "cache4" else relation_decode8
         step(qkv[:, 0], qkv[:, 1], qkv[:, 2], S, *rows, self.lam, m.tau_s, self.inv_freq, self.theta, m.layer_idx,
              advance, self.workspace, self.y, self.g, xm, run, rope_f32)
 
@@ -296,7 +301,7 @@ class RelationDecodeStep:
         B, T, Dm = x.shape
         H, dh = m.n_heads, m.d_head
         if self._generation != self.arena.generation and not self.arena.in_place:
-            # a grown arena in 4 bits: its workspace belongs to its capacity
+            # a grown arena in 4 or 8 bits: its workspace belongs to its capacity
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("the arena has grown: run the decode step once outside the capture first")
             self._new_workspace()

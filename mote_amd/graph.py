@@ -37,7 +37,8 @@ class RelationMainStep:
         position (0-d or [batch]). xm_dev: optional fp32 [n_layers] (batch 1) or [n_layers, batch]
         buffer that receives each layer's exchange mass. run: optional device flag (bool / uint8, one
         element), the predicate of every launch. advance: the last layer's launch moves S on. int8: the
-        layers' projections in 8-bit integers (see RelationDecodeStep). The arena may be a RelationArena4."""
+        layers' projections in 8-bit integers (see RelationDecodeStep). The arena may be a
+        RelationArena4 or a RelationArena8."""
         if S.dtype != torch.int64 or S.numel() != arena.batch or not S.is_contiguous():
             raise ValueError("S must be a contiguous int64 device tensor with one position per sequence")
         self.arena, self.S, self.xm_dev, self.run, self.advance = arena, S, xm_dev, run, advance

@@ -42,7 +42,7 @@ class Branch:
 
 def _rows_as_they_are(arena: RelationArena) -> None:
     if not arena.in_place:
-        raise TypeError("prefix-store pages hold an arena's rows as they are: not those of an arena in 4 bits")
+        raise TypeError("prefix-store pages hold an arena's rows as they are: not those of an arena in 4 or 8 bits")
 
 
 def _copy_rows(arena: RelationArena, seq: int, arena_row0: int, page: torch.Tensor, page_row0: int, rows: int,
