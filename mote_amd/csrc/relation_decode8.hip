@@ -124,7 +124,8 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
   const int64_t S64 = p.S[b + vzero];
   const int run_v = (p.run ? p.run : reinterpret_cast<const unsigned char*>(p.lam))[vzero];
   const int32_t* tab = p.table + b * p.table_sb;
-  const int t0 = split + nsp * wave, step = nsp * kD8Waves;  // this wave's pages: t0 + j step
+  const int psp = nsp > 1 ? nsp - 1 : 1;  // splits of the pages; the tail has the last one to itself
+  const int t0 = split + psp * wave, step = psp * kD8Waves;  // this wave's pages: t0 + j step
   int32_t pid = tab[min(t0 + int64_t(lane) * step, int64_t(p.blocks) - 1)];
   const float lam = p.lam[vzero];
   const int odd = h & 1, par = p.parity;
@@ -148,7 +149,7 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
   const bool bad = S64 < 0 || S64 >= int64_t(p.blocks) * kPage8;
   const int64_t S = bad ? 0 : S64;
   const int nfull = __builtin_amdgcn_readfirstlane(int(S / kPage8)), rest = __builtin_amdgcn_readfirstlane(int(S % kPage8));
-  const int np = nfull > t0 ? (nfull - t0 + step - 1) / step : 0;  // this wave's pages
+  const int np = split < psp && nfull > t0 ? (nfull - t0 + step - 1) / step : 0;  // this wave's pages
 
   // two register sets for pages, the next one's loads ahead of this one's sums
   bool gone = false;  // a block without a page
@@ -177,8 +178,8 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
     resolve(0);
     fetch(0, I0{});
   }
-  // the tail, by the last split (it has the fewest pages): 16 rows a wave, a quad of lanes a row of P2, and for I~ a lane
-  // the dims that it has of a page
+  // the tail, by the last split: 16 rows a wave, a quad of lanes a row of P2, and for I~ a lane the dims that it has of a
+  // page
   const int r0 = 16 * wave, quad = lane >> 2, part4 = lane & 3;
   const bool tailed = split == nsp - 1 && rest > r0;
   Chunk tk[(PIECES + 3) / 4];
@@ -483,14 +484,16 @@ __global__ void __launch_bounds__(kD8Threads) relation_decode8_kernel(const Dec8
 
 // Splits per head: a workgroup per CU over the whole batch, each with a page for every wave; two per CU where every wave
 // still has two pages (more loads in flight, and sequences of unlike lengths even out: 16 x 4700 rows of 4 x 48, fp32
-// 11.1 -> 10.1 us, 2 x 32768 of 8 x 128 27.3 -> 26.7; below, the merge costs more: 1 x 1000 rows 9.4 and 9.7). At most
-// one split per lane of the merging wave.
+// 11.1 -> 10.1 us, 2 x 32768 of 8 x 128 27.3 -> 26.7; below, the merge costs more: 1 x 1000 rows 9.4 and 9.7). Where there
+// are several, one more for the tail alone, which is as long a chain as a page (1 x 4130 rows of 8 x 96 9.5 -> 8.4 us,
+// 4 x 4130 10.8 -> 9.3, 16 x 4700 19.4 -> 18.8). At most one split per lane of the merging wave.
 static int splits8(const mote_relation_decode8_args* a) {
   const int64_t BH = int64_t(a->B) * a->H, blocks = a->cache.blocks;
   int64_t n = device_cu_count() / BH;
   if (n < 1) n = 1;
   if (blocks >= 2 * kD8Waves * 2 * n) n *= 2;
   n = std::min(n, (blocks + kD8Waves - 1) / kD8Waves);
+  if (n > 1) ++n;
   return int(n < kD8MaxSplits ? n : kD8MaxSplits);
 }
 

@@ -490,3 +490,53 @@ def test_shared_pages_another_stream_and_views_of_a_store(cuda):
     again = relation_decode8(four[:, 0], four[:, 1], four[:, 2], Sd, c, lamd)[0]
     relation_decode8(four[:, 0], four[:, 1], four[:, 2], Sd, c, lamd, y=four[:, 3])
     assert torch.equal(four[:, 3], again) and torch.equal(four[:, :3], xd)
+
+
+def test_offsets_past_32_bits(cuda):
+    """A pool of more than 2^32 code bytes: blocks in its last pages are written, read and swept there."""
+    from mote_amd.cache8 import Cache8, cache8_read, cache8_write, relation_decode8
+
+    B, H, D, P = 2, 4, 128, 140_000
+    codes = lambda *s: torch.empty(P, H, *s, dtype=torch.uint8, device=cuda)
+    scale = lambda: torch.empty(P, H, device=cuda)
+    c, k, v, x, lam, S = _step_case(cuda, 40, BF16, B, H, D, 4, [200, 255])
+    big = Cache8(codes(8, 64, 16), scale(), codes(128, 64), scale(), c.p2_tail.clone(), c.info_tail.clone(), P - 1 - c.table)
+    assert big.p2.numel() > 1 << 32
+    for t, s in zip(big[:4], c[:4]):
+        t[P - s.shape[0]:] = s.flip(0)
+    new = [_rows(41 + i, B, H, 60, D, BF16).to(cuda) for i in range(2)]
+    start = torch.tensor([140, 190], device=cuda)  # back to the middle of a block whose tail is gone: the same in both
+    xd, lamd = x.to(cuda), lam.to(cuda)
+    a = relation_decode8(xd[:, 0], xd[:, 1], xd[:, 2], S.to(cuda), big, lamd)
+    b = relation_decode8(xd[:, 0], xd[:, 1], xd[:, 2], S.to(cuda), c, lamd)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    for cache in (big, c):
+        cache8_write(cache, *new, start)
+    for g, w in zip(cache8_read(big, start + 60, 0, 256), cache8_read(c, start + 60, 0, 256)):
+        assert torch.equal(g, w)
+    for t, s in zip(big[:4], c[:4]):
+        assert torch.equal(t[P - s.shape[0]:], s.flip(0))
+
+
+def test_two_calls_at_once(cuda):
+    """Steps of two caches on two streams, each with a workspace of its own, against the same steps one by one."""
+    from mote_amd.cache8 import decode8_workspace, relation_decode8
+
+    cases = [_step_case(cuda, s, BF16, 4, 8, 96, 40, [2500, 100, 1999, 64]) for s in (50, 60)]
+    args = []
+    for c, k, v, x, lam, S in cases:
+        xd = x.to(cuda)
+        args.append((xd[:, 0], xd[:, 1], xd[:, 2], S.to(cuda), c, lam.to(cuda)))
+    want = [relation_decode8(*a) for a in args]
+    ws = [decode8_workspace(4, 8, 96, 40 * 64, cuda) for _ in args]
+    streams = [torch.cuda.Stream() for _ in args]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(relation_decode8(*args[i], workspace=ws[i]))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        for y, gate in g:
+            assert torch.equal(y, w[0]) and torch.equal(gate, w[1])
