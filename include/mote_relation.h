@@ -920,8 +920,8 @@ int mote_pages_reserve(const mote_pages_args* args, void* stream);
  * 0 on: codes [planes][pages][page_bytes] (planes codes_sp bytes apart; 16-byte multiples), scales
  * [planes][pages][H] (planes scale_sp elements apart), refs; refs2 past them zero, codes2 and scales2 left as they
  * were. table2 [B, blocks] (dense) is the table in the new numbers. Pages beyond the new pool are dropped, their
- * entries -1 and counted in *missing (device). Workspace: mote_pages_compact_workspace() bytes, contents on entry
- * do not matter. */
+ * entries -1 and counted in *missing (device). Workspace: mote_pages_compact_workspace() bytes (0 where none
+ * is needed), contents on entry do not matter. */
 typedef struct mote_pages_compact_args {
   int planes, pages, pages2, H, B, blocks;
   int64_t page_bytes;

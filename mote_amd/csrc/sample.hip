@@ -153,16 +153,23 @@ struct Row {
       }
     } else {
       const int whole = (to - from) / PER;
-      for (int c = threadIdx.x; c < whole; c += NT) {
-        const int i0 = from + c * PER;
-        const Chunk q = load_any(p + i0);
-        float v[PER];
+      constexpr int AHEAD = 4;  // loads in flight: 64 x 131072 fp32 in 56 us with one, 53 so
+      for (int c0 = threadIdx.x; c0 < whole; c0 += NT * AHEAD) {
+        Chunk q[AHEAD];
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-          if constexpr (sizeof(T) == 2) v[k] = __uint_as_float(k % 2 ? q.w[k / 2] & 0xffff0000u : q.w[k / 2] << 16);
-          else v[k] = __uint_as_float(q.w[k]);
+        for (int u = 0; u < AHEAD; ++u) q[u] = load_any(p + from + min(c0 + u * NT, whole - 1) * PER);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int c = c0 + u * NT;
+          if (c >= whole) break;
+          float v[PER];
+#pragma unroll
+          for (int k = 0; k < PER; ++k) {
+            if constexpr (sizeof(T) == 2) v[k] = __uint_as_float(k % 2 ? q[u].w[k / 2] & 0xffff0000u : q[u].w[k / 2] << 16);
+            else v[k] = __uint_as_float(q[u].w[k]);
+          }
+          many(v, from + c * PER);
         }
-        many(v, i0);
       }
       for (int i = from + whole * PER + int(threadIdx.x); i < to; i += NT) one(Elem<T>::to_f(p[i]), i);
     }

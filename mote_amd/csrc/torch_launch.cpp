@@ -1022,9 +1022,12 @@ std::tuple<Tensor, Tensor> pages_compact(const std::vector<Tensor>& pool, const 
   a.codes2 = into[0].data_ptr(); a.codes2_sp = a.planes > 1 ? into[0].stride(0) : 0;
   a.scales2 = fptr(into[1]); a.scale2_sp = a.planes > 1 ? into[1].stride(0) : 0;
   a.refs2 = iptr(into[2]); a.table2 = iptr(table2); a.missing = iptr(missing);
-  const Tensor ws = bytes(mote_pages_compact_workspace(&a), table);
-  a.workspace = ws.data_ptr();
-  a.workspace_bytes = size_t(ws.numel());
+  Tensor ws;
+  if (const size_t n = mote_pages_compact_workspace(&a)) {
+    ws = bytes(n, table);
+    a.workspace = ws.data_ptr();
+    a.workspace_bytes = n;
+  }
   check(mote_pages_compact(&a, on.stream), "mote_pages_compact");
   return {table2, missing};
 }

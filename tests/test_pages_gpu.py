@@ -129,7 +129,8 @@ def test_fork_copies_the_newest_rows(cuda, dtype, planes, B, H, D, rows):
 
 
 @pytest.mark.parametrize("planes,P,P2,H,size,B,blocks", [(2, 9, 9, 2, 16, 2, 4), (6, 40, 30, 3, 3 * 4096, 4, 7), (2, 1500, 1500, 2, 1040, 5, 300),
-                                                          (1, 64, 500, 8, 16384 + 16, 1, 64), (4, 33, 5, 1, 20000, 3, 6)])
+                                                          (1, 64, 500, 8, 16384 + 16, 1, 64), (4, 33, 5, 1, 20000, 3, 6),
+                                                          (2, 4096, 4096, 1, 16, 2, 3000), (1, 4097, 3000, 2, 32, 2, 3000), (1, 100, 90, 1, 48, 3, 6000)])
 def test_compact(cuda, planes, P, P2, H, size, B, blocks):
     """Pages in use in the order of their numbers, into a smaller, a larger or too small a pool; the old one is left as
     it was, the new one's other pages too."""
