@@ -278,14 +278,20 @@ static int pages_sizes(const mote_pages_args* a, const char* what) {
   if (a->B > 1 && a->table_sb < a->blocks) return set_error(MOTE_ERR_ARGUMENT, "%s: sequences lie over one another", what);
   return MOTE_OK;
 }
-// the listed sequences: each in the table, each once, none of them `src`
+// The listed sequences: each in the table, none of them `src`, and each once in a launch (in two launches one may come
+// twice: the second finds what the first left).
 static int pages_seqs(const mote_pages_args* a, int src, const char* what) {
   if (a->n < 0 || (a->n > 0 && !a->seqs)) return set_error(MOTE_ERR_ARGUMENT, "%s: bad list of sequences", what);
-  for (int i = 0; i < a->n; ++i) {
-    if (a->seqs[i] < 0 || a->seqs[i] >= a->B) return set_error(MOTE_ERR_ARGUMENT, "%s: no sequence %d of %d", what, a->seqs[i], a->B);
-    if (a->seqs[i] == src) return set_error(MOTE_ERR_ARGUMENT, "%s: sequence %d is the source", what, src);
-    for (int k = 0; k < i; ++k)
-      if (a->seqs[k] == a->seqs[i]) return set_error(MOTE_ERR_ARGUMENT, "%s: sequence %d twice", what, a->seqs[i]);
+  for (int i = 0; i < a->n; i += kSeqs) {
+    int32_t sorted[kSeqs];
+    const int n = std::min(kSeqs, a->n - i);
+    std::copy(a->seqs + i, a->seqs + i + n, sorted);
+    std::sort(sorted, sorted + n);
+    for (int k = 0; k < n; ++k) {
+      if (sorted[k] < 0 || sorted[k] >= a->B) return set_error(MOTE_ERR_ARGUMENT, "%s: no sequence %d of %d", what, sorted[k], a->B);
+      if (sorted[k] == src) return set_error(MOTE_ERR_ARGUMENT, "%s: sequence %d is the source", what, src);
+      if (k > 0 && sorted[k] == sorted[k - 1]) return set_error(MOTE_ERR_ARGUMENT, "%s: sequence %d twice", what, sorted[k]);
+    }
   }
   return MOTE_OK;
 }

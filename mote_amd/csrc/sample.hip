@@ -126,13 +126,23 @@ __device__ __forceinline__ void scan_block(u64& m, uint32_t& c, S& s) {
 // R > 0: a thread holds elements tid + r NT of the row; R == 0: the row is read each time, 16 bytes a thread
 template <typename T, int NT, int R>
 struct Row {
+  static constexpr int PER = 16 / int(sizeof(T));
+  static constexpr int AHEAD = 4;  // loads in flight, the first ones from open() on: 64 x 131072 fp32 in 56 us with one, 53 so
   const T* p;
   int from, to;
   float x[R > 0 ? R : 1];
+  Chunk head[R > 0 ? 1 : AHEAD];
+  __device__ __forceinline__ void load(Chunk (&q)[AHEAD], int c0) const {
+    const int whole = (to - from) / PER;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (c0 + u * NT < whole) q[u] = load_any(p + from + (c0 + u * NT) * PER);
+  }
   __device__ __forceinline__ void open(const T* row, int f, int t) {
     p = row;
     from = f;
     to = t;
+    if constexpr (R == 0) load(head, threadIdx.x);
     if constexpr (R > 0) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
@@ -142,7 +152,6 @@ struct Row {
     }
   }
   // many(v, i) for PER logits from i on, one(v, i) for single ones
-  static constexpr int PER = 16 / int(sizeof(T));
   template <typename Many, typename One>
   __device__ __forceinline__ void each(Many many, One one) const {
     if constexpr (R > 0) {
@@ -153,11 +162,11 @@ struct Row {
       }
     } else {
       const int whole = (to - from) / PER;
-      constexpr int AHEAD = 4;  // loads in flight: 64 x 131072 fp32 in 56 us with one, 53 so
-      for (int c0 = threadIdx.x; c0 < whole; c0 += NT * AHEAD) {
-        Chunk q[AHEAD];
+      Chunk q[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) q[u] = load_any(p + from + min(c0 + u * NT, whole - 1) * PER);
+      for (int u = 0; u < AHEAD; ++u) q[u] = head[u];
+      for (int c0 = threadIdx.x; c0 < whole; c0 += NT * AHEAD) {
+        if (c0 != int(threadIdx.x)) load(q, c0);
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
           const int c = c0 + u * NT;
@@ -578,13 +587,16 @@ __device__ __forceinline__ uint32_t resolve_list(const Goals& goals, const Prefi
     for (int i = threadIdx.x; i < n; i += NT) f(s.lkey[i], s.lidx[i], s.lbin[i], [&] { return s.lw[i]; });
   });
 }
-// (from memory each time: rare, and a step over registers is unrolled)
+// (a logit at a time from memory: rare, and anything wider takes registers that the common path needs)
 template <typename T, int NT, int BINS, typename S>
-__device__ __forceinline__ uint32_t resolve_row(const Goals& goals, const Prefix<BINS>& prefix, const Scale<BINS>& sc, u64 high, const T* logits, int V, S& s) {
-  Row<T, NT, 0> row;
-  row.open(logits, 0, V);
+__device__ __forceinline__ uint32_t resolve_row(const Goals& goals, const Prefix<BINS>& prefix, const Scale<BINS>& sc, u64 high,
+                                                const T* logits, int V, S& s) {
   return resolve<true, sizeof(T) == 2 ? 16 : 0, NT>(goals, prefix, sc, high, 0, V, s, [&](auto f) {
-    row.each([&](float x, int i) { f(key_of(x), uint32_t(i), sc.bin(x), [&] { return sc.weight(x); }); });
+#pragma unroll 1
+    for (int i = threadIdx.x; i < V; i += NT) {
+      const float x = Elem<T>::to_f(logits[i]);
+      f(key_of(x), uint32_t(i), sc.bin(x), [&] { return sc.weight(x); });
+    }
   });
 }
 
@@ -803,7 +815,7 @@ __device__ __forceinline__ Whole whole_row(const RowWs& w, const SampleParams& p
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kPieceThreads, 4) sample_hist_kernel(const SampleParams p) {
   constexpr int NT = kPieceThreads;
   __shared__ struct {
     u64 mass[kBins];
@@ -813,6 +825,8 @@ __global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(const Sample
     int last;
   } s;
   const int tid = threadIdx.x, b = blockIdx.x / p.pieces, g = blockIdx.x % p.pieces;
+  Row<T, NT, 0> row;
+  row.open(reinterpret_cast<const T*>(p.logits) + b * p.l_sr, g * p.piece, min(p.V, (g + 1) * p.piece));
   if (p.run && *p.run == 0) return;
   RowWs& w = reinterpret_cast<RowWs*>(p.ws)[b];
   const Setting o(p, b);
@@ -827,8 +841,6 @@ __global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(const Sample
     s.cnt[tid + i * NT] = 0;
   }
   __syncthreads();
-  Row<T, NT, 0> row;
-  row.open(reinterpret_cast<const T*>(p.logits) + b * p.l_sr, g * p.piece, min(p.V, (g + 1) * p.piece));
   const Scale<kBins> sc(o, all.top, all.low);
   u64 high = histogram<kBins>(row, sc, o.min_p, s);
   if (o.min_p > 0.f) {
@@ -875,10 +887,13 @@ __global__ void __launch_bounds__(kPieceThreads) sample_hist_kernel(const Sample
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kPieceThreads) sample_pick_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(kPieceThreads, 4) sample_pick_kernel(const SampleParams p) {
   constexpr int NT = kPieceThreads;
   __shared__ Lds<kBins, kRowList> s;
   const int tid = threadIdx.x, b = blockIdx.x / p.pieces, g = blockIdx.x % p.pieces;
+  const T* logits = reinterpret_cast<const T*>(p.logits) + b * p.l_sr;
+  Row<T, NT, 0> row;
+  row.open(logits, g * p.piece, min(p.V, (g + 1) * p.piece));
   if (p.run && *p.run == 0) return;
   RowWs& w = reinterpret_cast<RowWs*>(p.ws)[b];
   const Setting o(p, b);
@@ -888,11 +903,8 @@ __global__ void __launch_bounds__(kPieceThreads) sample_pick_kernel(const Sample
   const Plan plan = w.plan;
   const bool fits = plan.total <= kRowList;
   const Scale<kBins> sc(o, all.top, all.low);
-  const T* logits = reinterpret_cast<const T*>(p.logits) + b * p.l_sr;
   __syncthreads();
   if (fits) {
-    Row<T, NT, 0> row;
-    row.open(logits, g * p.piece, min(p.V, (g + 1) * p.piece));
     row.each([&](float x, int i) {
       if (!plan.has(sc.bin(x))) return;
       const int at = atomicAdd(&s.n, 1u);

@@ -860,6 +860,10 @@ std::tuple<Tensor, Tensor> relation_decode8(const Tensor& p1, const Tensor& p2, 
     bad_value(what, ": g must be a contiguous fp32 [B, H] tensor");
   if (y_)
     for (const Tensor* t : {&p1, &p2, &info}) apart(*y_, H * D, *t, H * D, B, what);
+  for (const OptTensor* t : {&y_, &g_, &xm})
+    if (*t)
+      for (const Tensor& held : c_)
+        if (!ranges_apart(**t, held)) bad_value(what, ": a result lies over the cache");
   no_grad(what, {&p1, &p2, &info, &lam});
   for (const OptTensor* t : {&inv_freq, &theta, &y_, &g_, &xm})
     if (*t) no_grad(what, {&**t});

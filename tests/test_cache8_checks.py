@@ -3,6 +3,8 @@ anything could be launched."""
 
 from __future__ import annotations
 
+import ctypes as C
+
 import pytest
 import torch
 
@@ -167,6 +169,8 @@ def test_decode8_refuses():
     qkv = torch.zeros(2, 3, 4, 48, dtype=BF16)
     with pytest.raises(ValueError, match="lies over an input"):
         relation_decode8(qkv[:, 0], qkv[:, 1], qkv[:, 2], S, c, lam, y=qkv[:, 2])
+    with pytest.raises(ValueError, match="over the cache"):
+        relation_decode8(x, x, x, S, c, lam, y=c.p2_tail[0].view(-1)[: 2 * 4 * 48].view(2, 4, 48))
     with pytest.raises(RuntimeError, match="no backward"):
         relation_decode8(x, x, x, S, c, torch.nn.Parameter(torch.tensor(0.5)))
     with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="dual"):
@@ -185,12 +189,12 @@ def test_the_c_entries_refuse():
     c = a.cache
     for f in ("p2", "p2_scale", "info", "info_scale", "p2_tail", "info_tail", "table"):
         setattr(c, f, 16)
-    c.pages, c.blocks, c.codes_sp, c.scale_sp, c.tail_sb, c.table_sb = 5, 2, 4 * 3072, 4, 4 * 64 * 48, 2
+    c.pages, c.blocks, c.codes_sp, c.scale_sp, c.tail_sb, c.table_sb = 5, 2, 4 * 64 * 48, 4, 4 * 64 * 48, 2
     need = int(lib.mote_relation_decode8_workspace(a))
     assert need > 0 and need % 32 == 0
     a.workspace_bytes = need - 1
     assert lib.mote_relation_decode8(a, None) == 3
-    for f, v, rc in (("codes_sp", 4 * 3072 - 16, 1), ("codes_sp", 4 * 3072 + 8, 1), ("scale_sp", 3, 1), ("tail_sb", 100, 1),
+    for f, v, rc in (("codes_sp", 4 * 64 * 48 - 16, 1), ("codes_sp", 4 * 64 * 48 + 8, 1), ("scale_sp", 3, 1), ("tail_sb", 100, 1),
                      ("table_sb", 1, 1), ("pages", 0, 1), ("blocks", 0, 1), ("p2", 24, 1), ("table", None, 1)):
         old = getattr(c, f)
         setattr(c, f, v)
@@ -219,6 +223,17 @@ def test_the_c_entries_refuse():
     assert lib.mote_sample(s, None) == 2
     s.V, s.B = 100, 0
     assert lib.mote_sample(s, None) == 0 and int(lib.mote_sample_workspace(s)) == 0
+    p = L.PagesArgs()
+    p.B, p.blocks, p.pages, p.table_sb, p.table, p.refs = 9, 4, 5, 4, 16, 16
+    for seqs, word in (([3, 9], b"no sequence 9"), ([2, 5, 2], b"sequence 2 twice"), ([-1], b"no sequence -1")):
+        held = (C.c_int32 * len(seqs))(*seqs)
+        p.seqs, p.n = C.addressof(held), len(seqs)
+        assert lib.mote_pages_free(p, None) == 1 and word in lib.mote_last_error()
+    held = (C.c_int32 * 1)(4)
+    p.seqs, p.n, p.src, p.S = C.addressof(held), 1, 4, 16
+    assert lib.mote_pages_fork(p, None) == 1 and b"is the source" in lib.mote_last_error()
+    p.n = 0
+    assert lib.mote_pages_free(p, None) == 0 and lib.mote_pages_fork(p, None) == 0  # nothing to do, nothing launched
     assert lib.mote_sample(None, None) == 1 and lib.mote_pages_free(None, None) == 1 and lib.mote_cache8_read(None, None) == 1
 
 
