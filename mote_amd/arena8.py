@@ -62,6 +62,7 @@ class RelationArena8(RelationArena):
         self.table = torch.full((self.batch, blocks), -1, device=self.device, dtype=torch.int32)
         self._rows: List[int] = [0] * self.batch    # rows that a sequence has pages for (host record)
         self._held: List[int] = [0] * self.n_layers  # rows that windows have stored, at least
+        self._shared = 0  # rows in blocks that forks may share
         if self.own:
             self.table.copy_(torch.arange(pages, dtype=torch.int32).view(self.batch, blocks))
             self.refs.fill_(1)
@@ -177,6 +178,8 @@ class RelationArena8(RelationArena):
         copied in every layer, S[dst] = S[src], and they get pages for as many rows as src has. Their own are released."""
         planes = self.tails.view(2 * self.n_layers, *self.tails.shape[2:])
         pages_fork(self.refs, self.table, S, src, dst, planes)
+        if len(dst):
+            self._shared = max(self._shared, min(int(S[src]), self.capacity) // PAGE * PAGE)
         rows = list(self._rows)
         for b in dst:
             rows[b], self._rows[b] = rows[src], 0
@@ -221,6 +224,10 @@ class ArenaLayer8(ArenaLayer):
             raise RuntimeError(f"no pages for rows up to {n + T}: ensure({n + T}) gives them out")
         if n % PAGE and n < a._held[self.layer]:
             raise ValueError(f"rows up to {a._held[self.layer]} are stored: a state goes back to a whole block of {PAGE}, not to {n}")
+        if n < a._shared:
+            pages = a.table[:, n // PAGE : (n + T) // PAGE]
+            if bool((a.refs[pages.clamp(min=0).long()] > 1).logical_and(pages >= 0).any()):
+                raise ValueError(f"rows {n} to {n + T} lie in blocks that forks share: release them first")
 
     def _cast(self, p2: torch.Tensor, info: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         return p2.to(self.arena.dtype), info.to(self.arena.dtype)

@@ -1,8 +1,8 @@
 """The next token of every sequence from its logits and one random number: temperature, top-k, top-p and min-p.
 
-The draw at the end of a decode step (GraphDecoder._sample, mote/infer/graph.py:243), one launch, for any number of
-sequences with settings of their own, and capturable: random numbers and settings may be device tensors that change
-between replays.
+The draw at the end of a decode step (GraphDecoder._sample, mote/infer/graph.py:243), for any number of sequences with
+settings of their own: one launch up to 8192 logits a row, three beyond. It can be captured: random numbers and settings
+may be device tensors that change between replays.
 
 Tokens stand in the order of their logits, the lowest index first among equal ones, with the weights
 w = exp((x - max) / temperature). Kept are the first `top_k`; of these the shortest run from the first on that holds at

@@ -78,3 +78,21 @@ def test_growth_keeps_every_sequence():
         a.release([1])
     with pytest.raises(ValueError, match="in use"):
         a.compact(47)
+
+
+def test_a_window_leaves_shared_blocks_alone():
+    """Back to a whole block that a fork shares: refused while it does, before anything is stored."""
+    a = RelationArena8(1, 2, 256, 32, "cpu", batch=2)
+    a.table[1, :2] = a.table[0, :2]
+    a.refs[a.table[0, :2].long()] = 2
+    a._shared = 128  # what a fork of 150 rows leaves
+    x = torch.zeros(2, 2, 70, 32)
+    for n in (0, 64):
+        with pytest.raises(ValueError, match="forks share"):
+            ArenaState(a, n)[0].write(x, x)
+    for n, T in ((128, 70), (64, 63)):  # behind them; no block of them becomes whole
+        with pytest.raises(RuntimeError, match="MI355X"):
+            ArenaState(a, n)[0].write(x[:, :, :T], x[:, :, :T])
+    a.refs[a.table[0, :2].long()] = 1  # released
+    with pytest.raises(RuntimeError, match="MI355X"):
+        ArenaState(a, 0)[0].write(x, x)

@@ -182,6 +182,8 @@ def test_a_group_of_continuations(cuda):
     assert int((shared.refs > 0).sum()) == 1
     shared.fork(0, [1, 2, 3, 4, 5], S)
     assert shared.refs.max() == 6 and int((shared.refs > 0).sum()) == 1 and S.tolist() == [100] * B
+    with pytest.raises(ValueError, match="forks share"):  # a window over a block that several sequences read
+        ArenaState(shared)[0].write(torch.zeros(B, H, 64, d // H, device=cuda, dtype=BF16), torch.zeros(B, H, 64, d // H, device=cuda, dtype=BF16))
     for t in shared.tails.flatten(0, 1):
         assert torch.equal(t[:, :, :36], t[:1, :, :36].expand(B, -1, -1, -1))
 
