@@ -12,7 +12,9 @@
 // scales are loaded a lane each, 64 pages a time, ahead of the pages.
 //
 // Grid, splits, predicate and the publish / count / merge protocol are those of relation_decode.hip; its comments
-// give the reasons. The last workgroup of a head appends: it counts itself after every other one has read.
+// give the reasons. The last workgroup of a head appends: it counts itself after every other one has read. 8 heads of 96,
+// bf16: 1 x 4130 rows 8.4 us (the chain of it), 16 sequences of up to 4700 19.9 (87 MB, 4.4 TB/s); of 128, 16 of up to
+// 32768 132 us (805 MB, 6.1 TB/s).
 #include <algorithm>
 #include <type_traits>
 

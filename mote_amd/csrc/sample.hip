@@ -15,6 +15,10 @@
 // Up to 8192 logits a workgroup has a row, in registers. Longer rows go in pieces over three launches: the maximum; the
 // histogram, and by a row's last piece its prefix sums and the intervals that a search can end in; the tokens of
 // those, and by the row's last piece the searches.
+//
+// A short row is a chain of a launch, its loads and some barriers: 1 x 271 5.0 us, 256 x 271 7.2. 64 x 131072 in fp32 (34 MB,
+// 6.6 us at a copy's rate): 6.3 + 24.5 + 23 us. The histogram's launch is bound by the weights' fp64 series (7) and the
+// LDS's additions (7); the last one by its read (7.5) and one workgroup's chain of searches (8).
 #include <algorithm>
 #include <type_traits>
 

@@ -1,8 +1,9 @@
 """Plain forms of the quantised formats, on the CPU in 64 bits with the formats' own rounding points.
 
 4 bits: groups of 32 values share a bf16 scale, codes are e2m1. 8 bits: a row shares an fp32 scale, and in the
-paged cache a block of 64 rows of a head does, whose codes are e4m3. Every 32-bit quotient and product of the definition is taken in fp64 and rounded (a quotient or product of two fp32
-values is rounded correctly that way), so codes and scales are the definition's bit for bit.
+paged cache a block of 64 rows of a head does, whose codes are e4m3. Every 32-bit quotient and product of the
+definition is taken in fp64 and rounded (a quotient or product of two fp32 values is rounded correctly that way), so
+codes and scales are the definition's bit for bit.
 """
 
 from __future__ import annotations
