@@ -198,3 +198,16 @@ def test_in_a_graph(cuda):
         torch.cuda.synchronize()
         assert torch.equal(got, eager)
         assert _check(xs, us, got, 0.5 + turn, 100 * turn) == 0
+
+
+@pytest.mark.parametrize("dtype,B,V", [(BF16, 300, 9000), (F32, 700, 8200), (F32, 1, 1 << 20), (BF16, 2, (1 << 20) - 5)])
+def test_many_rows_in_pieces_and_the_longest_rows(cuda, dtype, B, V):
+    """More rows than compute units, each in two pieces, and the longest rows there are; equal rows draw equal tokens."""
+    from mote_amd.sample import sample_tokens
+
+    x, u = _case(V + B, min(B, 40), V, dtype)
+    x, u = x.repeat(-(-B // 40), 1)[:B], u.repeat(-(-B // 40))[:B]
+    for T, k, p, m in ((1.0, 0, 0.97, 0.0), (0.8, 300, 1.0, 1e-3)):
+        got = sample_tokens(x.to(cuda), u.to(cuda), T, k, p, m)
+        assert torch.equal(got, got[:40].repeat(-(-B // 40))[:B])
+        assert _check(x[:40], u[:40], got, T, k, p, m) == 0
