@@ -13,12 +13,11 @@
 // equal ones by those of their indices.
 //
 // Up to 8192 logits a workgroup has a row, in registers. Longer rows go in pieces over three launches: the maximum; the
-// histogram, and by a row's last piece its prefix sums and the intervals that a search can end in; the tokens of
-// those, and by the row's last piece the searches.
+// histogram; then in every piece (a last one's, handed to the others, took two more trips) the prefix sums and the intervals
+// that a search can end in, of which it gathers its tokens, and the searches by the row's last piece.
 //
-// A short row is a chain of a launch, its loads and some barriers: 1 x 271 5.0 us, 256 x 271 7.2. 64 x 131072 in fp32 (34 MB,
-// 6.6 us at a copy's rate): 6.3 + 24.5 + 23 us. The histogram's launch is bound by the weights' fp64 series (7) and the
-// LDS's additions (7); the last one by its read (7.5) and one workgroup's chain of searches (8).
+// A short row is a chain of a launch, its loads and some barriers: 1 x 271 5.0 us, 256 x 271 7.0. 64 x 131072 in fp32 (34 MB,
+// 6.6 us at a copy's rate) with top-k 2000, top-p and min-p: 6.3 + 16.9 + 20.9 us.
 #include <algorithm>
 #include <type_traits>
 
@@ -49,7 +48,9 @@ struct SampleParams {
   int pieces, piece;  // logits of a piece: whole 16-byte chunks
 };
 
-constexpr int kBins = 2048;                      // intervals of a long row
+// intervals of a long row (512, 1024, 2048: 64 x 131072 fp32 with top-k 1000, top-p and min-p 43.5, 41.2, 44.7 us, 1 x
+// 131072 25.4, 22.5, 21.7; fewer cost less to add up, and more than 64 tokens in one cost a search in digits)
+constexpr int kBins = 1024;
 constexpr int kList = 1024;                      // tokens of an interval that are searched in LDS
 constexpr double kOne = 8796093022208.0;         // 2^43: the largest weight
 constexpr float kReach = 31.0f;                  // exp(-31) < 2^-44: no weight from there on
@@ -63,6 +64,15 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k); }
 
+// The intervals that each stage can end in (the weight that the ones before it leave is only known to within an interval
+// until they are searched), and how many tokens are in them.
+struct Plan {
+  int from[3], to[3];
+  uint32_t total;
+  __device__ __forceinline__ bool has(int bin) const {
+    return (bin >= from[0] && bin <= to[0]) || (bin >= from[1] && bin <= to[1]) || (bin >= from[2] && bin <= to[2]);
+  }
+};
 struct Digits {
   u64 mass[256];
   uint32_t cnt[256];
@@ -74,14 +84,16 @@ struct Lds {
   u64 lw[LIST];  // the tokens of the intervals that a search can end in
   uint32_t lkey[LIST], lidx[LIST];
   int lbin[LIST];
-  uint16_t slot[16][64];
+  u64 order[64];
+  uint16_t slot[64];
   Digits dig[3];
   u64 red64[16];
   uint32_t red32[16];
   float redf[16], redm[16];
-  u64 high;
-  uint32_t idx, n, first;
-  int last;
+  u64 high, kept;
+  uint32_t idx, n, first, token;
+  int last, stage;
+  Plan plan;
 };
 
 // wave prefix sums by DPP moves within and across rows of 16 lanes (a shuffle through LDS costs several times more)
@@ -216,40 +228,40 @@ struct Scale {
   float per;     // intervals per unit of the logit
   double rate;   // log2(e) / temperature
   __device__ __forceinline__ Scale(const Setting& o, float top_, float low) : top(top_) {
-    rate = 1.44269504088896340736 / double(o.temperature);
+    rate = fmax(1.44269504088896340736 / double(o.temperature), 1e-300);  // no 0 times infinity
     const float span = fminf(kReach * o.temperature, top - low);  // at most as far as weights reach
     per = span > 0.f ? float(BINS) / span : 0.f;
     if (!(per < __builtin_inff())) per = 3e38f;  // a span below the normal numbers
   }
-  __device__ __forceinline__ int bin(float x) const {  // never smaller for a smaller logit
-    if (x == top) return 0;
-    const float t = (top - x) * per;  // infinite or NaN where a logit is infinite: the last interval
-    return t < float(BINS - 1) ? int(t) : BINS - 1;
-  }
-  // The weight in units of 2^-43, from 2^f on |f| <= 1/2 by its power series up to f^11 (what follows is below 2^-47 of
-  // it) in fp64, without a branch: seventeen instructions, where an exponential to the last place takes three times as
-  // many.
+  // Never smaller for a smaller logit. Infinite differences end up in the last interval, and so does 0 times one; the
+  // NaN between two infinite logits is a difference of 0.
+  __device__ __forceinline__ int bin(float x) const { return int(fminf(fmaxf(top - x, 0.f) * per, float(BINS - 1))); }
+  // The weight in units of 2^-43, from 2^n (1 + f q(f)) with |f| <= 1/2, q of degree 9 through (2^f - 1) / f at Chebyshev's
+  // points (off by 2^-50), in fp64 without a branch.
   __device__ __forceinline__ u64 weight(float x) const {
-    // 0 for the largest logit; NaN where it is infinite goes as far down as any
-    const double y = fmax((double(x) - double(top)) * rate, -kReach2);
-    const double n = __builtin_rint(y), f = y - n;
-    constexpr double l = 0.693147180559945309417;
-    constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7,
-                     c8 = c7 * l / 8, c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11;
-    double e = fma(c11, f, c10);
-    e = fma(e, f, c9);
-    e = fma(e, f, c8);
-    e = fma(e, f, c7);
-    e = fma(e, f, c6);
-    e = fma(e, f, c5);
-    e = fma(e, f, c4);
-    e = fma(e, f, c3);
-    e = fma(e, f, c2);
-    e = fma(e, f, l);
+    constexpr double magic = 6755399441055744.0;  // 1.5 x 2^52: a sum with it holds the nearest whole number in its low bits
+    const double y = fmax(fmin((double(x) - double(top)) * rate, 0.0), -kReach2);  // NaN between two infinite logits: 0
+    const double t = y + magic, f = y - (t - magic);
+    double e = fma(0x1.e5e9f548e5725p-28, f, 0x1.b6571de2f2351p-24);
+    e = fma(e, f, 0x1.62bfe46117445p-20);
+    e = fma(e, f, 0x1.ffcb76789860fp-17);
+    e = fma(e, f, 0x1.4309130378460p-13);
+    e = fma(e, f, 0x1.5d87fe908f88ap-10);
+    e = fma(e, f, 0x1.3b2ab6fba385fp-7);
+    e = fma(e, f, 0x1.c6b08d7044119p-5);
+    e = fma(e, f, 0x1.ebfbdff82c590p-3);
+    e = fma(e, f, 0x1.62e42fefa39f7p-1);
     e = fma(e, f, 1.0);
-    // the sum with 2^52 holds the nearest whole number in its low bits
-    const u64 w = u64(__double_as_longlong(ldexp(e, int(n) + 43) + 4503599627370496.0)) & ((u64(1) << 52) - 1);
-    return x == top ? u64(kOne) : w;
+    const uint32_t n = uint32_t(__double_as_longlong(t));
+    const double scale = __longlong_as_double(static_cast<long long>(u64((n + 1023 + 43) << 20) << 32));  // 2^(n + 43)
+    return u64(__double_as_longlong(fma(e, scale, 4503599627370496.0))) & ((u64(1) << 52) - 1);
+  }
+  // Bounds of the logits of intervals `from` to `to` and of some beside them: half an interval covers the roundings of
+  // bin() and of `width` (1 / per), and the bounds' own are monotonic, so they pass no logit.
+  __device__ __forceinline__ void reach(int from, int to, float width, float& lo, float& hi) const {
+    const float a = fmaf(-(float(from) - 0.5f), width, top), b = fmaf(-(float(to) + 1.5f), width, top), inf = __builtin_inff();
+    hi = from > to ? -inf : from > 0 && a == a ? a : inf;
+    lo = from > to ? inf : to < BINS - 1 && b == b ? b : -inf;
   }
   // keys that an interval's logits lie between (bin() is off by less than 2^-10 of an interval)
   __device__ __forceinline__ void keys(int bin, uint32_t& lo, uint32_t& hi) const {
@@ -264,9 +276,7 @@ __device__ __forceinline__ u64 floor_of(float min_p) {
   return u64(__builtin_ceil(double(fminf(fmaxf(min_p, 0.f), 1.f)) * kOne));
 }
 // What a row's three searches are for: the last token that top-k keeps (of the running count), the last that top-p keeps,
-// the draw. They are stages of one loop, and its body is small: a row comes through it once, and instructions that no
-// wave has run before cost more than their execution (unrolled and specialised for each stage the searches of 77 tokens
-// took 8 us).
+// the draw.
 struct Goals {
   u64 fp, fu;  // top_p and u in units of 2^-64
   int64_t last;
@@ -445,24 +455,43 @@ __device__ __forceinline__ Found select(bool by_count, bool index, const Each& e
   return {mass0, m, s.idx};
 }
 
-// The same where there are at most 64 tokens, the lane's own being (key, idx, w) where `in`: each counts the ones before
-// it. Every wave does it for itself: no barrier.
+// The same by one wave where there are at most 64 tokens, the lane's own being (key, idx, w) where `in`: each counts the
+// ones before it. MANY: four instructions a token make its place in `order`, 64 words of LDS, and a scan the sums; else
+// the sums with the count, fifteen instructions and no scan (2000 of 131072 in 64 rows 44.4 us so, 43.1 by places; 1 x 271
+// 5.5, 5.7).
+template <bool MANY>
 __device__ __forceinline__ Found select_wave(bool by_count, bool in, uint32_t key, uint32_t idx, u64 w, u64 target, u64 mass0,
-                                             u64 cnt0) {
-  u64 mass = mass0;
-  uint32_t cnt = uint32_t(cnt0);
-  const uint32_t n = __popcll(__ballot(in));  // lanes 0 to n - 1
+                                             u64 cnt0, u64* order) {
+  const int lane = threadIdx.x & 63;
+  const int n = __popcll(__ballot(in));  // lanes 0 to n - 1
+  if constexpr (MANY) {
+    const u64 mine = (u64(key) << 32) | ~idx;
+    int place = 0;
+#pragma unroll 4
+    for (int j = 0; j < n; ++j) place += lane_u64(mine, j) > mine ? 1 : 0;
+    if (in) order[place] = w;
+    __builtin_amdgcn_wave_barrier();
+    const u64 here = lane < n ? order[lane] : 0, upto = mass0 + wave_scan(here), before = upto - here;
+    __builtin_amdgcn_wave_barrier();
+    const bool hit = by_count ? u64(lane) == target - cnt0 : before <= target && target < upto;
+    const int at = __ffsll(static_cast<u64>(__ballot(hit))) - 1;
+    const int src = __ffsll(static_cast<u64>(__ballot(in && place == at))) - 1;
+    return {lane_u64(before, at), lane_u64(here, at), lane_u32(idx, src)};
+  } else {
+    u64 mass = mass0;
+    uint32_t cnt = uint32_t(cnt0);
 #pragma unroll 1
-  for (uint32_t j = 0; j < n; ++j) {
-    const uint32_t kj = lane_u32(key, j), ij = lane_u32(idx, j);
-    const u64 wj = lane_u64(w, j);
-    const bool before = kj > key || (kj == key && ij < idx);
-    mass += before ? wj : 0;
-    cnt += before ? 1u : 0u;
+    for (int j = 0; j < n; ++j) {
+      const uint32_t kj = lane_u32(key, j), ij = lane_u32(idx, j);
+      const u64 wj = lane_u64(w, j);
+      const bool before = kj > key || (kj == key && ij < idx);
+      mass += before ? wj : 0;
+      cnt += before ? 1u : 0u;
+    }
+    const u64 lo = by_count ? u64(cnt) : mass;
+    const int src = __ffsll(static_cast<u64>(__ballot(in && lo <= target && target < lo + (by_count ? 1 : w)))) - 1;
+    return {lane_u64(mass, src), lane_u64(w, src), lane_u32(idx, src)};
   }
-  const u64 lo = by_count ? u64(cnt) : mass;
-  const int src = __ffsll(static_cast<u64>(__ballot(in && lo <= target && target < lo + (by_count ? 1 : w)))) - 1;
-  return {lane_u64(mass, src), lane_u64(w, src), lane_u32(idx, src)};
 }
 
 // Prefix sums of the intervals in LDS, every BINS / 64-th of them in a wave's registers.
@@ -486,7 +515,8 @@ struct Prefix {
   __device__ __forceinline__ u64 all() const { return lane_u64(m, 63); }
   // The interval in which the running count or weight passes `target` (below their sum): the first whose prefix sum is
   // larger, by two steps of 64. Every wave for itself, in scalar registers but for the comparisons.
-  __device__ __forceinline__ Interval find(bool by_count, u64 target) const {
+  __device__ __forceinline__ Interval find(int stage, u64 target) const {
+    const bool by_count = stage == 0;
     const int lane = threadIdx.x & 63;
     const int a = __ffsll(static_cast<u64>(__ballot(target < (by_count ? u64(c) : m)))) - 1;
     const int k = a * STEP + min(lane, STEP - 1);
@@ -504,15 +534,6 @@ struct Prefix {
   }
 };
 
-// The intervals that each stage can end in (the weight that the ones before it leave is only known to within an interval
-// until they are searched), and how many tokens are in them.
-struct Plan {
-  int from[3], to[3];
-  uint32_t total;
-  __device__ __forceinline__ bool has(int bin) const {
-    return (bin >= from[0] && bin <= to[0]) || (bin >= from[1] && bin <= to[1]) || (bin >= from[2] && bin <= to[2]);
-  }
-};
 template <int BINS>
 __device__ __forceinline__ Plan plan_row(const Goals& goals, u64 high, const Prefix<BINS>& prefix) {
   Plan r{{0, 0, 0}, {-1, -1, -1}, 0};
@@ -525,7 +546,7 @@ __device__ __forceinline__ Plan plan_row(const Goals& goals, u64 high, const Pre
       hi = min(hi, high);
     }
     const u64 t0 = goals.target(stage, lo), t1 = goals.target(stage, hi);
-    const Interval a = prefix.find(stage == 0, t0), b = t1 == t0 ? a : prefix.find(stage == 0, t1);
+    const Interval a = prefix.find(stage, t0), b = t1 == t0 ? a : prefix.find(stage, t1);
     lo = a.mass0;
     hi = b.mass1;
     r.total += b.cnt1 - a.cnt0;
@@ -536,58 +557,85 @@ __device__ __forceinline__ Plan plan_row(const Goals& goals, u64 high, const Pre
 }
 
 // The searches of a row: prefix sums in s, the tokens of its plan's intervals in the list (n of them), or FROM_ROW when
-// they do not fit, then each(f) gives f(key, index, interval, weight) of every token of the row. dig[0] is clear.
-template <bool FROM_ROW, int LOW, int NT, int BINS, typename S, typename Each>
+// they do not fit, then each(f) gives f(key, index, interval, weight) of every token of the row. dig[0] is clear. The
+// first wave goes by itself, the others asleep at the barrier (all of them beside it: 1 x 8000 16.9 us, 14.0 so), as long as
+// the intervals have at most 64 tokens; where one has more all go on from there.
+template <bool FROM_ROW, bool MANY, int LOW, int NT, int BINS, typename S, typename Each>
 __device__ __forceinline__ uint32_t resolve(const Goals& goals, const Prefix<BINS>& prefix, const Scale<BINS>& sc, u64 high, int n, int V,
                                             S& s, const Each& each) {
   const int lane = threadIdx.x & 63;
-  Turn turn;
   u64 kept = prefix.all();
   uint32_t token = 0;
+  int stage = 0;
+  if constexpr (!FROM_ROW) {
+    if (threadIdx.x < 64) {
+#pragma unroll
+      for (; stage < 3; ++stage) {
+        if (!goals.has(stage)) continue;
+        const u64 all = stage == 2 ? min(kept, high) : kept, target = goals.target(stage, all);
+        const Interval at = prefix.find(stage, target);
+        const int c = int(at.cnt1 - at.cnt0);
+        if (stage < 2 && c == 1) {  // the token is the interval
+          kept = at.mass1;
+          continue;
+        }
+        if (c > 64) break;
+        int have = 0;
 #pragma unroll 1
-  for (int stage = 0; stage < 3; ++stage) {
+        for (int i0 = 0; i0 < n; i0 += 64) {  // where in the list the interval's tokens are
+          const bool in = i0 + lane < n && s.lbin[min(i0 + lane, n - 1)] == at.bin;
+          const u64 mask = __ballot(in);
+          if (in) s.slot[have + __popcll(mask & ((u64(1) << lane) - 1))] = uint16_t(i0 + lane);
+          have += __popcll(mask);
+        }
+        __builtin_amdgcn_wave_barrier();
+        const int mine = lane < c ? s.slot[lane] : 0;
+        __builtin_amdgcn_wave_barrier();
+        const Found f = select_wave<MANY>(stage == 0, lane < c, s.lkey[mine], s.lidx[mine], s.lw[mine], target, at.mass0, at.cnt0, s.order);
+        kept = f.before + f.w;
+        token = f.idx;
+      }
+      if (lane == 0) {
+        s.kept = kept;
+        s.token = token;
+        s.stage = stage;
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64) {
+      stage = s.stage;
+      kept = s.kept;
+      token = s.token;
+    }
+  }
+  Turn turn;
+#pragma unroll 1
+  for (; stage < 3; ++stage) {
     if (!goals.has(stage)) continue;
     if (stage == 2) kept = min(kept, high);
     const u64 target = goals.target(stage, kept);
-    const Interval at = prefix.find(stage == 0, target);
+    const Interval at = prefix.find(stage, target);
     const uint32_t c = at.cnt1 - at.cnt0;
-    if (stage < 2 && c == 1) {  // the token is the interval
+    if (stage < 2 && c == 1) {
       kept = at.mass1;
       continue;
     }
-    Found f;
-    if (!FROM_ROW && c <= 64) {
-      uint16_t* slot = s.slot[threadIdx.x >> 6];  // the wave's: where in the list the interval's tokens are
-      int have = 0;
-#pragma unroll 1
-      for (int i0 = 0; i0 < n; i0 += 64) {
-        const bool in = i0 + lane < n && s.lbin[min(i0 + lane, n - 1)] == at.bin;
-        const u64 mask = __ballot(in);
-        if (in) slot[have + __popcll(mask & ((u64(1) << lane) - 1))] = uint16_t(i0 + lane);
-        have += __popcll(mask);
-      }
-      __builtin_amdgcn_wave_barrier();
-      const int mine = lane < int(c) ? slot[lane] : 0;
-      __builtin_amdgcn_wave_barrier();
-      f = select_wave(stage == 0, lane < int(c), s.lkey[mine], s.lidx[mine], s.lw[mine], target, at.mass0, at.cnt0);
-    } else {
-      uint32_t klo, khi;
-      sc.keys(at.bin, klo, khi);
-      auto of_bin = [&](auto g) {
-        each([&](uint32_t k, uint32_t i, int bin, auto weight) {
-          if (bin == at.bin) g(k, i, weight);
-        });
-      };
-      f = select<LOW, NT>(stage == 0, stage == 2, of_bin, target, at.mass0, at.cnt0, at.mass1 - at.mass0, c, klo, khi, V, s, turn);
-    }
+    uint32_t klo, khi;
+    sc.keys(at.bin, klo, khi);
+    auto of_bin = [&](auto g) {
+      each([&](uint32_t k, uint32_t i, int bin, auto weight) {
+        if (bin == at.bin) g(k, i, weight);
+      });
+    };
+    const Found f = select<LOW, NT>(stage == 0, stage == 2, of_bin, target, at.mass0, at.cnt0, at.mass1 - at.mass0, c, klo, khi, V, s, turn);
     kept = f.before + f.w;
     token = f.idx;
   }
   return token;
 }
-template <typename T, int NT, int BINS, typename S>
+template <typename T, bool MANY, int NT, int BINS, typename S>
 __device__ __forceinline__ uint32_t resolve_list(const Goals& goals, const Prefix<BINS>& prefix, const Scale<BINS>& sc, u64 high, int n, int V, S& s) {
-  return resolve<false, sizeof(T) == 2 ? 16 : 0, NT>(goals, prefix, sc, high, n, V, s, [&](auto f) {
+  return resolve<false, MANY, sizeof(T) == 2 ? 16 : 0, NT>(goals, prefix, sc, high, n, V, s, [&](auto f) {
     for (int i = threadIdx.x; i < n; i += NT) f(s.lkey[i], s.lidx[i], s.lbin[i], [&] { return s.lw[i]; });
   });
 }
@@ -595,7 +643,7 @@ __device__ __forceinline__ uint32_t resolve_list(const Goals& goals, const Prefi
 template <typename T, int NT, int BINS, typename S>
 __device__ __forceinline__ uint32_t resolve_row(const Goals& goals, const Prefix<BINS>& prefix, const Scale<BINS>& sc, u64 high,
                                                 const T* logits, int V, S& s) {
-  return resolve<true, sizeof(T) == 2 ? 16 : 0, NT>(goals, prefix, sc, high, 0, V, s, [&](auto f) {
+  return resolve<true, true, sizeof(T) == 2 ? 16 : 0, NT>(goals, prefix, sc, high, 0, V, s, [&](auto f) {
 #pragma unroll 1
     for (int i = threadIdx.x; i < V; i += NT) {
       const float x = Elem<T>::to_f(logits[i]);
@@ -707,7 +755,12 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
   high = cut ? s.high : ~u64(0);
   const Goals goals(o, p.V);
   const Prefix<BINS> prefix(s.mass, s.cnt);
-  const Plan plan = plan_row(goals, high, prefix);
+  if (tid < 64) {
+    const Plan plan = plan_row(goals, high, prefix);
+    if (tid == 0) s.plan = plan;
+  }
+  __syncthreads();
+  const Plan plan = s.plan;
   uint32_t token;
   if (plan.total <= LIST) {
     row.each([&](float x, int i) {
@@ -720,7 +773,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
       s.lbin[at] = bin;
     });
     __syncthreads();
-    token = resolve_list<T, NT>(goals, prefix, sc, high, int(s.n), p.V, s);
+    token = resolve_list<T, (R > 2), NT>(goals, prefix, sc, high, int(s.n), p.V, s);
   } else {
     token = resolve_row<T, NT>(goals, prefix, sc, high, row.p, p.V, s);
   }
@@ -731,12 +784,11 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
 constexpr int kPieceThreads = 512;
 constexpr int kRowList = 2048;  // tokens of the intervals that a row's searches can end in
 struct RowWs {                  // in the workspace: what a launch leaves for the next, and pieces for their row's last
-  u64 mass[kBins];              // prefix sums when the second launch has ended
+  u64 mass[kBins];
   u64 high;
   uint32_t cnt[kBins];
   float top[kMaxPieces], low[kMaxPieces];
   uint32_t nan[kMaxPieces], first[kMaxPieces];
-  Plan plan;
   uint32_t done, n;
   uint32_t key[kRowList], idx[kRowList];
 };
@@ -826,7 +878,6 @@ __global__ void __launch_bounds__(kPieceThreads, 4) sample_hist_kernel(const Sam
     uint32_t cnt[kBins];
     u64 red64[16];
     uint32_t red32[16];
-    int last;
   } s;
   const int tid = threadIdx.x, b = blockIdx.x / p.pieces, g = blockIdx.x % p.pieces;
   Row<T, NT, 0> row;
@@ -858,36 +909,6 @@ __global__ void __launch_bounds__(kPieceThreads, 4) sample_hist_kernel(const Sam
     if (s.cnt[k]) __hip_atomic_fetch_add(&w.cnt[k], s.cnt[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (s.mass[k]) __hip_atomic_fetch_add(&w.mass[k], s.mass[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  if (!last_piece(w, p.pieces, s.last)) return;
-
-  // ---- the row's last piece: prefix sums, and the intervals that a search can end in ----
-  {
-    u64 m[kBins / NT];
-    uint32_t c[kBins / NT];
-#pragma unroll
-    for (int i = 0; i < kBins / NT; ++i) {
-      m[i] = agent_load(&w.mass[tid + i * NT]);
-      c[i] = agent_load(&w.cnt[tid + i * NT]);
-    }
-#pragma unroll
-    for (int i = 0; i < kBins / NT; ++i) {
-      s.mass[tid + i * NT] = m[i];
-      s.cnt[tid + i * NT] = c[i];
-    }
-  }
-  high = o.min_p > 0.f ? agent_load(&w.high) : ~u64(0);
-  __syncthreads();
-  scan_bins<NT, kBins>(s);
-#pragma unroll
-  for (int i = 0; i < kBins / NT; ++i) {
-    w.mass[tid + i * NT] = s.mass[tid + i * NT];
-    w.cnt[tid + i * NT] = s.cnt[tid + i * NT];
-  }
-  const Plan plan = plan_row(Goals(o, p.V), high, Prefix<kBins>(s.mass, s.cnt));
-  if (tid == 0) {
-    w.plan = plan;
-    w.done = 0;
-  }
 }
 
 template <typename T>
@@ -898,18 +919,50 @@ __global__ void __launch_bounds__(kPieceThreads, 4) sample_pick_kernel(const Sam
   const T* logits = reinterpret_cast<const T*>(p.logits) + b * p.l_sr;
   Row<T, NT, 0> row;
   row.open(logits, g * p.piece, min(p.V, (g + 1) * p.piece));
-  if (p.run && *p.run == 0) return;
   RowWs& w = reinterpret_cast<RowWs*>(p.ws)[b];
+  u64 m[kBins / NT];
+  uint32_t c[kBins / NT];
+#pragma unroll
+  for (int i = 0; i < kBins / NT; ++i) {
+    m[i] = w.mass[tid + i * NT];
+    c[i] = w.cnt[tid + i * NT];
+  }
+  if (p.run && *p.run == 0) return;
   const Setting o(p, b);
   const Whole all = whole_row(w, p, o);
   if (all.over) return;
+#pragma unroll
+  for (int i = 0; i < kBins / NT; ++i) {
+    s.mass[tid + i * NT] = m[i];
+    s.cnt[tid + i * NT] = c[i];
+  }
+  for (int i = tid; i < 256; i += NT) {
+    s.dig[0].mass[i] = 0;
+    s.dig[0].cnt[i] = 0;
+  }
   if (tid == 0) s.n = 0;
-  const Plan plan = w.plan;
+  const u64 high = o.min_p > 0.f ? w.high : ~u64(0);
+  const Goals goals(o, p.V);
+  __syncthreads();
+  scan_bins<NT, kBins>(s);
+  const Prefix<kBins> prefix(s.mass, s.cnt);
+  if (tid < 64) {
+    const Plan plan = plan_row(goals, high, prefix);
+    if (tid == 0) s.plan = plan;
+  }
+  __syncthreads();
+  const Plan plan = s.plan;
   const bool fits = plan.total <= kRowList;
   const Scale<kBins> sc(o, all.top, all.low);
-  __syncthreads();
   if (fits) {
+    float l0, h0, l1, h1, l2, h2;
+    const float width = 1.0f / sc.per;
+    sc.reach(plan.from[0], plan.to[0], width, l0, h0);
+    sc.reach(plan.from[1], plan.to[1], width, l1, h1);
+    sc.reach(plan.from[2], plan.to[2], width, l2, h2);
     row.each([&](float x, int i) {
+      // six comparisons for nearly all; the interval is for the few
+      if (!(((x >= l0) & (x <= h0)) | ((x >= l1) & (x <= h1)) | ((x >= l2) & (x <= h2)))) return;
       if (!plan.has(sc.bin(x))) return;
       const int at = atomicAdd(&s.n, 1u);
       s.lkey[at] = key_of(x);
@@ -927,17 +980,6 @@ __global__ void __launch_bounds__(kPieceThreads, 4) sample_pick_kernel(const Sam
   if (!last_piece(w, p.pieces, s.last)) return;
 
   // ---- the row's last piece: the searches ----
-#pragma unroll
-  for (int i = 0; i < kBins / NT; ++i) {
-    s.mass[tid + i * NT] = w.mass[tid + i * NT];
-    s.cnt[tid + i * NT] = w.cnt[tid + i * NT];
-  }
-  for (int i = tid; i < 256; i += NT) {
-    s.dig[0].mass[i] = 0;
-    s.dig[0].cnt[i] = 0;
-  }
-  const u64 high = o.min_p > 0.f ? w.high : ~u64(0);
-  const Goals goals(o, p.V);
   uint32_t token;
   if (fits) {
     const int n = int(agent_load(&w.n));
@@ -950,10 +992,9 @@ __global__ void __launch_bounds__(kPieceThreads, 4) sample_pick_kernel(const Sam
       s.lbin[i] = sc.bin(x);
     }
     __syncthreads();
-    token = resolve_list<T, NT>(goals, Prefix<kBins>(s.mass, s.cnt), sc, high, n, p.V, s);
+    token = resolve_list<T, true, NT>(goals, prefix, sc, high, n, p.V, s);
   } else {
-    __syncthreads();
-    token = resolve_row<T, NT>(goals, Prefix<kBins>(s.mass, s.cnt), sc, high, logits, p.V, s);
+    token = resolve_row<T, NT>(goals, prefix, sc, high, logits, p.V, s);
   }
   if (tid == 0) p.tokens[b] = token;
 }
@@ -961,7 +1002,8 @@ __global__ void __launch_bounds__(kPieceThreads, 4) sample_pick_kernel(const Sam
 constexpr int kWholeRow = 8192;  // longer rows go in pieces
 
 // Pieces of a row: a workgroup a CU over the batch, two where a piece would be over 16384 logits, of at least 4096 (64 x
-// 131072 fp32 in 4, 8 pieces 56, 52 us; 16 x 131072 in 16, 32 pieces 33.8, 36.9; 1 x 32000 in 7, 3 pieces 24.5, 28).
+// 131072 in bf16 in 4, 8 pieces 46.4, 45.0 us; 1 x 131072 in fp32 in 32, 64 pieces 22.0, 24.6; 1 x 32000 in 3, 7, 15
+// 23.1, 19.5, 18.9, 16 x 32000 in 3, 7, 15 24.6, 22.1, 23.4).
 static int pieces_of(int B, int V) {
   if (V <= kWholeRow) return 1;
   int64_t n = std::max<int64_t>(device_cu_count() / B, 1);
@@ -1009,9 +1051,15 @@ int launch_sample(const mote_sample_args* a, hipStream_t stream) {
     return check_launch(what);
   }
 #define MOTE_SAMPLE(NT_, R_, BINS_) hipLaunchKernelGGL((sample_kernel<T, NT_, R_, BINS_>), dim3(a->B), dim3(NT_), 0, stream, p)
+  // few waves a row: their barriers and scans are its chain (16 x 2900 with 16 waves 12.0 us, 8 waves 10.8). Beyond 4096
+  // logits 16 waves are as fast while every row has a CU, two rows of 8 a CU when it has not (1 x 8000 15.1 and 15.6 us,
+  // 300 x 8000 28.7 and 20.6).
+  const bool crowded = a->B > device_cu_count();
 #define MOTE_SAMPLE_V                               \
   if (a->V <= 512) MOTE_SAMPLE(256, 2, 512);        \
   else if (a->V <= 1024) MOTE_SAMPLE(512, 2, 1024); \
+  else if (a->V <= 4096) MOTE_SAMPLE(512, 8, 1024); \
+  else if (crowded) MOTE_SAMPLE(512, 16, 1024);     \
   else MOTE_SAMPLE(1024, 8, 2048);
   if (a->dtype == MOTE_BF16) {
     using T = bf16_t;
