@@ -35,19 +35,6 @@ __device__ __forceinline__ uint32_t encode8(float a, float b, float c, float d) 
   return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true));
 }
 
-__device__ __forceinline__ uint32_t wave_umax(uint32_t x) {
-  u32x2 a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  x = max(a[0], a[1]);
-  a = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  x = max(a[0], a[1]);
-  auto step = [&](auto ctrl) { x = max(x, uint32_t(__builtin_amdgcn_mov_dpp(int(x), decltype(ctrl)::value, 0xF, 0xF, false))); };
-  step(std::integral_constant<int, kDppRor8>{});
-  step(std::integral_constant<int, kDppNext4>{});
-  step(std::integral_constant<int, kDppXor2>{});
-  step(std::integral_constant<int, kDppXor1>{});
-  return x;
-}
-
 // N elements (16-byte pieces) of a 16-byte aligned row
 template <int N, typename T>
 __device__ __forceinline__ void load_values(const T* p, float* x) {

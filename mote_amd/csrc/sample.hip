@@ -88,7 +88,7 @@ struct Lds {
   uint16_t slot[64];
   Digits dig[3];
   u64 red64[16];
-  uint32_t red32[16];
+  uint32_t red32[16], low32[16];
   float redf[16], redm[16];
   u64 high, kept;
   uint32_t idx, n, first, token;
@@ -230,7 +230,7 @@ struct Scale {
   __device__ __forceinline__ Scale(const Setting& o, float top_, float low) : top(top_) {
     rate = fmax(1.44269504088896340736 / double(o.temperature), 1e-300);  // no 0 times infinity
     const float span = fminf(kReach * o.temperature, top - low);  // at most as far as weights reach
-    per = span > 0.f ? float(BINS) / span : 0.f;
+    per = span > 0.f ? (float(BINS) - 1.5f) / span : 0.f;  // the last interval is for logits without weight: masked ones
     if (!(per < __builtin_inff())) per = 3e38f;  // a span below the normal numbers
   }
   // Never smaller for a smaller logit. Infinite differences end up in the last interval, and so does 0 times one; the
@@ -262,12 +262,6 @@ struct Scale {
     const float a = fmaf(-(float(from) - 0.5f), width, top), b = fmaf(-(float(to) + 1.5f), width, top), inf = __builtin_inff();
     hi = from > to ? -inf : from > 0 && a == a ? a : inf;
     lo = from > to ? inf : to < BINS - 1 && b == b ? b : -inf;
-  }
-  // keys that an interval's logits lie between (bin() is off by less than 2^-10 of an interval)
-  __device__ __forceinline__ void keys(int bin, uint32_t& lo, uint32_t& hi) const {
-    const float a = float(double(top) - (bin - 0.05) / double(per)), b = float(double(top) - (bin + 1.05) / double(per));
-    hi = bin == 0 || a != a ? key_of(top) : min(key_of(a) + 1, key_of(top));
-    lo = bin == BINS - 1 || b != b ? 0 : max(key_of(b), 1u) - 1;
   }
 };
 
@@ -346,9 +340,9 @@ __device__ __forceinline__ u64 histogram(const Rows& row, const Scale<BINS>& sc,
   return high;
 }
 // An addition to a histogram of digits; a wave whose lanes all have one digit makes one.
-__device__ __forceinline__ void add_to(Digits& d, int at, u64 w) {
+__device__ __forceinline__ void add_to(Digits& d, int at, bool weighs, u64 w) {
   if (__ballot(at == __builtin_amdgcn_readfirstlane(at)) == ~u64(0)) {
-    const u64 sum = wave_scan(w);
+    const u64 sum = weighs ? wave_scan(w) : 0;
     if ((threadIdx.x & 63) == 63) {
       atomicAdd(&d.mass[at], sum);
       atomicAdd(&d.cnt[at], 64u);
@@ -376,8 +370,8 @@ __device__ __forceinline__ u64 lane_u64(u64 x, int lane) {
 
 // The first of the tokens that each(f) gives f(key, index, weight) of, at which the running count (by_count) or weight,
 // `cnt0` and `mass0` before the first, passes `target`: by digits of 8 bits of the key, the largest first, until one token is
-// left, then of the index, the smallest first. There are `c` of them of the weight `m`; their keys lie between `klo` and
-// `khi` and differ from bit LOW on, indices are below `V`. Every thread is here; every wave has the result.
+// left, then of the index, the smallest first. There are `c` of them of the weight `m`; their least and largest keys are
+// `klo` and `khi` and differ from bit LOW on, indices are below `V`. Every thread is here; every wave has the result.
 template <int LOW, int NT, typename S, typename Each>
 __device__ __forceinline__ Found select(bool by_count, bool index, const Each& each, u64 target, u64 mass0, u64 cnt0, u64 m, uint32_t c, uint32_t klo,
                                         uint32_t khi, int V, S& s, Turn& turn) {
@@ -387,8 +381,15 @@ __device__ __forceinline__ Found select(bool by_count, bool index, const Each& e
   const uint32_t last = (1u << ibits) - 1;  // the inverse of index 0
   uint32_t kmask = above(kbits), kp = khi & kmask, ip = 0, imask = 0;
   auto mine = [&](uint32_t key, uint32_t inv) { return ((key ^ kp) & kmask) == 0 && ((inv ^ ip) & imask) == 0; };
+  bool weighs = true;
   while (c > 1 && (kbits > LOW || (index && ibits > 0))) {
     const bool on_key = kbits > LOW;
+    if (!on_key && weighs) {  // equal logits: the token by its place among them
+      weighs = false;
+      by_count = true;
+      target = (target - mass0) / (m / c);
+      cnt0 = 0;
+    }
     const int shift = on_key ? max(kbits - 8, LOW) : max(ibits - 8, 0), width = (on_key ? kbits : ibits) - shift;
     const uint32_t digits = (1u << width) - 1;
     Digits& now = s.dig[turn.digits % 3];
@@ -401,7 +402,7 @@ __device__ __forceinline__ Found select(bool by_count, bool index, const Each& e
     each([&](uint32_t key, uint32_t idx, auto weight) {
       const uint32_t inv = last - idx;
       if (!mine(key, inv)) return;
-      add_to(now, int(((on_key ? key : inv) >> shift) & digits), weight());
+      add_to(now, int(((on_key ? key : inv) >> shift) & digits), weighs, weighs ? weight() : 0);
     });
     __syncthreads();
     // lane l has digits 255 - 4 l and the three below it
@@ -549,6 +550,7 @@ __device__ __forceinline__ Plan plan_row(const Goals& goals, u64 high, const Pre
     const Interval a = prefix.find(stage, t0), b = t1 == t0 ? a : prefix.find(stage, t1);
     lo = a.mass0;
     hi = b.mass1;
+    if (stage == 0 && lo == hi) continue;  // of tokens without weight any number may go (top-k over masked ones)
     r.total += b.cnt1 - a.cnt0;
     r.from[stage] = a.bin;
     r.to[stage] = b.bin;
@@ -575,7 +577,7 @@ __device__ __forceinline__ uint32_t resolve(const Goals& goals, const Prefix<BIN
         const u64 all = stage == 2 ? min(kept, high) : kept, target = goals.target(stage, all);
         const Interval at = prefix.find(stage, target);
         const int c = int(at.cnt1 - at.cnt0);
-        if (stage < 2 && c == 1) {  // the token is the interval
+        if (stage < 2 && (c == 1 || at.mass1 == at.mass0)) {  // the token is the interval, or has no weight
           kept = at.mass1;
           continue;
         }
@@ -616,17 +618,33 @@ __device__ __forceinline__ uint32_t resolve(const Goals& goals, const Prefix<BIN
     const u64 target = goals.target(stage, kept);
     const Interval at = prefix.find(stage, target);
     const uint32_t c = at.cnt1 - at.cnt0;
-    if (stage < 2 && c == 1) {
+    if (stage < 2 && (c == 1 || at.mass1 == at.mass0)) {
       kept = at.mass1;
       continue;
     }
-    uint32_t klo, khi;
-    sc.keys(at.bin, klo, khi);
     auto of_bin = [&](auto g) {
       each([&](uint32_t k, uint32_t i, int bin, auto weight) {
         if (bin == at.bin) g(k, i, weight);
       });
     };
+    uint32_t klo = ~0u, khi = 0;  // the keys there are: one where logits are equal
+    of_bin([&](uint32_t k, uint32_t, auto) {
+      klo = min(klo, k);
+      khi = max(khi, k);
+    });
+    klo = ~wave_umax(~klo);
+    khi = wave_umax(khi);
+    __syncthreads();
+    if (lane == 0) {
+      s.red32[threadIdx.x >> 6] = khi;
+      s.low32[threadIdx.x >> 6] = klo;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) {
+      khi = max(khi, s.red32[w]);
+      klo = min(klo, s.low32[w]);
+    }
     const Found f = select<LOW, NT>(stage == 0, stage == 2, of_bin, target, at.mass0, at.cnt0, at.mass1 - at.mass0, c, klo, khi, V, s, turn);
     kept = f.before + f.w;
     token = f.idx;
@@ -639,15 +657,21 @@ __device__ __forceinline__ uint32_t resolve_list(const Goals& goals, const Prefi
     for (int i = threadIdx.x; i < n; i += NT) f(s.lkey[i], s.lidx[i], s.lbin[i], [&] { return s.lw[i]; });
   });
 }
-// (a logit at a time from memory: rare, and anything wider takes registers that the common path needs)
-template <typename T, int NT, int BINS, typename S>
+// (from memory, AHEAD loads at a time)
+template <typename T, int AHEAD, int NT, int BINS, typename S>
 __device__ __forceinline__ uint32_t resolve_row(const Goals& goals, const Prefix<BINS>& prefix, const Scale<BINS>& sc, u64 high,
                                                 const T* logits, int V, S& s) {
   return resolve<true, true, sizeof(T) == 2 ? 16 : 0, NT>(goals, prefix, sc, high, 0, V, s, [&](auto f) {
 #pragma unroll 1
-    for (int i = threadIdx.x; i < V; i += NT) {
-      const float x = Elem<T>::to_f(logits[i]);
-      f(key_of(x), uint32_t(i), sc.bin(x), [&] { return sc.weight(x); });
+    for (int i0 = threadIdx.x; i0 < V; i0 += AHEAD * NT) {
+      float x[AHEAD];
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) x[k] = Elem<T>::to_f(logits[min(i0 + k * NT, V - 1)]);
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int i = i0 + k * NT;
+        if (i < V) f(key_of(x[k]), uint32_t(i), sc.bin(x[k]), [&] { return sc.weight(x[k]); });
+      }
     }
   });
 }
@@ -706,7 +730,7 @@ __device__ __forceinline__ void extremes(const Rows& row, float& top, float& low
 
 // ---- a workgroup a row -------------------------------------------------------------------------------------
 template <typename T, int NT, int R, int BINS>
-__global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
+__global__ void __launch_bounds__(NT, 4) sample_kernel(const SampleParams p) {
   constexpr int LIST = BINS < kList ? BINS : kList;
   __shared__ Lds<BINS, LIST> s;
   const int tid = threadIdx.x, b = blockIdx.x;
@@ -775,7 +799,7 @@ __global__ void __launch_bounds__(NT) sample_kernel(const SampleParams p) {
     __syncthreads();
     token = resolve_list<T, (R > 2), NT>(goals, prefix, sc, high, int(s.n), p.V, s);
   } else {
-    token = resolve_row<T, NT>(goals, prefix, sc, high, row.p, p.V, s);
+    token = resolve_row<T, 1, NT>(goals, prefix, sc, high, row.p, p.V, s);
   }
   if (tid == 0) p.tokens[b] = token;
 }
@@ -994,7 +1018,7 @@ __global__ void __launch_bounds__(kPieceThreads, 4) sample_pick_kernel(const Sam
     __syncthreads();
     token = resolve_list<T, true, NT>(goals, prefix, sc, high, n, p.V, s);
   } else {
-    token = resolve_row<T, NT>(goals, prefix, sc, high, logits, p.V, s);
+    token = resolve_row<T, 8, NT>(goals, prefix, sc, high, logits, p.V, s);
   }
   if (tid == 0) p.tokens[b] = token;
 }

@@ -211,3 +211,29 @@ def test_many_rows_in_pieces_and_the_longest_rows(cuda, dtype, B, V):
         got = sample_tokens(x.to(cuda), u.to(cuda), T, k, p, m)
         assert torch.equal(got, got[:40].repeat(-(-B // 40))[:B])
         assert _check(x[:40], u[:40], got, T, k, p, m) == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [271, 3000, 7000, 40001])
+def test_top_k_beyond_the_unmasked_and_coarse_logits(cuda, dtype, V):
+    """A top-k that reaches into tokens at -inf, or at the type's lowest value, keeps what there is; many tokens that share few
+    values are told apart by their indices."""
+    from mote_amd.sample import sample_tokens
+
+    x, u = _case(V, 9, V, dtype)
+    for low in (-float("inf"), torch.finfo(dtype).min):
+        y = x.clone()
+        for b, left in enumerate((1, 2, 5, 30, 49, 50, 51, 100, 200)):
+            keep = torch.randperm(V, generator=torch.Generator().manual_seed(b))[:left]
+            y[b] = low
+            y[b, keep] = x[b, keep]
+        for p, m in ((1.0, 0.0), (0.9, 0.01)):
+            got = sample_tokens(y.to(cuda), u.to(cuda), 0.8, 50, p, m)
+            assert _check(y, u, got, 0.8, 50, p, m) == 0
+            whole = sample_tokens(y.to(cuda), u.to(cuda), 0.8, 0, p, m)
+            assert got[:6].tolist() == whole[:6].tolist()
+    # eighths below 1: ties of V / 8 tokens and more
+    x = (x.float().abs() * 4).floor().clamp(max=7).to(dtype) / 8
+    for T, k, p, m in ((1.0, 0, 1.0, 0.0), (0.7, V // 2, 0.9, 0.0), (1.5, V // 3, 1.0, 0.5)):
+        got = sample_tokens(x.to(cuda), u.to(cuda), T, k, p, m)
+        assert _check(x, u, got, T, k, p, m) == 0
