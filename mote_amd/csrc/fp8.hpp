@@ -8,6 +8,7 @@
 
 #include "params.hpp"
 #include "stream.hpp"
+#include "wave_uint.hpp"
 
 namespace mote {
 

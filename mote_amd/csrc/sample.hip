@@ -25,6 +25,7 @@
 #include "device.hpp"
 #include "params.hpp"
 #include "stream.hpp"
+#include "wave_uint.hpp"
 
 namespace mote {
 
