@@ -237,3 +237,19 @@ def test_top_k_beyond_the_unmasked_and_coarse_logits(cuda, dtype, V):
     for T, k, p, m in ((1.0, 0, 1.0, 0.0), (0.7, V // 2, 0.9, 0.0), (1.5, V // 3, 1.0, 0.5)):
         got = sample_tokens(x.to(cuda), u.to(cuda), T, k, p, m)
         assert _check(x, u, got, T, k, p, m) == 0
+
+
+@pytest.mark.parametrize("dtype,V", [(BF16, 131072), (F32, 60001), (F32, 6000)])
+def test_a_row_alone_and_in_a_batch(cuda, dtype, V):
+    """A row goes in other pieces, or by another kernel, when it is alone; its token is the same."""
+    from mote_amd.sample import sample_tokens
+
+    B = 300
+    x, u = _case(V, B, V, dtype)
+    xd, ud = x.to(cuda), u.to(cuda)
+    kw = dict(temperature=1.2, top_k=V // 5, top_p=0.98, min_p=1e-5)
+    whole = sample_tokens(xd, ud, **kw)
+    part = sample_tokens(xd[:20], ud[:20], **kw)
+    assert torch.equal(part, whole[:20])
+    for b in (0, 7, 19, 299):
+        assert int(sample_tokens(xd[b: b + 1], ud[b: b + 1], **kw)) == int(whole[b])
