@@ -219,7 +219,8 @@ struct Setting {
   __device__ __forceinline__ bool nan() const {
     return u != u || temperature != temperature || top_p != top_p || min_p != min_p;
   }
-  __device__ __forceinline__ bool greedy() const { return !(temperature > 0.f); }
+  // the first of the order is all that is kept: no weight reaches a min-p above 1, not even those equal to the first's
+  __device__ __forceinline__ bool greedy() const { return !(temperature > 0.f) || min_p > 1.f; }
 };
 
 // intervals and weights of a row
@@ -266,10 +267,8 @@ struct Scale {
   }
 };
 
-// the smallest weight that min_p keeps: the exact product is a whole number or lies between two
-__device__ __forceinline__ u64 floor_of(float min_p) {
-  return u64(__builtin_ceil(double(fminf(fmaxf(min_p, 0.f), 1.f)) * kOne));
-}
+// the smallest weight that min_p (at most 1) keeps: the exact product is a whole number or lies between two
+__device__ __forceinline__ u64 floor_of(float min_p) { return u64(__builtin_ceil(double(fmaxf(min_p, 0.f)) * kOne)); }
 // What a row's three searches are for: the last token that top-k keeps (of the running count), the last that top-p keeps,
 // the draw.
 struct Goals {

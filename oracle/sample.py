@@ -15,7 +15,7 @@ def sample_ref(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     if np.isnan(x).any() or not x.max() > -inf or any(t != t for t in (u, T, p, m)):
         return -1, inf
     order = np.lexsort((np.arange(V), -x))
-    if not T > 0:
+    if not T > 0 or m > 1:  # no weight reaches a min_p above 1: the first is all that is kept
         return int(order[0]), inf
     xs = x[order]
     w = np.ones(V, dtype=np.longdouble)
@@ -29,9 +29,9 @@ def sample_ref(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         t = max(p, 0.0) * total[-1]
         kept = min(int(np.searchsorted(total, t, side="left")), len(w) - 1) + 1
         margin = min(margin, float(np.abs(total - t).min()))
-    high = max(1, int((w >= min(m, 1.0)).sum()))
+    high = max(1, int((w >= m).sum()))
     if m > 0:
-        margin = min(margin, float(np.abs(w[1:] - min(m, 1.0)).min()) if len(w) > 1 else inf)
+        margin = min(margin, float(np.abs(w[1:] - m).min()) if len(w) > 1 else inf)
     kept = min(kept, high)
     t = min(max(u, 0.0), 1 - 2.0 ** -24) * total[kept - 1]
     at = min(int(np.searchsorted(total[:kept], t, side="right")), kept - 1)

@@ -1,0 +1,43 @@
+"""sample_tokens at the ends of its settings, on rows of every kernel: in registers and in pieces."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [3, 271, 5000, 8192, 20000, 131072])
+def test_min_p_above_one_keeps_the_first_alone(cuda, dtype, V):
+    """w >= min_p holds for no token, and the first of the order is always kept: of equal largest logits the first one."""
+    from mote_amd.sample import sample_tokens
+
+    B = 6
+    g = torch.Generator().manual_seed(V)
+    x = torch.randn(B, V, generator=g).clamp(max=2.0)
+    ties = torch.rand(B, V, generator=g) < 0.3
+    ties[:, -1] = True
+    x = torch.where(ties, 2.5, x).to(dtype).to(cuda)
+    first = ties.int().argmax(1).tolist()
+    u = torch.tensor([0.0, 0.3, 0.6, 0.9, 0.999, 1.0 - 2.0 ** -24], device=cuda)
+    f = lambda *t: torch.tensor(t, dtype=F32, device=cuda)
+    for m in (float(np.nextafter(np.float32(1), np.float32(2))), 5.0, math.inf):
+        for kw in (dict(), dict(top_k=2), dict(top_p=0.9, temperature=0.5), dict(temperature=f(*[0.7] * B))):
+            assert sample_tokens(x, u, min_p=m, **kw).tolist() == first
+            assert sample_tokens(x, u, min_p=f(*[m] * B), **kw).tolist() == first
+    # beside rows whose setting says otherwise, and rows without a token
+    mixed = sample_tokens(x, u, min_p=f(5.0, 1.0, 5.0, 0.0, 1.0, 5.0)).tolist()
+    alone = sample_tokens(x, u, min_p=1.0).tolist()
+    free = sample_tokens(x, u).tolist()
+    assert mixed == [first[0], alone[1], first[2], free[3], alone[4], first[5]]
+    places = [torch.nonzero(t).flatten().tolist() for t in ties]
+    assert alone == [p[int(float(t) * len(p))] for p, t in zip(places, u.double())]
+    x[0, 1], u[1] = float("nan"), float("nan")
+    assert sample_tokens(x, u, min_p=2.0).tolist() == [-1, -1] + first[2:]
