@@ -232,7 +232,7 @@ struct Scale {
   __device__ __forceinline__ Scale(const Setting& o, float top_, float low) : top(top_) {
     rate = fmax(1.44269504088896340736 / double(o.temperature), 1e-300);  // no 0 times infinity
     const float span = fminf(kReach * o.temperature, top - low);  // at most as far as weights reach
-    per = span > 0.f ? (float(BINS) - 1.5f) / span : 0.f;  // the last interval is for logits without weight: masked ones
+    per = span > 0.f ? (float(BINS) - 1.5f) / span : 0.f;  // the last interval is for masked logits (see reach())
     if (!(per < __builtin_inff())) per = 3e38f;  // a span below the normal numbers
   }
   // Never smaller for a smaller logit. Infinite differences end up in the last interval, and so does 0 times one; the
@@ -259,10 +259,11 @@ struct Scale {
     return u64(__double_as_longlong(fma(e, scale, 4503599627370496.0))) & ((u64(1) << 52) - 1);
   }
   // Bounds of the logits of intervals `from` to `to` and of some beside them: half an interval covers the roundings of
-  // bin() and of `width` (1 / per), and the bounds' own are monotonic, so they pass no logit.
+  // bin() and of `width` (1 / per), and the bounds' own are monotonic, so they pass no logit. A bound that is not finite is
+  // none: where differences and 31 T overflow, `per` is 0 and the last interval holds logits that have weight.
   __device__ __forceinline__ void reach(int from, int to, float width, float& lo, float& hi) const {
     const float a = fmaf(-(float(from) - 0.5f), width, top), b = fmaf(-(float(to) + 1.5f), width, top), inf = __builtin_inff();
-    hi = from > to ? -inf : from > 0 && a == a ? a : inf;
+    hi = from > to ? -inf : from > 0 && a > -inf ? a : inf;
     lo = from > to ? inf : to < BINS - 1 && b == b ? b : -inf;
   }
 };

@@ -8,6 +8,8 @@ import numpy as np
 import pytest
 import torch
 
+from oracle.sample import sample_ref
+
 pytestmark = pytest.mark.gpu
 
 BF16, F32 = torch.bfloat16, torch.float32
@@ -41,3 +43,45 @@ def test_min_p_above_one_keeps_the_first_alone(cuda, dtype, V):
     assert alone == [p[int(float(t) * len(p))] for p, t in zip(places, u.double())]
     x[0, 1], u[1] = float("nan"), float("nan")
     assert sample_tokens(x, u, min_p=2.0).tolist() == [-1, -1] + first[2:]
+
+
+def _near(V):
+    """Weights are rounded by 2^-44 of the largest, V of them add up to V 2^-44 at most, and the weight kept that u and p
+    are taken of is such a sum itself."""
+    return 2 * V * 2.0 ** -44 + 2.0 ** -40
+
+
+def _check(x, u, got, T, k, p, m):
+    """Every row against the oracle; returns how many rows have a comparison too near to a border to be told."""
+    near = 0
+    for b in range(len(x)):
+        want, margin = sample_ref(x[b].double().numpy(), float(u[b]), *(t[b] if isinstance(t, list) else t for t in (T, k, p, m)))
+        if margin <= _near(x.shape[1]):
+            near += 1
+        else:
+            assert int(got[b]) == want, (b, int(got[b]), want, margin)
+    return near
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [5000, 8193, 20000, 70001])
+@pytest.mark.parametrize("few", [100, 3000])
+def test_differences_beyond_fp32(cuda, dtype, V, few):
+    """Logits whose differences overflow fp32, with temperatures at which all of them have weight, masked ones among them."""
+    from mote_amd.sample import sample_tokens
+
+    g = torch.Generator().manual_seed(V + few)
+    u = torch.tensor([0.0, 0.4, 0.9, 0.9973, 0.9999, 1.0 - 2.0 ** -24])
+    x = torch.full((len(u), V), 2e38)
+    for row in x:
+        row[torch.randperm(V, generator=g)[:few]] = -2e38
+    x[1, torch.randperm(V, generator=g)[:50]] = -math.inf
+    x[2, torch.randperm(V, generator=g)[: V - 40]] = -math.inf
+    x[2, 1], x[2, V - 1] = 2e38, -2e38
+    x[4] = -x[4]  # nearly all far below the largest
+    x = x.to(dtype)
+    xd, ud = x.to(cuda), u.to(cuda)
+    for T in (1e38, 3e38, math.inf, 1e37):
+        for k, p, m in ((0, 1.0, 0.0), (V - 30, 1.0, 0.0), (0, 0.99973, 0.0), (V - 7, 0.9997, 1e-3)):
+            got = sample_tokens(xd, ud, T, k, p, m)
+            assert _check(x, u, got, T, k, p, m) == 0, (T, k, p, m)
