@@ -85,3 +85,29 @@ def test_differences_beyond_fp32(cuda, dtype, V, few):
         for k, p, m in ((0, 1.0, 0.0), (V - 30, 1.0, 0.0), (0, 0.99973, 0.0), (V - 7, 0.9997, 1e-3)):
             got = sample_tokens(xd, ud, T, k, p, m)
             assert _check(x, u, got, T, k, p, m) == 0, (T, k, p, m)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [5000, 20000])
+def test_settings_of_each_row(cuda, dtype, V):
+    """Greedy and drawing rows in one batch, settings at the ends of their ranges, as device tensors and one by one."""
+    from mote_amd.sample import sample_tokens
+
+    B = 120
+    g = torch.Generator().manual_seed(V)
+    x, u = (torch.randn(B, V, generator=g) * 2.5).to(dtype), torch.rand(B, generator=g)
+    T = [[0.0, 1.0, 0.3, 1e-30, 1e30, math.inf, 2.0][b % 7] for b in range(B)]
+    k = [[0, 1, 5, V - 1, V, 1 << 40][b % 6] for b in range(B)]
+    p = [[1.0, 0.0, 0.5, 0.999, 2.0][b % 5] for b in range(B)]
+    m = [[0.0, 1.0, 0.01, 5.0][b % 4] for b in range(B)]
+    u[:8] = torch.tensor([0.0, 1.0 - 2.0 ** -24, 2.0 ** -40, 0.5, 0.0, 1.0 - 2.0 ** -24, 1.0, -1.0])
+    xd, ud = x.to(cuda), u.to(cuda)
+    f = lambda t: torch.tensor(t, dtype=F32, device=cuda)
+    got = sample_tokens(xd, ud, f(T), torch.tensor(k, device=cuda), f(p), f(m))
+    # a temperature that makes every weight one, and logits rounded to few values, meet borders exactly
+    assert _check(x, u, got, T, k, p, m) < B // 4
+    assert bool(((got >= 0) & (got < V)).all())
+    for b in range(0, B, 7):
+        assert int(sample_tokens(xd[b: b + 1], ud[b: b + 1], T[b], k[b], p[b], m[b])) == int(got[b])
+    again = sample_tokens(xd.flip(0), ud.flip(0), f(T).flip(0), torch.tensor(k, device=cuda).flip(0), f(p).flip(0), f(m).flip(0))
+    assert torch.equal(again.flip(0), got)
