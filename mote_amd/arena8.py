@@ -173,9 +173,10 @@ class RelationArena8(RelationArena):
         self._rows = rows
         return bool(missing)
 
-    def fork(self, src: int, dst: Sequence[int], S: torch.Tensor) -> None:
+    def fork(self, src: int, dst: Sequence[int], S: torch.Tensor) -> bool:
         """The sequences `dst` continue `src`, which holds S[src] rows: they share its whole blocks, its newest rows are
-        copied in every layer, S[dst] = S[src], and they get pages for as many rows as src has. Their own are released."""
+        copied in every layer, S[dst] = S[src], and they get pages for as many rows as src has. Their own are released.
+        Returns True when a tensor of the arena was reallocated for those pages, as `ensure` does."""
         planes = self.tails.view(2 * self.n_layers, *self.tails.shape[2:])
         pages_fork(self.refs, self.table, S, src, dst, planes)
         if len(dst):
@@ -183,7 +184,7 @@ class RelationArena8(RelationArena):
         rows = list(self._rows)
         for b in dst:
             rows[b], self._rows[b] = rows[src], 0
-        self._reserve(rows)
+        return self._reserve(rows)
 
     def release(self, seqs: Sequence[int]) -> None:
         """The sequences have ended: their pages are free. `ensure` gives them pages again."""

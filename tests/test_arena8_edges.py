@@ -1,0 +1,90 @@
+"""The life of a RelationArena8 on the host: its calls over plain loops in the place of the pages' kernels (which have
+tests of their own against such loops), so that what it gives out, records and reports can be followed step by step."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from mote_amd import arena8
+from mote_amd.arena8 import RelationArena8
+
+
+def _free(refs, table, seqs):
+    for s in list(seqs):
+        for t in table[s].tolist():
+            if 0 <= t < len(refs):
+                refs[t] -= 1
+        table[s] = -1
+
+
+def _fork(refs, table, S, src, dst, tails=None):
+    n = min(max(int(S[src]), 0) // 64, table.shape[1])
+    for s in list(dst):
+        _free(refs, table, [s])
+        table[s, :n] = table[src, :n]
+        for t in table[s].tolist():
+            if t >= 0:
+                refs[t] += 1
+        S[s] = S[src]
+        if tails is not None:
+            tails[:, s, :, : int(S[src]) % 64] = tails[:, src, :, : int(S[src]) % 64]
+
+
+def _reserve(refs, table, rows):
+    missing = 0
+    free = iter([p for p, n in enumerate(refs.tolist()) if n == 0])
+    per = rows.tolist() if torch.is_tensor(rows) else [rows] * table.shape[0]
+    for b, row in enumerate(table):
+        for j in range(min(max(per[b], 0) // 64, len(row))):
+            if row[j] < 0:
+                row[j] = next(free, -1)
+                if row[j] < 0:
+                    missing += 1
+                else:
+                    refs[row[j]] = 1
+    return torch.tensor([missing], dtype=torch.int32)
+
+
+def _compact(pool, table, into):
+    live = (pool.refs > 0).nonzero().flatten().tolist()
+    number = {old: new for new, old in enumerate(live)}
+    for old, new in number.items():
+        into.codes[:, new], into.scales[:, new], into.refs[new] = pool.codes[:, old], pool.scales[:, old], pool.refs[old]
+    into.refs[len(live):] = 0
+    return torch.tensor([[number.get(t, -1) for t in row] for row in table.tolist()], dtype=torch.int32), torch.tensor([0])
+
+
+@pytest.fixture
+def on_host(monkeypatch):
+    for name, body in (("pages_free", _free), ("pages_fork", _fork), ("pages_reserve", _reserve), ("pages_compact", _compact)):
+        monkeypatch.setattr(arena8, name, body)
+
+
+def _sound(a):
+    """Counts are the table's entries, and every sequence has the pages that the host's record says."""
+    counts = torch.zeros(a.pages, dtype=torch.int32)
+    for t in a.table[a.table >= 0].tolist():
+        counts[t] += 1
+    assert torch.equal(counts, a.refs)
+    for b, rows in enumerate(a._rows):
+        assert (a.table[b, : rows // 64] >= 0).all(), (b, rows)
+
+
+def test_a_fork_that_grows_the_pool_says_so(on_host):
+    """True when a tensor of the arena was reallocated, as `ensure` answers: what was captured over it is void."""
+    a = RelationArena8(1, 2, 640, 32, "cpu", batch=4, pages=20)
+    S = torch.full((4,), 200)
+    assert not a.ensure(320) and (a.refs > 0).sum() == 20
+    a.release([1, 2, 3])
+    store, generation = a.store, a.generation
+    assert a.fork(0, [1], S) is False  # two pages for the blocks after the three that are shared
+    assert a.store is store and a.generation == generation and (a.refs > 0).sum() == 7
+    _sound(a)
+    a.compact(8)
+    store, generation = a.store, a.generation
+    assert a.fork(0, [], S) is False and a.generation == generation
+    assert a.fork(0, [2, 3], S) is True
+    assert a.store is not store and a.generation > generation and (a.refs > 0).sum() == 11
+    assert a.cache(0).p2.data_ptr() == a.store.data_ptr()
+    _sound(a)
