@@ -122,17 +122,24 @@ class RelationArena8(RelationArena):
         self._no_views()
 
     # ---- growth and pages ------------------------------------------------------------------------
-    def ensure(self, n_chunks: int) -> bool:
-        """Make room for `n_chunks` rows of every sequence: a table that reaches them, and pages for them. Returns True when
-        a tensor of the arena was reallocated. Pages that are given out within the pool change the table in place, which
-        captured graphs see; a call that gives none out costs no launch."""
+    def ensure(self, n_chunks: int, seqs: Optional[Sequence[int]] = None) -> bool:
+        """Make room for `n_chunks` rows of every sequence, or of `seqs`: a table that reaches them, and pages for them. The
+        others keep what they have: name those that run, and the ended ones hold no pages, shorter ones no more than they
+        need. Returns True when a tensor of the arena was reallocated. Pages that are given out within the pool change the
+        table in place, which captured graphs see; a call that gives none out costs no launch."""
+        named = range(self.batch) if seqs is None else list(seqs)
+        for b in named:
+            if not 0 <= b < self.batch:
+                raise ValueError(f"no sequence {b} of {self.batch}")
         grown = False
         if n_chunks > self.capacity:
             factor = 1 << max(0, (int(n_chunks) - 1) // self.capacity).bit_length()
             self._widen(self.capacity * factor)
             grown = True
         want = self.capacity if self.own else int(n_chunks)
-        rows = [max(r, want) for r in self._rows]
+        rows = list(self._rows)
+        for b in named:
+            rows[b] = max(rows[b], want)
         return self._reserve(rows) or grown
 
     def _widen(self, capacity: int) -> None:
@@ -187,7 +194,7 @@ class RelationArena8(RelationArena):
         return self._reserve(rows)
 
     def release(self, seqs: Sequence[int]) -> None:
-        """The sequences have ended: their pages are free. `ensure` gives them pages again."""
+        """The sequences have ended: their pages are free. An `ensure` that names them, or nobody, gives them pages again."""
         pages_free(self.refs, self.table, seqs)
         for b in seqs:
             self._rows[b] = 0

@@ -88,3 +88,41 @@ def test_a_fork_that_grows_the_pool_says_so(on_host):
     assert a.store is not store and a.generation > generation and (a.refs > 0).sum() == 11
     assert a.cache(0).p2.data_ptr() == a.store.data_ptr()
     _sound(a)
+
+
+def test_the_ended_stay_without_pages(on_host):
+    """`ensure` for the sequences that run: the ended ones, and shorter ones, hold no pages for the longest's rows."""
+    a = RelationArena8(1, 2, 1024, 32, "cpu", batch=4, pages=16)
+    assert not a.ensure(256) and (a.refs > 0).sum() == 16
+    a.release([1, 2, 3])
+    assert a.compact() == 4 and a.pages == 4
+    assert a.ensure(320, [0]) is True and a.pages == 8  # a growth at least doubles the pool
+    assert (a.table[1:] == -1).all() and (a.refs > 0).sum() == 5
+    assert a.ensure(512, range(1)) is False and (a.refs > 0).sum() == 8 and a.pages == 8
+    _sound(a)
+    S = torch.full((4,), 130)
+    assert a.fork(0, [2], S) is True  # eight blocks as its source, two of them shared
+    assert a.ensure(128, [1]) is False and (a.table[1, :2] >= 0).all() and (a.table[1, 2:] == -1).all()
+    assert (a.table[3] == -1).all()
+    _sound(a)
+    assert a.ensure(128, []) is False
+    a.ensure(128)  # all of them, as without a list
+    assert (a.table[3, :2] >= 0).all()
+    assert a.ensure(1025, [3]) is True and a.capacity == 2048 and (a.table[3, :16] >= 0).all() and (a.table[1, 2:] == -1).all()
+    _sound(a)
+    for bad in ([4], [-1], [0, 9]):
+        with pytest.raises(ValueError, match="no sequence"):
+            a.ensure(64, bad)
+
+
+def test_pages_of_their_own_for_the_named(on_host):
+    """Without a pool size every sequence owns pages for its whole capacity, the ended ones once they are named again."""
+    a = RelationArena8(2, 2, 128, 32, "cpu", batch=3)
+    a.release([1])
+    assert a.ensure(129, [0, 2]) is True and a.capacity == 256
+    assert (a.table[[0, 2]] >= 0).all() and (a.table[1] == -1).all()
+    _sound(a)
+    a.ensure(1, [1])
+    assert (a.table >= 0).all() and a._rows == [256] * 3
+    assert a.ensure(257) is True and a.capacity == 512 and (a.table >= 0).all()
+    _sound(a)
