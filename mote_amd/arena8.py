@@ -233,8 +233,11 @@ class ArenaLayer8(ArenaLayer):
         if n % PAGE and n < a._held[self.layer]:
             raise ValueError(f"rows up to {a._held[self.layer]} are stored: a state goes back to a whole block of {PAGE}, not to {n}")
         if n < a._shared:
-            pages = a.table[:, n // PAGE : (n + T) // PAGE]
-            if bool((a.refs[pages.clamp(min=0).long()] > 1).logical_and(pages >= 0).any()):
+            first, pages = n // PAGE, a.table[:, n // PAGE : a._shared // PAGE]
+            shared = (a.refs[pages.clamp(min=0).long()] > 1).logical_and(pages >= 0).any(0).nonzero().flatten().tolist()
+            # the record goes down to what the counts still say, so that a window asks them only while there is more
+            a._shared = PAGE * (first + shared[-1] + 1) if shared else PAGE * first
+            if shared and first + shared[0] < (n + T) // PAGE:
                 raise ValueError(f"rows {n} to {n + T} lie in blocks that forks share: release them first")
 
     def _cast(self, p2: torch.Tensor, info: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -126,3 +126,33 @@ def test_pages_of_their_own_for_the_named(on_host):
     assert (a.table >= 0).all() and a._rows == [256] * 3
     assert a.ensure(257) is True and a.capacity == 512 and (a.table >= 0).all()
     _sound(a)
+
+
+def test_windows_wait_for_the_device_only_while_blocks_are_shared(on_host, monkeypatch):
+    """What a window asks of the counts is asked once: the record of shared rows goes down with the answer."""
+    from mote_amd.arena import ArenaState
+
+    monkeypatch.setattr(arena8, "cache8_write", lambda *a: None)
+    a = RelationArena8(2, 2, 512, 32, "cpu", batch=3)
+    S = torch.full((3,), 300)
+    a.fork(0, [1], S)
+    assert a._shared == 256
+    x = torch.zeros(3, 2, 70, 32)
+    for n in (0, 64, 190):
+        with pytest.raises(ValueError, match="forks share"):
+            ArenaState(a, n)[0].write(x, x)
+    assert a._shared == 256
+    ArenaState(a, 256)[0].write(x, x)  # behind them: nothing to ask
+    a.fork(2, [1], torch.full((3,), 64))  # one shared block in the place of four
+    a._held = [0, 0]
+    ArenaState(a, 128)[0].write(x, x)
+    assert a._shared == 128  # nothing is shared from there on; the rows before were not asked about
+    with pytest.raises(ValueError, match="forks share"):
+        ArenaState(a, 0)[0].write(x, x)
+    assert a._shared == 64
+    a.release([1])
+    a.ensure(512)
+    ArenaState(a, 0)[1].write(x, x)
+    assert a._shared == 0
+    a.fork(0, [2], torch.full((3,), 130))
+    assert a._shared == 128
