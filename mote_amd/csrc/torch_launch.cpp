@@ -482,6 +482,23 @@ bool ranges_apart(const Tensor& a, const Tensor& b) {
   if (a.numel() == 0 || b.numel() == 0) return true;
   return reinterpret_cast<int64_t>(a.data_ptr()) >= end(b) || reinterpret_cast<int64_t>(b.data_ptr()) >= end(a);
 }
+// rows of `width` bytes back to back, `step` bytes apart
+struct Rows {
+  int64_t at, n, width, step;
+};
+Rows rows_of(const Tensor& t) {  // its first axis; the others lie back to back
+  const int64_t e = t.element_size(), n = t.size(0);
+  return {reinterpret_cast<int64_t>(t.data_ptr()), n, t.numel() / n * e, n > 1 ? t.stride(0) * e : 0};
+}
+// Whether the rows of two views have no byte in common: apart in their ranges, or each in the gaps of the other, which
+// rows of one step are everywhere when they are once. The rows of a view with several are apart from each other.
+bool rows_apart(const Rows& a, const Rows& b) {
+  if (a.at >= b.at + (b.n - 1) * b.step + b.width || b.at >= a.at + (a.n - 1) * a.step + a.width) return true;
+  const int64_t step = a.n > 1 ? a.step : b.step;
+  if (step <= 0 || (b.n > 1 && b.step != step)) return false;
+  const int64_t d = ((a.at - b.at) % step + step) % step;
+  return d >= b.width && d + a.width <= step;
+}
 // an int64 position per sequence (read, and with `advance` written, by the kernel as it is)
 void positions(const Tensor& t, int64_t B, c10::Device dev, const char* what, const char* name) {
   if (t.scalar_type() != at::kLong || t.device() != dev || t.numel() != B || !t.is_contiguous())
@@ -719,9 +736,12 @@ Cache8 cache8(const std::vector<Tensor>& t, int64_t B, int64_t H, int64_t D, c10
   if (writes) {
     for (const Tensor* x : {&p2, &info, &s2, &si, &t2, &ti})
       if (!separate(*x)) bad_value(what, ": pages or sequences lie over one another");
-    if (!ranges_apart(t2, ti) && !separate(t2, &ti)) bad_value(what, ": P2 and I~ must not be the same rows");
-    if (p2.data_ptr() == info.data_ptr() || s2.data_ptr() == si.data_ptr() || t2.data_ptr() == ti.data_ptr())
-      bad_value(what, ": P2 and I~ must not be the same rows");
+    std::array<Rows, 7> rows;
+    for (size_t i = 0; i < rows.size(); ++i) {
+      rows[i] = rows_of(t[i]);
+      for (size_t k = 0; k < i; ++k)
+        if (!rows_apart(rows[i], rows[k])) bad_value(what, ": two tensors of the cache lie over one another");
+    }
   }
   Cache8 r;
   r.c = mote_cache8{p2.data_ptr(), fptr(s2), info.data_ptr(), fptr(si), t2.data_ptr(), ti.data_ptr(), iptr(table),
@@ -755,9 +775,12 @@ void cache8_write(const std::vector<Tensor>& c_, Tensor p2, Tensor info, int64_t
     a.lens = static_cast<const int64_t*>(lens->data_ptr());
   }
   no_grad(what, {&p2, &info});
-  for (const Tensor* x : {&p2, &info})
-    for (const Tensor& held : c_)
+  for (const Tensor& held : c_) {
+    for (const Tensor* x : {&p2, &info})
       if (!ranges_apart(*x, held)) bad_value(what, ": the rows lie over the cache");
+    for (const OptTensor* x : {&start_dev, &lens})
+      if (*x && !ranges_apart(**x, held)) bad_value(what, ": start or lens lies over the cache");
+  }
   on_gpu(p2, what);
   const On on(p2);
   p2 = aligned(p2); info = aligned(info);
@@ -860,10 +883,11 @@ std::tuple<Tensor, Tensor> relation_decode8(const Tensor& p1, const Tensor& p2, 
     bad_value(what, ": g must be a contiguous fp32 [B, H] tensor");
   if (y_)
     for (const Tensor* t : {&p1, &p2, &info}) apart(*y_, H * D, *t, H * D, B, what);
-  for (const OptTensor* t : {&y_, &g_, &xm})
-    if (*t)
-      for (const Tensor& held : c_)
-        if (!ranges_apart(**t, held)) bad_value(what, ": a result lies over the cache");
+  for (const Tensor& held : c_) {
+    for (const OptTensor* t : {&y_, &g_, &xm})
+      if (*t && !ranges_apart(**t, held)) bad_value(what, ": a result lies over the cache");
+    if (!ranges_apart(S, held)) bad_value(what, ": S lies over the cache");
+  }
   no_grad(what, {&p1, &p2, &info, &lam});
   for (const OptTensor* t : {&inv_freq, &theta, &y_, &g_, &xm})
     if (*t) no_grad(what, {&**t});
@@ -941,6 +965,7 @@ void pages_fork(const Tensor& refs, const Tensor& table, const Tensor& S, int64_
   const char* what = "pages_fork";
   mote_pages_args a = page_table(refs, table, what);
   positions(S, a.B, table.device(), what, "S");
+  if (!ranges_apart(S, table) || !ranges_apart(S, refs)) bad_value(what, ": S lies over the table or refs");
   if (src < 0 || src >= a.B) bad_value(what, ": no sequence ", src, " of ", a.B);
   const std::vector<int32_t> list = sequences(dst, a.B, src, what);
   if (tails) {
@@ -971,6 +996,7 @@ Tensor pages_reserve(const Tensor& refs, const Tensor& table, int64_t rows, cons
   mote_pages_args a = page_table(refs, table, what);
   if (rows_dev) {
     positions(*rows_dev, a.B, table.device(), what, "rows");
+    if (!ranges_apart(*rows_dev, table) || !ranges_apart(*rows_dev, refs)) bad_value(what, ": rows lies over the table or refs");
     a.rows_dev = static_cast<const int64_t*>(rows_dev->data_ptr());
   } else if (rows < 0 || rows / 64 > a.blocks) {
     throw std::runtime_error(c10::str(what, ": ", rows, " rows in a table of ", int64_t(a.blocks) * 64));
@@ -1109,9 +1135,10 @@ Tensor int8_linear(const Tensor& x_, const Tensor& wq, const Tensor& ws, int64_t
 }
 
 // ---- the next token ---------------------------------------------------------------------------------------
-// a setting: one number, or a device tensor of one per row
+// a setting: one number, or a device tensor of one per row, apart from the result
 template <typename N, typename D>
-void setting(const py::object& x, at::ScalarType dt, int64_t B, const Tensor& like, N& number, const D*& dev, const char* name) {
+void setting(const py::object& x, at::ScalarType dt, int64_t B, const Tensor& like, const OptTensor& out, N& number, const D*& dev,
+             const char* name) {
   const char* what = "sample_tokens";
   if (!THPVariable_Check(x.ptr())) {
     try {
@@ -1126,6 +1153,7 @@ void setting(const py::object& x, at::ScalarType dt, int64_t B, const Tensor& li
     bad_value(what, ": ", name, " must be a number, or a contiguous tensor of B = ", B, " on the logits' device");
   if (t.scalar_type() != dt) throw py::type_error(c10::str(what, ": ", name, " must be ", c10::toString(dt), ", one per row"));
   no_grad(what, {&t});
+  if (out && !ranges_apart(*out, t)) bad_value(what, ": out lies over ", name);
   dev = static_cast<const D*>(t.data_ptr());
 }
 
@@ -1140,10 +1168,10 @@ Tensor sample_tokens(const Tensor& x_, const Tensor& u, const py::object& temper
   if (u.dim() != 1 || u.numel() != B || !u.is_contiguous() || u.device() != x_.device())
     bad_value(what, ": u must be a contiguous tensor of B = ", B, " on the logits' device");
   if (u.scalar_type() != at::kFloat) throw py::type_error("sample_tokens: u must be float32");
-  setting(temperature, at::kFloat, B, x_, a.temperature, a.temperature_dev, "temperature");
-  setting(top_k, at::kLong, B, x_, a.top_k, a.top_k_dev, "top_k");
-  setting(top_p, at::kFloat, B, x_, a.top_p, a.top_p_dev, "top_p");
-  setting(min_p, at::kFloat, B, x_, a.min_p, a.min_p_dev, "min_p");
+  setting(temperature, at::kFloat, B, x_, out, a.temperature, a.temperature_dev, "temperature");
+  setting(top_k, at::kLong, B, x_, out, a.top_k, a.top_k_dev, "top_k");
+  setting(top_p, at::kFloat, B, x_, out, a.top_p, a.top_p_dev, "top_p");
+  setting(min_p, at::kFloat, B, x_, out, a.min_p, a.min_p_dev, "min_p");
   if (!a.temperature_dev && !(a.temperature >= 0.f)) bad_value(what, ": temperature ", a.temperature, " (0 or more)");
   if (!a.top_k_dev && a.top_k < 0) bad_value(what, ": top_k ", a.top_k, " (0 for all, or more)");
   if (!a.top_p_dev && !(a.top_p >= 0.f)) bad_value(what, ": top_p ", a.top_p, " (0 or more)");
@@ -1152,6 +1180,8 @@ Tensor sample_tokens(const Tensor& x_, const Tensor& u, const py::object& temper
   if (out && (out->dim() != 1 || out->numel() != B || out->scalar_type() != at::kLong || out->device() != x_.device() ||
               !out->is_contiguous()))
     bad_value(what, ": out must be a contiguous int64 tensor of B = ", B, " on the logits' device");
+  if (out && (!ranges_apart(*out, x_) || !ranges_apart(*out, u) || (run && !ranges_apart(*out, *run))))
+    bad_value(what, ": out lies over the logits, u or run");
   no_grad(what, {&x_, &u});
   on_gpu(x_, what);
   const On on(x_);
