@@ -733,6 +733,7 @@ Cache8 cache8(const std::vector<Tensor>& t, int64_t B, int64_t H, int64_t D, c10
     bad_value(what, ": P2 and I~ must have the same strides");
   if (B > 1 && t2.stride(0) != ti.stride(0)) bad_value(what, ": the tails must have the same strides");
   if (P > INT_MAX || M > (int64_t(1) << 24)) bad_value(what, ": ", P, " pages, ", M, " blocks (at most 2^31 and 2^24)");
+  no_grad(what, {&s2, &si, &t2, &ti});
   if (writes) {
     for (const Tensor* x : {&p2, &info, &s2, &si, &t2, &ti})
       if (!separate(*x)) bad_value(what, ": pages or sequences lie over one another");
@@ -829,7 +830,6 @@ std::tuple<Tensor, Tensor> cache8_read(const std::vector<Tensor>& c_, int64_t he
     if (p2.requires_grad() || info.requires_grad()) throw std::runtime_error("cache8_read: out must not require a gradient");
     no_tangent(what, {&p2, &info});
   }
-  no_grad(what, {&c_[1], &c_[3], &c_[4], &c_[5]});
   a.dtype = code(out2 ? p2.scalar_type() : dtype);
   a.tail_dtype = code(like);
   on_gpu(like, what);
