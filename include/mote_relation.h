@@ -952,8 +952,9 @@ int mote_pages_compact(const mote_pages_compact_args* args, void* stream);
  * Weights w = exp((x - max) / temperature); order: by logit, ties to the lowest index first. Kept are the first
  * top_k (0: all), of these the shortest run from the first on that holds at least top_p of their weight (1: all),
  * and of those the ones with w >= min_p; the first is always kept. The token is the first in that order whose
- * running weight exceeds u times the weight kept. A temperature of 0 takes the first of the order. Each setting is
- * one number, or a device array of one per row where its _dev is not NULL.
+ * running weight exceeds u times the weight kept. A temperature of 0 takes the first of the order, and
+ * so does a min_p above 1, which no weight reaches. Each setting is one number, or a device array of one per row where
+ * its _dev is not NULL.
  * A row whose logits are all -inf, one with a NaN, and one with a NaN among u and its settings give -1. Of several
  * logits +inf each has the same weight. Weights are sums of fixed-point numbers (2^-43): no order of summation.
  * With run (device flag) 0 no token is written. Workspace: mote_sample_workspace() bytes (0 where none is needed),

@@ -13,7 +13,10 @@ blocks that are shared by a fork are held once). What a window or a step adds ta
 rows of a block that is not whole yet; the rows before are read at their 8-bit values.
 
 Rows are appended. A state may go back to a whole block (n % 64 == 0) that no other sequence shares, and replace what
-was behind it, but not into the middle of a block: a block is in 8 bits once it is whole.
+was behind it, but not into the middle of a block: a block is in 8 bits once it is whole. The arena sees windows and forks,
+not the positions of steps, which are the caller's on the device: a window that begins inside a block that steps have gone
+past is not refused and finds rows of a later block in the tail, and a step moved back to a block that forks share
+writes into their page.
 """
 
 from __future__ import annotations

@@ -4,7 +4,8 @@
 // Bookkeeping is integer work over tables of a few KB, bound by launches and by the chain of a scan; counts go by
 // integer atomics, whose order does not matter. What moves bytes is the tails' copy of a fork and the copy of a
 // compaction, both bound by memory: 15 forks of 4133 rows in 12 layers 6.8 us, 824 MB of pages moved in 313 (5.3
-// TB/s of reads and writes); 16 x 73 entries reserved 4.7, freed 2.7.
+// TB/s of reads and writes); 16 x 73 entries reserved 4.7, freed 2.7. A reservation walks the whole table by one workgroup,
+// 1024 entries a turn of 0.9 us, 2.1 where all of them need pages: 16 x 1024 entries 15 and 34 us, 2^20 0.9 and 2.1 ms.
 #include <algorithm>
 
 #include "common.hpp"

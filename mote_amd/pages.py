@@ -47,7 +47,8 @@ def pages_fork(refs: torch.Tensor, table: torch.Tensor, S: torch.Tensor, src: in
 def pages_reserve(refs: torch.Tensor, table: torch.Tensor, rows: Union[int, torch.Tensor]) -> torch.Tensor:
     """Every sequence gets pages for the rows // 64 whole blocks of its first `rows` rows where it has none yet. rows:
     one number, or int64 [B] on the device. Returns how many entries the pool had no page for (int32 [1], on the
-    device): those stay -1."""
+    device): those stay -1. The whole table is walked, 1 to 2 us for every 1024 entries: a call for a token that
+    completes no block is better not made."""
     n, dev = (0, rows) if torch.is_tensor(rows) else (int(rows), None)
     return L.native().pages_reserve(refs, table, n, dev)
 

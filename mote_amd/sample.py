@@ -26,8 +26,8 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, temperature: Union[floa
     """Token ids int64 [B] for logits [B, V] (bf16 or fp32, V <= 2^20) and u fp32 [B] in [0, 1).
 
     temperature, top_p, min_p: a number, or fp32 [B] on the device; top_k: a number, or int64 [B]. A temperature of 0
-        takes the first token; top_k 0, top_p 1 and min_p 0 leave all.
-    out: int64 [B] to write instead of a new tensor.
+        and a min_p above 1 take the first token; top_k 0, top_p 1 and min_p 0 leave all.
+    out: int64 [B] to write instead of a new tensor, apart from every operand.
     run: optional one-element bool / uint8 device tensor: when it holds 0 nothing is written.
     A row without a logit above -inf, with a NaN, or whose u or a setting is NaN gives -1. There is no derivative:
     logits that require a gradient are refused under grad mode, dual tensors always."""
